@@ -21,6 +21,9 @@ DASH_ERR_WORKSPACE = 4
 DASH_DEV_TIMEOUT = 1
 DASH_DEV_BAD_BLOCK = 2
 DASH_DEV_BAD_PAGE = 3
+DASH_DEV_BAD_TREE = 4
+DASH_DEV_NO_PAGE = 5
+DASH_DEV_BAD_ROW = 6
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
@@ -223,12 +226,67 @@ class DashCosSin2DArgs(C.Structure):
                 ("num_tokens", _i32), ("dim", _i32), ("n_tok", _i32), ("out_bf16", _i32)]
 
 
+class DashTreePlanArgs(C.Structure):
+    _fields_ = [("parents", _p), ("q_start", _p), ("ctx_len", _p), ("block_table", _p),
+                ("bt_stride", _i64), ("num_pages", _i64), ("n_seq", _i32), ("rows", _i32),
+                ("max_nodes", _i32), ("block_size", _i32), ("bt_width", _i32), ("mask_words", _i32),
+                ("depth", _p), ("row_pos", _p), ("row_seq", _p), ("mask", _p), ("slots", _p),
+                ("device_error", _p)]
+
+
+class DashTreeAttnArgs(C.Structure):
+    _fields_ = [("seqs", DashSeqs), ("kv", DashKV), ("routes", DashRoutes), ("qo", DashQO),
+                ("ctx_len", _p), ("row_pos", _p), ("mask", _p), ("mask_stride", _i64),
+                ("mask_words", _i32), ("bt_width", _i32), ("scale", _f32), ("block_size", _i32),
+                ("local_window", _i32), ("num_splits", _i32), ("device_error", _p)]
+
+
+class DashVerifyArgs(C.Structure):
+    _fields_ = [("tokens", _p), ("parents", _p), ("q_start", _p), ("target", _p),
+                ("target_stride", _i64), ("draft", _p), ("draft_stride", _i64), ("u_accept", _p),
+                ("u_sample", _p), ("n_seq", _i32), ("rows", _i32), ("max_nodes", _i32),
+                ("vocab", _i32), ("dtype", _i32), ("mode", _i32), ("n_accept", _p), ("path", _p),
+                ("next_token", _p), ("out_tokens", _p), ("device_error", _p)]
+
+
+class DashCacheTensor(C.Structure):
+    _fields_ = [("base", _p), ("page_stride", _i64), ("tok_stride", _i64), ("tok_bytes", _i32),
+                ("page_toks", _i32)]
+
+
+class DashCommitArgs(C.Structure):
+    _fields_ = [("tensors", _p), ("n_tensors", _i32), ("n_seq", _i32), ("max_nodes", _i32),
+                ("block_size", _i32), ("bt_width", _i32), ("pad0", _i32), ("num_pages", _i64),
+                ("path", _p), ("path_stride", _i64), ("n_accept", _p), ("ctx_len", _p),
+                ("block_table", _p), ("bt_stride", _i64), ("device_error", _p)]
+
+
+class DashPagesCopyArgs(C.Structure):
+    _fields_ = [("tensors", _p), ("n_tensors", _i32), ("n", _i32), ("src", _p), ("dst", _p),
+                ("count", _p), ("list", _p), ("num_pages", _i64), ("check", _i32), ("pad0", _i32),
+                ("device_error", _p)]
+
+
+class DashPagePool(C.Structure):
+    _fields_ = [("ref", _p), ("free_list", _p), ("n_free", _p), ("block_table", _p),
+                ("bt_stride", _i64), ("n_blocks", _p), ("num_pages", _i32), ("max_rows", _i32),
+                ("bt_width", _i32), ("block_size", _i32)]
+
+
+class DashPagesArgs(C.Structure):
+    _fields_ = [("pool", DashPagePool), ("into", DashPagePool), ("rows", _p), ("src", _p),
+                ("lens", _p), ("n", _i32), ("pad0", _i32), ("copy_src", _p), ("copy_dst", _p),
+                ("n_moves", _p), ("device_error", _p)]
+
+
 ABI_ORDER = [DashSeqs, DashKV, DashRoutes, DashQO, DashKbarArgs, DashRouteArgs,
              DashBlockMaxArgs, DashPrefillArgs, DashDecodeArgs, DashDeviceError,
              DashPageIdsArgs, DashPageStateArgs, DashPageAllowArgs, DashPageDecodeArgs,
              DashBlockAnyArgs, DashPageBlocksArgs, DashIndexProjArgs, DashRopeKVArgs,
              DashAttnBwdArgs, DashEntmaxArgs, DashServingPlanArgs, DashPeerHandle,
-             DashPageCoordArgs, DashCosSin2DArgs]
+             DashPageCoordArgs, DashCosSin2DArgs, DashTreePlanArgs, DashTreeAttnArgs,
+             DashVerifyArgs, DashCacheTensor, DashCommitArgs, DashPagesCopyArgs, DashPagePool,
+             DashPagesArgs]
 
 # every function the header declares
 EXPORTS = [
@@ -241,6 +299,9 @@ EXPORTS = [
     "dash_attn_bwd", "dash_attn_bwd_flag_words", "dash_entmax15_fwd", "dash_entmax15_bwd",
     "dash_serving_plan", "dash_peer_export", "dash_peer_import", "dash_peer_close",
     "dash_page_coords", "dash_cos_sin_2d", "dash_route_refresh",
+    "dash_tree_plan", "dash_tree_attn", "dash_draft_verify", "dash_draft_commit",
+    "dash_pages_copy", "dash_pages_reserve", "dash_pages_free", "dash_pages_fork",
+    "dash_pages_compact",
 ]
 
 
@@ -283,6 +344,15 @@ def load(path: str = LIB_PATH):
         ("dash_serving_plan", [C.POINTER(DashServingPlanArgs), _p]),
         ("dash_page_coords", [C.POINTER(DashPageCoordArgs), _p]),
         ("dash_cos_sin_2d", [C.POINTER(DashCosSin2DArgs), _p]),
+        ("dash_tree_plan", [C.POINTER(DashTreePlanArgs), _p]),
+        ("dash_tree_attn", [C.POINTER(DashTreeAttnArgs), _p]),
+        ("dash_draft_verify", [C.POINTER(DashVerifyArgs), _p]),
+        ("dash_draft_commit", [C.POINTER(DashCommitArgs), _p]),
+        ("dash_pages_copy", [C.POINTER(DashPagesCopyArgs), _p]),
+        ("dash_pages_reserve", [C.POINTER(DashPagesArgs), _p]),
+        ("dash_pages_free", [C.POINTER(DashPagesArgs), _p]),
+        ("dash_pages_fork", [C.POINTER(DashPagesArgs), _p]),
+        ("dash_pages_compact", [C.POINTER(DashPagesArgs), _p]),
     ]:
         f = getattr(L, name)
         f.argtypes = args

@@ -4,6 +4,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <climits>
 #include <mutex>
 #include <atomic>
 
@@ -133,7 +134,7 @@ int dash_count_launches(int reset) {
 }
 
 int dash_abi_sizes(int64_t* out, int n) {
-  const int64_t s[24] = {(int64_t)sizeof(DashSeqs),           (int64_t)sizeof(DashKV),
+  const int64_t s[32] = {(int64_t)sizeof(DashSeqs),           (int64_t)sizeof(DashKV),
                          (int64_t)sizeof(DashRoutes),         (int64_t)sizeof(DashQO),
                          (int64_t)sizeof(DashKbarArgs),       (int64_t)sizeof(DashRouteArgs),
                          (int64_t)sizeof(DashBlockMaxArgs),   (int64_t)sizeof(DashPrefillArgs),
@@ -144,9 +145,13 @@ int dash_abi_sizes(int64_t* out, int n) {
                          (int64_t)sizeof(DashIndexProjArgs),  (int64_t)sizeof(DashRopeKVArgs),
                          (int64_t)sizeof(DashAttnBwdArgs),    (int64_t)sizeof(DashEntmaxArgs),
                          (int64_t)sizeof(DashServingPlanArgs), (int64_t)sizeof(DashPeerHandle),
-                         (int64_t)sizeof(DashPageCoordArgs),   (int64_t)sizeof(DashCosSin2DArgs)};
-  for (int i = 0; i < n && i < 24; ++i) out[i] = s[i];
-  return 24;
+                         (int64_t)sizeof(DashPageCoordArgs),   (int64_t)sizeof(DashCosSin2DArgs),
+                         (int64_t)sizeof(DashTreePlanArgs),   (int64_t)sizeof(DashTreeAttnArgs),
+                         (int64_t)sizeof(DashVerifyArgs),     (int64_t)sizeof(DashCacheTensor),
+                         (int64_t)sizeof(DashCommitArgs),     (int64_t)sizeof(DashPagesCopyArgs),
+                         (int64_t)sizeof(DashPagePool),       (int64_t)sizeof(DashPagesArgs)};
+  for (int i = 0; i < n && i < 32; ++i) out[i] = s[i];
+  return 32;
 }
 
 static int validate_kbar(const DashKbarArgs* a) {
@@ -516,6 +521,162 @@ int dash_cos_sin_2d(const DashCosSin2DArgs* a, dash_stream_t stream) {
   if (!a->tok_pos || !a->page_pos || !a->inv_tok || !a->inv_page || !a->cos || !a->sin)
     return set_error(DASH_ERR_INVALID, "null pointer");
   return launch_cos_sin_2d(*a, (cudaStream_t)stream);
+}
+
+static int check_nodes(int n_seq, int rows, int max_nodes) {
+  if (n_seq < 0 || rows < 0) return set_error(DASH_ERR_INVALID, "negative size");
+  if (max_nodes < 1) return set_error(DASH_ERR_INVALID, "max_nodes must be >= 1");
+  if (max_nodes > 256) return set_error(DASH_ERR_UNSUPPORTED, "max_nodes %d > 256 drafted tokens", max_nodes);
+  return DASH_OK;
+}
+
+int dash_tree_plan(const DashTreePlanArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  int rc = check_nodes(a->n_seq, a->rows, a->max_nodes);
+  if (rc) return rc;
+  if (a->n_seq == 0 || a->rows == 0) return DASH_OK;
+  if (!a->q_start || !a->ctx_len) return set_error(DASH_ERR_INVALID, "null q_start/ctx_len");
+  if (a->mask && a->mask_words < (a->max_nodes + 31) / 32)
+    return set_error(DASH_ERR_INVALID, "mask_words %d too few for %d drafted tokens", a->mask_words, a->max_nodes);
+  if (a->slots) {
+    if (!a->block_table || a->block_size <= 0 || a->bt_width <= 0 || a->bt_stride < a->bt_width || a->num_pages <= 0)
+      return set_error(DASH_ERR_INVALID, "slots need a block table, block_size, bt_width and num_pages > 0");
+  }
+  return launch_tree_plan(*a, (cudaStream_t)stream);
+}
+
+int dash_tree_attn(const DashTreeAttnArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  int rc = check_nodes(a->seqs.n_seq, a->seqs.q_len_fixed, a->seqs.max_q_len);
+  if (rc) return rc;
+  if (a->seqs.n_seq == 0 || a->seqs.q_len_fixed == 0) return DASH_OK;
+  if (a->qo.n_heads <= 0) return set_error(DASH_ERR_INVALID, "n_heads must be > 0");
+  rc = check_kv(a->kv, a->qo.n_heads, a->block_size);
+  if (!rc) rc = check_routes(a->routes, a->qo.n_heads, a->kv.n_kv_heads);
+  if (!rc) rc = check_qo(a->qo);
+  if (rc) return rc;
+  if (!a->kv.block_table) return set_error(DASH_ERR_UNSUPPORTED, "draft trees run on a paged cache (null block_table)");
+  if (a->kv.num_pages >= INT32_MAX) return set_error(DASH_ERR_UNSUPPORTED, "num_pages must be < 2^31 - 1");
+  if (!a->seqs.q_start || !a->ctx_len || !a->row_pos || !a->mask)
+    return set_error(DASH_ERR_INVALID, "null q_start/ctx_len/row_pos/mask");
+  if (a->bt_width <= 0) return set_error(DASH_ERR_INVALID, "bt_width must be > 0");
+  if (a->mask_words < (a->seqs.max_q_len + 31) / 32 || a->mask_stride < a->mask_words)
+    return set_error(DASH_ERR_INVALID, "mask needs %d words per row and rows that far apart",
+                     (a->seqs.max_q_len + 31) / 32);
+  if (a->local_window < 0) return set_error(DASH_ERR_INVALID, "local_window must be >= 0");
+  if (a->num_splits < 0 || a->num_splits > 8) return set_error(DASH_ERR_INVALID, "num_splits %d not in [0, 8]", a->num_splits);
+  return launch_tree_attn(*a, (cudaStream_t)stream);
+}
+
+int dash_draft_verify(const DashVerifyArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  int rc = check_nodes(a->n_seq, a->rows, a->max_nodes);
+  if (rc) return rc;
+  if (a->n_seq == 0) return DASH_OK;
+  if (a->mode < 0 || a->mode > 2) return set_error(DASH_ERR_INVALID, "mode %d not in {0,1,2}", a->mode);
+  if (a->dtype != DASH_DTYPE_F32 && a->dtype != DASH_DTYPE_BF16 && a->dtype != DASH_DTYPE_F16)
+    return set_error(DASH_ERR_UNSUPPORTED, "target dtype must be fp32, bf16 or fp16");
+  if (a->vocab <= 0) return set_error(DASH_ERR_INVALID, "vocab must be > 0");
+  if (!a->q_start || !a->n_accept || !a->path || !a->next_token || !a->out_tokens)
+    return set_error(DASH_ERR_INVALID, "null q_start or output");
+  if (a->rows > 0 && (!a->tokens || !a->target)) return set_error(DASH_ERR_INVALID, "null tokens/target");
+  if (a->target_stride < a->vocab) return set_error(DASH_ERR_INVALID, "target rows shorter than vocab");
+  if (a->mode == 0 && a->rows > 0 && (!a->draft || a->draft_stride < a->vocab))
+    return set_error(DASH_ERR_INVALID, "mode 0 needs the draft's distributions (rows of vocab)");
+  if (a->mode < 2 && ((a->rows > 0 && !a->u_accept) || !a->u_sample))
+    return set_error(DASH_ERR_INVALID, "modes 0 and 1 need u_accept and u_sample");
+  return launch_verify(*a, (cudaStream_t)stream);
+}
+
+static int check_tensors(const DashCacheTensor* t, int n, int page_toks) {
+  if (n < 0) return set_error(DASH_ERR_INVALID, "n_tensors < 0");
+  if (n > 0 && !t) return set_error(DASH_ERR_INVALID, "null tensors");
+  for (int i = 0; i < n; ++i) {
+    if (!t[i].base) return set_error(DASH_ERR_INVALID, "cache tensor %d: null base", i);
+    if (t[i].tok_bytes <= 0 || t[i].page_toks <= 0 || t[i].tok_stride < t[i].tok_bytes ||
+        t[i].page_stride < (int64_t)(t[i].page_toks - 1) * t[i].tok_stride + t[i].tok_bytes)
+      return set_error(DASH_ERR_INVALID, "cache tensor %d: tokens or pages overlap", i);
+    if ((int64_t)t[i].tok_bytes * t[i].page_toks > ((int64_t)1 << 30))
+      return set_error(DASH_ERR_UNSUPPORTED, "cache tensor %d: pages above 1 GiB", i);
+    if (page_toks && t[i].page_toks != page_toks)
+      return set_error(DASH_ERR_INVALID, "cache tensor %d: %d tokens per page, not %d", i, t[i].page_toks, page_toks);
+  }
+  return DASH_OK;
+}
+
+int dash_draft_commit(const DashCommitArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  int rc = check_nodes(a->n_seq, 0, a->max_nodes);
+  if (rc) return rc;
+  if (a->n_seq > 65535) return set_error(DASH_ERR_UNSUPPORTED, "n_seq %d > 65535", a->n_seq);
+  if (a->block_size <= 0 || a->bt_width <= 0 || a->num_pages <= 0)
+    return set_error(DASH_ERR_INVALID, "block_size, bt_width and num_pages must be > 0");
+  rc = check_tensors(a->tensors, a->n_tensors, a->block_size);
+  if (rc || a->n_seq == 0 || a->n_tensors == 0) return rc;
+  if (!a->path || !a->n_accept || !a->ctx_len || !a->block_table) return set_error(DASH_ERR_INVALID, "null pointer");
+  if (a->path_stride < a->max_nodes || a->bt_stride < a->bt_width)
+    return set_error(DASH_ERR_INVALID, "path or block table rows overlap");
+  return launch_draft_commit(*a, (cudaStream_t)stream);
+}
+
+int dash_pages_copy(const DashPagesCopyArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  if (a->n < 0) return set_error(DASH_ERR_INVALID, "n < 0");
+  if (a->num_pages <= 0) return set_error(DASH_ERR_INVALID, "num_pages must be > 0");
+  int rc = check_tensors(a->tensors, a->n_tensors, 0);
+  if (rc || a->n == 0 || a->n_tensors == 0) return rc;
+  if (!a->src || !a->dst) return set_error(DASH_ERR_INVALID, "null src/dst");
+  if (a->check && !a->list) return set_error(DASH_ERR_INVALID, "a checked copy needs its list");
+  if (a->check && a->num_pages > (1 << 19))
+    return set_error(DASH_ERR_UNSUPPORTED, "num_pages %lld > 2^19", (long long)a->num_pages);
+  return launch_pages_copy(*a, (cudaStream_t)stream);
+}
+
+static int check_pool(const DashPagePool& p) {
+  if (!p.ref || !p.free_list || !p.n_free || !p.block_table || !p.n_blocks)
+    return set_error(DASH_ERR_INVALID, "null pool tensor");
+  if (p.num_pages <= 0 || p.max_rows <= 0 || p.bt_width <= 0 || p.block_size <= 0 || p.bt_stride < p.bt_width)
+    return set_error(DASH_ERR_INVALID, "pool sizes must be > 0 and table rows must not overlap");
+  if (p.num_pages > (1 << 19)) return set_error(DASH_ERR_UNSUPPORTED, "num_pages %d > 2^19", p.num_pages);
+  if (p.max_rows > 8192) return set_error(DASH_ERR_UNSUPPORTED, "max_rows %d > 8192", p.max_rows);
+  return DASH_OK;
+}
+
+static int check_pages(const DashPagesArgs* a, bool lens) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  const int rc = check_pool(a->pool);
+  if (rc) return rc;
+  if (a->n < 0) return set_error(DASH_ERR_INVALID, "n < 0");
+  if (a->n > 0 && (!a->rows || (lens && !a->lens))) return set_error(DASH_ERR_INVALID, "null rows/lens");
+  return DASH_OK;
+}
+
+int dash_pages_reserve(const DashPagesArgs* a, dash_stream_t stream) {
+  const int rc = check_pages(a, true);
+  return rc || a->n == 0 ? rc : launch_pages_reserve(*a, (cudaStream_t)stream);
+}
+
+int dash_pages_free(const DashPagesArgs* a, dash_stream_t stream) {
+  const int rc = check_pages(a, false);
+  return rc || a->n == 0 ? rc : launch_pages_free(*a, (cudaStream_t)stream);
+}
+
+int dash_pages_fork(const DashPagesArgs* a, dash_stream_t stream) {
+  const int rc = check_pages(a, true);
+  if (rc || a->n == 0) return rc;
+  if (!a->src || !a->copy_src || !a->copy_dst) return set_error(DASH_ERR_INVALID, "null src/copy_src/copy_dst");
+  return launch_pages_fork(*a, (cudaStream_t)stream);
+}
+
+int dash_pages_compact(const DashPagesArgs* a, dash_stream_t stream) {
+  int rc = check_pages(a, false);
+  if (!rc) rc = check_pool(a->into);
+  if (rc) return rc;
+  if (a->into.num_pages != a->pool.num_pages || a->into.max_rows != a->pool.max_rows ||
+      a->into.bt_width != a->pool.bt_width)
+    return set_error(DASH_ERR_INVALID, "`into` must have the pool's sizes");
+  if (!a->copy_src || !a->copy_dst || !a->n_moves) return set_error(DASH_ERR_INVALID, "null copy_src/copy_dst/n_moves");
+  return launch_pages_compact(*a, (cudaStream_t)stream);
 }
 
 int dash_entmax15_fwd(const DashEntmaxArgs* a, dash_stream_t stream) {

@@ -45,5 +45,14 @@ int launch_entmax15(const DashEntmaxArgs& a, bool backward, cudaStream_t st);
 int launch_serving_plan(const DashServingPlanArgs& a, cudaStream_t st);
 int launch_page_coords(const DashPageCoordArgs& a, cudaStream_t st);
 int launch_cos_sin_2d(const DashCosSin2DArgs& a, cudaStream_t st);
+int launch_tree_plan(const DashTreePlanArgs& a, cudaStream_t st);
+int launch_tree_attn(const DashTreeAttnArgs& a, cudaStream_t st);
+int launch_verify(const DashVerifyArgs& a, cudaStream_t st);
+int launch_draft_commit(const DashCommitArgs& a, cudaStream_t st);
+int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st);
+int launch_pages_reserve(const DashPagesArgs& a, cudaStream_t st);
+int launch_pages_free(const DashPagesArgs& a, cudaStream_t st);
+int launch_pages_fork(const DashPagesArgs& a, cudaStream_t st);
+int launch_pages_compact(const DashPagesArgs& a, cudaStream_t st);
 
 }  // namespace dash

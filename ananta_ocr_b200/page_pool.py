@@ -1,0 +1,220 @@
+"""Pages of a block-paged cache: handed out, shared, copied, freed, compacted
+(``dash_pages_*`` of libdash_b200.so).
+
+A serving cache keeps K, V, index keys and k-bar rows of every layer in pages
+with common ids.  :class:`CacheLayers` names those tensors once; every move of a
+page runs over all of them in one launch.  :class:`PagePool` holds the tables on
+the GPU: which pages a sequence owns, how many sequences hold a page, which
+pages are free.  Nothing here waits for the GPU, and everything can be captured
+into a CUDA graph; requests that do not fit leave their row as it was and are
+recorded in the ``device_error`` word.  CUDA tensors only; every non-zero
+library status raises.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import _lib as L
+from .ops import DeviceErrorWord, _need_cuda, _ptr
+
+
+def _call(fn: str, args, device) -> None:
+    """Launch on ``device``'s current stream, whatever the current device is."""
+    if torch.cuda.current_device() == device.index:
+        L.call(fn, args)
+    else:
+        with torch.cuda.device(device):
+            L.call(fn, args)
+
+
+def _ints(t: Optional[torch.Tensor], name: str, device, n: Optional[int] = None) -> Optional[torch.Tensor]:
+    """``t`` as a contiguous int32 vector (of ``n`` values) on ``device``."""
+    if t is None:
+        return None
+    _need_cuda(t)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not {device}")
+    if t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{name} must be an int32 vector" + ("" if n is None else f" of {n} values"))
+    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+class CacheLayers:
+    """The tensors of a paged cache, all indexed by the same page ids.
+
+    Each is [num_pages, page_tokens, ...] with a contiguous entry per token (any
+    stride between tokens and pages; [num_pages, 1, n] holds one entry per page,
+    like k-bar rows).  Any dtype.  The handle keeps the tensors alive; build it
+    once per set of caches."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("a cache needs at least one tensor")
+        first = self.tensors[0]
+        self.device, self.num_pages = first.device, int(first.shape[0])
+        self.c = (L.DashCacheTensor * len(self.tensors))()
+        toks = set()
+        for d, t in zip(self.c, self.tensors):
+            _need_cuda(t)
+            if t.device != self.device:
+                raise ValueError("cache tensors must be on one device")
+            if t.dim() < 2 or t.shape[0] != self.num_pages:
+                raise ValueError(f"cache tensors must be [{self.num_pages}, page_tokens, ...], got {tuple(t.shape)}")
+            e, inner = t.element_size(), 1
+            for k in range(t.dim() - 1, 1, -1):
+                if t.shape[k] != 1 and t.stride(k) != inner:
+                    raise ValueError("a token's entry must be contiguous")
+                inner *= t.shape[k]
+            d.base, d.tok_bytes, d.page_toks = t.data_ptr(), inner * e, t.shape[1]
+            d.tok_stride = inner * e if d.page_toks == 1 else t.stride(1) * e
+            d.page_stride = t.stride(0) * e if self.num_pages > 1 else d.page_toks * d.tok_stride
+            toks.add(int(d.page_toks))
+        # tokens per page, where all tensors agree
+        self.page_tokens = toks.pop() if len(toks) == 1 else None
+
+
+Layers = Union[CacheLayers, Sequence[torch.Tensor]]
+
+
+def _layers(caches: Layers) -> CacheLayers:
+    return caches if isinstance(caches, CacheLayers) else CacheLayers(caches)
+
+
+def _copy(layers: CacheLayers, src, dst, n, *, count=None, scratch=None, device_error=None) -> None:
+    a = L.DashPagesCopyArgs()
+    a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
+    a.n, a.src, a.dst, a.count = n, src, dst, count
+    a.num_pages = layers.num_pages
+    a.check, a.list = int(scratch is not None), _ptr(scratch)
+    a.device_error = device_error.ptr if device_error is not None else None
+    _call("dash_pages_copy", a, layers.device)
+
+
+def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
+               device_error: Optional[DeviceErrorWord] = None) -> None:
+    """Page ``src[i]`` -> page ``dst[i]`` in every cache tensor (int32 vectors; a
+    negative id skips the pair).  The pairs run at the same time: one whose
+    destination is another pair's source or destination is left out and
+    recorded, as is one with an id past the last page."""
+    layers = _layers(caches)
+    src = _ints(src, "src", layers.device)
+    n = int(src.shape[0])
+    dst = _ints(dst, "dst", layers.device, n)
+    if n:
+        scratch = torch.empty(2 * n, dtype=torch.int32, device=layers.device)
+        _copy(layers, src.data_ptr(), dst.data_ptr(), n, scratch=scratch, device_error=device_error)
+
+
+class PagePool:
+    """Page tables of up to ``max_rows`` sequences over ``num_pages`` pages.
+
+    ``block_table`` int32 [max_rows, max_blocks] (-1 behind a row's pages),
+    ``n_blocks`` [max_rows], ``ref`` [num_pages] (rows holding the page),
+    ``free_list`` [num_pages] (a stack, -1 behind its top), ``n_free`` [1]: CUDA
+    tensors that the attention calls read directly."""
+
+    def __init__(self, num_pages: int, max_rows: int, max_blocks: int, block_size: int, device="cuda"):
+        i32 = dict(dtype=torch.int32, device=device)
+        self._set(block_size, torch.zeros(num_pages, **i32),
+                  torch.arange(num_pages - 1, -1, -1, **i32), torch.full((1,), num_pages, **i32),
+                  torch.full((max_rows, max_blocks), -1, **i32), torch.zeros(max_rows, **i32))
+
+    @classmethod
+    def from_tensors(cls, *, block_size: int, ref, free_list, n_free, block_table, n_blocks) -> "PagePool":
+        """A pool over existing tables (kept by reference)."""
+        self = cls.__new__(cls)
+        self._set(block_size, ref, free_list, n_free, block_table, n_blocks)
+        return self
+
+    def _set(self, block_size, ref, free_list, n_free, block_table, n_blocks):
+        vecs = (ref, free_list, n_free, block_table, n_blocks)
+        _need_cuda(*vecs)
+        for t in vecs:
+            if t.dtype != torch.int32 or t.device != ref.device or t.stride(-1) != 1:
+                raise ValueError("pool tensors must be int32 on one device with unit inner stride")
+        if block_table.dim() != 2 or free_list.shape != ref.shape or n_free.numel() != 1 or \
+                n_blocks.shape != block_table.shape[:1]:
+            raise ValueError("pool tensors do not fit one another")
+        self.ref, self.free_list, self.n_free = ref, free_list, n_free
+        self.block_table, self.n_blocks = block_table, n_blocks
+        self.block_size, self.device = int(block_size), ref.device
+        c = self.c = L.DashPagePool()
+        c.ref, c.free_list, c.n_free = ref.data_ptr(), free_list.data_ptr(), n_free.data_ptr()
+        c.block_table, c.bt_stride = block_table.data_ptr(), block_table.stride(0)
+        c.n_blocks, c.num_pages = n_blocks.data_ptr(), ref.shape[0]
+        c.max_rows, c.bt_width, c.block_size = block_table.shape[0], block_table.shape[1], self.block_size
+
+    def _args(self, rows, device_error) -> L.DashPagesArgs:
+        a = L.DashPagesArgs()
+        a.pool = self.c
+        if rows is not None:
+            a.rows, a.n = rows.data_ptr(), rows.shape[0]
+        a.device_error = device_error.ptr if device_error is not None else None
+        return a
+
+    def _own(self, caches: Layers) -> CacheLayers:
+        layers = _layers(caches)
+        if layers.device != self.device or layers.num_pages < self.c.num_pages:
+            raise ValueError(f"the caches need {self.c.num_pages} pages on {self.device}")
+        return layers
+
+    def reserve(self, rows: torch.Tensor, lens: torch.Tensor,
+                device_error: Optional[DeviceErrorWord] = None) -> None:
+        """Row ``rows[i]`` gets pages for ``lens[i]`` tokens (it never loses any)."""
+        rows = _ints(rows, "rows", self.device)
+        lens = _ints(lens, "lens", self.device, rows.shape[0])
+        a = self._args(rows, device_error)
+        a.lens = lens.data_ptr()
+        _call("dash_pages_reserve", a, self.device)
+
+    def free(self, rows: torch.Tensor, keep: Optional[torch.Tensor] = None,
+             device_error: Optional[DeviceErrorWord] = None) -> None:
+        """Row ``rows[i]`` keeps its first ``keep[i]`` blocks (default none)."""
+        rows = _ints(rows, "rows", self.device)
+        keep = _ints(keep, "keep", self.device, rows.shape[0])
+        a = self._args(rows, device_error)
+        a.lens = _ptr(keep)
+        _call("dash_pages_free", a, self.device)
+
+    def fork(self, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor, caches: Layers,
+             device_error: Optional[DeviceErrorWord] = None) -> None:
+        """The empty row ``dst[i]`` becomes a copy of the first ``lens[i]`` tokens
+        of row ``src[i]``: full pages are shared, a partly filled last one is
+        copied to a page of its own in every tensor of ``caches``."""
+        layers = self._own(caches)
+        src = _ints(src, "src", self.device)
+        n = int(src.shape[0])
+        dst, lens = _ints(dst, "dst", self.device, n), _ints(lens, "lens", self.device, n)
+        if n == 0:
+            return
+        pairs = torch.empty(2 * n, dtype=torch.int32, device=self.device)
+        a = self._args(dst, device_error)
+        a.src, a.lens = src.data_ptr(), lens.data_ptr()
+        a.copy_src, a.copy_dst = pairs.data_ptr(), pairs.data_ptr() + 4 * n
+        _call("dash_pages_fork", a, self.device)
+        _copy(layers, a.copy_src, a.copy_dst, n)
+
+    def compact(self, caches: Layers, into: Optional["PagePool"] = None,
+                device_error: Optional[DeviceErrorWord] = None) -> torch.Tensor:
+        """Moves the held pages to the lowest ids.  With ``into`` (a pool of the
+        same sizes) the new tables go there and this pool keeps the old ones,
+        which stay usable until a page is handed out again: no page that they
+        name is overwritten.  Returns the number of moved pages (int32 [1],
+        on the GPU)."""
+        layers, to = self._own(caches), self if into is None else into
+        if to.device != self.device or to.block_size != self.block_size:
+            raise ValueError("`into` must be a pool of the same device and block size")
+        half = self.c.num_pages // 2
+        buf = torch.empty(2 * half + 1, dtype=torch.int32, device=self.device)
+        a = self._args(None, device_error)
+        a.into = to.c
+        a.copy_src, a.copy_dst = buf.data_ptr(), buf.data_ptr() + 4 * half
+        a.n_moves = buf.data_ptr() + 8 * half
+        _call("dash_pages_compact", a, self.device)
+        if half:
+            _copy(layers, a.copy_src, a.copy_dst, half, count=a.n_moves)
+        return buf[2 * half:]

@@ -15,6 +15,9 @@
  *   dash_prefill_attn   gather attention for many query tokens (tcgen05/TMEM)
  *   dash_decode_attn    gather attention for decode tokens over a block-paged
  *                       KV cache (split-KV with fused combine)
+ *   dash_tree_attn,     speculative decoding over that cache: attention of a tree
+ *   dash_draft_verify,  of drafted tokens, their verification, and the pages
+ *   dash_pages_*        themselves (copied, forked, compacted, freed)
  *
  * Conventions
  *  - All pointers are DEVICE pointers unless stated; strides are in ELEMENTS.
@@ -46,6 +49,10 @@ extern "C" {
 #define DASH_DEV_TIMEOUT 1     /* a bounded wait inside a kernel ran out               */
 #define DASH_DEV_BAD_BLOCK 2   /* routed block id outside [0, blocks of the sequence)   */
 #define DASH_DEV_BAD_PAGE 3    /* block-table page id outside [0, num_pages)            */
+#define DASH_DEV_BAD_TREE 4    /* draft tree: a parent not before its child, a path out of order,
+                                  more drafted tokens than the call allows              */
+#define DASH_DEV_NO_PAGE 5     /* the page pool has too few free pages for a request     */
+#define DASH_DEV_BAD_ROW 6     /* page pool: a row, length or page that does not fit     */
 
 #define DASH_DTYPE_F32 0
 #define DASH_DTYPE_BF16 1
@@ -800,6 +807,218 @@ int dash_entmax15_fwd(const DashEntmaxArgs* args, dash_stream_t stream);
 int dash_entmax15_bwd(const DashEntmaxArgs* args, dash_stream_t stream);
 
 /* ---------------------------------------------------------------------- */
+/* Speculative decoding over the paged cache (no counterpart in the reference,
+ * which decodes one token at a time).  One step checks a tree of drafted
+ * tokens per sequence: sequence s with ctx_len[s] committed tokens drafts
+ * n = q_start[s+1] - q_start[s] tokens, token i being row q_start[s] + i of the
+ * packed rows.  Token 0 is the last sampled token (the root), the others
+ * follow their parent; parents come before their children.  The K/V of token
+ * i is written at token ctx_len[s] + i of the sequence before the attention.
+ * Rows from q_start[n_seq] on are padding and stay as they were.
+ *
+ * dash_tree_plan -- per row, from the parents: depth (root 0), position
+ * ctx_len + depth, the set of the row's ancestors and itself (bit j of the
+ * row's mask words: token j), the cache slot of its K/V
+ * (block_table[s, t / block_size] * block_size + t % block_size at t = ctx_len
+ * + i; -1 where the page does not exist) and the sequence.  Every output is
+ * optional.  parents NULL: a chain.  A parent outside [0, i) records
+ * DASH_DEV_BAD_TREE and counts as none (row 0 has none).  max_nodes <= 256. */
+typedef struct {
+  const int32_t* parents;      /* [rows] token index within the sequence, -1 = none */
+  const int32_t* q_start;      /* [n_seq + 1] */
+  const int32_t* ctx_len;      /* [n_seq] */
+  const int32_t* block_table;  /* [n_seq, bt_width], for slots */
+  int64_t bt_stride;
+  int64_t num_pages;
+  int32_t n_seq, rows, max_nodes, block_size, bt_width, mask_words;
+  int32_t* depth;              /* [rows] */
+  int32_t* row_pos;            /* [rows] */
+  int32_t* row_seq;            /* [rows] */
+  uint32_t* mask;              /* [rows, mask_words], mask_words >= ceil(max_nodes / 32) */
+  int64_t* slots;              /* [rows] */
+  DashDeviceError* device_error;
+} DashTreePlanArgs;
+int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
+
+/* dash_tree_attn -- DASH attention of the drafted tokens over the paged cache.
+ * Row r = token i of sequence s at position p = row_pos[r] (>= ctx = ctx_len[s])
+ * and head h attends
+ *   committed keys j < ctx:  j > p - local_window: scale*<q,k_j>;
+ *                            else, block j/block_size routed for the row:
+ *                            scale*<q,k_j> + bias of that slot
+ *   drafted keys ctx + u, u < n:  bit u of the row's mask set: scale*<q,k>
+ * out = softmax @ V; a row without a key gets 0 and lse -inf.  Ids repeated
+ * in a row count once (first occurrence), -1 slots are unused.  Keys on a page
+ * outside [0, num_pages) are left out and recorded.  K/V, q and out are bf16
+ * or fp16, paged (block_table set), head_dim 128, page size == block_size;
+ * block_size 16, 32 and multiples of 64 up to 256 run on the tensor cores
+ * with up to 128 query heads per kv head, other sizes on the CUDA cores.
+ * seqs: n_seq, q_start, q_len_fixed = rows, max_q_len = most drafted tokens of
+ * a sequence (<= 256); pos0 and kv_len are not read.  num_splits 0: automatic
+ * (1..8 CTAs share a sequence's keys and join their parts over the cluster's
+ * shared memory; no workspace).                                            */
+typedef struct {
+  DashSeqs seqs;
+  DashKV kv;
+  DashRoutes routes;
+  DashQO qo;
+  const int32_t* ctx_len;      /* [n_seq] */
+  const int32_t* row_pos;      /* [rows] */
+  const uint32_t* mask;        /* [rows, mask_words] */
+  int64_t mask_stride;         /* words between rows */
+  int32_t mask_words;
+  int32_t bt_width;            /* columns of the block table */
+  float scale;
+  int32_t block_size;
+  int32_t local_window;
+  int32_t num_splits;
+  DashDeviceError* device_error;
+} DashTreeAttnArgs;
+int dash_tree_attn(const DashTreeAttnArgs* args, dash_stream_t stream);
+
+/* dash_draft_verify -- which drafted tokens are kept, and the next token.
+ * target[r] is the target's distribution behind row r (probabilities; mode 2:
+ * logits), draft[r] the draft's distribution that the children of row r were
+ * drawn from.  With cur = 0, c = 0, W = 1, tokens i = 1.. of a sequence whose
+ * parent is cur are tried in order (a token outside [0, vocab) is passed over):
+ *   mode 0 (drawn drafts):   kept iff u_accept[i] * W * draft[cur][x] <
+ *                            target[cur][x] - c * draft[cur][x]; otherwise
+ *                            c += W, W = sum_v max(target - c * draft, 0)
+ *   mode 1 (certain drafts): kept iff u_accept[i] * W < target[cur][x]; otherwise
+ *                            W -= target[cur][x] and x counts as 0 from now on
+ *   mode 2 (greedy):         kept iff x is the argmax of target[cur] (lowest
+ *                            index among equals; NaN is the largest)
+ * A kept token becomes cur, with c = 0 and W = 1.  next_token: mode 2 the argmax
+ * behind the last kept token, else the first v whose running sum of the
+ * residual max(target - c * draft, 0) (mode 1: target without the rejected
+ * tokens) exceeds u_sample[s] times its sum; the row itself where the residual is
+ * empty, -1 where that is empty too (or the sequence drafts nothing).  The
+ * distribution of the tokens is the target's.  Arithmetic is 64-bit.
+ * path[s] = the kept tokens' indices (0 first), out_tokens[s] = their ids
+ * without token 0, then next_token; both -1 behind that, max_nodes wide.   */
+typedef struct {
+  const int64_t* tokens;       /* [rows] */
+  const int32_t* parents;      /* [rows], NULL: a chain */
+  const int32_t* q_start;      /* [n_seq + 1] */
+  const void* target; int64_t target_stride;   /* [rows, vocab], elements */
+  const void* draft;  int64_t draft_stride;    /* [rows, vocab], mode 0 */
+  const float* u_accept;       /* [rows], modes 0 and 1 */
+  const float* u_sample;       /* [n_seq], modes 0 and 1 */
+  int32_t n_seq, rows, max_nodes, vocab;
+  int32_t dtype;               /* DASH_DTYPE_* of target and draft */
+  int32_t mode;
+  int32_t* n_accept;           /* [n_seq] */
+  int32_t* path;               /* [n_seq, max_nodes] */
+  int64_t* next_token;         /* [n_seq] */
+  int64_t* out_tokens;         /* [n_seq, max_nodes] */
+  DashDeviceError* device_error;
+} DashVerifyArgs;
+int dash_draft_verify(const DashVerifyArgs* args, dash_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
+/* Pages of a cache.  A cache tensor holds page_toks tokens per page; every
+ * tensor of a call is indexed by the same page ids (K, V, index keys, k-bar
+ * rows of every layer).  The descriptors are HOST memory.                  */
+typedef struct {
+  void* base;
+  int64_t page_stride;         /* bytes between pages */
+  int64_t tok_stride;          /* bytes between the tokens of a page */
+  int32_t tok_bytes;           /* bytes of one token's entry (contiguous) */
+  int32_t page_toks;
+} DashCacheTensor;
+
+/* dash_draft_commit -- the kept tokens' entries moved behind the committed
+ * ones: token ctx_len[s] + path[s, i] -> ctx_len[s] + i for 0 < i <= n_accept[s],
+ * in every tensor.  path rises strictly (as dash_draft_verify writes it); from
+ * an entry that does not, or is >= max_nodes, the rest of the sequence stays
+ * (DASH_DEV_BAD_TREE).                                                       */
+typedef struct {
+  const DashCacheTensor* tensors;   /* host, each of block_size tokens per page */
+  int32_t n_tensors;
+  int32_t n_seq, max_nodes, block_size, bt_width, pad0;
+  int64_t num_pages;
+  const int32_t* path; int64_t path_stride;
+  const int32_t* n_accept;
+  const int32_t* ctx_len;
+  const int32_t* block_table; int64_t bt_stride;
+  DashDeviceError* device_error;
+} DashCommitArgs;
+int dash_draft_commit(const DashCommitArgs* args, dash_stream_t stream);
+
+/* dash_pages_copy -- page src[i] -> page dst[i] in every tensor, i < n (a pair
+ * with a negative id or src == dst is skipped).  check != 0: pairs whose dst is
+ * another pair's source or dst are left out and recorded (DASH_DEV_BAD_ROW), as are
+ * ids >= num_pages; list (device, [2 n] scratch) receives the pairs that run.
+ * check == 0: the caller knows that no such pair exists.                    */
+typedef struct {
+  const DashCacheTensor* tensors;   /* host */
+  int32_t n_tensors;
+  int32_t n;
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* count;             /* optional: live pairs (<= n) */
+  int32_t* list;
+  int64_t num_pages;
+  int32_t check;
+  int32_t pad0;
+  DashDeviceError* device_error;
+} DashPagesCopyArgs;
+int dash_pages_copy(const DashPagesCopyArgs* args, dash_stream_t stream);
+
+/* A pool of pages shared by up to max_rows sequences.  Page p is held by ref[p]
+ * table entries; the n_free pages without a holder are the first entries of
+ * free_list (a stack, -1 behind its top).  Row r of the table holds n_blocks[r]
+ * pages, -1 behind them.                                                    */
+typedef struct {
+  int32_t* ref;                     /* [num_pages] */
+  int32_t* free_list;               /* [num_pages] */
+  int32_t* n_free;                  /* [1] */
+  int32_t* block_table; int64_t bt_stride;   /* [max_rows, bt_width] */
+  int32_t* n_blocks;                /* [max_rows] */
+  int32_t num_pages, max_rows, bt_width, block_size;
+} DashPagePool;
+
+/* Requests name rows; of several that name the same row (fork: dst) the first
+ * runs, the others are recorded (DASH_DEV_BAD_ROW), as is a request that does
+ * not fit the table.  num_pages <= 2^19, max_rows <= 8192.
+ *
+ * dash_pages_reserve  rows[i] gets pages for lens[i] tokens (none are taken
+ *                     back).  Pages are taken from the stack's top in request
+ *                     order; from the first request that does not fit on, those
+ *                     that need a page get none (DASH_DEV_NO_PAGE).
+ * dash_pages_free     rows[i] keeps its first keep[i] blocks (keep NULL: none);
+ *                     pages without a holder go onto the stack in ascending order.
+ * dash_pages_fork     dst[i] (an empty row) becomes a copy of the first lens[i]
+ *                     tokens of row src[i]: full pages are shared, the last one,
+ *                     if partly filled, is a page of its own; copy_src/dst[i] =
+ *                     the pages to copy (-1: none), to be passed to
+ *                     dash_pages_copy.  Pages are taken as by dash_pages_reserve.
+ * dash_pages_compact  with L held pages, the k-th held page >= L moves to the
+ *                     k-th unheld page < L: copy_src/dst[k] (k < *n_moves, num_pages
+ *                     / 2 entries) list the moves (sources and targets are disjoint,
+ *                     so the old tables stay valid until their pages are reused),
+ *                     `into` receives the new ref, free_list (the lowest page on
+ *                     top), n_free, block_table and n_blocks; into may be the pool
+ *                     itself.                                               */
+typedef struct {
+  DashPagePool pool;
+  DashPagePool into;                /* compact */
+  const int32_t* rows;              /* reserve, free: rows; fork: dst */
+  const int32_t* src;               /* fork */
+  const int32_t* lens;              /* reserve, fork: tokens; free: blocks kept or NULL */
+  int32_t n;
+  int32_t pad0;
+  int32_t* copy_src;
+  int32_t* copy_dst;
+  int32_t* n_moves;
+  DashDeviceError* device_error;
+} DashPagesArgs;
+int dash_pages_reserve(const DashPagesArgs* args, dash_stream_t stream);
+int dash_pages_free(const DashPagesArgs* args, dash_stream_t stream);
+int dash_pages_fork(const DashPagesArgs* args, dash_stream_t stream);
+int dash_pages_compact(const DashPagesArgs* args, dash_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
 /* Diagnostics */
 int dash_last_error(char* buf, int len);     /* copies the last host-side error message */
 int dash_library_version(void);              /* (major << 16) | minor */
@@ -809,7 +1028,9 @@ int dash_count_launches(int reset);          /* kernels launched by this library
  * DashDecodeArgs, DashDeviceError, DashPageIdsArgs, DashPageStateArgs,
  * DashPageAllowArgs, DashPageDecodeArgs, DashBlockAnyArgs, DashPageBlocksArgs,
  * DashIndexProjArgs, DashRopeKVArgs, DashAttnBwdArgs, DashEntmaxArgs,
- * DashServingPlanArgs, DashPeerHandle, DashPageCoordArgs, DashCosSin2DArgs.
+ * DashServingPlanArgs, DashPeerHandle, DashPageCoordArgs, DashCosSin2DArgs,
+ * DashTreePlanArgs, DashTreeAttnArgs, DashVerifyArgs, DashCacheTensor,
+ * DashCommitArgs, DashPagesCopyArgs, DashPagePool, DashPagesArgs.
  * Lets a binding
  * verify its struct layouts; returns the number of sizes available. */
 int dash_abi_sizes(int64_t* out, int n);

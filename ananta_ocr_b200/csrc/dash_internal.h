@@ -47,6 +47,9 @@ int launch_page_coords(const DashPageCoordArgs& a, cudaStream_t st);
 int launch_cos_sin_2d(const DashCosSin2DArgs& a, cudaStream_t st);
 int launch_tree_plan(const DashTreePlanArgs& a, cudaStream_t st);
 int launch_tree_attn(const DashTreeAttnArgs& a, cudaStream_t st);
+// draft-tree attention on the tensor cores (dash_tree_tc.cu)
+bool tree_tc_supported(const DashTreeAttnArgs& a);
+int launch_tree_tc(const DashTreeAttnArgs& a, cudaStream_t st);
 int launch_verify(const DashVerifyArgs& a, cudaStream_t st);
 int launch_draft_commit(const DashCommitArgs& a, cudaStream_t st);
 int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st);

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kTreeRowWarps * 32) tree_rows_kernel(const __g
 }
 
 int launch_tree_attn(const DashTreeAttnArgs& a, cudaStream_t st) {
+  if (tree_tc_supported(a)) return launch_tree_tc(a, st);
   const int64_t units = (int64_t)a.seqs.q_len_fixed * a.qo.n_heads;
   const unsigned grid = (unsigned)((units + kTreeRowWarps - 1) / kTreeRowWarps);
   if (a.kv.dtype == DASH_DTYPE_BF16)

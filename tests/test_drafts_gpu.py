@@ -134,10 +134,16 @@ def test_rows_without_a_key():
 
 def test_not_finite_keys_and_values_stay_in_their_rows():
     """A block with NaN and infinite values that one token routed, and a drafted
-    token with NaN: the rows that attend them get NaN or infinity, all others
-    exactly what they get without."""
+    token with NaN: the rows that attend them get NaN, all others what they get
+    without.  (Such a row may be computed on another path, with the weights in
+    fp32 instead of the caches' type: it is held to the exact result with the
+    tolerance of any row, not to the bits of the other path.)"""
     t = make_tree(10, [12, 6], [900, 700], H=2, Hkv=2, bs=64, window=1, K=3, branch=2)
     clean, _ = attend(t)
+    ref, lse, A = DO.tree_attend(t["q"].float().numpy(), t["kc"].float().numpy(), t["vc"].float().numpy(), t["idx"],
+                                 t["bias"], t["bt"], t["starts"], t["ctx"], t["pos"], t["vis"], t["bs"], t["window"],
+                                 SCALE)
+    tol = attention_tolerance(ref, A, t["dtype"])
     b = 1
     page = int(t["bt"][0, b])
     rows = set(r for r in range(12) if b in t["idx"][0, r].tolist())
@@ -152,12 +158,13 @@ def test_not_finite_keys_and_values_stay_in_their_rows():
     rows |= {12 + i for i in range(6) if t["vis"][12 + i, 4]}
     for splits in (0, 1, 3):
         out, z = attend(bad, splits=splits)
+        got, zz = out.float().cpu().numpy(), z.cpu().numpy()
         for r in range(18):
             if r in rows:
                 assert torch.isnan(out[r]).any() and torch.isnan(z[r]).all()
             else:
-                ref, _ = attend(t, splits=splits)
-                assert torch.equal(out[r], ref[r]), r
+                assert (np.abs(got[r] - ref[r]) <= tol[r]).all(), r
+                assert (np.abs(zz[r] - lse[r]) <= 1e-4 + 1e-6 * np.abs(lse[r])).all()
     assert not torch.isnan(clean).any()
 
 
@@ -181,9 +188,11 @@ def test_single_tokens_equal_the_decode_operator():
 
 def test_strides_and_wide_tables():
     """q and output as parts of wider rows, caches as parts of a joint K/V
-    tensor, a table with more columns and another row distance, int64 ids."""
+    tensor, a table with more columns and another row distance, int64 ids: the
+    same bits at the same number of splits (the automatic number goes by the
+    table's width)."""
     t = make_tree(13, [9, 4], [500, 260], H=4, Hkv=2, bs=64, window=2, K=5)
-    ref, _ = attend(t)
+    ref, _ = attend(t, splits=2)
     qkv = torch.randn(13, 4 * 128 * 3, dtype=t["dtype"], device="cuda")
     q = qkv[:, 512:1024].view(13, 4, 128)
     q.copy_(t["q"])
@@ -193,9 +202,10 @@ def test_strides_and_wide_tables():
     wide = torch.full((2, 40), -5, dtype=torch.int32, device="cuda")
     wide[:, 8:8 + t["bt"].shape[1]].copy_(t["t_bt"])
     obuf = torch.full((13, 4, 256), 7.0, dtype=t["dtype"], device="cuda")
-    out, _ = attend(t, out=obuf[:, :, 128:], q=q, kc=both[:, 0], vc=both[:, 1], t_bt=wide[:, 8:],
+    out, z = attend(t, splits=2, out=obuf[:, :, 128:], q=q, kc=both[:, 0], vc=both[:, 1], t_bt=wide[:, 8:],
                     t_idx=t["t_idx"].cuda().long())
     assert torch.equal(out, ref) and (obuf[:, :, :128] == 7.0).all()
+    check(t, out, z)
 
 
 def test_bad_ids_are_recorded_and_left_out():

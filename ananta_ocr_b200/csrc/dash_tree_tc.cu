@@ -10,21 +10,29 @@
 // what bounds the kernel: 32 KB of K and V per tile against ~0.5 k cycles of
 // tensor work (M = 128 rows, padded) and ~0.6 k of softmax per SM sub-partition.
 //
-//   setup (all)       union bit set and its prefix sums in shared memory
+//   setup             union bit set and its prefix sums in shared memory, while Q
+//                     arrives by cp.async
 //   warp 4  TMA       block table -> page boxes {64 dims, GR tokens} of K and V
-//                     (128-byte swizzle), K and V in rings of their own (2 x
-//                     16 KB each): a K slot is free after Q K^T, a V slot after P V
+//                     (128-byte swizzle), K and V in rings of their own (16 KB per
+//                     slot): a K slot is free after Q K^T, a V slot after P V
 //   warp 5  MMA       S = Q K^T (M 128, N 64, two TMEM buffers), O += P V (N 128, P
 //                     from TMEM)
 //   warps 0-3 softmax one thread per row; warps without a row sleep.  The additive
 //                     terms of the routed granules lie in a [granule][token]
-//                     table (first occurrence of a repeated id by atomicMin on
+//                     table (first occurrence of a repeated id by atomicMax on
 //                     the slot), refilled when a part outgrows it
 //
-// 96 KB of Q, K and V stages and 256 TMEM columns per CTA: two CTAs per SM, whose
-// phases interleave.  At the end the CTAs leave O, the running maximum and the
-// sum in their shared memory and each joins its share of the rows over the
-// cluster (no workspace, no atomics, fixed order).
+// Units of up to 32 rows keep 8 KB of Q and three K and V slots, of up to 64 rows 16 KB,
+// three and two, larger ones 32 KB and two (the rows of Q's operand tile that do not exist are whatever lies
+// behind them: they make rows of S that nobody reads).  Either way two CTAs fit an SM
+// (256 TMEM columns each), and their phases interleave.  At the end the CTAs leave O,
+// the running maximum and the sum in their shared memory and each joins its share
+// of the rows over the cluster (no workspace, no atomics, fixed order); a CTA
+// that holds a unit alone writes it from its registers.
+//
+// A CTA lives for some 20 us and runs most of its code once, so instruction fetches
+// count: loops that are not in the tiles' path stay rolled (unrolled, warps waited
+// 5 us per CTA for instructions).
 //
 // A masked key has P = 0, and 0 * v is 0 only for finite v.  V rows behind the last
 // drafted token are zeroed; a row whose joined output is not finite for any
@@ -43,43 +51,116 @@ namespace {
 constexpr int kRows = 128;                       // M of both MMAs
 constexpr int kKeys = 64;                        // N of Q K^T, K of P V
 constexpr int kThreads = 192;
-constexpr int kStages = 2;
 constexpr int kSlot = 16384;                     // one tile of K or of V: 2 x [64 x 128 B]
-constexpr int kCells = 3000;                     // additive terms held at a time
-constexpr int kMaxWords = 512;                   // 16384 granules of a sequence
+constexpr int kMaxWords = 256;                   // 8192 granules of a sequence
 constexpr uint32_t kTmemCols = 256;              // S0 | S1 | O
 constexpr float kGrow = 8.0f;                    // O is rescaled when a row's maximum grows by 2^8
 
+// QR: rows of Q that are kept (32, 64 or 128)
+template <int QR>
 struct TreeSmem {
-  uint8_t q[2 * kRows * 128];                    // two halves of 64 dims, swizzled
-  uint8_t k[kStages][kSlot];                     // k and v together receive O (128 x 512 B) at the end
-  uint8_t v[kStages][kSlot];
-  float cell[kCells];
+  static constexpr int kKSlots = QR <= 64 ? 3 : 2, kVSlots = QR == 32 ? 3 : 2;
+  static constexpr int kCells = QR == 32 ? 1500 : QR == 64 ? 3456 : 3360;     // additive terms held at a time
+  uint8_t q[2 * QR * 128];                       // two halves of 64 dims, swizzled
+  uint8_t k[kKSlots][kSlot];                     // receives O (QR x 512 B) at the end
+  uint8_t v[kVSlots][kSlot];
+  int cell[kCells];
   uint32_t bits[kMaxWords];
-  uint16_t before[kMaxWords + 1];
-  int tok[kStages][4];                           // first token of the tile's granules, -1 = none
-  float m[kRows], l[kRows];
-  uint64_t kfull[kStages], kempty[kStages], vfull[kStages], vempty[kStages];
+  uint16_t before[kMaxWords + 2];
+  int tok[8][4];                                 // first token of the tile's granules, -1 = none (K runs < 8 tiles ahead)
+  float m[QR], l[QR];
+  uint64_t kfull[kKSlots], kempty[kKSlots], vfull[kVSlots], vempty[kVSlots];
   uint64_t sfull[2], pfull[2], pvdone[2], qfull, alldone;
   uint32_t tmem;
   int abort_flag;
 };
-static_assert(offsetof(TreeSmem, v) == offsetof(TreeSmem, k) + kStages * kSlot, "O spans the K and V slots");
-static_assert(kStages * kSlot * 2 == kRows * 512, "O spans the K and V slots");
-static_assert(sizeof(TreeSmem) + 1024 <= 233472 / 2 - 1024, "two CTAs per SM");
+template <int QR>
+constexpr bool fits() {
+  using S = TreeSmem<QR>;
+  // two CTAs per SM; O fits the K and V slots; Q's operand tile stays inside
+  return sizeof(S) + 1024 <= 233472 / 2 - 1024 && QR * 512 <= (S::kKSlots + S::kVSlots) * kSlot &&
+         QR * 128 + kRows * 128 <= (int)sizeof(S::q) + S::kKSlots * kSlot && offsetof(S, k) == sizeof(S::q) &&
+         offsetof(S, v) == offsetof(S, k) + sizeof(S::k);
+}
+static_assert(fits<32>() && fits<64>() && fits<128>(), "shared memory of a CTA");
+
+// Row m of a unit from its own keys only (the whole warp).
+template <typename T>
+__device__ __noinline__ void redo_row(const DashTreeAttnArgs& a, TreeSeq sq, int s, int64_t r0, int m, int G,
+                                      int hk) {
+  const int node = m / G, hq = hk * G + m - node * G;
+  float ms, ls, os[16];
+  tree_row_attend<T>(a, sq, s, r0 + node, hq, ms, ls, os);
+  tree_row_store<T>(a, r0 + node, hq, ms, ls, os);
+}
 
 // the j-th set bit of w (j < popc(w))
 __device__ __forceinline__ int nth_bit(uint32_t w, int j) { return (int)__fns(w, 0, j + 1); }
 
+// Bounded wait (see mbar_wait), small enough to stand in many places: a few polls,
+// then out of line.
+__device__ __noinline__ bool tree_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DeviceError* err,
+                                            int where) {
+  return mbar_wait(bar, parity, abort_flag, err, where);
+}
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DeviceError* err,
+                                          int where) {
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  return tree_wait_long(bar, parity, abort_flag, err, where);
+}
+__device__ __forceinline__ bool tree_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                               DeviceError* err, int where) {
+  return __all_sync(0xffffffffu, tree_wait(bar, parity, abort_flag, err, where));
+}
+
+// whether the phase is complete, without waiting
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16f(uint32_t taddr, const float (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+      "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 }  // namespace
 
-template <typename T, int GR>
+template <typename T, int GR, int QR>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const __grid_constant__ DashTreeAttnArgs a, int n_tiles_seq) {
   constexpr int NG = kKeys / GR;                 // granules per tile
+  using Smem = TreeSmem<QR>;
+  constexpr int kKSlots = Smem::kKSlots, kVSlots = Smem::kVSlots;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TreeSmem& S = *reinterpret_cast<TreeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   cg::cluster_group cluster = cg::this_cluster();
   const int nsp = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -97,65 +178,105 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int64_t r0 = sq.row0 + node0;            // packed row of the tile's first token
   const int nrows = nt * G, nact = (nrows + 31) >> 5;
   const int nih = a.routes.n_index_heads > 0 ? a.routes.n_index_heads : 1;
-  const int64_t ioff = (int64_t)((hk * G) / (H / nih)) * a.routes.ihead_stride;
   const int K = a.routes.K;
+  const int64_t rbase = r0 * a.routes.row_stride + (int64_t)((hk * G) / (H / nih)) * a.routes.ihead_stride;
   DeviceError* derr = a.device_error;
   const int ctx = sq.ctx, end = ctx + total_n;
   // tokens behind the table's last column do not exist
   const int64_t room = (int64_t)a.bt_width * bs;
-  const int words = min(kMaxWords, (int)((min((int64_t)end, room) + 32 * GR - 1) / (32 * GR)));
-  if ((int64_t)end > room && tid == 0 && hk == 0 && split == 0) record_error(derr, DASH_DEV_BAD_PAGE, 75, a.bt_width);
   const int live_end = (int)min((int64_t)end, room);
+  const int words = min(kMaxWords, (live_end + 32 * GR - 1) / (32 * GR));
+  if (live_end < end && tid == 0 && hk == 0 && split == 0) record_error(derr, DASH_DEV_BAD_PAGE, 75, a.bt_width);
   const int nblk = (end + bs - 1) / bs;
   volatile int* abort_flag = &S.abort_flag;
+  constexpr int kNone = (int)0xff800000u;        // -inf, below every slot's key
+  constexpr int kKey = 0x40000000;
 
-  // ---- setup ----
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&S.kfull[i], 1);
-      mbar_init(&S.kempty[i], 1);
-      mbar_init(&S.vfull[i], 1);
-      mbar_init(&S.vempty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&S.sfull[i], 1);
-      mbar_init(&S.pfull[i], nact);
-      mbar_init(&S.pvdone[i], 1);
-    }
-    mbar_init(&S.qfull, nact);
-    mbar_init(&S.alldone, 1);
-    S.abort_flag = 0;
-    mbar_init_fence();
-    prefetch_tmap(&tmK);
-    prefetch_tmap(&tmV);
-  }
-  if (warp == 5) { tmem_alloc(&S.tmem, kTmemCols); tmem_relinquish(); }
-  for (int w = tid; w < words; w += kThreads) S.bits[w] = 0u;
-  __syncthreads();
-  // first key of a token's window
+  // first key of a row's window
   auto window_of = [&](int64_t r) -> int {
-    const int64_t e = (int64_t)a.row_pos[r] - a.local_window + 1;
+    const int64_t e = (int64_t)__ldg(a.row_pos + r) - a.local_window + 1;
     return (int)max((int64_t)0, min(e, (int64_t)ctx));
   };
-  // keys [t0, t1) join the union
-  auto add_range = [&](int t0, int t1) {
-    t1 = min(t1, live_end);
-    for (int g = t0 / GR; t0 < t1 && g * GR < t1; ++g) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
+  // entry e = (token, slot of its list), lists padded to a power of two: the
+  // slot's remote keys from t0 on, in granules
+  const int pad = K > 1 ? 32 - __clz(K - 1) : 0;
+  const int entries = K > 0 ? nt << pad : 0;
+  auto remote = [&](int e, int& node, int& slot, int& t0) -> int {
+    node = e >> pad;
+    slot = e & ((1 << pad) - 1);
+    if (slot >= K) return 0;
+    const int b = __ldg(a.routes.idx + rbase + (int64_t)node * a.routes.row_stride + slot);
+    const int edge = min(window_of(r0 + node), live_end);
+    if (b < 0) return 0;
+    if (b >= nblk) { record_error(derr, DASH_DEV_BAD_BLOCK, 76, b); return 0; }
+    t0 = (int)min((int64_t)b * bs, (int64_t)ctx);
+    const int t1 = (int)min((int64_t)(b + 1) * bs, (int64_t)edge);
+    return t1 > t0 ? (t1 - t0 + GR - 1) / GR : 0;
   };
-  for (int e = tid; e < nt * K; e += kThreads) {
-    const int node = e / K;
-    const int b = a.routes.idx[(r0 + node) * a.routes.row_stride + ioff + (e - node * K)];
-    if (b < 0) continue;
-    if (b >= nblk) { record_error(derr, DASH_DEV_BAD_BLOCK, 76, b); continue; }
-    const int64_t t0 = (int64_t)b * bs;
-    add_range((int)min(t0, (int64_t)ctx), (int)min(t0 + bs, (int64_t)window_of(r0 + node)));
+
+  // ---- setup ----
+  if (warp == 5) {
+    tmem_alloc(&S.tmem, kTmemCols);
+    tmem_relinquish();
+    if (lane < kKSlots) {
+      mbar_init(&S.kfull[lane], 1);
+      mbar_init(&S.kempty[lane], 1);
+    }
+    if (lane < kVSlots) {
+      mbar_init(&S.vfull[lane], 1);
+      mbar_init(&S.vempty[lane], 1);
+    }
+    if (lane < 2) {
+      mbar_init(&S.sfull[lane], 1);
+      mbar_init(&S.pfull[lane], nact);
+      mbar_init(&S.pvdone[lane], 1);
+    }
+    if (lane == 0) {
+      mbar_init(&S.qfull, 2);
+      mbar_init(&S.alldone, 1);
+      S.abort_flag = 0;
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+    mbar_init_fence();
   }
-  {
-    int lo = ctx;                                // the earliest window of the tile
-    for (int i = lane; i < nt; i += 32) lo = min(lo, window_of(r0 + i));
-    lo = __reduce_min_sync(0xffffffffu, lo);
+  int lo = ctx;                                  // warp 5: the earliest window of the tile
+  if (warp < 4) {
+    for (int w = tid; w < kMaxWords; w += kRows) S.bits[w] = 0u;
+  } else {
+    // the table's row on its way to the L1, for the producer
+    for (int b = (tid - kRows) * 32; b < min(a.bt_width, nblk); b += (kThreads - kRows) * 32)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(a.kv.block_table + (int64_t)s * a.kv.bt_stride + b));
+    // Q (rows of the operand tile beyond the unit's stay as they are)
+#pragma unroll 1
+    for (int c = tid - kRows; c < nrows * 16; c += kThreads - kRows) {
+      const int m = c >> 4, cc = c & 15, node = m / G;
+      const T* src = reinterpret_cast<const T*>(a.qo.q) + (r0 + node) * a.qo.q_stride_tok +
+                     (int64_t)(hk * G + m - node * G) * a.qo.q_stride_head + cc * 8;
+      const uint32_t dst = smem_u32(S.q + (cc >> 3) * (QR * 128) + m * 128 + (((cc & 7) ^ (m & 7)) << 4));
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    }
+    if (warp == 5) {
+#pragma unroll 1
+      for (int i = lane; i < nt; i += 32) lo = min(lo, window_of(r0 + i));
+      lo = __reduce_min_sync(0xffffffffu, lo);
+    }
+  }
+  __syncthreads();
+  // ---- the union ----
+  if (warp < 4) {
+#pragma unroll 4
+    for (int e = tid; e < entries; e += kRows) {
+      int node, slot, t0 = 0;
+      const int n = remote(e, node, slot, t0);
+      // the biases are read next, by the same threads
+      if (n && a.routes.bias)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.routes.bias + rbase + (int64_t)node * a.routes.row_stride + slot));
+      for (int g = t0 / GR, g1 = g + n; g < g1; ++g) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
+    }
+  } else if (warp == 5) {
     const int g0 = lo / GR, g1 = (live_end + GR - 1) / GR;        // [g0, g1): window and drafts
-    for (int w = (g0 >> 5) + tid; w < words && w * 32 < g1; w += kThreads) {
+    for (int w = (g0 >> 5) + lane; w * 32 < g1; w += 32) {
       uint32_t m = 0xffffffffu;
       if (w * 32 < g0) m &= 0xffffffffu << (g0 & 31);
       if (w * 32 + 32 > g1) m &= 0xffffffffu >> (32 - (g1 & 31));
@@ -165,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   if (warp == 0) {                               // prefix sums of the words' counts
     int base = 0;
+#pragma unroll 1
     for (int w0 = 0; w0 < words; w0 += 32) {
       const int c = w0 + lane < words ? __popc(S.bits[w0 + lane]) : 0;
       int x = c;
@@ -189,71 +311,106 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int first = min(n_tile, split * share), tiles = min(n_tile, first + share) - first;
   const int rank0 = first * NG;
 
+  if (warp >= 4) {
+    // Q has come (requested at the start)
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (a.scale < 0.0f) {
+      // a negative scale is folded into q, so that a row's largest product is
+      // its largest logit
+#pragma unroll 1
+      for (int c = tid - kRows; c < nrows * 16; c += kThreads - kRows) {
+        const int m = c >> 4, cc = c & 15;
+        uint4* p = reinterpret_cast<uint4*>(S.q + (cc >> 3) * (QR * 128) + m * 128 + (((cc & 7) ^ (m & 7)) << 4));
+        uint4 v = *p;
+        v.x ^= 0x80008000u; v.y ^= 0x80008000u; v.z ^= 0x80008000u; v.w ^= 0x80008000u;
+        *p = v;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&S.qfull);
+  }
   if (warp == 4) {
     // =================== TMA producer ===================
-    int it = 0;
+    // K runs a tile ahead of V, so that a V slot that is still read does not keep
+    // the next K from being requested.
+    int kn = 0, vn = 0;                          // tiles requested
+    int page = 0, tok = 0;                       // a lane's granule of the current 32
+    int vpg[NG], vtk[NG];                        // the tile whose V is next
     bool alive = true;
-    for (int b0 = 0; b0 < tiles * NG && alive; b0 += 32) {
-      // a lane per granule: its place in the union, its page
-      const int rk = rank0 + b0 + lane;
-      int tok = -1, page = (int)a.kv.num_pages;  // out of range: the box reads as zeros
-      if (b0 + lane < tiles * NG && rk < n_gran) {
-        int lo = 0, hi = words - 1;
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if ((int)S.before[mid] <= rk) lo = mid; else hi = mid - 1;
+#pragma unroll 1
+    for (int it = 0; it <= tiles && alive; ++it) {
+      int pg[NG], tk[NG];
+      if (it < tiles) {
+        const int at = it * NG & 31;
+        if (at == 0) {
+          // a lane per granule: its place in the union, its page
+          const int rk = rank0 + it * NG + lane;
+          tok = -1;
+          page = (int)a.kv.num_pages;            // out of range: the box reads as zeros
+          if (it * NG + lane < tiles * NG && rk < n_gran) {
+            int lo = 0, hi = words - 1;
+            while (lo < hi) {
+              const int mid = (lo + hi + 1) >> 1;
+              if ((int)S.before[mid] <= rk) lo = mid; else hi = mid - 1;
+            }
+            const int t = (lo * 32 + nth_bit(S.bits[lo], rk - S.before[lo])) * GR;
+            const int64_t p = __ldg(a.kv.block_table + (int64_t)s * a.kv.bt_stride + t / bs);
+            if (p >= 0 && p < a.kv.num_pages) { page = (int)p; tok = t; }
+            else record_error(derr, DASH_DEV_BAD_PAGE, 77, p);
+          }
         }
-        const int t = (lo * 32 + nth_bit(S.bits[lo], rk - S.before[lo])) * GR;
-        const int64_t p = a.kv.block_table[(int64_t)s * a.kv.bt_stride + t / bs];
-        if (p >= 0 && p < a.kv.num_pages) { page = (int)p; tok = t; }
-        else record_error(derr, DASH_DEV_BAD_PAGE, 77, p);
-      }
-      const int n = min(32, tiles * NG - b0);
-      for (int i = 0; i < n && alive; i += NG, ++it) {
-        const int st = it % kStages;
-        const uint32_t ph = (uint32_t)((it / kStages) - 1) & 1u;
-        int pg[NG], tk[NG];
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
-          pg[g] = __shfl_sync(0xffffffffu, page, i + g);
-          tk[g] = __shfl_sync(0xffffffffu, tok, i + g);
+          pg[g] = __shfl_sync(0xffffffffu, page, at + g);
+          tk[g] = __shfl_sync(0xffffffffu, tok, at + g);
         }
         if (lane == 0) {
-          if (it >= kStages && !mbar_wait(&S.kempty[st], ph, abort_flag, derr, 40)) alive = false;
-          if (alive) {
+          const int st = it % kKSlots;
+          if (it >= kKSlots && !tree_wait(&S.kempty[st], (uint32_t)((it / kKSlots) - 1) & 1u, abort_flag, derr, 40)) {
+            alive = false;
+          } else {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) S.tok[it & 7][g] = tk[g];
             mbar_arrive_expect_tx(&S.kfull[st], kSlot);
+            ++kn;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               const int row = tk[g] < 0 ? 0 : tk[g] % bs;
               tma_load_4d(S.k[st] + g * GR * 128, &tmK, &S.kfull[st], 0, row, hk, pg[g]);
               tma_load_4d(S.k[st] + 8192 + g * GR * 128, &tmK, &S.kfull[st], 64, row, hk, pg[g]);
             }
-            if (it >= kStages && !mbar_wait(&S.vempty[st], ph, abort_flag, derr, 41)) alive = false;
-          }
-          if (alive) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) S.tok[st][g] = tk[g];
-            mbar_arrive_expect_tx(&S.vfull[st], kSlot);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-              const int row = tk[g] < 0 ? 0 : tk[g] % bs;
-              tma_load_4d(S.v[st] + g * GR * 128, &tmV, &S.vfull[st], 0, row, hk, pg[g]);
-              tma_load_4d(S.v[st] + 8192 + g * GR * 128, &tmV, &S.vfull[st], 64, row, hk, pg[g]);
-            }
-          } else {
-            ++it;                                // this tile's K was requested, its V was not
           }
         }
-        alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
       }
+      if (it > 0 && lane == 0 && alive) {
+        const int j = it - 1, st = j % kVSlots;
+        if (j >= kVSlots && !tree_wait(&S.vempty[st], (uint32_t)((j / kVSlots) - 1) & 1u, abort_flag, derr, 41)) {
+          alive = false;
+        } else {
+          mbar_arrive_expect_tx(&S.vfull[st], kSlot);
+          ++vn;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const int row = vtk[g] < 0 ? 0 : vtk[g] % bs;
+            tma_load_4d(S.v[st] + g * GR * 128, &tmV, &S.vfull[st], 0, row, hk, vpg[g]);
+            tma_load_4d(S.v[st] + 8192 + g * GR * 128, &tmV, &S.vfull[st], 64, row, hk, vpg[g]);
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) { vpg[g] = pg[g]; vtk[g] = tk[g]; }
+      alive = __shfl_sync(0xffffffffu, alive ? 1 : 0, 0) != 0;
     }
     // never leave with bulk copies in flight (after an abort the waits run out)
     if (lane == 0) {
       volatile int no_abort = 0;
-      for (int k = max(0, it - kStages); k < it; ++k) {
-        mbar_wait(&S.kfull[k % kStages], (uint32_t)(k / kStages) & 1u, &no_abort, nullptr, 42);
-        mbar_wait(&S.vfull[k % kStages], (uint32_t)(k / kStages) & 1u, &no_abort, nullptr, 42);
-      }
+#pragma unroll 1
+      for (int k = max(0, kn - kKSlots); k < kn; ++k)
+        tree_wait(&S.kfull[k % kKSlots], (uint32_t)(k / kKSlots) & 1u, &no_abort, nullptr, 42);
+#pragma unroll 1
+      for (int k = max(0, vn - kVSlots); k < vn; ++k)
+        tree_wait(&S.vfull[k % kVSlots], (uint32_t)(k / kVSlots) & 1u, &no_abort, nullptr, 42);
     }
     __syncwarp();
   } else if (warp == 5) {
@@ -263,202 +420,206 @@ __global__ void __launch_bounds__(kThreads, 2)
       constexpr uint32_t idesc_qk = make_idesc(fmt, 0, 0, kRows, kKeys);
       constexpr uint32_t idesc_pv = make_idesc(fmt, 0, 1, kRows, 128);
       const uint32_t sQ = smem_u32(S.q);
-      bool alive = mbar_wait(&S.qfull, 0, abort_flag, derr, 50);
-      auto issue_pv = [&](int j) -> bool {
-        const int pb = j & 1, st = j % kStages;
-        if (!mbar_wait(&S.vfull[st], (uint32_t)(j / kStages) & 1u, abort_flag, derr, 51)) return false;
-        if (!mbar_wait(&S.pfull[pb], (uint32_t)(j >> 1) & 1u, abort_flag, derr, 52)) return false;
-        tc_fence_after();
-        const uint32_t sV = smem_u32(S.v[st]);
+      // S(qk) = Q K^T and O += P(pv) V are issued as their operands come, whichever is
+      // first: a K tile that is late does not hold back the P V that frees a V slot.
+      // S buffer qk & 1 held P(qk - 2), whose P V was issued before by this thread.
+      int qk = 0, pv = tree_wait(&S.qfull, 0, abort_flag, derr, 50) ? 0 : tiles;
+      uint32_t idle = 0;
+      uint64_t since = 0;
+#pragma unroll 1
+      while (pv < tiles) {
+        bool did = false;
+        if (pv < qk && mbar_test(&S.pfull[pv & 1], (uint32_t)(pv >> 1) & 1u) &&
+            mbar_test(&S.vfull[pv % kVSlots], (uint32_t)(pv / kVSlots) & 1u)) {
+          tc_fence_after();
+          const uint32_t sV = smem_u32(S.v[pv % kVSlots]);
 #pragma unroll
-        for (int kk = 0; kk < kKeys / 16; ++kk)
-          umma_ts(tO, tmem + pb * kKeys + kk * 8, sw128_desc(sV + kk * 2048, 8192, 1024), idesc_pv,
-                  (j > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&S.pvdone[pb]);
-        umma_commit(&S.vempty[st]);
-        return true;
-      };
-      int it = 0;
-      for (; alive && it < tiles; ++it) {
-        const int st = it % kStages, sb = it & 1;
-        if (!mbar_wait(&S.kfull[st], (uint32_t)(it / kStages) & 1u, abort_flag, derr, 53)) { alive = false; break; }
-        // S buffer sb held P(it-2); PV(it-2) was issued before this by the same thread
-        tc_fence_after();
-        const uint32_t sK = smem_u32(S.k[st]);
+          for (int kk = 0; kk < kKeys / 16; ++kk)
+            umma_ts(tO, tmem + (pv & 1) * kKeys + kk * 8, sw128_desc(sV + kk * 2048, 8192, 1024), idesc_pv,
+                    (pv > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&S.pvdone[pv & 1]);
+          umma_commit(&S.vempty[pv % kVSlots]);
+          ++pv;
+          did = true;
+        }
+        if (qk < tiles && qk <= pv + 1 && mbar_test(&S.kfull[qk % kKSlots], (uint32_t)(qk / kKSlots) & 1u)) {
+          tc_fence_after();
+          const uint32_t sK = smem_u32(S.k[qk % kKSlots]);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_ss(tmem + sb * kKeys, sw128_desc(sQ + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024),
-                  sw128_desc(sK + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
-        umma_commit(&S.sfull[sb]);
-        umma_commit(&S.kempty[st]);
-        if (it >= 1 && !issue_pv(it - 1)) { alive = false; break; }
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ss(tmem + (qk & 1) * kKeys, sw128_desc(sQ + (kk >> 2) * (QR * 128) + (kk & 3) * 32, 16, 1024),
+                    sw128_desc(sK + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024), idesc_qk, kk > 0 ? 1u : 0u);
+          umma_commit(&S.sfull[qk & 1]);
+          umma_commit(&S.kempty[qk % kKSlots]);
+          ++qk;
+          did = true;
+        }
+        if (did) {
+          idle = 0;
+        } else if ((++idle & 255u) == 0) {       // the wait is bounded as all others are
+          if (idle == 256u) since = globaltimer_ns();
+          if (*abort_flag) break;
+          if (globaltimer_ns() - since > 2000000000ull) {
+            *abort_flag = 1;
+            record_error(derr, DASH_DEV_TIMEOUT, 51, qk);
+            break;
+          }
+        }
       }
-      if (alive) issue_pv(tiles - 1);
       // every MMA is done before TMEM is given back
       umma_commit(&S.alldone);
       volatile int no_abort = 0;
-      mbar_wait(&S.alldone, 0, &no_abort, nullptr, 54);
+      tree_wait(&S.alldone, 0, &no_abort, nullptr, 54);
     }
     __syncwarp();
-  } else if (warp < nact) {
+  } else {
     // =================== softmax: one thread per row ===================
-    const int m = tid;                           // row of the tile = (token m / G, head m % G)
-    const bool row_ok = m < nrows;
+    const int m = tid;                           // row of the unit = (token m / G, head m % G)
+    const bool row_ok = m < nrows, warp_on = warp < nact;
     const int node = row_ok ? m / G : 0;
     const int64_t r = r0 + node;
     const int hq = hk * G + (row_ok ? m - node * G : 0);
-    {
-      // a negative scale is folded into q, so that a row's largest product is
-      // its largest logit
-      const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
-      const T* qp = reinterpret_cast<const T*>(a.qo.q) + r * a.qo.q_stride_tok + (int64_t)hq * a.qo.q_stride_head;
-#pragma unroll
-      for (int cc = 0; cc < 16; ++cc) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row_ok) v = __ldg(reinterpret_cast<const uint4*>(qp + cc * 8));
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-        *reinterpret_cast<uint4*>(S.q + (cc >> 3) * 16384 + m * 128 + (((cc & 7) ^ (m & 7)) << 4)) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.qfull);
-    }
     const int lstart = window_of(r);
     const uint32_t* vis = a.mask + r * a.mask_stride;
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(vis));
     const float sl2 = fabsf(a.scale) * kTreeLog2e;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-    // granules whose terms fit the table
-    const int cap = kCells / nt / NG * NG;
-    int c0 = 0, c1 = 0;                          // ranks (from rank0) held by the table
+    // The additive terms of granules [c0, c1) of this CTA's part, -inf where no slot
+    // of the token names the block: the lowest slot that names a cell wins it (pass
+    // 0; slots as large positive keys, above -inf's bits), then leaves its bias there
+    // (pass 1).  By all four warps.
+    const int cap = Smem::kCells / nt / NG * NG;
+    int c0 = 0, c1 = 0;
     auto fill = [&](int from) {
+      asm volatile("bar.sync 1, 128;" ::: "memory");         // the old terms have been read
       c0 = from;
       c1 = min(from + cap, tiles * NG);
-      const int nthr = nact * 32;
-      asm volatile("bar.sync 1, %0;" ::"r"(nthr) : "memory");          // the old terms have been read
-      const int cells = (c1 - c0) * nt;
-      int* cell_i = reinterpret_cast<int*>(S.cell);
-      for (int i = m; i < cells; i += nthr) cell_i[i] = INT32_MAX;
-      asm volatile("bar.sync 1, %0;" ::"r"(nthr) : "memory");
-      for (int e = m; e < nt * K; e += nthr) {
-        const int nd = e / K, slot = e - nd * K;
-        const int b = a.routes.idx[(r0 + nd) * a.routes.row_stride + ioff + slot];
-        if (b < 0 || b >= nblk) continue;
-        const int64_t t0 = (int64_t)b * bs;
-        const int t1 = min((int)min(t0 + bs, (int64_t)window_of(r0 + nd)), live_end);
-        for (int t = (int)min(t0, (int64_t)ctx); t < t1; t += GR) {
-          const int g = t / GR;
-          const int rk = (int)S.before[g >> 5] + __popc(S.bits[g >> 5] & ((1u << (g & 31)) - 1u)) - rank0;
-          if (rk >= c0 && rk < c1) atomicMin(cell_i + (rk - c0) * nt + nd, slot);
+      for (int i = m; i < (c1 - c0) * nt; i += kRows) S.cell[i] = kNone;
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll 1
+        for (int e = m; e < entries; e += kRows) {
+          int nd, slot, t0 = 0;
+          const int n = remote(e, nd, slot, t0);
+          if (n == 0) continue;
+          // a block's granules follow one another in the union
+          const int g = t0 / GR;
+          int rk = (int)S.before[g >> 5] + __popc(S.bits[g >> 5] & ((1u << (g & 31)) - 1u)) - rank0;
+          const int rk1 = min(rk + n, c1);
+          float bias = 0.0f;
+          if (pass && a.routes.bias)
+            bias = __ldg(a.routes.bias + rbase + (int64_t)nd * a.routes.row_stride + slot) * kTreeLog2e;
+#pragma unroll 1
+          for (rk = max(rk, c0); rk < rk1; ++rk) {
+            int* c = S.cell + (rk - c0) * nt + nd;
+            if (pass == 0) atomicMax(c, kKey - slot);
+            else if (*c == kKey - slot) *c = __float_as_int(bias);
+          }
         }
       }
-      asm volatile("bar.sync 1, %0;" ::"r"(nthr) : "memory");
-      for (int i = m; i < cells; i += nthr) {
-        const int slot = cell_i[i];
-        float t = -INFINITY;
-        if (slot != INT32_MAX)
-          t = a.routes.bias
-                  ? a.routes.bias[(r0 + i % nt) * a.routes.row_stride + ioff + slot] * kTreeLog2e
-                  : 0.0f;
-        S.cell[i] = t;
-      }
-      asm volatile("bar.sync 1, %0;" ::"r"(nthr) : "memory");
+      asm volatile("bar.sync 1, 128;" ::: "memory");
     };
     float m_run = -INFINITY, l_run = 0.0f;
     bool alive = true;
+#pragma unroll 1
     for (int it = 0; it < tiles; ++it) {
       if (it * NG >= c1) fill(it * NG);
-      if (!alive) continue;                      // after an abort: only the table's barriers
-      const int st = it % kStages, sb = it & 1;
-      if (!mbar_wait_warp(&S.vfull[st], (uint32_t)(it / kStages) & 1u, abort_flag, derr, 60)) { alive = false; continue; }
-      int t0[NG];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) t0[g] = S.tok[st][g];
-      // V rows behind the last drafted token: P = 0 must not meet a NaN
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if (t0[g] >= 0 && t0[g] + GR > end) {
-          const int q0 = max(0, end - t0[g]);
-          for (int e = m; e < (GR - q0) * 16; e += nact * 32) {
-            const int row = g * GR + q0 + e / 16, ch = e % 16;
-            *reinterpret_cast<uint4*>(S.v[st] + (ch >> 3) * 8192 + row * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-      }
-      if (!mbar_wait_warp(&S.sfull[sb], (uint32_t)(it >> 1) & 1u, abort_flag, derr, 61)) { alive = false; continue; }
+      if (!alive || !warp_on) continue;          // only the table's barriers
+      const int sb = it & 1;
+      if (!tree_wait_warp(&S.sfull[sb], (uint32_t)(it >> 1) & 1u, abort_flag, derr, 61)) { alive = false; continue; }
       tc_fence_after();
       const uint32_t tS = tmem + sb * kKeys + lane_base;
       float x[kKeys];
       tmem_ld32f(tS, x);
       tmem_ld32f(tS + 32, x + 32);
-      // additive term of each granule for this row; pure: one term for all GR keys
+      // additive term of each granule for this row; pure: one term for all its keys
       float add[NG];
-      bool pure = true, none = true;
+      bool pure = true, none = true, tail = false;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
+        const int t0 = S.tok[it & 7][g];
         add[g] = -INFINITY;
-        if (t0[g] >= 0 && row_ok) {
-          const bool remote = t0[g] < lstart;
-          if (remote) add[g] = S.cell[(it * NG + g - c0) * nt + node];
-          else if (t0[g] + GR <= ctx) add[g] = 0.0f;
-          const bool p = remote ? t0[g] + GR <= lstart : t0[g] + GR <= ctx;
+        tail |= t0 >= 0 && t0 + GR > end;
+        if (t0 >= 0 && row_ok) {
+          const bool far = t0 < lstart;
+          if (far) add[g] = __int_as_float(S.cell[(it * NG + g - c0) * nt + node]);
+          else if (t0 + GR <= ctx) add[g] = 0.0f;
+          const bool p = far ? t0 + GR <= lstart : t0 + GR <= ctx;
           pure &= p;
           none &= p && add[g] == -INFINITY;
         }
       }
-      tmem_ld_wait();
-      uint32_t pk[kKeys / 2];
-      if (__all_sync(0xffffffffu, none)) {
+      const bool all_none = __all_sync(0xffffffffu, none), all_pure = __all_sync(0xffffffffu, pure);
+      if (tail) {
+        // V rows behind the last drafted token: P = 0 must not meet a NaN
+        const int st = it % kVSlots;
+        if (!tree_wait_warp(&S.vfull[st], (uint32_t)(it / kVSlots) & 1u, abort_flag, derr, 60)) alive = false;
+#pragma unroll 1
+        for (int e = m; alive && e < kKeys * 16; e += nact * 32) {
+          const int row = e >> 4, ch = e & 15, t0 = S.tok[it & 7][row / GR];
+          if (t0 >= 0 && t0 + row % GR >= end)
+            *reinterpret_cast<uint4*>(S.v[st] + (ch >> 3) * 8192 + row * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      if (all_none) {
         // no row of this warp attends the tile
+        tmem_ld_wait();
+        uint32_t pk[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int e = 0; e < kKeys / 2; ++e) pk[e] = 0u;
+        for (int c = 0; c < 4; ++c) tmem_st8(tS + c * 8, pk);
       } else {
-        const bool all_pure = __all_sync(0xffffffffu, pure);
-        float mx = -INFINITY;
-        if (all_pure) {
-#pragma unroll
+        float sl = sl2;
+        if (!all_pure) {
+          // which keys: before the window with the granule's term, window and
+          // visible drafted tokens without, nothing else
+          uint64_t far = 0, near = 0;
+#pragma unroll 1
           for (int g = 0; g < NG; ++g) {
-            float h = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < GR; ++c) h = fmaxf(h, x[g * GR + c]);
-            mx = fmaxf(mx, fmaf(h, sl2, add[g]));                       // sl2 >= 0
-          }
-        } else {
-          // key by key: remote keys take the granule's term, window and
-          // visible drafted keys none, all others -inf
-#pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            uint64_t on = 0;                     // columns attended without a term
-            int rem = 0;                         // columns [0, rem) are remote
-            if (t0[g] >= 0 && row_ok) {
-              rem = min(GR, max(0, lstart - t0[g]));
-              const int loc = min(GR, max(0, ctx - t0[g]));            // columns [rem, loc) are the window
-              const uint64_t below = loc >= 64 ? ~0ull : (1ull << loc) - 1ull;
-              on = below & (rem >= 64 ? 0ull : ~0ull << rem);
-              if (loc < GR) {
-                const int v0 = t0[g] + loc - ctx;                       // drafted token of column loc
-                uint64_t bits = 0;
-#pragma unroll
-                for (int w = 0; w < 3; ++w) {
-                  const int wi = (v0 >> 5) + w;
-                  if (wi < a.mask_words && wi * 32 < total_n) {
-                    uint32_t mw = vis[wi];
-                    if (total_n - wi * 32 < 32) mw &= (1u << (total_n - wi * 32)) - 1u;
-                    const int sh = wi * 32 - v0;                        // column of the word's first token - loc
-                    if (sh >= 0) { if (sh < 64) bits |= (uint64_t)mw << sh; }
-                    else bits |= (uint64_t)(mw >> -sh);
-                  }
-                }
-                on |= bits << loc;
+            const int t0 = S.tok[it & 7][g];
+            if (t0 < 0 || !row_ok) continue;
+            const int rem = min(GR, max(0, lstart - t0)), loc = min(GR, max(0, ctx - t0));
+            uint64_t f = rem >= 64 ? ~0ull : (1ull << rem) - 1ull;
+            uint64_t on = (loc >= 64 ? ~0ull : (1ull << loc) - 1ull) & ~f;
+            if (loc < GR) {
+              const int v0 = t0 + loc - ctx;     // drafted token of column loc
+              uint64_t bits = 0;
+#pragma unroll 1
+              for (int w = 0; w < 3; ++w) {
+                const int wi = (v0 >> 5) + w, sh = wi * 32 - v0;        // column of the word's first token - loc
+                if (wi >= a.mask_words || wi * 32 >= total_n || sh >= 64) break;
+                uint32_t mw = __ldg(vis + wi);
+                if (total_n - wi * 32 < 32) mw &= (1u << (total_n - wi * 32)) - 1u;
+                bits |= sh >= 0 ? (uint64_t)mw << sh : (uint64_t)(mw >> -sh);
               }
+              on |= bits << loc;
             }
-#pragma unroll
-            for (int c = 0; c < GR; ++c) {
-              const float y = fmaf(x[g * GR + c], sl2, c < rem ? add[g] : 0.0f);
-              x[g * GR + c] = (c < rem || ((on >> c) & 1ull)) ? y : -INFINITY;
-              mx = fmaxf(mx, x[g * GR + c]);
-            }
+            if (GR < 64) on &= (1ull << (GR & 63)) - 1ull;
+            far |= f << (g * GR & 63);
+            near |= on << (g * GR & 63);
           }
+          tmem_ld_wait();
+          const uint32_t fw[2] = {(uint32_t)far, (uint32_t)(far >> 32)};
+          const uint32_t kw[2] = {(uint32_t)(far | near), (uint32_t)((far | near) >> 32)};
+#pragma unroll
+          for (int c = 0; c < kKeys; ++c) {
+            const uint32_t bit = 1u << (c & 31);
+            const float y = fmaf(x[c], sl2, fw[c >> 5] & bit ? add[c / GR] : 0.0f);
+            x[c] = kw[c >> 5] & bit ? y : -INFINITY;
+          }
+          sl = 1.0f;                             // x holds logits: nothing is left to add
+#pragma unroll
+          for (int g = 0; g < NG; ++g) add[g] = 0.0f;
+        }
+        tmem_ld_wait();
+        float mx = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          float h = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < GR; ++c) h = fmaxf(h, x[g * GR + c]);
+          mx = fmaxf(mx, fmaf(h, sl, add[g]));                          // sl >= 0
         }
         // running maximum; O follows it only when it grew by more than 2^kGrow
         const bool grow = mx > m_run + kGrow;
@@ -466,19 +627,19 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (__any_sync(0xffffffffu, scale_o)) {
           const float f = scale_o ? fast_exp2(m_run - mx) : 1.0f;
           if (it > 0) {
-            if (!mbar_wait_warp(&S.pvdone[(it - 1) & 1], (uint32_t)((it - 1) >> 1) & 1u, abort_flag, derr, 62)) {
+            if (!tree_wait_warp(&S.pvdone[(it - 1) & 1], (uint32_t)((it - 1) >> 1) & 1u, abort_flag, derr, 62)) {
               alive = false;
               continue;
             }
             tc_fence_after();
 #pragma unroll 1
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t o[32];
-              tmem_ld32(tO + q4 * 32 + lane_base, o);
+            for (int c = 0; c < 128; c += 16) {
+              float o[16];
+              tmem_ld16f(tO + c + lane_base, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-              tmem_st32(tO + q4 * 32 + lane_base, o);
+              for (int k = 0; k < 16; ++k) o[k] *= f;
+              tmem_st16f(tO + c + lane_base, o);
             }
             tmem_st_wait();
           }
@@ -486,96 +647,124 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (grow) m_run = mx;
         const float mu = m_run == -INFINITY ? 0.0f : m_run;
+        // P is rounded to the caches' type for the matrix product (half a unit
+        // in the last place per weight); the sum keeps the unrounded weights
+        // because lse is an fp32 result
         uint64_t ls = f2_pack(0.0f, 0.0f);
-        if (all_pure) {
-          const uint64_t sl = f2_pack(sl2, sl2);
+        const uint64_t slv = f2_pack(sl, sl);
+        uint32_t pk[kKeys / 2];
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const uint64_t ad = f2_pack(add[g] - mu, add[g] - mu);
+        for (int g = 0; g < NG; ++g) {
+          const uint64_t ad = f2_pack(add[g] - mu, add[g] - mu);
 #pragma unroll
-            for (int c = 0; c < GR; c += 2) {
-              float y0, y1;
-              f2_unpack(ffma2(f2_pack(x[g * GR + c], x[g * GR + c + 1]), sl, ad), y0, y1);
-              const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
-              ls = fadd2(ls, f2_pack(p0, p1));
-              pk[(g * GR + c) >> 1] = pack2(p0, p1, (T*)nullptr);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < kKeys; c += 2) {
-            const float p0 = fast_exp2(x[c] - mu), p1 = fast_exp2(x[c + 1] - mu);
+          for (int c = 0; c < GR; c += 2) {
+            float y0, y1;
+            f2_unpack(ffma2(f2_pack(x[g * GR + c], x[g * GR + c + 1]), slv, ad), y0, y1);
+            const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
             ls = fadd2(ls, f2_pack(p0, p1));
-            pk[c >> 1] = pack2(p0, p1, (T*)nullptr);
+            pk[(g * GR + c) >> 1] = pack2(p0, p1, (T*)nullptr);
           }
         }
+        tmem_st32(tS, pk);
         float l0, l1;
         f2_unpack(ls, l0, l1);
         l_run += l0 + l1;
       }
-      tmem_st32(tS, pk);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.pfull[sb]);
     }
-    // ---- O, maximum and sum into shared memory (the K and V slots are free) ----
-    if (tiles > 0 && alive)
-      alive = mbar_wait_warp(&S.pvdone[(tiles - 1) & 1], (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag, derr, 63);
-    tc_fence_after();
-    if (tiles > 0) {
+    // ---- the end: O from TMEM ----
+    if (warp_on) {
+      if (tiles > 0 && alive)
+        alive = tree_wait_warp(&S.pvdone[(tiles - 1) & 1], (uint32_t)((tiles - 1) >> 1) & 1u, abort_flag, derr, 63);
+      tc_fence_after();
+      const float inv = l_run > 0.0f ? 1.0f / l_run : 0.0f;
+      T* op = reinterpret_cast<T*>(a.qo.out) + r * a.qo.o_stride_tok + (int64_t)hq * a.qo.o_stride_head;
+      float chk = l_run * 0.0f;                  // x * 0 is 0 for a finite x only
 #pragma unroll 1
-      for (int q4 = 0; q4 < 4; ++q4) {
-        uint32_t o[32];
-        tmem_ld32(tO + q4 * 32 + lane_base, o);
+      for (int c = 0; c < 128; c += 32) {
+        float o[32];
+        tmem_ld32f(tO + c + lane_base, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int v = 0; v < 8; ++v)
-          *reinterpret_cast<uint4*>(S.k[0] + m * 512 + (((q4 * 8 + v) ^ (m & 7)) << 4)) =
-              make_uint4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        for (int k = 0; k < 32; ++k) {
+          if (tiles == 0) o[k] = 0.0f;
+          chk = fmaf(o[k], 0.0f, chk);
+        }
+        if (nsp == 1) {
+          // the unit is this CTA's alone
+          if (row_ok) {
+#pragma unroll
+            for (int v = 0; v < 4; ++v)
+              *reinterpret_cast<uint4*>(op + c + v * 8) =
+                  make_uint4(pack2(o[8 * v] * inv, o[8 * v + 1] * inv, (T*)nullptr),
+                             pack2(o[8 * v + 2] * inv, o[8 * v + 3] * inv, (T*)nullptr),
+                             pack2(o[8 * v + 4] * inv, o[8 * v + 5] * inv, (T*)nullptr),
+                             pack2(o[8 * v + 6] * inv, o[8 * v + 7] * inv, (T*)nullptr));
+          }
+        } else {
+          // into shared memory (the K and V slots are free)
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            *reinterpret_cast<float4*>(S.k[0] + m * 512 + ((((c >> 2) + v) ^ (m & 7)) << 4)) =
+                make_float4(o[4 * v], o[4 * v + 1], o[4 * v + 2], o[4 * v + 3]);
+        }
+      }
+      if (nsp == 1) {
+        if (row_ok && a.qo.lse)
+          a.qo.lse[r * a.qo.lse_stride_tok + (int64_t)hq * a.qo.lse_stride_head] =
+              l_run > 0.0f ? (m_run + log2f(l_run)) * kTreeLn2 : -INFINITY;
+        __syncwarp();                            // these stores come before those of redo_row
+        for (uint32_t bad = __ballot_sync(0xffffffffu, row_ok && !(chk == 0.0f)); bad; bad &= bad - 1)
+          redo_row<T>(a, sq, s, r0, warp * 32 + __ffs(bad) - 1, G, hk);
+      } else {
+        S.m[m] = m_run;
+        S.l[m] = tiles > 0 ? l_run : -1.0f;      // -1: this CTA had no tile
       }
     }
-    S.m[m] = m_run;
-    S.l[m] = tiles > 0 ? l_run : -1.0f;          // -1: this CTA had no tile
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
+  if (nsp == 1) return;
   cluster.sync();
   // ---- join: row m by CTA m % nsp, a warp per row, lane = 4 dims ----
+#pragma unroll 1
   for (int m = split + nsp * warp; m < nrows; m += nsp * (kThreads / 32)) {
     const int node = m / G;
     const int64_t r = r0 + node;
     const int hq = hk * G + m - node * G;
-    float M = -INFINITY;
     float mk = -INFINITY, lk = -1.0f;            // lane k holds CTA k's
     if (lane < nsp) {
       mk = *cluster.map_shared_rank(&S.m[m], lane);
       lk = *cluster.map_shared_rank(&S.l[m], lane);
     }
-    M = mk;
+    float M = mk;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int x = 4; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
     M = __shfl_sync(0xffffffffu, M, 0);
+    // a part without a key for the row has weight 0, and 0 * NaN shows below;
+    // one without a tile is left out
+    const float wk = mk == -INFINITY ? 0.0f : fast_exp2(mk - M);
     float L = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
     for (int k = 0; k < nsp; ++k) {
-      const float m1 = __shfl_sync(0xffffffffu, mk, k), l1 = __shfl_sync(0xffffffffu, lk, k);
-      if (l1 == -1.0f) continue;
-      const float w = m1 == -INFINITY ? 0.0f : fast_exp2(m1 - M);
+      const float w = __shfl_sync(0xffffffffu, wk, k), l1 = __shfl_sync(0xffffffffu, lk, k);
       const float4 o =
           *reinterpret_cast<const float4*>(cluster.map_shared_rank(&S.k[0][0], k) + m * 512 + ((lane ^ (m & 7)) << 4));
-      L += l1 * w;
-      O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+      if (l1 != -1.0f) {
+        L += l1 * w;
+        O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+      }
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    // x * 0 is 0 for a finite x only
-    const bool fine = (O.x + O.y + O.z + O.w) * 0.0f + L * 0.0f == 0.0f;
+    const bool fine = (O.x + O.y + O.z + O.w + L) * 0.0f == 0.0f;
     if (!__all_sync(0xffffffffu, fine)) {
-      float ms, ls, os[16];
-      tree_row_attend<T>(a, sq, s, r, hq, ms, ls, os);
-      tree_row_store<T>(a, r, hq, ms, ls, os);
+      redo_row<T>(a, sq, s, r0, m, G, hk);
       continue;
     }
     T* op = reinterpret_cast<T*>(a.qo.out) + r * a.qo.o_stride_tok + (int64_t)hq * a.qo.o_stride_head + lane * 4;
@@ -628,35 +817,37 @@ static int page_map(CUtensorMap* map, const void* base, const DashTreeAttnArgs& 
   return DASH_OK;
 }
 
-// CTAs per sequence and kv head: (whole waves of CTAs, two per SM) x (tiles of a
-// CTA + setup and join, worth about 3 tiles).  The number of tiles is not known
-// here; its upper bound is.
-static int tree_splits(const DashTreeAttnArgs& a, int64_t units, int gr) {
+// CTAs per unit.  A CTA costs about 10 us before and after its tiles; a tile takes
+// 0.95 us (its chain of S, softmax and P V), or what the memory gives: 1.49 us with
+// two CTAs on every SM.  Past one wave the last one is about half full.  (Measured, us,
+// 1 / 2 / 3 / 8 CTAs: 320 units of 37 tiles 103 / 101 / 102 / 151, 160 of 34
+// 51 / 64 / 57 / 89, 80 of 15 31 / 25 / 23 / 45, 10 of 20 29 / 23 / 21 / 17.)  The number of tiles
+// is not known here; the drafted tokens of a sequence route similar blocks: twice K are
+// assumed.
+static int tree_splits(const DashTreeAttnArgs& a, int64_t units) {
   if (a.num_splits) return a.num_splits;
-  const int64_t per = kRows / (a.qo.n_heads / a.kv.n_kv_heads);
-  const int64_t nodes = a.seqs.max_q_len < per ? a.seqs.max_q_len : per;
-  int64_t gran = nodes * a.routes.K * (a.block_size / gr) + (a.local_window + nodes) / gr + 2;
-  const int64_t most = (int64_t)a.bt_width * a.block_size / gr;
-  if (gran > most) gran = most;
-  const int64_t tiles = (gran * gr + kKeys - 1) / kKeys;
+  int64_t keys = (int64_t)(a.seqs.max_q_len == 1 ? 1 : 2) * a.routes.K * a.block_size + a.local_window + a.seqs.max_q_len;
+  const int64_t most = (int64_t)a.bt_width * a.block_size;
+  const double tiles = (double)((keys < most ? keys : most) + kKeys - 1) / kKeys;
   int best = 1;
-  int64_t cost = INT64_MAX;
+  double least = 1e30;
   for (int sp = 1; sp <= 8 && sp <= tiles; ++sp) {
-    const int64_t waves = (units * sp + 295) / 296, c = waves * ((tiles + sp - 1) / sp + 3);
-    if (c < cost) { cost = c; best = sp; }
+    const double waves = (double)units * sp / 296, tile = waves < 1 ? 1.49 * waves : 1.49;
+    const double own = 10.0 + tiles / sp * (tile > 0.95 ? tile : 0.95), t = own * (waves <= 1 ? 1.0 : waves + 0.5);
+    if (t < least) { least = t; best = sp; }
   }
   return best;
 }
 
-template <typename T, int GR>
+template <typename T, int GR, int QR>
 static int launch_tc(const DashTreeAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, cudaStream_t st) {
   const int per = kRows / (a.qo.n_heads / a.kv.n_kv_heads);
   const int n_tiles = (a.seqs.max_q_len + per - 1) / per;
   const int64_t units = (int64_t)a.seqs.n_seq * a.kv.n_kv_heads * n_tiles;
-  const int sp = tree_splits(a, units, GR);
+  const int sp = tree_splits(a, units);
   if (units * sp > INT32_MAX) return set_error(DASH_ERR_UNSUPPORTED, "too many sequences x kv heads");
-  const int smem = (int)sizeof(TreeSmem) + 1024;
-  auto kernel = tree_tc_kernel<T, GR>;
+  const int smem = (int)sizeof(TreeSmem<QR>) + 1024;
+  auto kernel = tree_tc_kernel<T, GR, QR>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
@@ -684,9 +875,14 @@ static int launch_tc_gr(const DashTreeAttnArgs& a, cudaStream_t st) {
   int rc = page_map(&mk, a.kv.k, a, gr);
   if (rc == DASH_OK) rc = page_map(&mv, a.kv.v, a, gr);
   if (rc != DASH_OK) return rc;
-  if (gr == 16) return launch_tc<T, 16>(a, mk, mv, st);
-  if (gr == 32) return launch_tc<T, 32>(a, mk, mv, st);
-  return launch_tc<T, 64>(a, mk, mv, st);
+  const int G = a.qo.n_heads / a.kv.n_kv_heads;
+  const int rows = (a.seqs.max_q_len < kRows / G ? a.seqs.max_q_len : kRows / G) * G;
+  if (rows <= 32) return gr == 16 ? launch_tc<T, 16, 32>(a, mk, mv, st)
+                       : gr == 32 ? launch_tc<T, 32, 32>(a, mk, mv, st) : launch_tc<T, 64, 32>(a, mk, mv, st);
+  if (rows <= 64) return gr == 16 ? launch_tc<T, 16, 64>(a, mk, mv, st)
+                       : gr == 32 ? launch_tc<T, 32, 64>(a, mk, mv, st) : launch_tc<T, 64, 64>(a, mk, mv, st);
+  return gr == 16 ? launch_tc<T, 16, 128>(a, mk, mv, st)
+       : gr == 32 ? launch_tc<T, 32, 128>(a, mk, mv, st) : launch_tc<T, 64, 128>(a, mk, mv, st);
 }
 
 int launch_tree_tc(const DashTreeAttnArgs& a, cudaStream_t st) {

@@ -26,7 +26,6 @@ from . import _lib as L
 from . import ops
 from .ops import DeviceErrorWord, _need_cuda, _ptr
 from .page_pool import Layers, _call, _ints, _layers
-from .unlimited_dash_ops.attend_triton import _paged_kv, _routes_from
 
 
 @dataclass
@@ -49,11 +48,11 @@ def tree_plan(parents: Optional[torch.Tensor], cu_seqlens_q: torch.Tensor, ctx_l
     within its sequence (-1: none); None: every sequence drafts a chain.
     ``slots`` are filled when a ``block_table`` [n_seq, W] is given."""
     _need_cuda(cu_seqlens_q, parents, block_table)
-    dev = cu_seqlens_q.device
-    cu = _ints(cu_seqlens_q, "cu_seqlens_q", dev)
+    dev, index = cu_seqlens_q.device, cu_seqlens_q.get_device()
+    cu = _ints(cu_seqlens_q, "cu_seqlens_q", index)
     n_seq = cu.shape[0] - 1
-    ctx = _ints(ctx_lens, "ctx_lens", dev, n_seq)
-    par = _ints(parents, "parents", dev, rows)
+    ctx = _ints(ctx_lens, "ctx_lens", index, n_seq)
+    par = _ints(parents, "parents", index, rows)
     words = (max_nodes + 31) // 32
     # rows behind the last sequence keep these values
     buf = torch.zeros((3 + words) * rows, dtype=torch.int32, device=dev)
@@ -65,19 +64,15 @@ def tree_plan(parents: Optional[torch.Tensor], cu_seqlens_q: torch.Tensor, ctx_l
     a.depth, a.row_pos, a.row_seq, a.mask = depth.data_ptr(), pos.data_ptr(), seq.data_ptr(), mask.data_ptr()
     slots = None
     if block_table is not None:
-        bt = block_table if block_table.dtype == torch.int32 and block_table.stride(1) == 1 else \
-            block_table.to(torch.int32).contiguous()
-        if bt.shape[0] != n_seq:
-            raise ValueError(f"block_table has {bt.shape[0]} rows for {n_seq} sequences")
+        bt = _table(block_table, index, n_seq)
         slots = torch.full((rows,), -1, dtype=torch.int64, device=dev)
         a.block_table, a.bt_stride, a.bt_width = bt.data_ptr(), bt.stride(0), bt.shape[1]
         a.block_size, a.num_pages, a.slots = int(block_size), int(num_pages), slots.data_ptr()
     a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_tree_plan", a, dev)
+    _call("dash_tree_plan", a, index)
     return TreePlan(depth, pos, seq, mask, slots)
 
 
-@torch.no_grad()
 def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                           topk_idx: torch.Tensor, blk_bias: Optional[torch.Tensor],
                           block_table: torch.Tensor, cu_seqlens_q: torch.Tensor, ctx_lens: torch.Tensor,
@@ -99,64 +94,97 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     (with their biases) before it, and the drafted tokens of its mask.  Rows
     from ``cu_seqlens_q[-1]`` on are left as they were.  lse [rows, H] fp32:
     natural-log sums.  num_splits: CTAs per sequence and kv head (0 = automatic)."""
-    _need_cuda(q, k_cache, v_cache, topk_idx, block_table, tree_mask, output, lse)
-    dev, dt = q.device, k_cache.dtype
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("topk_idx", topk_idx), ("blk_bias", blk_bias),
-                    ("block_table", block_table), ("tree_mask", tree_mask), ("output", output), ("lse", lse)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, not {dev}")
+    index, dt = q.get_device(), q.dtype
+    ks, kst = k_cache.shape, k_cache.stride()
+    # the usual call passes one test; what is wrong with any other is said below
+    if not (q.dim() == 3 == topk_idx.dim() and len(ks) == 4 and output.shape == q.shape and
+            ks == v_cache.shape and kst == v_cache.stride() and
+            tuple(ks[1:]) == (sparse_block_size, num_kv_heads, q.shape[2]) and
+            dt is k_cache.dtype is v_cache.dtype is output.dtype and
+            index == k_cache.get_device() == v_cache.get_device() == output.get_device() ==
+            topk_idx.get_device() == tree_mask.get_device() and index >= 0):
+        _refuse_tree(q, k_cache, v_cache, output, topk_idx, tree_mask, sparse_block_size, num_kv_heads)
+    rows, H, _ = q.shape
+    if rows == 0:
+        return
+    qst, ost, mst, ist = q.stride(), output.stride(), tree_mask.stride(), topk_idx.stride()
+    if qst[2] != 1 or ost[2] != 1 or kst[3] != 1:
+        raise ValueError("q, output and the caches must have a unit inner stride")
+    K = topk_idx.shape[2]
+    if topk_idx.shape[0] != num_kv_heads or topk_idx.shape[1] != rows:
+        raise ValueError(f"topk_idx must be [{num_kv_heads}, {rows}, K]")
+    if tree_mask.dtype is not torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] != rows or \
+            (tree_mask.shape[1] > 1 and mst[1] != 1):
+        raise ValueError(f"tree_mask must be int32 [{rows}, words]")
+    cu = _ints(cu_seqlens_q, "cu_seqlens_q", index)
+    n_seq = cu.shape[0] - 1
+    ctx = _ints(ctx_lens, "ctx_lens", index, n_seq)
+    pos = _ints(row_pos, "row_pos", index, rows)
+    bt = _table(block_table, index, n_seq)
+    if n_seq == 0:
+        return
+    a = L.DashTreeAttnArgs()
+    sq, kv, ro, qo = a.seqs, a.kv, a.routes, a.qo
+    sq.n_seq, sq.q_len_fixed, sq.max_q_len, sq.q_start = n_seq, rows, max_nodes, cu.data_ptr()
+    kv.k, kv.v, kv.dtype = k_cache.data_ptr(), v_cache.data_ptr(), ops._DT.get(dt, -1)
+    kv.n_kv_heads, kv.head_dim = num_kv_heads, ks[3]
+    kv.stride_seq, kv.stride_tok, kv.stride_head, _ = kst
+    kv.block_table, kv.bt_stride, kv.num_pages = bt.data_ptr(), bt.stride(0), ks[0]
+    if blk_bias is not None:
+        if blk_bias.shape != topk_idx.shape or blk_bias.dtype is not torch.float32 or blk_bias.get_device() != index:
+            raise ValueError(f"blk_bias must be fp32 of topk_idx's shape on cuda:{index}")
+    if K:
+        if topk_idx.dtype is not torch.int32 or ist[2] != 1 or (blk_bias is not None and blk_bias.stride() != ist):
+            # one layout for both; a router head that all kv heads share is kept once
+            one = ist[0] == 0 or num_kv_heads == 1
+            topk_idx = (topk_idx[:1] if one else topk_idx).to(torch.int32).contiguous()
+            if blk_bias is not None:
+                blk_bias = (blk_bias[:1] if one else blk_bias).contiguous()
+            ist = (0 if one else topk_idx.stride(0),) + topk_idx.stride()[1:]
+        one = ist[0] == 0 or num_kv_heads == 1
+        ro.idx, ro.K, ro.row_stride = topk_idx.data_ptr(), K, ist[1]
+        ro.n_index_heads, ro.ihead_stride = (1, 0) if one else (num_kv_heads, ist[0])
+        if blk_bias is not None:
+            ro.bias = blk_bias.data_ptr()
+    qo.q, qo.out, qo.n_heads = q.data_ptr(), output.data_ptr(), H
+    qo.q_stride_tok, qo.q_stride_head = qst[0], qst[1]
+    qo.o_stride_tok, qo.o_stride_head = ost[0], ost[1]
+    if lse is not None:
+        if lse.shape != (rows, H) or lse.dtype is not torch.float32 or lse.get_device() != index:
+            raise ValueError(f"lse must be fp32 [{rows}, {H}] on cuda:{index}")
+        qo.lse = lse.data_ptr()
+        qo.lse_stride_tok, qo.lse_stride_head = lse.stride()
+    a.ctx_len, a.row_pos, a.mask = ctx.data_ptr(), pos.data_ptr(), tree_mask.data_ptr()
+    a.mask_stride, a.mask_words, a.bt_width = mst[0], tree_mask.shape[1], bt.shape[1]
+    a.scale, a.block_size = sm_scale, sparse_block_size
+    a.local_window, a.num_splits = local_blocks * sparse_block_size, num_splits
+    if device_error is not None:
+        a.device_error = device_error.ptr
+    _call("dash_tree_attn", a, index)
+
+
+def _table(block_table: torch.Tensor, index: int, n_seq: int) -> torch.Tensor:
+    """The block table as int32 rows of unit inner stride."""
+    if block_table.dim() != 2 or block_table.shape[0] != n_seq or block_table.get_device() != index:
+        _need_cuda(block_table)
+        raise ValueError(f"block_table must be [{n_seq}, W] on cuda:{index}")
+    return block_table if block_table.dtype is torch.int32 and block_table.stride(1) == 1 else \
+        block_table.to(torch.int32).contiguous()
+
+
+def _refuse_tree(q, k_cache, v_cache, output, topk_idx, tree_mask, block, n_kv):
+    _need_cuda(q, k_cache, v_cache, output, topk_idx, tree_mask)
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("output", output), ("topk_idx", topk_idx),
+                    ("tree_mask", tree_mask)):
+        if t.device != q.device:
+            raise ValueError(f"{name} is on {t.device}, not {q.device}")
     if q.dim() != 3 or output.shape != q.shape:
         raise ValueError("q and output must be [rows, heads, head_dim]")
-    rows, H, hd = q.shape
-    if q.dtype != dt or v_cache.dtype != dt or output.dtype != dt:
+    if not q.dtype == k_cache.dtype == v_cache.dtype == output.dtype:
         raise ValueError("q, k_cache, v_cache and output must have one dtype")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or \
-            k_cache.shape[1:] != (sparse_block_size, num_kv_heads, hd):
-        raise ValueError(f"caches must be [pages, {sparse_block_size}, {num_kv_heads}, {hd}] with common strides")
-    for name, t in (("q", q), ("output", output), ("k_cache", k_cache)):
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name} must have a unit inner stride")
-    if topk_idx.dim() != 3 or topk_idx.shape[:2] != (num_kv_heads, rows):
-        raise ValueError(f"topk_idx must be [{num_kv_heads}, {rows}, K]")
-    if blk_bias is not None and (blk_bias.shape != topk_idx.shape or blk_bias.dtype != torch.float32):
-        raise ValueError("blk_bias must be fp32 of topk_idx's shape")
-    cu = _ints(cu_seqlens_q, "cu_seqlens_q", dev)
-    n_seq = cu.shape[0] - 1
-    ctx = _ints(ctx_lens, "ctx_lens", dev, n_seq)
-    pos = _ints(row_pos, "row_pos", dev, rows)
-    if tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] != rows or \
-            (tree_mask.shape[1] > 1 and tree_mask.stride(1) != 1):
-        raise ValueError(f"tree_mask must be int32 [{rows}, words]")
-    if block_table.dim() != 2 or block_table.shape[0] != n_seq:
-        raise ValueError(f"block_table must be [{n_seq}, W]")
-    bt = block_table if block_table.dtype == torch.int32 and block_table.stride(1) == 1 else \
-        block_table.to(torch.int32).contiguous()
-    if rows == 0 or n_seq == 0:
-        return
-    if topk_idx.shape[2]:
-        routes, idx_keep, bias_keep = _routes_from(topk_idx, blk_bias, num_kv_heads)
-    else:
-        routes, idx_keep, bias_keep = ops._routes(None, None, 0, 0, 1), None, None
-    a = L.DashTreeAttnArgs()
-    a.seqs = ops.Seqs(n_seq=n_seq, q_start=cu, total_rows=rows, max_q_len=int(max_nodes)).c()
-    a.kv = _paged_kv(k_cache, v_cache, bt, num_kv_heads)
-    a.routes = routes
-    lse_strides = (0, 0, 0)
-    if lse is not None:
-        if lse.shape != (rows, H) or lse.dtype != torch.float32:
-            raise ValueError(f"lse must be fp32 [{rows}, {H}]")
-        lse_strides = (0, lse.stride(0), lse.stride(1))
-    a.qo = ops._qo(q, output, (0, q.stride(0), q.stride(1)), (0, output.stride(0), output.stride(1)), H,
-                   lse, lse_strides)
-    a.ctx_len, a.row_pos = ctx.data_ptr(), pos.data_ptr()
-    a.mask, a.mask_stride, a.mask_words = tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1]
-    a.bt_width = bt.shape[1]
-    a.scale, a.block_size = float(sm_scale), int(sparse_block_size)
-    a.local_window = int(local_blocks) * int(sparse_block_size)
-    a.num_splits = int(num_splits)
-    a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_tree_attn", a, dev)
-    del idx_keep, bias_keep
+    if topk_idx.dim() != 3:
+        raise ValueError("topk_idx must be [kv heads, rows, K]")
+    raise ValueError(f"caches must be [pages, {block}, {n_kv}, {q.shape[2]}] with common strides")
 
 
 @dataclass
@@ -187,50 +215,53 @@ def verify_drafts(tokens: torch.Tensor, parents: Optional[torch.Tensor], cu_seql
     distribution.  ``greedy``: target are logits (or probabilities), a draft is kept
     where it is the row's argmax (lowest index among equals), and no random
     numbers are read."""
-    _need_cuda(tokens, target, draft, u_accept, u_sample)
-    dev = target.device
-    cu = _ints(cu_seqlens_q, "cu_seqlens_q", dev)
+    index = target.get_device()
+    if index < 0:
+        _need_cuda(target)
+    cu = _ints(cu_seqlens_q, "cu_seqlens_q", index)
     n_seq = cu.shape[0] - 1
     if target.dim() != 2 or target.dtype not in ops._DT:
         raise ValueError("target must be [rows, vocab] in fp32, bf16 or fp16")
     rows, V = target.shape
-    par = _ints(parents, "parents", dev, rows)
-    if tokens.shape != (rows,) or tokens.dtype != torch.int64 or tokens.device != dev:
-        raise ValueError(f"tokens must be int64 [{rows}] on {dev}")
-    if target.stride(1) != 1 and V > 1:
+    par = _ints(parents, "parents", index, rows)
+    if tokens.shape != (rows,) or tokens.dtype is not torch.int64 or tokens.get_device() != index:
+        raise ValueError(f"tokens must be int64 [{rows}] on cuda:{index}")
+    if greedy:
+        if draft is not None or u_accept is not None or u_sample is not None:
+            raise ValueError("greedy verification takes neither draft probabilities nor random numbers")
+    else:
+        if u_accept is None or u_sample is None:
+            raise ValueError("u_accept and u_sample are needed unless greedy")
+        for name, u, n in (("u_accept", u_accept, rows), ("u_sample", u_sample, n_seq)):
+            if u.shape != (n,) or u.dtype is not torch.float32 or u.get_device() != index:
+                raise ValueError(f"{name} must be fp32 [{n}] on cuda:{index}")
+        u_accept, u_sample = u_accept.contiguous(), u_sample.contiguous()
+    tst = target.stride()
+    if tst[1] != 1 and V > 1:
         target = target.contiguous()
-    if greedy and (draft is not None or u_accept is not None or u_sample is not None):
-        raise ValueError("greedy verification takes neither draft probabilities nor random numbers")
-    if not greedy and (u_accept is None or u_sample is None):
-        raise ValueError("u_accept and u_sample are needed unless greedy")
+        tst = target.stride()
+    tokens = tokens.contiguous()
+    dev, i32, i64 = target.device, torch.int32, torch.int64
+    r = Verified(torch.empty(n_seq, dtype=i32, device=dev), torch.empty(n_seq, max_nodes, dtype=i32, device=dev),
+                 torch.empty(n_seq, dtype=i64, device=dev), torch.empty(n_seq, max_nodes, dtype=i64, device=dev))
+    a = L.DashVerifyArgs()
+    a.tokens, a.parents, a.q_start = tokens.data_ptr(), _ptr(par), cu.data_ptr()
+    a.target, a.target_stride = target.data_ptr(), tst[0] if rows > 1 else V
+    a.n_seq, a.rows, a.max_nodes, a.vocab = n_seq, rows, max_nodes, V
+    a.dtype, a.mode = ops._DT[target.dtype], 2 if greedy else 1
     if draft is not None:
-        if draft.shape != target.shape or draft.dtype != target.dtype or draft.device != dev:
+        if draft.shape != target.shape or draft.dtype is not target.dtype or draft.get_device() != index:
             raise ValueError("draft must have target's shape, dtype and device")
         if draft.stride(1) != 1 and V > 1:
             draft = draft.contiguous()
-    for name, u, n in (("u_accept", u_accept, rows), ("u_sample", u_sample, n_seq)):
-        if u is not None and (u.shape != (n,) or u.dtype != torch.float32 or u.device != dev):
-            raise ValueError(f"{name} must be fp32 [{n}] on {dev}")
-    tokens = tokens.contiguous()
-    u_accept = None if u_accept is None else u_accept.contiguous()
-    u_sample = None if u_sample is None else u_sample.contiguous()
-    max_nodes = int(max_nodes)
-    i64 = torch.empty(n_seq * (max_nodes + 1), dtype=torch.int64, device=dev)
-    i32 = torch.empty(n_seq * (max_nodes + 1), dtype=torch.int32, device=dev)
-    r = Verified(i32[:n_seq], i32[n_seq:].view(n_seq, max_nodes), i64[:n_seq],
-                 i64[n_seq:].view(n_seq, max_nodes))
-    a = L.DashVerifyArgs()
-    a.tokens, a.parents, a.q_start = tokens.data_ptr(), _ptr(par), cu.data_ptr()
-    a.target, a.target_stride = target.data_ptr(), target.stride(0) if rows > 1 else V
-    if draft is not None:
-        a.draft, a.draft_stride = draft.data_ptr(), draft.stride(0) if rows > 1 else V
-    a.u_accept, a.u_sample = _ptr(u_accept), _ptr(u_sample)
-    a.n_seq, a.rows, a.max_nodes, a.vocab = n_seq, rows, max_nodes, V
-    a.dtype, a.mode = ops._DT[target.dtype], 2 if greedy else 0 if draft is not None else 1
+        a.draft, a.draft_stride, a.mode = draft.data_ptr(), draft.stride(0) if rows > 1 else V, 0
+    if not greedy:
+        a.u_accept, a.u_sample = u_accept.data_ptr(), u_sample.data_ptr()
     a.n_accept, a.path = r.n_accept.data_ptr(), r.path.data_ptr()
     a.next_token, a.out_tokens = r.next_token.data_ptr(), r.tokens.data_ptr()
-    a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_draft_verify", a, dev)
+    if device_error is not None:
+        a.device_error = device_error.ptr
+    _call("dash_draft_verify", a, index)
     return r
 
 
@@ -242,20 +273,16 @@ def commit_drafts(caches: Layers, path: torch.Tensor, n_accept: torch.Tensor, ct
     returns them).  ``ctx_lens + 1 + n_accept`` tokens are committed afterwards;
     summaries of the touched pages (k-bar) have to be refreshed."""
     layers = _layers(caches)
-    dev = layers.device
+    index = layers.index
     if layers.page_tokens is None:
         raise ValueError("commit_drafts takes tensors with one entry per token")
-    _need_cuda(path, block_table)
-    if path.dim() != 2 or path.dtype != torch.int32 or path.device != dev or \
+    if path.dim() != 2 or path.dtype is not torch.int32 or path.get_device() != index or \
             (path.shape[1] > 1 and path.stride(1) != 1):
-        raise ValueError(f"path must be int32 [n_seq, max_nodes] on {dev}")
+        raise ValueError(f"path must be int32 [n_seq, max_nodes] on cuda:{index}")
     n_seq, max_nodes = path.shape
-    acc = _ints(n_accept, "n_accept", dev, n_seq)
-    ctx = _ints(ctx_lens, "ctx_lens", dev, n_seq)
-    if block_table.dim() != 2 or block_table.shape[0] != n_seq or block_table.device != dev:
-        raise ValueError(f"block_table must be [{n_seq}, W] on {dev}")
-    bt = block_table if block_table.dtype == torch.int32 and block_table.stride(1) == 1 else \
-        block_table.to(torch.int32).contiguous()
+    acc = _ints(n_accept, "n_accept", index, n_seq)
+    ctx = _ints(ctx_lens, "ctx_lens", index, n_seq)
+    bt = _table(block_table, index, n_seq)
     a = L.DashCommitArgs()
     a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
     a.n_seq, a.max_nodes, a.block_size = n_seq, max_nodes, layers.page_tokens
@@ -263,5 +290,6 @@ def commit_drafts(caches: Layers, path: torch.Tensor, n_accept: torch.Tensor, ct
     a.path, a.path_stride = path.data_ptr(), path.stride(0) if n_seq > 1 else max_nodes
     a.n_accept, a.ctx_len = acc.data_ptr(), ctx.data_ptr()
     a.block_table, a.bt_stride = bt.data_ptr(), bt.stride(0) if n_seq > 1 else bt.shape[1]
-    a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_draft_commit", a, dev)
+    if device_error is not None:
+        a.device_error = device_error.ptr
+    _call("dash_draft_commit", a, index)

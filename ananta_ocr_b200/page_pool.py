@@ -21,25 +21,30 @@ from . import _lib as L
 from .ops import DeviceErrorWord, _need_cuda, _ptr
 
 
-def _call(fn: str, args, device) -> None:
-    """Launch on ``device``'s current stream, whatever the current device is."""
-    if torch.cuda.current_device() == device.index:
-        L.call(fn, args)
-    else:
-        with torch.cuda.device(device):
-            L.call(fn, args)
+def _call(fn: str, args, index: int) -> None:
+    """Launch on the current stream of device ``index``, whatever the current
+    device is."""
+    if torch._C._cuda_getDevice() != index:
+        with torch.cuda.device(index):
+            return _call(fn, args, index)
+    rc = getattr(L.load(), fn)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc != L.DASH_OK:
+        raise L.DashError(rc, L.last_error())
 
 
-def _ints(t: Optional[torch.Tensor], name: str, device, n: Optional[int] = None) -> Optional[torch.Tensor]:
-    """``t`` as a contiguous int32 vector (of ``n`` values) on ``device``."""
+def _ints(t: Optional[torch.Tensor], name: str, index: int, n: Optional[int] = None) -> Optional[torch.Tensor]:
+    """``t`` as a contiguous int32 vector (of ``n`` values) on CUDA device ``index``."""
     if t is None:
         return None
-    _need_cuda(t)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, not {device}")
-    if t.dtype not in (torch.int32, torch.int64) or t.dim() != 1 or (n is not None and t.shape[0] != n):
+    if t.get_device() != index:
+        _need_cuda(t)
+        raise ValueError(f"{name} is on {t.device}, not cuda:{index}")
+    if t.dim() != 1 or (n is not None and t.shape[0] != n) or t.dtype not in _INTS:
         raise ValueError(f"{name} must be an int32 vector" + ("" if n is None else f" of {n} values"))
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+
+_INTS = (torch.int32, torch.int64)
 
 
 class CacheLayers:
@@ -56,6 +61,7 @@ class CacheLayers:
             raise ValueError("a cache needs at least one tensor")
         first = self.tensors[0]
         self.device, self.num_pages = first.device, int(first.shape[0])
+        self.index = first.get_device()
         self.c = (L.DashCacheTensor * len(self.tensors))()
         toks = set()
         for d, t in zip(self.c, self.tensors):
@@ -91,7 +97,7 @@ def _copy(layers: CacheLayers, src, dst, n, *, count=None, scratch=None, device_
     a.num_pages = layers.num_pages
     a.check, a.list = int(scratch is not None), _ptr(scratch)
     a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_pages_copy", a, layers.device)
+    _call("dash_pages_copy", a, layers.index)
 
 
 def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
@@ -101,9 +107,9 @@ def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
     destination is another pair's source or destination is left out and
     recorded, as is one with an id past the last page."""
     layers = _layers(caches)
-    src = _ints(src, "src", layers.device)
-    n = int(src.shape[0])
-    dst = _ints(dst, "dst", layers.device, n)
+    src = _ints(src, "src", layers.index)
+    n = src.shape[0]
+    dst = _ints(dst, "dst", layers.index, n)
     if n:
         scratch = torch.empty(2 * n, dtype=torch.int32, device=layers.device)
         _copy(layers, src.data_ptr(), dst.data_ptr(), n, scratch=scratch, device_error=device_error)
@@ -141,7 +147,7 @@ class PagePool:
             raise ValueError("pool tensors do not fit one another")
         self.ref, self.free_list, self.n_free = ref, free_list, n_free
         self.block_table, self.n_blocks = block_table, n_blocks
-        self.block_size, self.device = int(block_size), ref.device
+        self.block_size, self.device, self.index = int(block_size), ref.device, ref.get_device()
         c = self.c = L.DashPagePool()
         c.ref, c.free_list, c.n_free = ref.data_ptr(), free_list.data_ptr(), n_free.data_ptr()
         c.block_table, c.bt_stride = block_table.data_ptr(), block_table.stride(0)
@@ -165,20 +171,20 @@ class PagePool:
     def reserve(self, rows: torch.Tensor, lens: torch.Tensor,
                 device_error: Optional[DeviceErrorWord] = None) -> None:
         """Row ``rows[i]`` gets pages for ``lens[i]`` tokens (it never loses any)."""
-        rows = _ints(rows, "rows", self.device)
-        lens = _ints(lens, "lens", self.device, rows.shape[0])
+        rows = _ints(rows, "rows", self.index)
+        lens = _ints(lens, "lens", self.index, rows.shape[0])
         a = self._args(rows, device_error)
         a.lens = lens.data_ptr()
-        _call("dash_pages_reserve", a, self.device)
+        _call("dash_pages_reserve", a, self.index)
 
     def free(self, rows: torch.Tensor, keep: Optional[torch.Tensor] = None,
              device_error: Optional[DeviceErrorWord] = None) -> None:
         """Row ``rows[i]`` keeps its first ``keep[i]`` blocks (default none)."""
-        rows = _ints(rows, "rows", self.device)
-        keep = _ints(keep, "keep", self.device, rows.shape[0])
+        rows = _ints(rows, "rows", self.index)
+        keep = _ints(keep, "keep", self.index, rows.shape[0])
         a = self._args(rows, device_error)
         a.lens = _ptr(keep)
-        _call("dash_pages_free", a, self.device)
+        _call("dash_pages_free", a, self.index)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor, caches: Layers,
              device_error: Optional[DeviceErrorWord] = None) -> None:
@@ -186,16 +192,16 @@ class PagePool:
         of row ``src[i]``: full pages are shared, a partly filled last one is
         copied to a page of its own in every tensor of ``caches``."""
         layers = self._own(caches)
-        src = _ints(src, "src", self.device)
-        n = int(src.shape[0])
-        dst, lens = _ints(dst, "dst", self.device, n), _ints(lens, "lens", self.device, n)
+        src = _ints(src, "src", self.index)
+        n = src.shape[0]
+        dst, lens = _ints(dst, "dst", self.index, n), _ints(lens, "lens", self.index, n)
         if n == 0:
             return
         pairs = torch.empty(2 * n, dtype=torch.int32, device=self.device)
         a = self._args(dst, device_error)
         a.src, a.lens = src.data_ptr(), lens.data_ptr()
         a.copy_src, a.copy_dst = pairs.data_ptr(), pairs.data_ptr() + 4 * n
-        _call("dash_pages_fork", a, self.device)
+        _call("dash_pages_fork", a, self.index)
         _copy(layers, a.copy_src, a.copy_dst, n)
 
     def compact(self, caches: Layers, into: Optional["PagePool"] = None,
@@ -214,7 +220,7 @@ class PagePool:
         a.into = to.c
         a.copy_src, a.copy_dst = buf.data_ptr(), buf.data_ptr() + 4 * half
         a.n_moves = buf.data_ptr() + 8 * half
-        _call("dash_pages_compact", a, self.device)
+        _call("dash_pages_compact", a, self.index)
         if half:
             _copy(layers, a.copy_src, a.copy_dst, half, count=a.n_moves)
         return buf[2 * half:]

@@ -275,8 +275,8 @@ class DashPagePool(C.Structure):
 
 class DashPagesArgs(C.Structure):
     _fields_ = [("pool", DashPagePool), ("into", DashPagePool), ("rows", _p), ("src", _p),
-                ("lens", _p), ("n", _i32), ("pad0", _i32), ("copy_src", _p), ("copy_dst", _p),
-                ("n_moves", _p), ("device_error", _p)]
+                ("lens", _p), ("n", _i32), ("n_tensors", _i32), ("tensors", _p), ("copy_src", _p),
+                ("copy_dst", _p), ("n_moves", _p), ("new_id", _p), ("device_error", _p)]
 
 
 ABI_ORDER = [DashSeqs, DashKV, DashRoutes, DashQO, DashKbarArgs, DashRouteArgs,

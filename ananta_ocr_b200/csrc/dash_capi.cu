@@ -665,6 +665,8 @@ int dash_pages_fork(const DashPagesArgs* a, dash_stream_t stream) {
   const int rc = check_pages(a, true);
   if (rc || a->n == 0) return rc;
   if (!a->src || !a->copy_src || !a->copy_dst) return set_error(DASH_ERR_INVALID, "null src/copy_src/copy_dst");
+  const int rt = check_tensors(a->tensors, a->n_tensors, 0);
+  if (rt) return rt;
   return launch_pages_fork(*a, (cudaStream_t)stream);
 }
 
@@ -675,7 +677,10 @@ int dash_pages_compact(const DashPagesArgs* a, dash_stream_t stream) {
   if (a->into.num_pages != a->pool.num_pages || a->into.max_rows != a->pool.max_rows ||
       a->into.bt_width != a->pool.bt_width)
     return set_error(DASH_ERR_INVALID, "`into` must have the pool's sizes");
-  if (!a->copy_src || !a->copy_dst || !a->n_moves) return set_error(DASH_ERR_INVALID, "null copy_src/copy_dst/n_moves");
+  if (!a->copy_src || !a->copy_dst || !a->n_moves || !a->new_id)
+    return set_error(DASH_ERR_INVALID, "null copy_src/copy_dst/n_moves/new_id");
+  rc = check_tensors(a->tensors, a->n_tensors, 0);
+  if (rc) return rc;
   return launch_pages_compact(*a, (cudaStream_t)stream);
 }
 

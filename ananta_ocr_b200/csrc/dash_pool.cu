@@ -104,9 +104,33 @@ constexpr int kPoolThreads = 1024;
 // ---------------------------------------------------------------------------
 // page copies
 // ---------------------------------------------------------------------------
+// A block table whose pages get new ids while their data moves (compaction).
+struct TableMap {
+  const int32_t* from;
+  int32_t* to;
+  const int32_t* new_id;
+  int64_t from_stride, to_stride;
+  int32_t rows, width;
+};
+constexpr int kMapBlocks = 32;
+
 __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_constant__ TensorSet ts,
                                                                   const int32_t* src, const int32_t* dst, int n,
-                                                                  const int32_t* count, int64_t num_pages) {
+                                                                  const int32_t* count, int64_t num_pages,
+                                                                  const __grid_constant__ TableMap tm) {
+  // starts while the kernel that writes the pairs runs
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // the table's entries, in the first CTAs, beside the copies
+  if (tm.rows && blockIdx.x < kMapBlocks) {
+    const int64_t entries = (int64_t)tm.rows * tm.width;
+#pragma unroll 4
+    for (int64_t e = (int64_t)blockIdx.x * kCopyThreads + threadIdx.x; e < entries;
+         e += (int64_t)kMapBlocks * kCopyThreads) {
+      const int row = (int)(e / tm.width), col = (int)(e - (int64_t)row * tm.width);
+      const int page = tm.from[row * tm.from_stride + col];
+      tm.to[row * tm.to_stride + col] = page >= 0 && page < num_pages ? tm.new_id[page] : page;
+    }
+  }
   const int live = count ? min(n, *count) : n;
   const int64_t units = (int64_t)live * ts.items;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
@@ -132,6 +156,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_check_kernel(const int32_t
                                                                    const int32_t* count, int num_pages, int32_t* list,
                                                                    DeviceError* err) {
   extern __shared__ uint32_t s_bits[];
+  asm volatile("griddepcontrol.launch_dependents;");          // the copy's CTAs may take their places
   const int words = (num_pages + 31) / 32;
   uint32_t *once = s_bits, *more = s_bits + words, *from = s_bits + 2 * words;
   const int live = count ? min(n, *count) : n;
@@ -309,6 +334,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_kernel(const DashPage
   extern __shared__ int s_first[];
   __shared__ int s_warp[32];
   __shared__ int4 s_req[kPoolThreads];
+  asm volatile("griddepcontrol.launch_dependents;");          // the copy's CTAs may take their places
   const DashPagePool& p = a.pool;
   const int bs = p.block_size;
   first_requests(s_first, a.rows, a.n, p.max_rows);
@@ -438,6 +464,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_free_kernel(const DashPage
 __global__ void __launch_bounds__(kPoolThreads) pages_compact_kernel(const DashPagesArgs a) {
   extern __shared__ int s_mem[];                   // held pages' bits, prefix sums
   __shared__ int s_warp[32];
+  asm volatile("griddepcontrol.launch_dependents;");          // the copy's CTAs may take their places
   const DashPagePool &p = a.pool, &q = a.into;
   const int P = p.num_pages, words = (P + 31) / 32;
   uint32_t* held = reinterpret_cast<uint32_t*>(s_mem);
@@ -460,7 +487,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_compact_kernel(const DashP
     if (page >= L && on(page)) a.copy_src[rank(page) - at_L] = page;
   }
   for (int k = moves + threadIdx.x; k < P / 2; k += kPoolThreads) a.copy_src[k] = a.copy_dst[k] = -1;
-  __syncthreads();                                 // copy_dst is read below (same CTA)
+  __syncthreads();                                 // the lists are read below (same CTA)
   // counts: a target takes its source's, pages >= L have none
   for (int page = threadIdx.x; page < P; page += kPoolThreads) {
     int c = 0;
@@ -472,13 +499,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_compact_kernel(const DashP
   for (int page = threadIdx.x; page < P; page += kPoolThreads) {
     if (page >= L) q.ref[page] = 0;
     q.free_list[page] = page < P - L ? P - 1 - page : -1;
-  }
-  const int64_t entries = (int64_t)p.max_rows * p.bt_width;
-  for (int64_t e = threadIdx.x; e < entries; e += kPoolThreads) {
-    const int64_t row = e / p.bt_width, col = e - row * p.bt_width;
-    int page = p.block_table[row * p.bt_stride + col];
-    if (page >= L && page < P && on(page)) page = a.copy_dst[rank(page) - at_L];
-    q.block_table[row * q.bt_stride + col] = page;
+    a.new_id[page] = page >= L && on(page) ? a.copy_dst[rank(page) - at_L] : page;
   }
   for (int r = threadIdx.x; r < p.max_rows; r += kPoolThreads) q.n_blocks[r] = p.n_blocks[r];
   if (threadIdx.x == 0) {
@@ -520,21 +541,33 @@ static void make_set(TensorSet& ts, const DashCacheTensor* t, int n, bool whole_
 }
 
 static int copy_pages(const DashCacheTensor* t, int n_tensors, const int32_t* src, const int32_t* dst, int n,
-                      const int32_t* count, int64_t num_pages, cudaStream_t st) {
+                      const int32_t* count, int64_t num_pages, const TableMap& tm, cudaStream_t st) {
+  TableMap map = tm;
   for (int i0 = 0; i0 < n_tensors; i0 += kMaxTensors) {
     TensorSet ts;
     make_set(ts, t + i0, n_tensors - i0 < kMaxTensors ? n_tensors - i0 : kMaxTensors, true, [](const TensorDesc& d) {
       const int64_t acc = ((int64_t)d.tok_bytes >> d.log_vec) * d.page_toks;
       return (int)((acc + kCopyThreads * kCopyBatch - 1) / (kCopyThreads * kCopyBatch));
     });
-    const int64_t units = (int64_t)n * ts.items;
+    int64_t units = (int64_t)n * ts.items;
+    if (map.rows && units < kMapBlocks) units = kMapBlocks;
     if (units == 0) continue;
     const int64_t most = 148 * 8;
-    pages_copy_kernel<<<(unsigned)(units < most ? units : most), kCopyThreads, 0, st>>>(ts, src, dst, n, count,
-                                                                                       num_pages);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units < most ? units : most));
+    cfg.blockDim = dim3(kCopyThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, pages_copy_kernel, ts, src, dst, n, count, num_pages, map);
+    if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "pages_copy_kernel launch failed: %s", cudaGetErrorString(e));
     count_launch();
     const int rc = check_launch("pages_copy_kernel");
     if (rc) return rc;
+    map.rows = 0;                                  // once
   }
   return DASH_OK;
 }
@@ -549,7 +582,7 @@ static int allow_smem(K kernel, size_t bytes, const char* name) {
 }
 
 int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st) {
-  if (!a.check) return copy_pages(a.tensors, a.n_tensors, a.src, a.dst, a.n, a.count, a.num_pages, st);
+  if (!a.check) return copy_pages(a.tensors, a.n_tensors, a.src, a.dst, a.n, a.count, a.num_pages, TableMap{}, st);
   const size_t smem = (size_t)((a.num_pages + 31) / 32) * 3 * 4;
   int rc = allow_smem(pages_check_kernel, smem, "pages_check_kernel");
   if (rc) return rc;
@@ -558,7 +591,7 @@ int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st) {
   count_launch();
   rc = check_launch("pages_check_kernel");
   if (rc) return rc;
-  return copy_pages(a.tensors, a.n_tensors, a.list, a.list + a.n, a.n, nullptr, a.num_pages, st);
+  return copy_pages(a.tensors, a.n_tensors, a.list, a.list + a.n, a.n, nullptr, a.num_pages, TableMap{}, st);
 }
 
 int launch_draft_commit(const DashCommitArgs& a, cudaStream_t st) {
@@ -591,7 +624,10 @@ int launch_pages_fork(const DashPagesArgs& a, cudaStream_t st) {
   if (rc) return rc;
   pages_fork_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();
-  return check_launch("pages_fork_kernel");
+  const int rl = check_launch("pages_fork_kernel");
+  return rl || a.n_tensors == 0 ? rl
+                                : copy_pages(a.tensors, a.n_tensors, a.copy_src, a.copy_dst, a.n, nullptr,
+                                             a.pool.num_pages, TableMap{}, st);
 }
 
 int launch_pages_free(const DashPagesArgs& a, cudaStream_t st) {
@@ -611,7 +647,16 @@ int launch_pages_compact(const DashPagesArgs& a, cudaStream_t st) {
   if (rc) return rc;
   pages_compact_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();
-  return check_launch("pages_compact_kernel");
+  const int rl = check_launch("pages_compact_kernel");
+  if (rl) return rl;
+  // the data and the table's ids, in one launch (64 tensors each); a call without
+  // tensors still maps the table
+  const TableMap map = {a.pool.block_table, a.into.block_table, a.new_id, a.pool.bt_stride, a.into.bt_stride,
+                        a.pool.max_rows, a.pool.bt_width};
+  static const DashCacheTensor none = {};
+  return a.n_tensors ? copy_pages(a.tensors, a.n_tensors, a.copy_src, a.copy_dst, a.pool.num_pages / 2, a.n_moves,
+                                  a.pool.num_pages, map, st)
+                     : copy_pages(&none, 1, a.copy_src, a.copy_dst, 0, a.n_moves, a.pool.num_pages, map, st);
 }
 
 }  // namespace dash

@@ -90,16 +90,6 @@ def _layers(caches: Layers) -> CacheLayers:
     return caches if isinstance(caches, CacheLayers) else CacheLayers(caches)
 
 
-def _copy(layers: CacheLayers, src, dst, n, *, count=None, scratch=None, device_error=None) -> None:
-    a = L.DashPagesCopyArgs()
-    a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
-    a.n, a.src, a.dst, a.count = n, src, dst, count
-    a.num_pages = layers.num_pages
-    a.check, a.list = int(scratch is not None), _ptr(scratch)
-    a.device_error = device_error.ptr if device_error is not None else None
-    _call("dash_pages_copy", a, layers.index)
-
-
 def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
                device_error: Optional[DeviceErrorWord] = None) -> None:
     """Page ``src[i]`` -> page ``dst[i]`` in every cache tensor (int32 vectors; a
@@ -112,7 +102,12 @@ def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
     dst = _ints(dst, "dst", layers.index, n)
     if n:
         scratch = torch.empty(2 * n, dtype=torch.int32, device=layers.device)
-        _copy(layers, src.data_ptr(), dst.data_ptr(), n, scratch=scratch, device_error=device_error)
+        a = L.DashPagesCopyArgs()
+        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
+        a.n, a.src, a.dst = n, src.data_ptr(), dst.data_ptr()
+        a.num_pages, a.check, a.list = layers.num_pages, 1, scratch.data_ptr()
+        a.device_error = device_error.ptr if device_error is not None else None
+        _call("dash_pages_copy", a, layers.index)
 
 
 class PagePool:
@@ -201,8 +196,8 @@ class PagePool:
         a = self._args(dst, device_error)
         a.src, a.lens = src.data_ptr(), lens.data_ptr()
         a.copy_src, a.copy_dst = pairs.data_ptr(), pairs.data_ptr() + 4 * n
+        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
         _call("dash_pages_fork", a, self.index)
-        _copy(layers, a.copy_src, a.copy_dst, n)
 
     def compact(self, caches: Layers, into: Optional["PagePool"] = None,
                 device_error: Optional[DeviceErrorWord] = None) -> torch.Tensor:
@@ -214,13 +209,13 @@ class PagePool:
         layers, to = self._own(caches), self if into is None else into
         if to.device != self.device or to.block_size != self.block_size:
             raise ValueError("`into` must be a pool of the same device and block size")
-        half = self.c.num_pages // 2
-        buf = torch.empty(2 * half + 1, dtype=torch.int32, device=self.device)
+        P = self.c.num_pages
+        half = P // 2
+        buf = torch.empty(2 * half + P + 1, dtype=torch.int32, device=self.device)
         a = self._args(None, device_error)
         a.into = to.c
-        a.copy_src, a.copy_dst = buf.data_ptr(), buf.data_ptr() + 4 * half
-        a.n_moves = buf.data_ptr() + 8 * half
+        a.copy_src = at = buf.data_ptr()
+        a.copy_dst, a.new_id, a.n_moves = at + 4 * half, at + 8 * half, at + 8 * half + 4 * P
+        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
         _call("dash_pages_compact", a, self.index)
-        if half:
-            _copy(layers, a.copy_src, a.copy_dst, half, count=a.n_moves)
-        return buf[2 * half:]
+        return buf[2 * half + P:]

@@ -990,16 +990,18 @@ typedef struct {
  *                     pages without a holder go onto the stack in ascending order.
  * dash_pages_fork     dst[i] (an empty row) becomes a copy of the first lens[i]
  *                     tokens of row src[i]: full pages are shared, the last one,
- *                     if partly filled, is a page of its own; copy_src/dst[i] =
- *                     the pages to copy (-1: none), to be passed to
- *                     dash_pages_copy.  Pages are taken as by dash_pages_reserve.
+ *                     if partly filled, is copied to a page of its own in every
+ *                     tensor; copy_src/dst[i] = the pages copied (-1: none).  Pages
+ *                     are taken as by dash_pages_reserve.
  * dash_pages_compact  with L held pages, the k-th held page >= L moves to the
- *                     k-th unheld page < L: copy_src/dst[k] (k < *n_moves, num_pages
- *                     / 2 entries) list the moves (sources and targets are disjoint,
- *                     so the old tables stay valid until their pages are reused),
- *                     `into` receives the new ref, free_list (the lowest page on
- *                     top), n_free, block_table and n_blocks; into may be the pool
- *                     itself.                                               */
+ *                     k-th unheld page < L in every tensor: copy_src/dst[k] (k <
+ *                     *n_moves, num_pages / 2 entries) list the moves, new_id[p]
+ *                     (num_pages entries) is page p's new id.  Sources and targets
+ *                     are disjoint, so the old tables stay valid until their pages
+ *                     are reused.  `into` receives the new ref, free_list (the lowest
+ *                     page on top), n_free, block_table and n_blocks; into may be
+ *                     the pool itself.
+ * tensors (fork, compact): as for dash_pages_copy; n_tensors 0: tables only.  */
 typedef struct {
   DashPagePool pool;
   DashPagePool into;                /* compact */
@@ -1007,10 +1009,12 @@ typedef struct {
   const int32_t* src;               /* fork */
   const int32_t* lens;              /* reserve, fork: tokens; free: blocks kept or NULL */
   int32_t n;
-  int32_t pad0;
+  int32_t n_tensors;
+  const DashCacheTensor* tensors;   /* host */
   int32_t* copy_src;
   int32_t* copy_dst;
   int32_t* n_moves;
+  int32_t* new_id;
   DashDeviceError* device_error;
 } DashPagesArgs;
 int dash_pages_reserve(const DashPagesArgs* args, dash_stream_t stream);

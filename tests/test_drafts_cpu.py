@@ -179,7 +179,7 @@ def pages_args():
         p.ref = p.free_list = p.n_free = p.block_table = p.n_blocks = 1 << 16
         p.bt_stride = p.bt_width = 8
         p.num_pages, p.max_rows, p.block_size = 32, 4, 16
-    a.rows = a.src = a.lens = a.copy_src = a.copy_dst = a.n_moves = 1 << 16
+    a.rows = a.src = a.lens = a.copy_src = a.copy_dst = a.n_moves = a.new_id = 1 << 16
     a.n = 2
     return a
 

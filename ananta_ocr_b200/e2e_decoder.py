@@ -21,16 +21,24 @@ Attention per layer, all through libdash_b200:
   dash_sparse_attn*   paged prefill (tcgen05) / decode (split-KV) attention
 The GEMMs and the MoE are PyTorch (cuBLAS).  ``decode_step`` allocates nothing
 that changes between steps and is captured in a CUDA graph by the caller.
+
+``draft_step`` checks a tree of drafted tokens per sequence in one pass over the
+layers (speculative decoding, drafts.py), keeps a path of it and commits its cache
+entries.  With ``pool_pages`` the sequences draw their pages from a page_pool.PagePool
+instead of owning a fixed part of the cache; ``fork`` continues one sequence in
+another row, sharing its full pages when there is a pool.
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List
+from typing import List, Optional, Sequence
 
 import torch
 import torch.nn.functional as F
 
+from . import drafts
+from .page_pool import CacheLayers, PagePool, copy_pages
 from .unlimited_dash_ops import attend_triton as AT
 from .unlimited_dash_ops import decode_meta_triton as DM
 from .unlimited_dash_ops import index_frontend as IF
@@ -77,10 +85,11 @@ def rmsnorm(x, w, eps):
 
 class DashDecoder:
     """Random-init bf16 decoder with paged caches for ``batch`` sequences of
-    up to ``max_len`` tokens."""
+    up to ``max_len`` tokens.  ``pool_pages``: that many pages shared by the
+    sequences through a page pool (default: a fixed set for each)."""
 
     def __init__(self, cfg: DecoderConfig, batch: int, max_len: int, device, seed: int = 0,
-                 page_cfg=None, page_mask: bool = False):
+                 page_cfg=None, page_mask: bool = False, pool_pages: int = 0):
         self.cfg = c = cfg
         self.B = batch
         self.dev = device
@@ -121,10 +130,19 @@ class DashDecoder:
         P = batch * self.pps
         self.num_pages = P
         self.block_table = torch.randperm(P, generator=g, device=device).to(torch.int32).view(batch, self.pps).contiguous()
+        self.pool = None
+        self.rows = torch.arange(batch, dtype=torch.int32, device=device)
+        if pool_pages:
+            self.num_pages = P = pool_pages
+            self.pool = PagePool(P, batch, self.pps, bs, device)
+            self.block_table = self.pool.block_table
         self.kc = [torch.zeros(P, bs, c.kv_heads, c.head_dim, dtype=bf, device=device) for _ in range(c.layers)]
         self.vc = [torch.zeros_like(self.kc[0]) for _ in range(c.layers)]
         self.ic = [torch.zeros(P, bs, c.index_dim, device=device) for _ in range(c.layers)]
         self.kbar = [torch.zeros(P, c.index_dim, device=device) for _ in range(c.layers)]
+        # the caches of all layers: per token (commits), and with the k-bar rows (page copies)
+        self.token_caches = CacheLayers(self.kc + self.vc + self.ic)
+        self.page_caches = CacheLayers(self.kc + self.vc + self.ic + [k[:, None] for k in self.kbar])
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         inv = 1.0 / (c.rope_theta ** (torch.arange(0, c.head_dim // 2, device=device).float() / (c.head_dim // 2)))
         self.inv_freq = inv
@@ -216,8 +234,11 @@ class DashDecoder:
         req = torch.arange(B, device=dev).repeat_interleave(S)
         pos = torch.arange(S, device=dev).repeat(B)
         cos, sin = self.rope_tables(pos)
-        slots = self.slots_of(pos, req)
         self.seq_lens.fill_(S)
+        if self.pool is not None:
+            self.pool.free(self.rows)
+            self.pool.reserve(self.rows, self.seq_lens)
+        slots = self.slots_of(pos, req)
         cu = (torch.arange(B + 1, device=dev) * S).to(torch.int32)
         ctx = torch.zeros(B, dtype=torch.int32, device=dev)
         row2req = RT.prefill_row2req(cu_seqlens_q=cu, device=dev, total_q=T)
@@ -286,8 +307,10 @@ class DashDecoder:
         pos = self.seq_lens.long()
         req = torch.arange(B, device=dev)
         cos, sin = self.rope_tables(pos)
-        slots = self.slots_of(pos, req)
         sl = self.seq_lens + 1
+        if self.pool is not None:
+            self.pool.reserve(self.rows, sl)
+        slots = self.slots_of(pos, req)
         tail = RT.kbar_tail_plan(block_table=self.block_table, seq_lens=sl,
                                  block_size=c.block_size, tail_pages=1, device=dev)
         domain = allow = None
@@ -331,3 +354,118 @@ class DashDecoder:
         self.tok.copy_(logits.argmax(-1))
         self.seq_lens.add_(1)
         return logits
+
+    # ---------------------------------------------------------------- drafts
+    @torch.no_grad()
+    def draft_step(self, drafted: torch.Tensor, parents: Optional[torch.Tensor] = None, *,
+                   temperature: float = 0.0, draft_probs: Optional[torch.Tensor] = None,
+                   u_accept: Optional[torch.Tensor] = None, u_sample: Optional[torch.Tensor] = None):
+        """Checks drafted tokens [B, n - 1] (int64) behind ``self.tok`` at once.
+
+        With the root ``self.tok`` as token 0, ``parents`` [B, n] int32 gives each
+        token's parent (None: chains).  temperature 0 keeps the drafts that greedy
+        decoding would have chosen; otherwise the drafts are accepted against the
+        softmax of logits / temperature with the random numbers ``u_accept`` [B * n]
+        and ``u_sample`` [B] (``draft_probs`` [B * n, vocab]: the distributions that the
+        drafts were drawn from).  The kept tokens' cache entries are moved
+        together, the k-bar rows of their pages refreshed, ``self.seq_lens``
+        advanced by the kept tokens and the root, and ``self.tok`` becomes the
+        next token.  Returns (drafts.Verified, logits [B, n, vocab])."""
+        c = self.cfg
+        if self.pst is not None:
+            raise NotImplementedError("draft_step has no page-aware candidates (page state has no rewind)")
+        B, H, dev = self.B, c.hidden, self.tok.device
+        n = drafted.shape[1] + 1
+        if n - 1 > (c.local_blocks - 1) * c.block_size:
+            # a deeper token would route among blocks that hold drafts
+            raise ValueError(f"{n - 1} drafts reach past the local window's whole blocks "
+                             f"({(c.local_blocks - 1) * c.block_size} tokens)")
+        T = B * n
+        tokens = torch.cat([self.tok[:, None], drafted], 1).reshape(T)
+        if parents is not None:
+            parents = parents.to(torch.int32).reshape(T)
+        ctx = self.seq_lens
+        if self.pool is not None:
+            self.pool.reserve(self.rows, ctx + n)
+        cu = torch.arange(B + 1, dtype=torch.int32, device=dev) * n
+        plan = drafts.tree_plan(parents, cu, ctx, rows=T, max_nodes=n, block_table=self.block_table,
+                                block_size=c.block_size, num_pages=self.num_pages)
+        cos, sin = self.rope_tables(plan.row_pos)
+        table = self.block_table.index_select(0, plan.row_seq)          # a row per token, for the router
+        sl = plan.row_pos + 1
+        x = self.embed[tokens]
+        oi = torch.empty(T, c.slots, dtype=torch.int32, device=dev)
+        ob = torch.empty(T, c.slots, dtype=torch.float32, device=dev)
+        attn = torch.empty(T, c.heads, c.head_dim, dtype=torch.bfloat16, device=dev)
+        for li, L in enumerate(self.layers):
+            h = rmsnorm(x, L["ln1"], c.eps)
+            qkv = F.linear(h, L["wqkv"])
+            q, k, v = qkv[:, :H], qkv[:, H:2 * H], qkv[:, 2 * H:]
+            IF.rope_and_store_kv(q, k, v, cos, sin, self.kc[li], self.vc[li], plan.slots, c.head_dim)
+            idx_q, _ = IF.index_qk_fused(h, L["wiq"], L["wik"], L["niq"], L["nik"], c.eps, cos, sin,
+                                         index_cache=self.ic[li], slot_mapping=plan.slots)
+            RT.route_decode_triton(idx_q=idx_q, k_bar=self.kbar[li], block_table=table, seq_lens=sl,
+                                   image_allow=None, out_idx=oi, out_bias=ob, max_block=self.pps,
+                                   block_size=c.block_size, local_blocks=c.local_blocks, decode_query_len=1,
+                                   idx_scale=self.idx_scale, prior_floor=c.prior_floor, sigma=c.sigma,
+                                   topm=c.topm, budget=c.K, out_slots=c.slots)
+            drafts.dash_sparse_attn_tree(q.view(T, c.heads, c.head_dim), self.kc[li], self.vc[li],
+                                         oi[None].expand(c.kv_heads, T, c.slots),
+                                         ob[None].expand(c.kv_heads, T, c.slots), self.block_table, cu, ctx,
+                                         plan.row_pos, plan.mask, n, c.kv_heads, 1.0 / math.sqrt(c.head_dim), attn,
+                                         local_blocks=c.local_blocks, sparse_block_size=c.block_size)
+            x = x + F.linear(attn.view(T, H), L["wo"])
+            x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
+        logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
+        if temperature > 0:
+            target = (logits.float() / temperature).softmax(-1)
+            kept = drafts.verify_drafts(tokens, parents, cu, target, max_nodes=n, draft=draft_probs,
+                                        u_accept=u_accept, u_sample=u_sample)
+        else:
+            kept = drafts.verify_drafts(tokens, parents, cu, logits, max_nodes=n, greedy=True)
+        drafts.commit_drafts(self.token_caches, kept.path, kept.n_accept, ctx, self.block_table)
+        now = ctx + kept.n_accept + 1
+        fresh = RT.kbar_all_plan(block_table=self.block_table, seq_lens=now, context_lens=ctx,
+                                 block_size=c.block_size, max_block=self.pps, max_query_len=n, device=dev)
+        for li, L in enumerate(self.layers):
+            RT.kbar_refresh_tail_triton(kv_cache=self.ic[li], k_bar=self.kbar[li], block_table=self.block_table,
+                                        seq_lens=now, head_cls=L["head_cls"], block_size=c.block_size, plan=fresh)
+        self.seq_lens.copy_(now)
+        self.tok.copy_(kept.next_token)
+        if self.pool is not None:
+            # pages that only dropped drafts reached go back
+            self.pool.free(self.rows, (now + c.block_size - 1) // c.block_size)
+        return kept, logits.view(B, n, -1)
+
+    # ---------------------------------------------------------------- sequences
+    @torch.no_grad()
+    def fork(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Row ``dst[i]`` becomes a copy of row ``src[i]``: with a page pool full
+        pages are shared and the last one is copied, without one all pages of the
+        sequence are copied into the row's own."""
+        if self.pst is not None:
+            raise NotImplementedError("fork has no page-aware candidates")
+        dev = self.tok.device
+        if len(src) != len(dst) or len(set(dst)) != len(dst) or set(src) & set(dst) or \
+                not all(0 <= r < self.B for r in (*src, *dst)):
+            raise ValueError("fork takes distinct rows, none of them source and destination")
+        if not src:
+            return
+        s, d = (torch.tensor(list(x), dtype=torch.int32, device=dev) for x in (src, dst))
+        lens = self.seq_lens.index_select(0, s)
+        if self.pool is not None:
+            self.pool.free(d)
+            self.pool.fork(s, d, lens, self.page_caches)
+        else:
+            used = torch.arange(self.pps, device=dev) * self.cfg.block_size < lens[:, None]
+            pages = self.block_table.index_select(0, s).masked_fill(~used, -1)
+            copy_pages(self.page_caches, pages.reshape(-1), self.block_table.index_select(0, d).reshape(-1))
+        self.seq_lens.index_copy_(0, d.long(), lens)
+        self.tok.index_copy_(0, d.long(), self.tok.index_select(0, s))
+
+    @torch.no_grad()
+    def compact(self) -> None:
+        """Moves the pool's pages to the lowest ids."""
+        if self.pool is None:
+            raise ValueError("compact needs a page pool (pool_pages)")
+        self.pool.compact(self.page_caches)

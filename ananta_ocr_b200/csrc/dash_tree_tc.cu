@@ -60,11 +60,13 @@ constexpr float kGrow = 8.0f;                    // O is rescaled when a row's m
 template <int QR>
 struct TreeSmem {
   static constexpr int kKSlots = QR <= 64 ? 3 : 2, kVSlots = QR == 32 ? 3 : 2;
-  static constexpr int kCells = QR == 32 ? 1500 : QR == 64 ? 3456 : 3360;     // additive terms held at a time
+  static constexpr int kCells = QR == 32 ? 980 : QR == 64 ? 2900 : 2800;      // additive terms held at a time
+  static constexpr int kSlots = 512;             // routed slots held
   uint8_t q[2 * QR * 128];                       // two halves of 64 dims, swizzled
   uint8_t k[kKSlots][kSlot];                     // receives O (QR x 512 B) at the end
   uint8_t v[kVSlots][kSlot];
   int cell[kCells];
+  uint32_t slot[kSlots];                         // (first granule << 8) | granules
   uint32_t bits[kMaxWords];
   uint16_t before[kMaxWords + 2];
   int tok[8][4];                                 // first token of the tile's granules, -1 = none (K runs < 8 tiles ahead)
@@ -155,7 +157,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 template <typename T, int GR, int QR>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ DashTreeAttnArgs a, int n_tiles_seq) {
+                   const __grid_constant__ DashTreeAttnArgs a, int n_tiles_seq, int unit0) {
   constexpr int NG = kKeys / GR;                 // granules per tile
   using Smem = TreeSmem<QR>;
   constexpr int kKSlots = Smem::kKSlots, kVSlots = Smem::kVSlots;
@@ -164,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   cg::cluster_group cluster = cg::this_cluster();
   const int nsp = (int)cluster.num_blocks(), split = (int)cluster.block_rank();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int u = blockIdx.x / nsp;
+  int u = unit0 + blockIdx.x / nsp;
   const int tile_i = u % n_tiles_seq;
   u /= n_tiles_seq;
   const int hk = u % a.kv.n_kv_heads, s = u / a.kv.n_kv_heads;
@@ -197,21 +199,23 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t e = (int64_t)__ldg(a.row_pos + r) - a.local_window + 1;
     return (int)max((int64_t)0, min(e, (int64_t)ctx));
   };
-  // entry e = (token, slot of its list), lists padded to a power of two: the
-  // slot's remote keys from t0 on, in granules
+  // entry e = (token, slot of its list), lists padded to a power of two
   const int pad = K > 1 ? 32 - __clz(K - 1) : 0;
   const int entries = K > 0 ? nt << pad : 0;
-  auto remote = [&](int e, int& node, int& slot, int& t0) -> int {
-    node = e >> pad;
-    slot = e & ((1 << pad) - 1);
-    if (slot >= K) return 0;
-    const int b = __ldg(a.routes.idx + rbase + (int64_t)node * a.routes.row_stride + slot);
-    const int edge = min(window_of(r0 + node), live_end);
-    if (b < 0) return 0;
-    if (b >= nblk) { record_error(derr, DASH_DEV_BAD_BLOCK, 76, b); return 0; }
-    t0 = (int)min((int64_t)b * bs, (int64_t)ctx);
-    const int t1 = (int)min((int64_t)(b + 1) * bs, (int64_t)edge);
-    return t1 > t0 ? (t1 - t0 + GR - 1) / GR : 0;
+  // remote granules of block b for a row at position pos: (first << 8) | count
+  auto remote = [&](int b, int pos) -> uint32_t {
+    if (b >= nblk) record_error(derr, DASH_DEV_BAD_BLOCK, 76, b);
+    const int64_t e = (int64_t)pos - a.local_window + 1;
+    const int edge = (int)max((int64_t)0, min(e, (int64_t)min(ctx, live_end)));
+    const int64_t t0 = (int64_t)b * bs, t1 = min(t0 + bs, (int64_t)edge);
+    return b >= 0 && t1 > t0 ? (uint32_t)(t0 / GR) << 8 | (uint32_t)((t1 - t0 + GR - 1) / GR) : 0u;
+  };
+  // the same for entry e, from memory
+  auto remote_of = [&](int e) -> uint32_t {
+    const int node = e >> pad, slot = e & ((1 << pad) - 1);
+    return slot < K ? remote(__ldg(a.routes.idx + rbase + (int64_t)node * a.routes.row_stride + slot),
+                             __ldg(a.row_pos + r0 + node))
+                    : 0u;
   };
 
   // ---- setup ----
@@ -265,14 +269,31 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   // ---- the union ----
   if (warp < 4) {
-#pragma unroll 4
-    for (int e = tid; e < entries; e += kRows) {
-      int node, slot, t0 = 0;
-      const int n = remote(e, node, slot, t0);
-      // the biases are read next, by the same threads
-      if (n && a.routes.bias)
-        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.routes.bias + rbase + (int64_t)node * a.routes.row_stride + slot));
-      for (int g = t0 / GR, g1 = g + n; g < g1; ++g) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
+#pragma unroll 1
+    for (int e0 = tid; e0 < entries; e0 += 4 * kRows) {
+      int b[4], pos[4];                          // the loads of four entries at once
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kRows, node = e >> pad, slot = e & ((1 << pad) - 1);
+        b[i] = -1;
+        pos[i] = 0;
+        if (e < entries && slot < K) {
+          const int64_t at = rbase + (int64_t)node * a.routes.row_stride + slot;
+          b[i] = __ldg(a.routes.idx + at);
+          pos[i] = __ldg(a.row_pos + r0 + node);
+          // the biases are read next, by the same threads
+          if (a.routes.bias) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.routes.bias + at));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = e0 + i * kRows;
+        const uint32_t v = remote(b[i], pos[i]);
+        if (e < Smem::kSlots) S.slot[e] = v;
+        // (tokens of a tree name the same blocks: a set bit needs no atomic)
+        for (uint32_t g = v >> 8, g1 = g + (v & 255u); g < g1; ++g)
+          if (!((*(volatile uint32_t*)&S.bits[g >> 5] >> (g & 31)) & 1u)) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
+      }
     }
   } else if (warp == 5) {
     const int g0 = lo / GR, g1 = (live_end + GR - 1) / GR;        // [g0, g1): window and drafts
@@ -500,13 +521,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll 1
         for (int e = m; e < entries; e += kRows) {
-          int nd, slot, t0 = 0;
-          const int n = remote(e, nd, slot, t0);
-          if (n == 0) continue;
+          const uint32_t v = e < Smem::kSlots ? S.slot[e] : remote_of(e);
+          if (v == 0u) continue;
+          const int nd = e >> pad, slot = e & ((1 << pad) - 1);
           // a block's granules follow one another in the union
-          const int g = t0 / GR;
+          const int g = v >> 8;
           int rk = (int)S.before[g >> 5] + __popc(S.bits[g >> 5] & ((1u << (g & 31)) - 1u)) - rank0;
-          const int rk1 = min(rk + n, c1);
+          const int rk1 = min(rk + (int)(v & 255u), c1);
           float bias = 0.0f;
           if (pass && a.routes.bias)
             bias = __ldg(a.routes.bias + rbase + (int64_t)nd * a.routes.row_stride + slot) * kTreeLog2e;
@@ -555,11 +576,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         // V rows behind the last drafted token: P = 0 must not meet a NaN
         const int st = it % kVSlots;
         if (!tree_wait_warp(&S.vfull[st], (uint32_t)(it / kVSlots) & 1u, abort_flag, derr, 60)) alive = false;
+        // (16 threads per row of 256 bytes)
 #pragma unroll 1
-        for (int e = m; alive && e < kKeys * 16; e += nact * 32) {
-          const int row = e >> 4, ch = e & 15, t0 = S.tok[it & 7][row / GR];
-          if (t0 >= 0 && t0 + row % GR >= end)
-            *reinterpret_cast<uint4*>(S.v[st] + (ch >> 3) * 8192 + row * 128 + ((ch & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        for (int g = 0; alive && g < NG; ++g) {
+          const int t0 = S.tok[it & 7][g];
+          uint8_t* v = S.v[st] + ((m & 15) >> 3) * 8192 + g * GR * 128 + ((m & 7) << 4);
+          for (int q = t0 < 0 ? GR : max(0, end - t0) + (m >> 4); q < GR; q += nact * 2)
+            *reinterpret_cast<uint4*>(v + q * 128) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
@@ -742,6 +765,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       mk = *cluster.map_shared_rank(&S.m[m], lane);
       lk = *cluster.map_shared_rank(&S.l[m], lane);
     }
+    float4 o[8];                                 // all parts in flight
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < nsp)
+        o[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&S.k[0][0], k) + m * 512 + ((lane ^ (m & 7)) << 4));
     float M = mk;
 #pragma unroll
     for (int x = 4; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
@@ -751,14 +779,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float wk = mk == -INFINITY ? 0.0f : fast_exp2(mk - M);
     float L = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int k = 0; k < nsp; ++k) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
       const float w = __shfl_sync(0xffffffffu, wk, k), l1 = __shfl_sync(0xffffffffu, lk, k);
-      const float4 o =
-          *reinterpret_cast<const float4*>(cluster.map_shared_rank(&S.k[0][0], k) + m * 512 + ((lane ^ (m & 7)) << 4));
-      if (l1 != -1.0f) {
+      if (l1 != -1.0f) {                         // lanes k >= nsp hold -1
         L += l1 * w;
-        O.x += o.x * w; O.y += o.y * w; O.z += o.z * w; O.w += o.w * w;
+        O.x += o[k].x * w; O.y += o[k].y * w; O.z += o[k].z * w; O.w += o[k].w * w;
       }
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
@@ -817,26 +843,40 @@ static int page_map(CUtensorMap* map, const void* base, const DashTreeAttnArgs& 
   return DASH_OK;
 }
 
-// CTAs per unit.  A CTA costs about 10 us before and after its tiles; a tile takes
-// 0.95 us (its chain of S, softmax and P V), or what the memory gives: 1.49 us with
-// two CTAs on every SM.  Past one wave the last one is about half full.  (Measured, us,
-// 1 / 2 / 3 / 8 CTAs: 320 units of 37 tiles 103 / 101 / 102 / 151, 160 of 34
-// 51 / 64 / 57 / 89, 80 of 15 31 / 25 / 23 / 45, 10 of 20 29 / 23 / 21 / 17.)  The number of tiles
-// is not known here; the drafted tokens of a sequence route similar blocks: twice K are
-// assumed.
-static int tree_splits(const DashTreeAttnArgs& a, int64_t units) {
-  if (a.num_splits) return a.num_splits;
+// How the units are cut into CTAs: `whole` units of one CTA each, the rest of `sp` CTAs.
+struct TreeCut {
+  int64_t whole;
+  int sp;
+};
+
+// A CTA costs about 10 us before and after its tiles; a tile takes 0.95 us (its chain
+// of S, softmax and P V), or what the memory gives: 1.49 us with two CTAs on every SM.
+// Past one wave of CTAs the last one is about half full; full waves of whole units with a
+// launch of split ones behind them waste less where the units are long.  (Measured,
+// us, 1 / 2 / 3 / 8 CTAs per unit: 160 units of 34 tiles 49 / 64 / 56 / 85, 80 of 15
+// 31 / 23 / 21 / 41, 10 of 20 29 / 21 / 19 / 15; 320 of 37 100 / 97 / 99 / 151, as 296 whole
+// ones and 24 of 8 CTAs 84; 640 of 24 148 / 160 / 181 / 313, as 592 whole ones and 48 of 6 146.)
+// The number of tiles is not known here; the drafted tokens of a sequence route similar
+// blocks: twice K are assumed.
+static TreeCut tree_cut(const DashTreeAttnArgs& a, int64_t units) {
+  if (a.num_splits) return {0, a.num_splits};
   int64_t keys = (int64_t)(a.seqs.max_q_len == 1 ? 1 : 2) * a.routes.K * a.block_size + a.local_window + a.seqs.max_q_len;
   const int64_t most = (int64_t)a.bt_width * a.block_size;
   const double tiles = (double)((keys < most ? keys : most) + kKeys - 1) / kKeys;
-  int best = 1;
-  double least = 1e30;
-  for (int sp = 1; sp <= 8 && sp <= tiles; ++sp) {
-    const double waves = (double)units * sp / 296, tile = waves < 1 ? 1.49 * waves : 1.49;
-    const double own = 10.0 + tiles / sp * (tile > 0.95 ? tile : 0.95), t = own * (waves <= 1 ? 1.0 : waves + 0.5);
-    if (t < least) { least = t; best = sp; }
-  }
-  return best;
+  auto best = [&](int64_t n, int& sp) {
+    double least = 1e30;
+    for (int k = 1; k <= 8 && k <= tiles; ++k) {
+      const double waves = (double)n * k / 296, tile = waves < 1 ? 1.49 * waves : 1.49;
+      const double own = 10.0 + tiles / k * (tile > 0.95 ? tile : 0.95), t = own * (waves <= 1 ? 1.0 : waves + 0.5);
+      if (t < least) { least = t; sp = k; }
+    }
+    return least;
+  };
+  TreeCut one = {0, 1}, two = {units / 296 * 296, 1};
+  const double t1 = best(units, one.sp);
+  if (two.whole == 0 || two.whole == units) return one;
+  const double t2 = (double)(two.whole / 296) * (10.0 + tiles * 1.49) + best(units - two.whole, two.sp) + 3.0;
+  return t2 < t1 ? two : one;
 }
 
 template <typename T, int GR, int QR>
@@ -844,14 +884,17 @@ static int launch_tc(const DashTreeAttnArgs& a, const CUtensorMap& mk, const CUt
   const int per = kRows / (a.qo.n_heads / a.kv.n_kv_heads);
   const int n_tiles = (a.seqs.max_q_len + per - 1) / per;
   const int64_t units = (int64_t)a.seqs.n_seq * a.kv.n_kv_heads * n_tiles;
-  const int sp = tree_splits(a, units);
-  if (units * sp > INT32_MAX) return set_error(DASH_ERR_UNSUPPORTED, "too many sequences x kv heads");
+  const TreeCut cut = tree_cut(a, units);
+  if (units * cut.sp > INT32_MAX) return set_error(DASH_ERR_UNSUPPORTED, "too many sequences x kv heads");
   const int smem = (int)sizeof(TreeSmem<QR>) + 1024;
   auto kernel = tree_tc_kernel<T, GR, QR>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e == cudaSuccess) {
+  for (int part = 0; part < 2 && e == cudaSuccess; ++part) {
+    const int64_t n = part == 0 ? cut.whole : units - cut.whole;
+    if (n == 0) continue;
+    const int sp = part == 0 ? 1 : cut.sp;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * sp));
+    cfg.gridDim = dim3((unsigned)(n * sp));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -861,10 +904,10 @@ static int launch_tc(const DashTreeAttnArgs& a, const CUtensorMap& mk, const CUt
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, n_tiles);
+    e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, n_tiles, part == 0 ? 0 : (int)cut.whole);
+    count_launch();
   }
   if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "tree_tc_kernel launch failed: %s", cudaGetErrorString(e));
-  count_launch();
   return check_launch("tree_tc_kernel");
 }
 

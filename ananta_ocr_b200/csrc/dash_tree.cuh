@@ -28,7 +28,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const int32_t* q_start, const int32_
   TreeSeq t;
   const int a = q_start[s];
   t.row0 = a;
-  t.n = max(0, min(min(q_start[s + 1], rows) - a, max_nodes));
+  t.n = a < 0 ? 0 : max(0, min(min(q_start[s + 1], rows) - a, max_nodes));
   t.ctx = min(max(0, ctx_len[s]), INT32_MAX / 2);
   return t;
 }

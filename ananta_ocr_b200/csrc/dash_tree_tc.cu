@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int nblk = (end + bs - 1) / bs;
   volatile int* abort_flag = &S.abort_flag;
   constexpr int kNone = (int)0xff800000u;        // -inf, below every slot's key
-  constexpr int kKey = 0x40000000;
+  constexpr int kKey = 0x7ffffffe;               // slots as keys: NaNs that no product has
 
   // first key of a row's window
   auto window_of = [&](int64_t r) -> int {
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     // The additive terms of granules [c0, c1) of this CTA's part, -inf where no slot
     // of the token names the block: the lowest slot that names a cell wins it (pass
-    // 0; slots as large positive keys, above -inf's bits), then leaves its bias there
+    // 0; slots as keys above -inf's bits that no bias equals), then leaves its bias there
     // (pass 1).  By all four warps.
     const int cap = Smem::kCells / nt / NG * NG;
     int c0 = 0, c1 = 0;

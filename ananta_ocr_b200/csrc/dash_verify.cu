@@ -86,8 +86,10 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const __grid_con
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int s = blockIdx.x / C;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  // the other CTAs' shared memory is written once they run: waited for in the first pass
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int r0 = a.q_start[s];
-  const int n = max(0, min(min(a.q_start[s + 1], a.rows) - r0, a.max_nodes));
+  const int n = r0 < 0 ? 0 : max(0, min(min(a.q_start[s + 1], a.rows) - r0, a.max_nodes));
   if (tid == 0 && rank == 0 && a.q_start[s + 1] - r0 > a.max_nodes)
     record_error(a.device_error, DASH_DEV_BAD_TREE, 80, a.q_start[s + 1] - r0);
   const T* target = reinterpret_cast<const T*>(a.target);
@@ -119,6 +121,9 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const __grid_con
   const int64_t v0 = min((int64_t)V, (rank * warps + warp) * per), v1 = min((int64_t)V, v0 + per);
 
   int cur = 0, kept = 0, n_rej = 0, pass = 0;
+  auto wait_started = [&]() {
+    if (pass == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  };
   double c = 0.0, W = 1.0;
   // the residual of element v (probabilities as stored, 64-bit arithmetic)
   auto residual = [&](int64_t v, double r, double q, int rej) -> double {
@@ -168,6 +173,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const __grid_con
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if (lane == 0) S.part[warp] = acc;
+    wait_started();
     __syncthreads();
     if (warp == 0 && lane < C) {
       double t = 0.0;
@@ -193,6 +199,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const __grid_con
       best = k > best ? k : best;
     }
     if (lane == 0) S.wkey[warp] = best;
+    wait_started();
     __syncthreads();
     if (warp == 0 && lane < C) {
       best = 0;
@@ -346,6 +353,7 @@ __global__ void __launch_bounds__(kVerThreads, 2) verify_kernel(const __grid_con
       }
     }
   }
+  wait_started();                      // no drafted token, no pass
   if (rank == 0) {
     __syncthreads();
     if (tid == 0) {

@@ -96,6 +96,20 @@ def test_repeated_ids_and_index_heads():
     check(t, *attend(t))
 
 
+def test_repeated_ids_with_biases_near_log4():
+    """The first of repeated ids counts whatever its bias is: in units of log2
+    these lie around 2.0, bit by bit from 16 units in the last place below to
+    above (a table entry that marked slots by such values would be taken twice)."""
+    t = make_tree(12, [32], [3000], H=1, Hkv=1, bs=64, window=1, K=12)
+    near = np.float32(np.log(4.0)).view(np.int32)
+    t["bias"][0] = -5.0
+    for r in range(32):
+        t["idx"][0, r, 1:] = t["idx"][0, r, 0]
+        t["bias"][0, r, 0] = (near - 24 + r).astype(np.int32).view(np.float32)
+    t["t_bias"], t["t_idx"] = torch.from_numpy(t["bias"]), torch.from_numpy(t["idx"])
+    check(t, *attend(t))
+
+
 def test_large_logits():
     """Rows whose logits span hundreds: the running maximum has to move."""
     t = make_tree(6, [16, 5], [900, 700], H=4, Hkv=2, bs=64, window=2, K=8, scale_q=30.0)

@@ -612,6 +612,9 @@ int dash_draft_commit(const DashCommitArgs* a, dash_stream_t stream) {
   if (a->block_size <= 0 || a->bt_width <= 0 || a->num_pages <= 0)
     return set_error(DASH_ERR_INVALID, "block_size, bt_width and num_pages must be > 0");
   rc = check_tensors(a->tensors, a->n_tensors, a->block_size);
+  for (int i = 0; i < a->n_tensors && !rc; ++i)
+    if (a->tensors[i].tok_bytes > (1 << 24))
+      rc = set_error(DASH_ERR_UNSUPPORTED, "cache tensor %d: tokens above 16 MiB", i);
   if (rc || a->n_seq == 0 || a->n_tensors == 0) return rc;
   if (!a->path || !a->n_accept || !a->ctx_len || !a->block_table) return set_error(DASH_ERR_INVALID, "null pointer");
   if (a->path_stride < a->max_nodes || a->bt_stride < a->bt_width)

@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kCommitThreads) draft_commit_kernel(const __gr
   const int32_t* bt = a.block_table + (int64_t)s * a.bt_stride;
   for (int i = threadIdx.x + 1; i <= acc; i += kCommitThreads) {
     const int p = path[i], q = i > 1 ? path[i - 1] : 0;
-    if (p <= q || p >= a.max_nodes || ctx < 0) {
+    if (p <= q || p >= a.max_nodes || ctx < 0 || ctx > INT32_MAX - kCommitNodes) {
       if (blockIdx.x == 0) record_error(a.device_error, DASH_DEV_BAD_TREE, 92, p);
       atomicMin(&s_n, i - 1);
       continue;
@@ -271,6 +271,11 @@ __device__ void first_requests(int* first, const int32_t* rows, int n, int max_r
   __syncthreads();
 }
 
+// a row's blocks, inside the table's row
+__device__ __forceinline__ int held_blocks(const DashPagePool& p, int row) {
+  return min(max(p.n_blocks[row], 0), p.bt_width);
+}
+
 // page popped as the k-th of this call, or -1 when the stack does not hold it
 __device__ __forceinline__ int pop_page(const DashPagePool& p, int n_free, int k) {
   const int at = n_free - 1 - k;
@@ -300,8 +305,9 @@ __global__ void __launch_bounds__(kPoolThreads) pages_reserve_kernel(const DashP
         record_error(a.device_error, DASH_DEV_BAD_ROW, 94, row);
         row = -1;
       } else {
-        have = p.n_blocks[row];
-        add = max(0, (int)((len + (int64_t)p.block_size - 1) / p.block_size) - have);
+        have = held_blocks(p, row);
+        // (more than all pages is one too many, so that the sums stay small)
+        add = min(max(0, (int)((len + (int64_t)p.block_size - 1) / p.block_size) - have), p.num_pages + 1);
       }
     }
     int total;
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_reserve_kernel(const DashP
     int given;
     block_scan(got ? add : 0, s_warp, given);      // also orders s_req
     used += given;
-    taken += total;
+    taken = min(taken + total, p.num_pages + 1);
     // a warp per request writes its pages
     for (int u = threadIdx.x >> 5; u < min(kPoolThreads, a.n - i0); u += kPoolThreads / 32) {
       const int4 rq = s_req[u];
@@ -351,7 +357,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_kernel(const DashPage
       // depends on another's row
       const bool ok = dst >= 0 && dst < p.max_rows && s_first[dst] == i && src >= 0 && src < p.max_rows &&
                       len >= 0 && s_first[src] == INT32_MAX && p.n_blocks[dst] == 0 &&
-                      (len + (int64_t)bs - 1) / bs <= p.n_blocks[src];
+                      (len + (int64_t)bs - 1) / bs <= held_blocks(p, src);
       if (!ok) {
         record_error(a.device_error, DASH_DEV_BAD_ROW, 96, dst);
         dst = -1;
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_free_kernel(const DashPage
       if (lane == 0) record_error(a.device_error, DASH_DEV_BAD_ROW, 98, row);
       continue;
     }
-    const int have = min(p.n_blocks[row], p.bt_width);
+    const int have = held_blocks(p, row);
     for (int b = keep + lane; b < have; b += 32) {
       int32_t* e = p.block_table + (int64_t)row * p.bt_stride + b;
       const int page = *e;

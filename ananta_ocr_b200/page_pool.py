@@ -75,6 +75,8 @@ class CacheLayers:
                 if t.shape[k] != 1 and t.stride(k) != inner:
                     raise ValueError("a token's entry must be contiguous")
                 inner *= t.shape[k]
+            if inner * e > 1 << 30:
+                raise ValueError("entries above 1 GiB are not supported")
             d.base, d.tok_bytes, d.page_toks = t.data_ptr(), inner * e, t.shape[1]
             d.tok_stride = inner * e if d.page_toks == 1 else t.stride(1) * e
             d.page_stride = t.stride(0) * e if self.num_pages > 1 else d.page_toks * d.tok_stride

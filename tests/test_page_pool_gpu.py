@@ -126,6 +126,34 @@ def test_pool_largest_sizes():
     assert torch.equal(pool.free_list[:P - held], torch.arange(P - 1, held - 1, -1, dtype=torch.int32, device="cuda"))
 
 
+def test_requests_whose_sum_passes_32_bits():
+    """8192 rows that ask for 2^18 + 64 pages each: 2^31 pages and more in sum,
+    none of which fits; a request that fits comes first."""
+    W = 2 ** 18 + 64
+    pool = PagePool(16, 8192, W, 1)
+    err = ops.DeviceErrorWord("cuda")
+    pool.reserve(i32([5]), i32([3]))
+    rows = torch.arange(8192, dtype=torch.int32, device="cuda")
+    pool.reserve(rows, torch.full_like(rows, W), err)
+    assert err.read()[0] == L.DASH_DEV_NO_PAGE
+    assert pool.n_free.item() == 13 and pool.n_blocks.sum().item() == 3 and pool.ref.sum().item() == 3
+    assert pool.free_list.tolist() == list(range(15, 2, -1)) + [-1] * 3
+
+
+def test_block_counts_outside_the_table():
+    """Counts that no call of the pool leaves (below 0, past the table) stay inside it."""
+    pool = PagePool(16, 4, 4, 1)
+    pool.n_blocks.copy_(i32([-5, 9, 0, 0]))
+    pool.reserve(i32([0]), i32([2]))
+    assert pool.block_table.tolist()[0] == [0, 1, -1, -1] and pool.n_blocks[0].item() == 2
+    t = torch.zeros(16, 1, 4, device="cuda")
+    err = ops.DeviceErrorWord("cuda")
+    pool.fork(i32([1]), i32([2]), i32([7]), [t], err)
+    assert err.read()[0] == L.DASH_DEV_BAD_ROW and pool.n_blocks.tolist() == [2, 9, 0, 0]
+    pool.free(i32([1, 0]))
+    assert pool.n_free.item() == 16 and pool.n_blocks.tolist() == [0, 0, 0, 0]
+
+
 def test_fork_copies_the_last_page_in_every_tensor():
     P, bs = 30, 16
     ts = caches(P, bs)
@@ -237,6 +265,13 @@ def test_commit_stops_at_a_bad_path():
         drafts.commit_drafts([t, torch.zeros(P, 1, 4, device="cuda")], i32([[0]]), i32([0]), i32([0]), bt)
     with pytest.raises(ValueError, match="path"):
         drafts.commit_drafts([t], i32([[0]]).long(), i32([0]), i32([0]), bt)
+
+
+def test_commit_behind_the_last_token_of_32_bits():
+    t = torch.arange(64, device="cuda", dtype=torch.float32).view(4, 4, 4)
+    want, err = t.clone(), ops.DeviceErrorWord("cuda")
+    drafts.commit_drafts([t], i32([[0, 2, 3, -1]]), i32([2]), i32([2 ** 31 - 2]), i32([[0, 1, 2, 3]]), err)
+    assert err.read()[0] == L.DASH_DEV_BAD_TREE and torch.equal(t, want)
 
 
 def test_graph_of_a_pool_step():

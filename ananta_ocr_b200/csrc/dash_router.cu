@@ -103,14 +103,14 @@ __host__ __device__ inline size_t kbar_pool_smem_floats(int block_size, int d) {
 }
 
 // Plan entry i of a paged pool: false when it is not a page slot (ntok <= 0,
-// route_triton.py:69-72).
+// route_triton.py:69-72) or its block has no page (a table entry below 0).
 __device__ __forceinline__ bool kbar_paged_entry(const DashKbarArgs& a, int i, int& n, int64_t& base,
                                                  int64_t& out_row) {
   n = a.ntok[i];
-  if (n <= 0) return false;
-  if (n > a.block_size) n = a.block_size;
-  base = a.pages[i] * a.page_stride;
   out_row = a.pages[i];
+  if (n <= 0 || out_row < 0) return false;
+  if (n > a.block_size) n = a.block_size;
+  base = out_row * a.page_stride;
   return true;
 }
 

@@ -26,7 +26,10 @@ that changes between steps and is captured in a CUDA graph by the caller.
 layers (speculative decoding, drafts.py), keeps a path of it and commits its cache
 entries.  With ``pool_pages`` the sequences draw their pages from a page_pool.PagePool
 instead of owning a fixed part of the cache; ``fork`` continues one sequence in
-another row, sharing its full pages when there is a pool.
+another row, sharing its full pages when there is a pool.  Nothing waits for the
+GPU: a row that got no page (the pool is empty, drafts pass ``max_len``) or a
+malformed tree is recorded in ``errors``; the row's tokens mean nothing from
+there on, other rows are not touched.
 """
 from __future__ import annotations
 
@@ -38,6 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from . import drafts
+from .ops import DeviceErrorWord
 from .page_pool import CacheLayers, PagePool, copy_pages
 from .unlimited_dash_ops import attend_triton as AT
 from .unlimited_dash_ops import decode_meta_triton as DM
@@ -131,6 +135,7 @@ class DashDecoder:
         self.num_pages = P
         self.block_table = torch.randperm(P, generator=g, device=device).to(torch.int32).view(batch, self.pps).contiguous()
         self.pool = None
+        self.errors = DeviceErrorWord(device)
         self.rows = torch.arange(batch, dtype=torch.int32, device=device)
         if pool_pages:
             self.num_pages = P = pool_pages
@@ -236,8 +241,11 @@ class DashDecoder:
         cos, sin = self.rope_tables(pos)
         self.seq_lens.fill_(S)
         if self.pool is not None:
+            pages = -(-S // c.block_size)
+            if pages > self.pps or B * pages > self.num_pages:
+                raise ValueError(f"{B} sequences of {S} tokens do not fit {self.num_pages} pages, {self.pps} each")
             self.pool.free(self.rows)
-            self.pool.reserve(self.rows, self.seq_lens)
+            self.pool.reserve(self.rows, self.seq_lens, self.errors)
         slots = self.slots_of(pos, req)
         cu = (torch.arange(B + 1, device=dev) * S).to(torch.int32)
         ctx = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -309,7 +317,7 @@ class DashDecoder:
         cos, sin = self.rope_tables(pos)
         sl = self.seq_lens + 1
         if self.pool is not None:
-            self.pool.reserve(self.rows, sl)
+            self.pool.reserve(self.rows, sl, self.errors)
         slots = self.slots_of(pos, req)
         tail = RT.kbar_tail_plan(block_table=self.block_table, seq_lens=sl,
                                  block_size=c.block_size, tail_pages=1, device=dev)
@@ -386,10 +394,10 @@ class DashDecoder:
             parents = parents.to(torch.int32).reshape(T)
         ctx = self.seq_lens
         if self.pool is not None:
-            self.pool.reserve(self.rows, ctx + n)
+            self.pool.reserve(self.rows, ctx + n, self.errors)
         cu = torch.arange(B + 1, dtype=torch.int32, device=dev) * n
         plan = drafts.tree_plan(parents, cu, ctx, rows=T, max_nodes=n, block_table=self.block_table,
-                                block_size=c.block_size, num_pages=self.num_pages)
+                                block_size=c.block_size, num_pages=self.num_pages, device_error=self.errors)
         cos, sin = self.rope_tables(plan.row_pos)
         table = self.block_table.index_select(0, plan.row_seq)          # a row per token, for the router
         sl = plan.row_pos + 1
@@ -413,17 +421,18 @@ class DashDecoder:
                                          oi[None].expand(c.kv_heads, T, c.slots),
                                          ob[None].expand(c.kv_heads, T, c.slots), self.block_table, cu, ctx,
                                          plan.row_pos, plan.mask, n, c.kv_heads, 1.0 / math.sqrt(c.head_dim), attn,
-                                         local_blocks=c.local_blocks, sparse_block_size=c.block_size)
+                                         local_blocks=c.local_blocks, sparse_block_size=c.block_size,
+                                         device_error=self.errors)
             x = x + F.linear(attn.view(T, H), L["wo"])
             x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
         logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
         if temperature > 0:
             target = (logits.float() / temperature).softmax(-1)
             kept = drafts.verify_drafts(tokens, parents, cu, target, max_nodes=n, draft=draft_probs,
-                                        u_accept=u_accept, u_sample=u_sample)
+                                        u_accept=u_accept, u_sample=u_sample, device_error=self.errors)
         else:
-            kept = drafts.verify_drafts(tokens, parents, cu, logits, max_nodes=n, greedy=True)
-        drafts.commit_drafts(self.token_caches, kept.path, kept.n_accept, ctx, self.block_table)
+            kept = drafts.verify_drafts(tokens, parents, cu, logits, max_nodes=n, greedy=True, device_error=self.errors)
+        drafts.commit_drafts(self.token_caches, kept.path, kept.n_accept, ctx, self.block_table, self.errors)
         now = ctx + kept.n_accept + 1
         fresh = RT.kbar_all_plan(block_table=self.block_table, seq_lens=now, context_lens=ctx,
                                  block_size=c.block_size, max_block=self.pps, max_query_len=n, device=dev)
@@ -455,7 +464,7 @@ class DashDecoder:
         lens = self.seq_lens.index_select(0, s)
         if self.pool is not None:
             self.pool.free(d)
-            self.pool.fork(s, d, lens, self.page_caches)
+            self.pool.fork(s, d, lens, self.page_caches, self.errors)
         else:
             used = torch.arange(self.pps, device=dev) * self.cfg.block_size < lens[:, None]
             pages = self.block_table.index_select(0, s).masked_fill(~used, -1)

@@ -15,6 +15,7 @@ import numpy as np
 import pytest
 import torch
 
+from ananta_ocr_b200 import _lib as L
 from ananta_ocr_b200.e2e_decoder import DashDecoder, DecoderConfig
 from oracle import draft_oracle as DO
 
@@ -200,6 +201,45 @@ def test_fork_continues_as_its_source(pool):
         dec.fork([0], [0])
     with pytest.raises(ValueError):
         dec.fork([0], [4])
+
+
+def test_no_page_left():
+    """A pool without a page for a row: recorded, and the other row goes on as
+    it would alone (bit for bit: the same rows in the same batch)."""
+    cfg, S = CFGS["bs32"], 64                              # two full pages each
+    ids = ids_of(S, 12)
+    rich, poor = make(cfg, pool_pages=12), make(cfg, pool_pages=5)
+    with pytest.raises(ValueError, match="do not fit"):
+        poor.prefill(poor.embed[ids_of(81, 1)])
+    for d in (rich, poor):
+        d.prefill(d.embed[ids])
+        d.tok.fill_(5)
+        guard = [k.clone() for k in d.kbar]
+    for step in range(3):
+        if step < 2:
+            a, b = (d.decode_step() for d in (rich, poor))
+        else:
+            x = ids_of(3, 13)
+            a, b = (d.draft_step(x)[1] for d in (rich, poor))
+        assert torch.equal(a[0], b[0]), step
+        assert rich.errors.read()[0] == 0 and poor.errors.read()[0] == L.DASH_DEV_NO_PAGE
+    assert poor.block_table[1, 2].item() == -1 and poor.pool.n_free.item() == 0
+    held = poor.block_table[1, :2].long()
+    for k, g in zip(poor.kbar, guard):
+        assert torch.equal(k[held], g[held])
+
+
+def test_a_root_alone():
+    """draft_step without drafts is a decode step."""
+    cfg, ids = CFGS["bs64"], ids_of(100, 14)
+    a, b = make(cfg), make(cfg, pool_pages=12)
+    for d in (a, b):
+        d.prefill(d.embed[ids])
+        d.tok.fill_(9)
+    one = a.decode_step()
+    kept, logits = b.draft_step(torch.zeros(2, 0, dtype=torch.int64, device="cuda"))
+    assert off(logits[:, 0], one) <= 0.1 and kept.n_accept.tolist() == [0, 0]
+    assert torch.equal(b.tok, logits[:, 0].argmax(-1)) and b.seq_lens.tolist() == [101, 101]
 
 
 def test_draft_step_refusals():

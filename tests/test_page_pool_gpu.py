@@ -274,6 +274,13 @@ def test_commit_behind_the_last_token_of_32_bits():
     assert err.read()[0] == L.DASH_DEV_BAD_TREE and torch.equal(t, want)
 
 
+def test_kbar_of_a_block_without_a_page():
+    """A plan entry below 0 writes no row (row -1 lies inside the tensors here)."""
+    cache, kbar = torch.ones(5, 16, 128, device="cuda")[1:], torch.zeros(5, 128, device="cuda")
+    ops.kbar_pool_paged(cache, torch.tensor([2, -1], device="cuda"), i32([16, 16]), None, kbar[1:])
+    assert (kbar[[0, 1, 2, 4]] == 0).all() and (kbar[3] != 0).any()
+
+
 def test_graph_of_a_pool_step():
     """free + fork + compact captured once and replayed: the tables of three
     eager steps."""

@@ -16,7 +16,6 @@ every non-zero library status raises.
 """
 from __future__ import annotations
 
-import ctypes
 from dataclasses import dataclass
 from typing import Optional
 
@@ -95,77 +94,79 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     from ``cu_seqlens_q[-1]`` on are left as they were.  lse [rows, H] fp32:
     natural-log sums.  num_splits: CTAs per sequence and kv head (0 = automatic)."""
     index, dt = q.get_device(), q.dtype
-    ks, kst = k_cache.shape, k_cache.stride()
+    qs, ks, ts, ms = q.shape, k_cache.shape, topk_idx.shape, tree_mask.shape
+    qst, kst, ist = q.stride(), k_cache.stride(), topk_idx.stride()
     # the usual call passes one test; what is wrong with any other is said below
-    if not (q.dim() == 3 == topk_idx.dim() and len(ks) == 4 and output.shape == q.shape and
+    if not (len(qs) == 3 == len(ts) and len(ks) == 4 and output.shape == qs and
             ks == v_cache.shape and kst == v_cache.stride() and
-            tuple(ks[1:]) == (sparse_block_size, num_kv_heads, q.shape[2]) and
+            ks[1] == sparse_block_size and ks[2] == num_kv_heads and ks[3] == qs[2] and
             dt is k_cache.dtype is v_cache.dtype is output.dtype and
             index == k_cache.get_device() == v_cache.get_device() == output.get_device() ==
             topk_idx.get_device() == tree_mask.get_device() and index >= 0):
         _refuse_tree(q, k_cache, v_cache, output, topk_idx, tree_mask, sparse_block_size, num_kv_heads)
-    rows, H, _ = q.shape
+    rows, H, D = qs
     if rows == 0:
         return
-    qst, ost, mst, ist = q.stride(), output.stride(), tree_mask.stride(), topk_idx.stride()
+    ost = output.stride()
     if qst[2] != 1 or ost[2] != 1 or kst[3] != 1:
         raise ValueError("q, output and the caches must have a unit inner stride")
-    K = topk_idx.shape[2]
-    if topk_idx.shape[0] != num_kv_heads or topk_idx.shape[1] != rows:
+    HI, trows, K = ts
+    if HI != num_kv_heads or trows != rows:
         raise ValueError(f"topk_idx must be [{num_kv_heads}, {rows}, K]")
-    if tree_mask.dtype is not torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] != rows or \
-            (tree_mask.shape[1] > 1 and mst[1] != 1):
+    mst = tree_mask.stride()
+    if tree_mask.dtype is not torch.int32 or len(ms) != 2 or ms[0] != rows or (ms[1] > 1 and mst[1] != 1):
         raise ValueError(f"tree_mask must be int32 [{rows}, words]")
     cu = _ints(cu_seqlens_q, "cu_seqlens_q", index)
-    n_seq = cu.shape[0] - 1
+    n_seq = cu.numel() - 1
     ctx = _ints(ctx_lens, "ctx_lens", index, n_seq)
     pos = _ints(row_pos, "row_pos", index, rows)
     bt = _table(block_table, index, n_seq)
     if n_seq == 0:
         return
-    a = L.DashTreeAttnArgs()
-    sq, kv, ro, qo = a.seqs, a.kv, a.routes, a.qo
-    sq.n_seq, sq.q_len_fixed, sq.max_q_len, sq.q_start = n_seq, rows, max_nodes, cu.data_ptr()
-    kv.k, kv.v, kv.dtype = k_cache.data_ptr(), v_cache.data_ptr(), ops._DT.get(dt, -1)
-    kv.n_kv_heads, kv.head_dim = num_kv_heads, ks[3]
-    kv.stride_seq, kv.stride_tok, kv.stride_head, _ = kst
-    kv.block_table, kv.bt_stride, kv.num_pages = bt.data_ptr(), bt.stride(0), ks[0]
+    idx = bias = 0
     if blk_bias is not None:
-        if blk_bias.shape != topk_idx.shape or blk_bias.dtype is not torch.float32 or blk_bias.get_device() != index:
+        if blk_bias.shape != ts or blk_bias.dtype is not torch.float32 or blk_bias.get_device() != index:
             raise ValueError(f"blk_bias must be fp32 of topk_idx's shape on cuda:{index}")
+    one = ist[0] == 0 or num_kv_heads == 1        # a router head that all kv heads share
     if K:
         if topk_idx.dtype is not torch.int32 or ist[2] != 1 or (blk_bias is not None and blk_bias.stride() != ist):
-            # one layout for both; a router head that all kv heads share is kept once
-            one = ist[0] == 0 or num_kv_heads == 1
+            # one layout for both; a shared router head is kept once
             topk_idx = (topk_idx[:1] if one else topk_idx).to(torch.int32).contiguous()
             if blk_bias is not None:
                 blk_bias = (blk_bias[:1] if one else blk_bias).contiguous()
-            ist = (0 if one else topk_idx.stride(0),) + topk_idx.stride()[1:]
-        one = ist[0] == 0 or num_kv_heads == 1
-        ro.idx, ro.K, ro.row_stride = topk_idx.data_ptr(), K, ist[1]
-        ro.n_index_heads, ro.ihead_stride = (1, 0) if one else (num_kv_heads, ist[0])
+            ist = topk_idx.stride()
+        idx = topk_idx.data_ptr()
         if blk_bias is not None:
-            ro.bias = blk_bias.data_ptr()
-    qo.q, qo.out, qo.n_heads = q.data_ptr(), output.data_ptr(), H
-    qo.q_stride_tok, qo.q_stride_head = qst[0], qst[1]
-    qo.o_stride_tok, qo.o_stride_head = ost[0], ost[1]
+            bias = blk_bias.data_ptr()
+    z, zst = 0, (0, 0)
     if lse is not None:
         if lse.shape != (rows, H) or lse.dtype is not torch.float32 or lse.get_device() != index:
             raise ValueError(f"lse must be fp32 [{rows}, {H}] on cuda:{index}")
-        qo.lse = lse.data_ptr()
-        qo.lse_stride_tok, qo.lse_stride_head = lse.stride()
-    a.ctx_len, a.row_pos, a.mask = ctx.data_ptr(), pos.data_ptr(), tree_mask.data_ptr()
-    a.mask_stride, a.mask_words, a.bt_width = mst[0], tree_mask.shape[1], bt.shape[1]
-    a.scale, a.block_size = sm_scale, sparse_block_size
-    a.local_window, a.num_splits = local_blocks * sparse_block_size, num_splits
-    if device_error is not None:
-        a.device_error = device_error.ptr
-    _call("dash_tree_attn", a, index)
+        z, zst = lse.data_ptr(), lse.stride()
+    _call("dash_tree_attn", _TREE(
+        # seqs: n_seq, q_len_fixed (all rows), kv_len_fixed, max_q_len, q_start, pos0, kv_len
+        n_seq, rows, 0, max_nodes, cu.data_ptr(), 0, 0,
+        # kv: k, v, dtype, n_kv_heads, head_dim, pad, strides of a page, a token, a head, table, its stride, num_pages
+        k_cache.data_ptr(), v_cache.data_ptr(), ops._DT.get(dt, -1), num_kv_heads, D, 0, kst[0], kst[1], kst[2],
+        bt.data_ptr(), bt.stride(0), ks[0],
+        # routes: idx, bias, row_stride, ihead_stride, K, n_index_heads
+        idx, bias, ist[1], 0 if one else ist[0], K, 1 if one else num_kv_heads,
+        # qo: q, out, q strides, out strides (sequence, token, head), n_heads, pad, lse, its strides
+        q.data_ptr(), output.data_ptr(), 0, qst[0], qst[1], 0, ost[0], ost[1], H, 0, z, 0, zst[0], zst[1],
+        # ctx_len, row_pos, mask, mask_stride, mask_words, bt_width, scale
+        ctx.data_ptr(), pos.data_ptr(), tree_mask.data_ptr(), mst[0], ms[1], bt.shape[1], sm_scale,
+        # block_size, local_window, num_splits, device_error
+        sparse_block_size, local_blocks * sparse_block_size, num_splits,
+        device_error.ptr if device_error is not None else 0), index)
+
+
+_TREE = L.packer(L.DashTreeAttnArgs)
 
 
 def _table(block_table: torch.Tensor, index: int, n_seq: int) -> torch.Tensor:
     """The block table as int32 rows of unit inner stride."""
-    if block_table.dim() != 2 or block_table.shape[0] != n_seq or block_table.get_device() != index:
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != n_seq or block_table.get_device() != index:
         _need_cuda(block_table)
         raise ValueError(f"block_table must be [{n_seq}, W] on cuda:{index}")
     return block_table if block_table.dtype is torch.int32 and block_table.stride(1) == 1 else \
@@ -219,12 +220,12 @@ def verify_drafts(tokens: torch.Tensor, parents: Optional[torch.Tensor], cu_seql
     if index < 0:
         _need_cuda(target)
     cu = _ints(cu_seqlens_q, "cu_seqlens_q", index)
-    n_seq = cu.shape[0] - 1
-    if target.dim() != 2 or target.dtype not in ops._DT:
+    n_seq = cu.numel() - 1
+    if target.ndim != 2 or target.dtype not in ops._DT:
         raise ValueError("target must be [rows, vocab] in fp32, bf16 or fp16")
     rows, V = target.shape
     par = _ints(parents, "parents", index, rows)
-    if tokens.shape != (rows,) or tokens.dtype is not torch.int64 or tokens.get_device() != index:
+    if tokens.ndim != 1 or tokens.numel() != rows or tokens.dtype is not torch.int64 or tokens.get_device() != index:
         raise ValueError(f"tokens must be int64 [{rows}] on cuda:{index}")
     if greedy:
         if draft is not None or u_accept is not None or u_sample is not None:
@@ -233,7 +234,7 @@ def verify_drafts(tokens: torch.Tensor, parents: Optional[torch.Tensor], cu_seql
         if u_accept is None or u_sample is None:
             raise ValueError("u_accept and u_sample are needed unless greedy")
         for name, u, n in (("u_accept", u_accept, rows), ("u_sample", u_sample, n_seq)):
-            if u.shape != (n,) or u.dtype is not torch.float32 or u.get_device() != index:
+            if u.ndim != 1 or u.numel() != n or u.dtype is not torch.float32 or u.get_device() != index:
                 raise ValueError(f"{name} must be fp32 [{n}] on cuda:{index}")
         u_accept, u_sample = u_accept.contiguous(), u_sample.contiguous()
     tst = target.stride()
@@ -244,25 +245,27 @@ def verify_drafts(tokens: torch.Tensor, parents: Optional[torch.Tensor], cu_seql
     dev, i32, i64 = target.device, torch.int32, torch.int64
     r = Verified(torch.empty(n_seq, dtype=i32, device=dev), torch.empty(n_seq, max_nodes, dtype=i32, device=dev),
                  torch.empty(n_seq, dtype=i64, device=dev), torch.empty(n_seq, max_nodes, dtype=i64, device=dev))
-    a = L.DashVerifyArgs()
-    a.tokens, a.parents, a.q_start = tokens.data_ptr(), _ptr(par), cu.data_ptr()
-    a.target, a.target_stride = target.data_ptr(), tst[0] if rows > 1 else V
-    a.n_seq, a.rows, a.max_nodes, a.vocab = n_seq, rows, max_nodes, V
-    a.dtype, a.mode = ops._DT[target.dtype], 2 if greedy else 1
+    q = q_stride = 0
     if draft is not None:
         if draft.shape != target.shape or draft.dtype is not target.dtype or draft.get_device() != index:
             raise ValueError("draft must have target's shape, dtype and device")
         if draft.stride(1) != 1 and V > 1:
             draft = draft.contiguous()
-        a.draft, a.draft_stride, a.mode = draft.data_ptr(), draft.stride(0) if rows > 1 else V, 0
-    if not greedy:
-        a.u_accept, a.u_sample = u_accept.data_ptr(), u_sample.data_ptr()
-    a.n_accept, a.path = r.n_accept.data_ptr(), r.path.data_ptr()
-    a.next_token, a.out_tokens = r.next_token.data_ptr(), r.tokens.data_ptr()
-    if device_error is not None:
-        a.device_error = device_error.ptr
-    _call("dash_draft_verify", a, index)
+        q, q_stride = draft.data_ptr(), draft.stride(0) if rows > 1 else V
+    _call("dash_draft_verify", _VERIFY(
+        # tokens, parents, q_start, target, target_stride, draft, draft_stride
+        tokens.data_ptr(), 0 if par is None else par.data_ptr(), cu.data_ptr(), target.data_ptr(),
+        tst[0] if rows > 1 else V, q, q_stride,
+        # u_accept, u_sample, n_seq, rows, max_nodes, vocab, dtype, mode
+        0 if greedy else u_accept.data_ptr(), 0 if greedy else u_sample.data_ptr(), n_seq, rows, max_nodes, V,
+        ops._DT[target.dtype], 2 if greedy else 1 if draft is None else 0,
+        # n_accept, path, next_token, out_tokens, device_error
+        r.n_accept.data_ptr(), r.path.data_ptr(), r.next_token.data_ptr(), r.tokens.data_ptr(),
+        device_error.ptr if device_error is not None else 0), index)
     return r
+
+
+_VERIFY = L.packer(L.DashVerifyArgs)
 
 
 def commit_drafts(caches: Layers, path: torch.Tensor, n_accept: torch.Tensor, ctx_lens: torch.Tensor,
@@ -276,20 +279,22 @@ def commit_drafts(caches: Layers, path: torch.Tensor, n_accept: torch.Tensor, ct
     index = layers.index
     if layers.page_tokens is None:
         raise ValueError("commit_drafts takes tensors with one entry per token")
-    if path.dim() != 2 or path.dtype is not torch.int32 or path.get_device() != index or \
-            (path.shape[1] > 1 and path.stride(1) != 1):
+    shape = path.shape
+    if len(shape) != 2 or path.dtype is not torch.int32 or path.get_device() != index or \
+            (shape[1] > 1 and path.stride(1) != 1):
         raise ValueError(f"path must be int32 [n_seq, max_nodes] on cuda:{index}")
-    n_seq, max_nodes = path.shape
+    n_seq, max_nodes = shape
     acc = _ints(n_accept, "n_accept", index, n_seq)
     ctx = _ints(ctx_lens, "ctx_lens", index, n_seq)
     bt = _table(block_table, index, n_seq)
-    a = L.DashCommitArgs()
-    a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
-    a.n_seq, a.max_nodes, a.block_size = n_seq, max_nodes, layers.page_tokens
-    a.bt_width, a.num_pages = bt.shape[1], layers.num_pages
-    a.path, a.path_stride = path.data_ptr(), path.stride(0) if n_seq > 1 else max_nodes
-    a.n_accept, a.ctx_len = acc.data_ptr(), ctx.data_ptr()
-    a.block_table, a.bt_stride = bt.data_ptr(), bt.stride(0) if n_seq > 1 else bt.shape[1]
-    if device_error is not None:
-        a.device_error = device_error.ptr
-    _call("dash_draft_commit", a, index)
+    many = n_seq > 1
+    _call("dash_draft_commit", _COMMIT(
+        # tensors, n_tensors, n_seq, max_nodes, block_size, bt_width, pad, num_pages, path, path_stride
+        layers.address, layers.n, n_seq, max_nodes, layers.page_tokens, bt.shape[1], 0, layers.num_pages,
+        path.data_ptr(), path.stride(0) if many else max_nodes,
+        # n_accept, ctx_len, block_table, bt_stride, device_error
+        acc.data_ptr(), ctx.data_ptr(), bt.data_ptr(), bt.stride(0) if many else bt.shape[1],
+        device_error.ptr if device_error is not None else 0), index)
+
+
+_COMMIT = L.packer(L.DashCommitArgs)

@@ -18,7 +18,7 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _lib as L
-from .ops import DeviceErrorWord, _need_cuda, _ptr
+from .ops import DeviceErrorWord, _need_cuda
 
 
 def _call(fn: str, args, index: int) -> None:
@@ -36,15 +36,20 @@ def _ints(t: Optional[torch.Tensor], name: str, index: int, n: Optional[int] = N
     """``t`` as a contiguous int32 vector (of ``n`` values) on CUDA device ``index``."""
     if t is None:
         return None
+    if t.dtype is torch.int32 and t.get_device() == index and t.ndim == 1 and t.is_contiguous() and \
+            (n is None or t.numel() == n):
+        return t
     if t.get_device() != index:
         _need_cuda(t)
         raise ValueError(f"{name} is on {t.device}, not cuda:{index}")
     if t.dim() != 1 or (n is not None and t.shape[0] != n) or t.dtype not in _INTS:
         raise ValueError(f"{name} must be an int32 vector" + ("" if n is None else f" of {n} values"))
-    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+    return t.to(torch.int32).contiguous()
 
 
 _INTS = (torch.int32, torch.int64)
+_COPY = L.packer(L.DashPagesCopyArgs)
+_PAGES = L.packer(L.DashPagesArgs, 2)             # behind the two pools
 
 
 class CacheLayers:
@@ -81,6 +86,7 @@ class CacheLayers:
             d.tok_stride = inner * e if d.page_toks == 1 else t.stride(1) * e
             d.page_stride = t.stride(0) * e if self.num_pages > 1 else d.page_toks * d.tok_stride
             toks.add(int(d.page_toks))
+        self.n, self.address = len(self.c), ctypes.addressof(self.c)
         # tokens per page, where all tensors agree
         self.page_tokens = toks.pop() if len(toks) == 1 else None
 
@@ -100,16 +106,13 @@ def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
     recorded, as is one with an id past the last page."""
     layers = _layers(caches)
     src = _ints(src, "src", layers.index)
-    n = src.shape[0]
+    n = src.numel()
     dst = _ints(dst, "dst", layers.index, n)
     if n:
         scratch = torch.empty(2 * n, dtype=torch.int32, device=layers.device)
-        a = L.DashPagesCopyArgs()
-        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
-        a.n, a.src, a.dst = n, src.data_ptr(), dst.data_ptr()
-        a.num_pages, a.check, a.list = layers.num_pages, 1, scratch.data_ptr()
-        a.device_error = device_error.ptr if device_error is not None else None
-        _call("dash_pages_copy", a, layers.index)
+        _call("dash_pages_copy", _COPY(layers.address, layers.n, n, src.data_ptr(), dst.data_ptr(), 0, scratch.data_ptr(),
+                                       layers.num_pages, 1, 0, device_error.ptr if device_error is not None else 0),
+              layers.index)
 
 
 class PagePool:
@@ -150,14 +153,14 @@ class PagePool:
         c.block_table, c.bt_stride = block_table.data_ptr(), block_table.stride(0)
         c.n_blocks, c.num_pages = n_blocks.data_ptr(), ref.shape[0]
         c.max_rows, c.bt_width, c.block_size = block_table.shape[0], block_table.shape[1], self.block_size
+        self.packed = bytes(c)
 
-    def _args(self, rows, device_error) -> L.DashPagesArgs:
-        a = L.DashPagesArgs()
-        a.pool = self.c
-        if rows is not None:
-            a.rows, a.n = rows.data_ptr(), rows.shape[0]
-        a.device_error = device_error.ptr if device_error is not None else None
-        return a
+    def _args(self, device_error, rows=0, src=0, lens=0, n=0, layers=None, copy_src=0, copy_dst=0, n_moves=0,
+              new_id=0, into=None) -> L.DashPagesArgs:
+        return L.DashPagesArgs.from_buffer_copy(
+            self.packed + (into or self).packed +
+            _PAGES(rows, src, lens, n, *((0, 0) if layers is None else (layers.n, layers.address)), copy_src, copy_dst,
+                   n_moves, new_id, device_error.ptr if device_error is not None else 0))
 
     def _own(self, caches: Layers) -> CacheLayers:
         layers = _layers(caches)
@@ -169,19 +172,18 @@ class PagePool:
                 device_error: Optional[DeviceErrorWord] = None) -> None:
         """Row ``rows[i]`` gets pages for ``lens[i]`` tokens (it never loses any)."""
         rows = _ints(rows, "rows", self.index)
-        lens = _ints(lens, "lens", self.index, rows.shape[0])
-        a = self._args(rows, device_error)
-        a.lens = lens.data_ptr()
-        _call("dash_pages_reserve", a, self.index)
+        n = rows.numel()
+        lens = _ints(lens, "lens", self.index, n)
+        _call("dash_pages_reserve", self._args(device_error, rows.data_ptr(), 0, lens.data_ptr(), n), self.index)
 
     def free(self, rows: torch.Tensor, keep: Optional[torch.Tensor] = None,
              device_error: Optional[DeviceErrorWord] = None) -> None:
         """Row ``rows[i]`` keeps its first ``keep[i]`` blocks (default none)."""
         rows = _ints(rows, "rows", self.index)
-        keep = _ints(keep, "keep", self.index, rows.shape[0])
-        a = self._args(rows, device_error)
-        a.lens = _ptr(keep)
-        _call("dash_pages_free", a, self.index)
+        n = rows.numel()
+        keep = _ints(keep, "keep", self.index, n)
+        _call("dash_pages_free", self._args(device_error, rows.data_ptr(), 0, 0 if keep is None else keep.data_ptr(), n),
+              self.index)
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor, caches: Layers,
              device_error: Optional[DeviceErrorWord] = None) -> None:
@@ -190,16 +192,14 @@ class PagePool:
         copied to a page of its own in every tensor of ``caches``."""
         layers = self._own(caches)
         src = _ints(src, "src", self.index)
-        n = src.shape[0]
+        n = src.numel()
         dst, lens = _ints(dst, "dst", self.index, n), _ints(lens, "lens", self.index, n)
         if n == 0:
             return
         pairs = torch.empty(2 * n, dtype=torch.int32, device=self.device)
-        a = self._args(dst, device_error)
-        a.src, a.lens = src.data_ptr(), lens.data_ptr()
-        a.copy_src, a.copy_dst = pairs.data_ptr(), pairs.data_ptr() + 4 * n
-        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
-        _call("dash_pages_fork", a, self.index)
+        at = pairs.data_ptr()
+        _call("dash_pages_fork", self._args(device_error, dst.data_ptr(), src.data_ptr(), lens.data_ptr(), n, layers, at,
+                                            at + 4 * n), self.index)
 
     def compact(self, caches: Layers, into: Optional["PagePool"] = None,
                 device_error: Optional[DeviceErrorWord] = None) -> torch.Tensor:
@@ -214,10 +214,7 @@ class PagePool:
         P = self.c.num_pages
         half = P // 2
         buf = torch.empty(2 * half + P + 1, dtype=torch.int32, device=self.device)
-        a = self._args(None, device_error)
-        a.into = to.c
-        a.copy_src = at = buf.data_ptr()
-        a.copy_dst, a.new_id, a.n_moves = at + 4 * half, at + 8 * half, at + 8 * half + 4 * P
-        a.tensors, a.n_tensors = ctypes.addressof(layers.c), len(layers.c)
-        _call("dash_pages_compact", a, self.index)
+        at = buf.data_ptr()
+        _call("dash_pages_compact", self._args(device_error, layers=layers, copy_src=at, copy_dst=at + 4 * half,
+                                               new_id=at + 8 * half, n_moves=at + 8 * half + 4 * P, into=to), self.index)
         return buf[2 * half + P:]

@@ -298,3 +298,26 @@ def test_pool_oracle_keeps_every_page_once():
                 held[p] += 1
         assert held == P.ref
         assert sorted(P.free) == [p for p in range(40) if P.ref[p] == 0]
+
+
+def test_packer_equals_setting_the_fields():
+    """Arguments packed at once hold what setting every field gives."""
+
+    def fill(c, values):
+        for name, t in type(c)._fields_:
+            if issubclass(t, C.Structure):
+                fill(getattr(c, name), values)
+            else:
+                setattr(c, name, next(values))
+
+    for cls in (L.DashTreeAttnArgs, L.DashVerifyArgs, L.DashCommitArgs, L.DashPagesCopyArgs):
+        want, n = cls(), 0
+        fill(want, iter(range(1, 100)))
+        def count(c):                                      # noqa: E306
+            return sum(count(t) if issubclass(t, C.Structure) else 1 for _, t in c._fields_)
+        n = count(cls)
+        assert bytes(L.packer(cls)(*range(1, n + 1))) == bytes(want), cls.__name__
+    want = L.DashPagesArgs()
+    fill(want, iter(range(1, 100)))
+    rest = L.packer(L.DashPagesArgs, 2)(*range(21, 32))
+    assert bytes(want.pool) + bytes(want.into) + rest == bytes(want)

@@ -244,15 +244,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     mbar_init_fence();
   }
-  int lo = ctx;                                  // warp 5: the earliest window of the tile
-  if (warp < 4) {
-    for (int w = tid; w < kMaxWords; w += kRows) S.bits[w] = 0u;
-  } else {
+  if (warp >= 4) {
     // the table's row on its way to the L1, for the producer
     for (int b = (tid - kRows) * 32; b < min(a.bt_width, nblk); b += (kThreads - kRows) * 32)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(a.kv.block_table + (int64_t)s * a.kv.bt_stride + b));
     // Q (rows of the operand tile beyond the unit's stay as they are)
-#pragma unroll 1
+#pragma unroll 4
     for (int c = tid - kRows; c < nrows * 16; c += kThreads - kRows) {
       const int m = c >> 4, cc = c & 15, node = m / G;
       const T* src = reinterpret_cast<const T*>(a.qo.q) + (r0 + node) * a.qo.q_stride_tok +
@@ -260,15 +257,11 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint32_t dst = smem_u32(S.q + (cc >> 3) * (QR * 128) + m * 128 + (((cc & 7) ^ (m & 7)) << 4));
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     }
-    if (warp == 5) {
-#pragma unroll 1
-      for (int i = lane; i < nt; i += 32) lo = min(lo, window_of(r0 + i));
-      lo = __reduce_min_sync(0xffffffffu, lo);
-    }
-  }
-  __syncthreads();
-  // ---- the union ----
-  if (warp < 4) {
+  } else {
+    // ---- the union ----
+    const int first_key = tid < nt ? window_of(r0 + tid) : ctx;
+    for (int w = tid; w < kMaxWords; w += kRows) S.bits[w] = 0u;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll 1
     for (int e0 = tid; e0 < entries; e0 += 4 * kRows) {
       int b[4], pos[4];                          // the loads of four entries at once
@@ -295,8 +288,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (!((*(volatile uint32_t*)&S.bits[g >> 5] >> (g & 31)) & 1u)) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
       }
     }
-  } else if (warp == 5) {
-    const int g0 = lo / GR, g1 = (live_end + GR - 1) / GR;        // [g0, g1): window and drafts
+    // the windows of the warp's tokens and the drafts: granules [g0, g1)
+    const int g0 = __reduce_min_sync(0xffffffffu, first_key) / GR, g1 = (live_end + GR - 1) / GR;
     for (int w = (g0 >> 5) + lane; w * 32 < g1; w += 32) {
       uint32_t m = 0xffffffffu;
       if (w * 32 < g0) m &= 0xffffffffu << (g0 & 31);

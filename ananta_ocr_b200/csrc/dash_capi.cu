@@ -564,7 +564,7 @@ int dash_tree_attn(const DashTreeAttnArgs* a, dash_stream_t stream) {
     return set_error(DASH_ERR_INVALID, "mask needs %d words per row and rows that far apart",
                      (a->seqs.max_q_len + 31) / 32);
   if (a->local_window < 0) return set_error(DASH_ERR_INVALID, "local_window must be >= 0");
-  if (a->num_splits < 0 || a->num_splits > 8) return set_error(DASH_ERR_INVALID, "num_splits %d not in [0, 8]", a->num_splits);
+  if (a->num_splits < 0 || a->num_splits > 16) return set_error(DASH_ERR_INVALID, "num_splits %d not in [0, 16]", a->num_splits);
   return launch_tree_attn(*a, (cudaStream_t)stream);
 }
 

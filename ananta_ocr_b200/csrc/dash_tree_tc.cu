@@ -1,7 +1,7 @@
 // dash_tree_tc.cu -- draft-tree attention on the sm_100a tensor cores.
 //
 // Work unit: up to 128 (drafted token, query head) rows of one sequence and kv
-// head, split over a cluster of 1..8 CTAs.  The keys that any row attends --
+// head, split over a cluster of 1..16 CTAs.  The keys that any row attends --
 // the union of the rows' routed blocks, their windows and the drafted tokens --
 // are cut into granules of GR tokens (GR = block size, 64 at most); a tile of 64
 // keys is 64 / GR granules of the union in ascending order, and each CTA of the
@@ -19,8 +19,8 @@
 //                     from TMEM)
 //   warps 0-3 softmax one thread per row; warps without a row sleep.  The additive
 //                     terms of the routed granules lie in a [granule][token]
-//                     table (first occurrence of a repeated id by atomicMax on
-//                     the slot), refilled when a part outgrows it
+//                     table (of a repeated id the lowest slot's), refilled when
+//                     a part outgrows it
 //
 // Units of up to 32 rows keep 8 KB of Q and three K and V slots, of up to 64 rows 16 KB,
 // three and two, larger ones 32 KB and two (the rows of Q's operand tile that do not exist are whatever lies
@@ -52,6 +52,7 @@ constexpr int kRows = 128;                       // M of both MMAs
 constexpr int kKeys = 64;                        // N of Q K^T, K of P V
 constexpr int kThreads = 192;
 constexpr int kSlot = 16384;                     // one tile of K or of V: 2 x [64 x 128 B]
+constexpr int kMaxCluster = 16;
 constexpr int kMaxWords = 256;                   // 8192 granules of a sequence
 constexpr uint32_t kTmemCols = 256;              // S0 | S1 | O
 constexpr float kGrow = 8.0f;                    // O is rescaled when a row's maximum grows by 2^8
@@ -61,12 +62,12 @@ template <int QR>
 struct TreeSmem {
   static constexpr int kKSlots = QR <= 64 ? 3 : 2, kVSlots = QR == 32 ? 3 : 2;
   static constexpr int kCells = QR == 32 ? 980 : QR == 64 ? 2900 : 2800;      // additive terms held at a time
-  static constexpr int kSlots = 512;             // routed slots held
+  static constexpr int kSlots = 1024;            // routed slots held
   uint8_t q[2 * QR * 128];                       // two halves of 64 dims, swizzled
   uint8_t k[kKSlots][kSlot];                     // receives O (QR x 512 B) at the end
   uint8_t v[kVSlots][kSlot];
-  int cell[kCells];
-  uint32_t slot[kSlots];                         // (first granule << 8) | granules
+  float cell[kCells];
+  uint16_t slot[kSlots];                         // (first granule << 3) | granules
   uint32_t bits[kMaxWords];
   uint16_t before[kMaxWords + 2];
   int tok[8][4];                                 // first token of the tile's granules, -1 = none (K runs < 8 tiles ahead)
@@ -191,8 +192,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (live_end < end && tid == 0 && hk == 0 && split == 0) record_error(derr, DASH_DEV_BAD_PAGE, 75, a.bt_width);
   const int nblk = (end + bs - 1) / bs;
   volatile int* abort_flag = &S.abort_flag;
-  constexpr int kNone = (int)0xff800000u;        // -inf, below every slot's key
-  constexpr int kKey = 0x7ffffffe;               // slots as keys: NaNs that no product has
 
   // first key of a row's window
   auto window_of = [&](int64_t r) -> int {
@@ -202,13 +201,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   // entry e = (token, slot of its list), lists padded to a power of two
   const int pad = K > 1 ? 32 - __clz(K - 1) : 0;
   const int entries = K > 0 ? nt << pad : 0;
-  // remote granules of block b for a row at position pos: (first << 8) | count
+  // remote granules of block b for a row at position pos: (first << 3) | count (13 and 3 bits)
   auto remote = [&](int b, int pos) -> uint32_t {
     if (b >= nblk) record_error(derr, DASH_DEV_BAD_BLOCK, 76, b);
     const int64_t e = (int64_t)pos - a.local_window + 1;
     const int edge = (int)max((int64_t)0, min(e, (int64_t)min(ctx, live_end)));
     const int64_t t0 = (int64_t)b * bs, t1 = min(t0 + bs, (int64_t)edge);
-    return b >= 0 && t1 > t0 ? (uint32_t)(t0 / GR) << 8 | (uint32_t)((t1 - t0 + GR - 1) / GR) : 0u;
+    return b >= 0 && t1 > t0 ? (uint32_t)(t0 / GR) << 3 | (uint32_t)((t1 - t0 + GR - 1) / GR) : 0u;
   };
   // the same for entry e, from memory
   auto remote_of = [&](int e) -> uint32_t {
@@ -282,9 +281,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i = 0; i < 4; ++i) {
         const int e = e0 + i * kRows;
         const uint32_t v = remote(b[i], pos[i]);
-        if (e < Smem::kSlots) S.slot[e] = v;
+        if (e < Smem::kSlots) S.slot[e] = (uint16_t)v;
         // (tokens of a tree name the same blocks: a set bit needs no atomic)
-        for (uint32_t g = v >> 8, g1 = g + (v & 255u); g < g1; ++g)
+        for (uint32_t g = v >> 3, g1 = g + (v & 7u); g < g1; ++g)
           if (!((*(volatile uint32_t*)&S.bits[g >> 5] >> (g & 31)) & 1u)) atomicOr(&S.bits[g >> 5], 1u << (g & 31));
       }
     }
@@ -499,38 +498,45 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float sl2 = fabsf(a.scale) * kTreeLog2e;
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     // The additive terms of granules [c0, c1) of this CTA's part, -inf where no slot
-    // of the token names the block: the lowest slot that names a cell wins it (pass
-    // 0; slots as keys above -inf's bits that no bias equals), then leaves its bias there
-    // (pass 1).  By all four warps.
+    // of the token names the block.  A warp takes 32 slots of one token, or all slots of
+    // several; of slots that name one block the lowest counts (in the warp by
+    // their lanes, later chunks of a token before earlier ones).
     const int cap = Smem::kCells / nt / NG * NG;
+    const int lp = min(pad, 5), span = max(pad, 5);
     int c0 = 0, c1 = 0;
     auto fill = [&](int from) {
       asm volatile("bar.sync 1, 128;" ::: "memory");         // the old terms have been read
       c0 = from;
       c1 = min(from + cap, tiles * NG);
-      for (int i = m; i < (c1 - c0) * nt; i += kRows) S.cell[i] = kNone;
+      for (int i = m; i < (c1 - c0) * nt; i += kRows) S.cell[i] = -INFINITY;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // entry of step j; its bias is loaded a step ahead
+      auto entry = [&](int j) {
+        return ((warp + (j >> (span - 5) << 2)) << span) + ((~j & ((1 << (span - 5)) - 1)) << 5) + lane;
+      };
+      auto bias_of = [&](int e) {
+        const int slot = e & ((1 << pad) - 1);
+        return a.routes.bias && e < entries && slot < K
+                   ? __ldg(a.routes.bias + rbase + (int64_t)(e >> pad) * a.routes.row_stride + slot) * kTreeLog2e : 0.0f;
+      };
+      float next = bias_of(entry(0));
 #pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      for (int j = 0, e = entry(0); e - lane < entries; ++j) {
+        const float bias = next;
+        const uint32_t v = e >= entries ? 0u : e < Smem::kSlots ? S.slot[e] : remote_of(e);
+        const int nd = e >> pad;
+        e = entry(j + 1);
+        next = bias_of(e);
+        // a block's granules follow one another in the union
+        const int g = v >> 3;
+        int rk = (int)S.before[g >> 5] + __popc(S.bits[g >> 5] & ((1u << (g & 31)) - 1u)) - rank0;
+        const int rk1 = min(rk + (int)(v & 7u), c1);
+        rk = max(rk, c0);
+        const uint32_t same = __match_any_sync(0xffffffffu, v << 5 | (uint32_t)(lane >> lp));
+        if (__ffs(same) - 1 == lane)
 #pragma unroll 1
-        for (int e = m; e < entries; e += kRows) {
-          const uint32_t v = e < Smem::kSlots ? S.slot[e] : remote_of(e);
-          if (v == 0u) continue;
-          const int nd = e >> pad, slot = e & ((1 << pad) - 1);
-          // a block's granules follow one another in the union
-          const int g = v >> 8;
-          int rk = (int)S.before[g >> 5] + __popc(S.bits[g >> 5] & ((1u << (g & 31)) - 1u)) - rank0;
-          const int rk1 = min(rk + (int)(v & 255u), c1);
-          float bias = 0.0f;
-          if (pass && a.routes.bias)
-            bias = __ldg(a.routes.bias + rbase + (int64_t)nd * a.routes.row_stride + slot) * kTreeLog2e;
-#pragma unroll 1
-          for (rk = max(rk, c0); rk < rk1; ++rk) {
-            int* c = S.cell + (rk - c0) * nt + nd;
-            if (pass == 0) atomicMax(c, kKey - slot);
-            else if (*c == kKey - slot) *c = __float_as_int(bias);
-          }
-        }
+          for (float* c = S.cell + (rk - c0) * nt + nd; rk < rk1; ++rk, c += nt) *c = bias;
+        __syncwarp();
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
     };
@@ -557,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tail |= t0 >= 0 && t0 + GR > end;
         if (t0 >= 0 && row_ok) {
           const bool far = t0 < lstart;
-          if (far) add[g] = __int_as_float(S.cell[(it * NG + g - c0) * nt + node]);
+          if (far) add[g] = S.cell[(it * NG + g - c0) * nt + node];
           else if (t0 + GR <= ctx) add[g] = 0.0f;
           const bool p = far ? t0 + GR <= lstart : t0 + GR <= ctx;
           pure &= p;
@@ -758,26 +764,30 @@ __global__ void __launch_bounds__(kThreads, 2)
       mk = *cluster.map_shared_rank(&S.m[m], lane);
       lk = *cluster.map_shared_rank(&S.l[m], lane);
     }
-    float4 o[8];                                 // all parts in flight
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < nsp)
-        o[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&S.k[0][0], k) + m * 512 + ((lane ^ (m & 7)) << 4));
     float M = mk;
 #pragma unroll
-    for (int x = 4; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    for (int x = 8; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
     M = __shfl_sync(0xffffffffu, M, 0);
     // a part without a key for the row has weight 0, and 0 * NaN shows below;
     // one without a tile is left out
     const float wk = mk == -INFINITY ? 0.0f : fast_exp2(mk - M);
     float L = 0.0f;
     float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int k0 = 0; k0 < nsp; k0 += 8) {
+      float4 o[8];                               // eight parts in flight
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const float w = __shfl_sync(0xffffffffu, wk, k), l1 = __shfl_sync(0xffffffffu, lk, k);
-      if (l1 != -1.0f) {                         // lanes k >= nsp hold -1
-        L += l1 * w;
-        O.x += o[k].x * w; O.y += o[k].y * w; O.z += o[k].z * w; O.w += o[k].w * w;
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < nsp)
+          o[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&S.k[0][0], k0 + k) + m * 512 +
+                                                  ((lane ^ (m & 7)) << 4));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = __shfl_sync(0xffffffffu, wk, k0 + k), l1 = __shfl_sync(0xffffffffu, lk, k0 + k);
+        if (l1 != -1.0f) {                       // lanes k >= nsp hold -1
+          L += l1 * w;
+          O.x += o[k].x * w; O.y += o[k].y * w; O.z += o[k].z * w; O.w += o[k].w * w;
+        }
       }
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
@@ -849,6 +859,9 @@ struct TreeCut {
 // us, 1 / 2 / 3 / 8 CTAs per unit: 160 units of 34 tiles 49 / 64 / 56 / 85, 80 of 15
 // 31 / 23 / 21 / 41, 10 of 20 29 / 21 / 19 / 15; 320 of 37 100 / 97 / 99 / 151, as 296 whole
 // ones and 24 of 8 CTAs 84; 640 of 24 148 / 160 / 181 / 313, as 592 whole ones and 48 of 6 146.)
+// More than 8 CTAs, which leave gaps in the GPU's processing clusters, only where most of
+// the GPU stays empty otherwise (4 units of some 250 tiles 33 -> 29 with 16 CTAs; 20
+// units of 20 tiles 17 -> 27 with 14).
 // The number of tiles is not known here; the drafted tokens of a sequence route similar
 // blocks: twice K are assumed.
 static TreeCut tree_cut(const DashTreeAttnArgs& a, int64_t units) {
@@ -858,7 +871,7 @@ static TreeCut tree_cut(const DashTreeAttnArgs& a, int64_t units) {
   const double tiles = (double)((keys < most ? keys : most) + kKeys - 1) / kKeys;
   auto best = [&](int64_t n, int& sp) {
     double least = 1e30;
-    for (int k = 1; k <= 8 && k <= tiles; ++k) {
+    for (int k = 1; k <= kMaxCluster && k <= tiles && (k <= 8 || n * k <= 160); ++k) {
       const double waves = (double)n * k / 296, tile = waves < 1 ? 1.49 * waves : 1.49;
       const double own = 10.0 + tiles / k * (tile > 0.95 ? tile : 0.95), t = own * (waves <= 1 ? 1.0 : waves + 0.5);
       if (t < least) { least = t; sp = k; }
@@ -882,6 +895,7 @@ static int launch_tc(const DashTreeAttnArgs& a, const CUtensorMap& mk, const CUt
   const int smem = (int)sizeof(TreeSmem<QR>) + 1024;
   auto kernel = tree_tc_kernel<T, GR, QR>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   for (int part = 0; part < 2 && e == cudaSuccess; ++part) {
     const int64_t n = part == 0 ? cut.whole : units - cut.whole;
     if (n == 0) continue;

@@ -855,7 +855,7 @@ int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
  * with up to 128 query heads per kv head, other sizes on the CUDA cores.
  * seqs: n_seq, q_start, q_len_fixed = rows, max_q_len = most drafted tokens of
  * a sequence (<= 256); pos0 and kv_len are not read.  num_splits 0: automatic
- * (1..8 CTAs share a sequence's keys and join their parts over the cluster's
+ * (1..16 CTAs share a sequence's keys and join their parts over the cluster's
  * shared memory; no workspace).                                            */
 typedef struct {
   DashSeqs seqs;

@@ -68,7 +68,7 @@ def tree_args(**kw):
     (dict(bt_width=0), L.DASH_ERR_INVALID, "bt_width"),
     (dict(block_size=0), L.DASH_ERR_INVALID, "block_size"),
     (dict(local_window=-1), L.DASH_ERR_INVALID, "local_window"),
-    (dict(num_splits=9), L.DASH_ERR_INVALID, "num_splits"),
+    (dict(num_splits=17), L.DASH_ERR_INVALID, "num_splits"),
 ])
 def test_tree_attn_refuses(change, code, words):
     refused("dash_tree_attn", tree_args(**change), code, words)

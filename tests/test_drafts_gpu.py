@@ -77,7 +77,7 @@ def test_tree_attention(name, poison):
     check(t, *attend(t))
 
 
-@pytest.mark.parametrize("splits", range(1, 9))
+@pytest.mark.parametrize("splits", [*range(1, 9), 11, 16])
 @pytest.mark.parametrize("name", ["decoder", "gqa", "short"])
 def test_every_split_count(name, splits):
     nodes, ctx, H, Hkv, bs, win, K, dt, branch = CASES[name]

@@ -158,7 +158,7 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 template <typename T, int GR, int QR>
 __global__ void __launch_bounds__(kThreads, 2)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const __grid_constant__ DashTreeAttnArgs a, int n_tiles_seq, int unit0) {
+                   const __grid_constant__ DashTreeAttnArgs a, int n_tiles_seq, int unit0, bool more) {
   constexpr int NG = kKeys / GR;                 // granules per tile
   using Smem = TreeSmem<QR>;
   constexpr int kKSlots = Smem::kKSlots, kVSlots = Smem::kVSlots;
@@ -176,7 +176,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   TreeSeq sq = tree_seq(a.seqs.q_start, a.ctx_len, a.seqs.q_len_fixed, a.seqs.max_q_len, s);
   const int node0 = tile_i * per_tile;
   const int nt = min(per_tile, sq.n - node0);    // this tile's tokens
-  if (nt <= 0) return;                           // the whole cluster leaves
+  // Of two launches the second takes the slots that the first leaves, as soon as it
+  // leaves them; it ends after the first, so that what follows sees both.
+  if (more) asm volatile("griddepcontrol.launch_dependents;");
+  auto after_first = [&]() {
+    if (unit0 > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  if (nt <= 0) {                                 // the whole cluster leaves
+    after_first();
+    return;
+  }
   const int total_n = sq.n;
   const int64_t r0 = sq.row0 + node0;            // packed row of the tile's first token
   const int nrows = nt * G, nact = (nrows + 31) >> 5;
@@ -751,7 +760,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
-  if (nsp == 1) return;
+  if (nsp == 1) {
+    after_first();
+    return;
+  }
   cluster.sync();
   // ---- join: row m by CTA m % nsp, a warp per row, lane = 4 dims ----
 #pragma unroll 1
@@ -804,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           L > 0.0f ? (M + log2f(L)) * kTreeLn2 : -INFINITY;
   }
   cluster.sync();                                // no CTA leaves while another reads its part
+  after_first();
 }
 
 // ---------------------------------------------------------------------------
@@ -905,13 +918,16 @@ static int launch_tc(const DashTreeAttnArgs& a, const CUtensorMap& mk, const CUt
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)sp;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, n_tiles, part == 0 ? 0 : (int)cut.whole);
+    cfg.numAttrs = part == 1 && cut.whole > 0 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, n_tiles, part == 0 ? 0 : (int)cut.whole,
+                           part == 0 && cut.whole < units);
     count_launch();
   }
   if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "tree_tc_kernel launch failed: %s", cudaGetErrorString(e));

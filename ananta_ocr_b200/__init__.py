@@ -14,8 +14,14 @@ keep the reference's module and function names so callers swap them in:
                                              route_triton.{route_prefill_triton,
                                              route_decode_triton, kbar_refresh_tail_triton},
                                              dash_router.DashRouterMath
+
+Speculative decoding on the paged cache (no counterpart in the reference):
+
+  ananta_ocr_b200.drafts                     tree_plan, dash_sparse_attn_tree,
+                                             verify_drafts, commit_drafts
+  ananta_ocr_b200.page_pool                  PagePool, CacheLayers, copy_pages
 """
 from . import _lib  # noqa: F401
 
 __all__ = ["ops", "sparse_gather_e2e_triton", "sparse_gather_triton", "modeling_deepseekv2",
-           "unlimited_dash_ops", "sharding"]
+           "unlimited_dash_ops", "sharding", "drafts", "page_pool"]

@@ -7,6 +7,12 @@
 // in order, so what pages a request gets depends on nothing but the state and
 // the requests; counts are integers and every page's fate is decided by its
 // final count, not by the order of the atomics that made it.
+//
+// Measured (CUDA graph): compaction of 1.1 GB of traffic in 12 layers 195 us (5.7 TB/s; a plain
+// copy 6.5), 64 forks with 243 MB of copied pages and their freeing 46 us, 2 forks
+// 12.4 us and a commit of 8 sequences 8.4 us (bound by launches and dependent loads).
+// The copy's CTAs take their places while the tables are still worked on
+// (programmatic dependent launch: fork 14.4 -> 12.4 us).
 #include "dash_common.cuh"
 #include "dash_internal.h"
 

@@ -144,8 +144,8 @@ typedef struct {
  *           (_kbar_page_kernel) and :707-726 (kbar_refresh_tail_triton).
  * contiguous (pages == NULL): summary of block b of sequence s (tokens
  *   [b*block_size, min(seq_len, (b+1)*block_size))) -> kbar row s*kbar_seq_rows+b.
- * paged: for each plan entry i with ntok[i] > 0, the first ntok[i] tokens of
- *   page pages[i] -> kbar row pages[i].                                    */
+ * paged: for each plan entry i with ntok[i] > 0 and pages[i] >= 0, the first
+ *   ntok[i] tokens of page pages[i] -> kbar row pages[i].                  */
 typedef struct {
   const void* keys;
   int32_t dtype;       /* DASH_DTYPE_F32 or DASH_DTYPE_BF16 */
@@ -822,7 +822,9 @@ int dash_entmax15_bwd(const DashEntmaxArgs* args, dash_stream_t stream);
  * (block_table[s, t / block_size] * block_size + t % block_size at t = ctx_len
  * + i; -1 where the page does not exist) and the sequence.  Every output is
  * optional.  parents NULL: a chain.  A parent outside [0, i) records
- * DASH_DEV_BAD_TREE and counts as none (row 0 has none).  max_nodes <= 256. */
+ * DASH_DEV_BAD_TREE and counts as none (row 0 has none), as does a sequence of
+ * more than max_nodes tokens, whose rows behind those no call of the step
+ * reads or writes.  max_nodes <= 256.                                      */
 typedef struct {
   const int32_t* parents;      /* [rows] token index within the sequence, -1 = none */
   const int32_t* q_start;      /* [n_seq + 1] */
@@ -852,7 +854,9 @@ int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
  * outside [0, num_pages) are left out and recorded.  K/V, q and out are bf16
  * or fp16, paged (block_table set), head_dim 128, page size == block_size;
  * block_size 16, 32 and multiples of 64 up to 256 run on the tensor cores
- * with up to 128 query heads per kv head, other sizes on the CUDA cores.
+ * with up to 128 query heads per kv head and tables of up to 8,192 granules of
+ * min(block_size, 64) tokens; other calls run on the CUDA cores (same results
+ * within rounding, six and more times slower).
  * seqs: n_seq, q_start, q_len_fixed = rows, max_q_len = most drafted tokens of
  * a sequence (<= 256); pos0 and kv_len are not read.  num_splits 0: automatic
  * (1..16 CTAs share a sequence's keys and join their parts over the cluster's

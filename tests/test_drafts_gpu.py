@@ -88,6 +88,34 @@ def test_every_split_count(name, splits):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("last", [7, 0], ids=["", "nothing_in_the_second"])
+def test_more_units_than_the_gpu_holds(last):
+    """320 units: 296 of one CTA each, the others in a second launch (whose
+    sequences may draft nothing), eager and captured, with work in front of it
+    and behind it in the stream."""
+    nodes = [3, 1, 0, 5] * 9 + [7] + [last] * 3
+    t = make_tree(21, nodes, [1100 + 17 * i for i in range(40)], H=8, Hkv=8, bs=64, window=2, K=16)
+    d = {k: v.cuda() for k, v in t.items() if isinstance(v, torch.Tensor)}
+    L.launches(reset=True)
+    out, z = attend(t, **d)
+    assert L.launches() == 2
+    check(t, out, z)
+    q, o = torch.empty_like(d["q"]), torch.empty_like(out)
+    sums = torch.empty_like(out, dtype=torch.float32)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for scale in (0.5, 1.0):                       # the first result must not be what is left
+            q.copy_(d["q"] * scale)
+            attend(t, out=o, lse=False, **{**d, "q": q})
+            sums.copy_(o)
+            o.zero_()
+    for _ in range(5):
+        g.replay()
+        torch.cuda.synchronize()
+        n = t["rows"]
+        assert torch.equal(sums[:n], out[:n].float()) and (o == 0).all()
+
+
 def test_repeated_ids_and_index_heads():
     """The first of repeated ids counts; two router heads pick their own blocks."""
     t = make_tree(3, [9, 14], [800, 600], H=4, Hkv=2, bs=64, window=2, K=6, index_heads=2, dup=True, pad_rows=2)

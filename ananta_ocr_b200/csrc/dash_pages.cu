@@ -390,7 +390,10 @@ __global__ void __cluster_dims__(kIdCluster, 1, 1) __launch_bounds__(kIdThreads)
 // page_state_kernel: one CTA per request, tiles of kStTile tokens scanned in
 // order with the running marker count, image run and pp carried across
 // tiles.  Restates page_state.py:217-313 and decode_meta_triton.py:38-87, and
-// page_state.py:315-328 for the bounds of the blocks it wrote.
+// page_state.py:315-328 for the bounds of the blocks it wrote.  A slot outside
+// [0, num_slots), or one in a block without a page (a table entry below 0), is
+// no slot: nothing is read or written there (the reference clamps it to the
+// first or last slot, which may be another request's).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int64_t warp_min64(int64_t v) {
 #pragma unroll
@@ -430,10 +433,12 @@ __global__ void __launch_bounds__(kStThreads) page_state_kernel(DashPageStateArg
   if (sp - 1 >= 0) {
     const int64_t p = sp - 1;
     const int64_t blk = min(p / bs, (int64_t)a.bt_width - 1);
-    const int64_t slot = clamp64((int64_t)bt[blk] * bs + p % bs, 0, ns - 1);
-    prev_m = a.slot_marker_cum[slot];
-    prev_i = a.slot_img_run[slot];
-    prev_pp = a.slot_prompt_pages[slot];
+    const int64_t slot = bt[blk] < 0 ? -1 : (int64_t)bt[blk] * bs + p % bs;
+    if (slot >= 0 && slot < ns) {
+      prev_m = a.slot_marker_cum[slot];
+      prev_i = a.slot_img_run[slot];
+      prev_pp = a.slot_prompt_pages[slot];
+    }
   }
   const int64_t gen0 = a.gen_start ? a.gen_start[r] : INT64_MAX;
 
@@ -489,11 +494,15 @@ __global__ void __launch_bounds__(kStThreads) page_state_kernel(DashPageStateArg
         const int resp = cm - 1 - pp;
         const int text = gen ? (resp >= 0 ? resp : -1) : (cm > pp ? cm - 1 : -1);
         a.q_page[t] = img ? ip : text;
-        const int64_t slot = clamp64(a.slot_mapping[t], 0, ns - 1);
-        a.slot_img_page[slot] = ip;
-        a.slot_marker_cum[slot] = cm;
-        a.slot_img_run[slot] = ci;
-        a.slot_prompt_pages[slot] = pp;
+        const int64_t slot = a.slot_mapping[t];
+        if (slot >= 0 && slot < ns) {
+          a.slot_img_page[slot] = ip;
+          a.slot_marker_cum[slot] = cm;
+          a.slot_img_run[slot] = ci;
+          a.slot_prompt_pages[slot] = pp;
+        } else {
+          record_error(a.device_error, DASH_DEV_BAD_PAGE, 82, slot);
+        }
       }
     }
     cm_carry += (int)(total >> 16);
@@ -507,9 +516,9 @@ __global__ void __launch_bounds__(kStThreads) page_state_kernel(DashPageStateArg
   const int64_t last_blk = clamp64(max(end - 1, (int64_t)0) / bs, 0, (int64_t)a.bt_width - 1);
   const int rem = (int)(end % bs);
   if (rem > 0) {
-    const int64_t phys = bt[last_blk];
-    for (int o = rem + tid; o < bs; o += kStThreads)
-      a.slot_img_page[clamp64(phys * bs + o, 0, ns - 1)] = -1;
+    const int64_t first = (int64_t)bt[last_blk] * bs;
+    if (first >= 0)
+      for (int64_t o = first + rem + tid; o < min(first + bs, ns); o += kStThreads) a.slot_img_page[o] = -1;
   }
   if (!a.blk_lo) return;
   __syncthreads();

@@ -322,8 +322,11 @@ int dash_page_ids(const DashPageIdsArgs* args, dash_stream_t stream);
  * negative) : (marker_cum > pp ? marker_cum - 1 : -1)).  A token is
  * generated iff its index < num_decode_tokens, or its position >=
  * gen_start[r] (gen_start optional).  The four slot arrays are written at
- * slot_mapping (clamped to [0, num_slots)); then slots past the last token
- * in each request's last block get image page -1.  When blk_lo/blk_hi are
+ * slot_mapping; then slots past the last token in each request's last block
+ * get image page -1.  A slot outside [0, num_slots), as a block without a page
+ * (a table entry below 0) gives, is left out (recorded where a token names it;
+ * the carry-in counts as 0): the reference clamps it into the range, where it
+ * may be another request's.  When blk_lo/blk_hi are
  * given, the image-page bounds of every physical block written in this step
  * are recomputed from the slot array (page_state.py:315-328).            */
 typedef struct {

@@ -563,7 +563,9 @@ __global__ void __launch_bounds__(kAllowWarps * 32) page_allow_kernel(DashPageAl
     if (q < 0 || b >= a.desc_width || (int64_t)b * a.block_size >= live) return false;
     int64_t i;
     if (a.block_table) {
-      i = clamp64(a.block_table[s * a.bt_stride + b], 0, a.num_desc - 1);
+      i = a.block_table[s * a.bt_stride + b];
+      if (i < 0) return false;                     // no page (an unused entry): it holds none
+      i = min(i, (int64_t)a.num_desc - 1);
     } else {
       i = s * a.desc_seq_rows + b;
       if (i >= a.num_desc) return false;

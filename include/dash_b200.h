@@ -368,7 +368,8 @@ int dash_page_state_step(const DashPageStateArgs* args, dash_stream_t stream);
  * fallback) and the decode branch of modeling_anantaocr.py:482-496.
  * Row r belongs to sequence s = row_seq ? row_seq[r] : r / rows_per_seq.
  * Block b < desc_width has descriptor i = block_table[s*bt_stride + b]
- * (clamped to [0, num_desc)) or s*desc_seq_rows + b; blocks >= desc_width
+ * (an entry below 0 holds no page; one past num_desc counts as the last, as in
+ * the reference) or s*desc_seq_rows + b; blocks >= desc_width
  * and (seq_lens given) blocks with b*block_size >= seq_lens[s] never match.
  * same = match as in dash_route's page mode; out = same, or 1 everywhere
  * when fallback != 0 and the row has no match.                             */

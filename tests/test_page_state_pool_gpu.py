@@ -111,3 +111,30 @@ def test_a_row_without_a_page_leaves_the_others_page_state():
         for x, y in zip(state_of_row(rich, 0), state_of_row(poor, 0)):
             assert torch.equal(x, y), step
     assert poor.block_table[1, 4].item() == -1
+
+
+def test_unused_table_entries_are_no_block():
+    """The dense mask: an entry below 0 holds no page, whatever page 0 holds."""
+    lo = torch.tensor([3, 1, -1], dtype=torch.int32).cuda()
+    hi = torch.tensor([3, 2, -1], dtype=torch.int32).cuda()
+    bt = torch.tensor([[1, 2, -1, -7], [1, 0, -1, -1]], dtype=torch.int32).cuda()
+    q = torch.tensor([3, 3, 2], dtype=torch.int32).cuda()
+    seq = torch.tensor([0, 1, 0], dtype=torch.int32).cuda()
+    out = P.page_allow(q, lo, hi, width=4, rows=3, row_seq=seq, block_table=bt, desc_width=4, fallback=True)
+    # row 0: no block of its sequence holds page 3: open; row 1: its block 1 does
+    assert out.bool().tolist() == [[True] * 4, [False, True, False, False], [True, False, False, False]]
+
+
+@pytest.mark.parametrize("mask", [False, True], ids=["domain", "mask"])
+def test_pool_decodes_as_the_fixed_table(mask):
+    """The same pages' contents under other ids, with unused table entries behind
+    them: the same routes and logits, bit for bit."""
+    ids = doc_ids(2, 1000, 4, 3)
+    a, b = make(2, mask=mask), make(2, pool=40, mask=mask)
+    assert torch.equal(a.prefill(a.embed[ids], token_ids=ids), b.prefill(b.embed[ids], token_ids=ids))
+    assert torch.equal(a.last_q_page, b.last_q_page) and torch.equal(a.last_route[0], b.last_route[0])
+    for i, t in enumerate((7, PG, 7, 8, IMG, IMG, 9)):
+        for d in (a, b):
+            d.tok.fill_(t)
+        assert torch.equal(a.decode_step(), b.decode_step()), i
+        assert torch.equal(a.oi, b.oi), i

@@ -474,7 +474,12 @@ class DashDecoder:
 
     @torch.no_grad()
     def compact(self) -> None:
-        """Moves the pool's pages to the lowest ids."""
+        """Moves the pool's pages to the lowest ids, with all that is kept by page:
+        caches, k-bar rows and the page state."""
         if self.pool is None:
             raise ValueError("compact needs a page pool (pool_pages)")
-        self.pool.compact(self.page_caches)
+        layers = self.page_caches
+        state = self.pst.page_tensors(self.num_pages) if self.pst is not None else []
+        if state:
+            layers = CacheLayers(layers.tensors + state)
+        self.pool.compact(layers)

@@ -95,6 +95,18 @@ class PageIsolationState:
         return (self._slot_img_page, self._slot_marker_cum, self._slot_img_run,
                 self._slot_prompt_pages)
 
+    def page_tensors(self, num_pages: int):
+        """The state as tensors indexed by physical page, [num_pages, block_size]
+        per slot and [num_pages, 1] per block (views): what has to move when pages
+        move.  Empty before the first step."""
+        if self._slot_img_page is None:
+            return []
+        n = num_pages * self.block_size
+        if self._num_slots < n:
+            raise ValueError(f"the state has {self._num_slots} slots, not {n}")
+        return [t[:n].view(num_pages, self.block_size) for t in self._slots] + \
+            [t[:num_pages, None] for t in (self._blk_lo, self._blk_hi)]
+
     @torch.no_grad()
     def step(self, input_ids: torch.Tensor, layout: BatchLayout, slot_mapping: torch.Tensor,
              num_slots: int) -> torch.Tensor:

@@ -138,3 +138,42 @@ def test_pool_decodes_as_the_fixed_table(mask):
             d.tok.fill_(t)
         assert torch.equal(a.decode_step(), b.decode_step()), i
         assert torch.equal(a.oi, b.oi), i
+
+
+@pytest.mark.parametrize("mask", [False, True], ids=["domain", "mask"])
+def test_compaction_takes_the_page_state_along(mask):
+    """Row 0 gives its pages back and the others' move down: rows 1 and 2 decode
+    as without the move, over page boundaries too, and their state is where their
+    pages are."""
+    ids = doc_ids(3, 1000, 4, 5)
+    a, b = make(3, pool=60, mask=mask), make(3, pool=60, mask=mask)
+    for d in (a, b):
+        d.prefill(d.embed[ids], token_ids=ids)
+        d.pool.free(d.rows[:1])
+        d.seq_lens[0] = 0
+    moved = b.block_table.clone()
+    b.compact()
+    assert (moved[1:] != b.block_table[1:]).any()
+    for r in (1, 2):
+        for x, y in zip(state_of_row(a, r), state_of_row(b, r)):
+            assert torch.equal(x, y), r
+    assert b.pst._blk_lo.numel() >= 60
+    lo, hi = b.pst.block_page_bounds(60)
+    held = b.block_table[1:].flatten().long()
+    held = held[held >= 0]
+    assert torch.equal(b.pst._blk_lo[held], lo.int()[held]) and torch.equal(b.pst._blk_hi[held], hi.int()[held])
+    for i, t in enumerate((7, PG, 7, IMG, IMG) + (9,) * 30):
+        for d in (a, b):
+            d.tok.fill_(t)
+        x, y = a.decode_step(), b.decode_step()
+        assert torch.equal(a.oi[1:], b.oi[1:]), i
+        assert torch.equal(x[1:], y[1:]), i
+
+
+def test_compaction_before_any_page_state():
+    """A decoder that has seen no token ids yet has no state to move."""
+    d = make(2, pool=40)
+    d.prefill(d.embed[doc_ids(2, 200, 1, 6)])
+    d.pool.free(d.rows[:1])
+    d.compact()
+    assert d.block_table[1].max().item() == 3

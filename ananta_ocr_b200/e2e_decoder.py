@@ -27,9 +27,10 @@ layers (speculative decoding, drafts.py), keeps a path of it and commits its cac
 entries.  With ``pool_pages`` the sequences draw their pages from a page_pool.PagePool
 instead of owning a fixed part of the cache; ``fork`` continues one sequence in
 another row, sharing its full pages when there is a pool.  Nothing waits for the
-GPU: a row that got no page (the pool is empty, drafts pass ``max_len``) or a
-malformed tree is recorded in ``errors``; the row's tokens mean nothing from
-there on, other rows are not touched.
+GPU: a token without a page (the pool is empty, the row is full) or a malformed
+tree is recorded in ``errors``.  A draft without a page is passed over, as if it
+had not been drafted.  A row whose next token has no page stays as long as its
+pages allow and its tokens mean nothing from there on; other rows are not touched.
 """
 from __future__ import annotations
 
@@ -131,12 +132,14 @@ class DashDecoder:
         # paged caches: one block of block_size tokens per page, random block table
         bs = c.block_size
         self.pps = -(-max_len // bs)
+        self.capacity = self.pps * bs                                   # tokens that a row's table holds
         P = batch * self.pps
         self.num_pages = P
         self.block_table = torch.randperm(P, generator=g, device=device).to(torch.int32).view(batch, self.pps).contiguous()
         self.pool = None
         self.errors = DeviceErrorWord(device)
         self.rows = torch.arange(batch, dtype=torch.int32, device=device)
+        self.one_each = torch.arange(batch + 1, dtype=torch.int32, device=device)
         if pool_pages:
             self.num_pages = P = pool_pages
             self.pool = PagePool(P, batch, self.pps, bs, device)
@@ -235,6 +238,8 @@ class DashDecoder:
         B, S, H = embeds.shape
         T = B * S
         dev = embeds.device
+        if S > self.capacity:
+            raise ValueError(f"sequences of {S} tokens do not fit the tables' {self.capacity}")
         x = embeds.reshape(T, H).clone()
         req = torch.arange(B, device=dev).repeat_interleave(S)
         pos = torch.arange(S, device=dev).repeat(B)
@@ -312,13 +317,15 @@ class DashDecoder:
         B, H = self.B, c.hidden
         dev = self.tok.device
         x = self.embed[self.tok]
-        pos = self.seq_lens.long()
-        req = torch.arange(B, device=dev)
-        cos, sin = self.rope_tables(pos)
+        cos, sin = self.rope_tables(self.seq_lens)
         sl = self.seq_lens + 1
         if self.pool is not None:
             self.pool.reserve(self.rows, sl, self.errors)
-        slots = self.slots_of(pos, req)
+        # a token behind the table's end has no slot, and the row's keys end there
+        slots = drafts.tree_plan(None, self.one_each, self.seq_lens, rows=B, max_nodes=1,
+                                 block_table=self.block_table, block_size=c.block_size, num_pages=self.num_pages,
+                                 device_error=self.errors).slots
+        sl.clamp_(max=self.capacity)
         tail = RT.kbar_tail_plan(block_table=self.block_table, seq_lens=sl,
                                  block_size=c.block_size, tail_pages=1, device=dev)
         domain = allow = None
@@ -360,7 +367,7 @@ class DashDecoder:
             x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
         logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
         self.tok.copy_(logits.argmax(-1))
-        self.seq_lens.add_(1)
+        self.seq_lens.copy_(sl)
         return logits
 
     # ---------------------------------------------------------------- drafts
@@ -378,7 +385,8 @@ class DashDecoder:
         drafts were drawn from).  The kept tokens' cache entries are moved
         together, the k-bar rows of their pages refreshed, ``self.seq_lens``
         advanced by the kept tokens and the root, and ``self.tok`` becomes the
-        next token.  Returns (drafts.Verified, logits [B, n, vocab])."""
+        next token.  A draft without a page (the row is full, the pool is empty) is
+        not kept.  Returns (drafts.Verified, logits [B, n, vocab])."""
         c = self.cfg
         if self.pst is not None:
             raise NotImplementedError("draft_step has no page-aware candidates (page state has no rewind)")
@@ -394,13 +402,16 @@ class DashDecoder:
             parents = parents.to(torch.int32).reshape(T)
         ctx = self.seq_lens
         if self.pool is not None:
-            self.pool.reserve(self.rows, ctx + n, self.errors)
+            # every root has its page before any draft, so that drafts cost no row its next token
+            self.pool.reserve(self.rows, ctx + 1, self.errors)
+            if n > 1:
+                self.pool.reserve(self.rows, (ctx + n).clamp_(max=self.capacity), self.errors)
         cu = torch.arange(B + 1, dtype=torch.int32, device=dev) * n
         plan = drafts.tree_plan(parents, cu, ctx, rows=T, max_nodes=n, block_table=self.block_table,
                                 block_size=c.block_size, num_pages=self.num_pages, device_error=self.errors)
         cos, sin = self.rope_tables(plan.row_pos)
         table = self.block_table.index_select(0, plan.row_seq)          # a row per token, for the router
-        sl = plan.row_pos + 1
+        sl = (plan.row_pos + 1).clamp_(max=self.capacity)
         x = self.embed[tokens]
         oi = torch.empty(T, c.slots, dtype=torch.int32, device=dev)
         ob = torch.empty(T, c.slots, dtype=torch.float32, device=dev)
@@ -426,6 +437,8 @@ class DashDecoder:
             x = x + F.linear(attn.view(T, H), L["wo"])
             x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
         logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
+        # a draft whose keys could not be stored is passed over
+        tokens = tokens.masked_fill(plan.slots < 0, -1)
         if temperature > 0:
             target = (logits.float() / temperature).softmax(-1)
             kept = drafts.verify_drafts(tokens, parents, cu, target, max_nodes=n, draft=draft_probs,
@@ -433,7 +446,7 @@ class DashDecoder:
         else:
             kept = drafts.verify_drafts(tokens, parents, cu, logits, max_nodes=n, greedy=True, device_error=self.errors)
         drafts.commit_drafts(self.token_caches, kept.path, kept.n_accept, ctx, self.block_table, self.errors)
-        now = ctx + kept.n_accept + 1
+        now = (ctx + kept.n_accept + 1).clamp_(max=self.capacity)
         fresh = RT.kbar_all_plan(block_table=self.block_table, seq_lens=now, context_lens=ctx,
                                  block_size=c.block_size, max_block=self.pps, max_query_len=n, device=dev)
         for li, L in enumerate(self.layers):

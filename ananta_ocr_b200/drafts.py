@@ -86,7 +86,7 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
 
     q, output [rows, H, 128]; k/v cache [num_pages, block, Hkv, 128] (bf16 or
     fp16, block == ``sparse_block_size``); topk_idx / blk_bias [Hkv, rows, K]
-    (usually one router head, expanded); block_table [n_seq, W]; cu_seqlens_q
+    (usually one router head, both expanded: anything else is copied first); block_table [n_seq, W]; cu_seqlens_q
     [n_seq + 1]; ctx_lens [n_seq] committed tokens; row_pos [rows] and tree_mask
     [rows, words] as ``tree_plan`` makes them.  A row attends its window of
     ``local_blocks * sparse_block_size`` committed tokens, its routed blocks
@@ -127,7 +127,8 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     if blk_bias is not None:
         if blk_bias.shape != ts or blk_bias.dtype is not torch.float32 or blk_bias.get_device() != index:
             raise ValueError(f"blk_bias must be fp32 of topk_idx's shape on cuda:{index}")
-    one = ist[0] == 0 or num_kv_heads == 1        # a router head that all kv heads share
+    # a router head that all kv heads share: ids and biases both
+    one = num_kv_heads == 1 or ist[0] == 0 and (blk_bias is None or blk_bias.stride(0) == 0)
     if K:
         if topk_idx.dtype is not torch.int32 or ist[2] != 1 or (blk_bias is not None and blk_bias.stride() != ist):
             # one layout for both; a shared router head is kept once

@@ -1,0 +1,63 @@
+"""Draft-tree attention at its edges: router heads shared in part.
+"""
+import numpy as np
+import pytest
+import torch
+
+from ananta_ocr_b200 import drafts
+from oracle import draft_oracle as DO
+from draft_testutil import attention_tolerance, make_tree
+
+pytestmark = pytest.mark.gpu
+SCALE = 1.0 / np.sqrt(128)
+LOW = np.finfo(np.float32).min
+
+
+def attend(t, idx, bias, *, splits=0, out=None, q=None, scale=SCALE, **over):
+    d = {k: over.get(k, v).cuda() for k, v in t.items() if isinstance(v, torch.Tensor)}
+    q = d["q"] if q is None else q
+    out = torch.full(q.shape, 7.0, dtype=t["dtype"], device="cuda") if out is None else out
+    z = torch.full(q.shape[:2], 7.0, device="cuda")
+    drafts.dash_sparse_attn_tree(q, d["kc"], d["vc"], idx, bias, d["t_bt"], d["t_cu"], d["t_ctx"], d["t_pos"],
+                                 d["t_mask"], max(t["nodes"]), t["Hkv"], scale, out, local_blocks=t["local_blocks"],
+                                 sparse_block_size=t["bs"], num_splits=splits, lse=z)
+    return out, z
+
+
+def exact(t, idx, bias, scale=SCALE):
+    return DO.tree_attend(t["q"].float().numpy(), t["kc"].float().numpy(), t["vc"].float().numpy(), idx, bias, t["bt"],
+                          t["starts"], t["ctx"], t["pos"], t["vis"], t["bs"], t["window"], scale)
+
+
+def close(t, got, want, rows=slice(None)):
+    out, z = (x.float().cpu().numpy()[rows] for x in got)
+    ref, lse, A = (x[rows] for x in want)
+    assert (np.abs(out - ref) <= attention_tolerance(ref, A, t["dtype"])).all()
+    none = np.isneginf(lse)
+    assert (np.isneginf(z) == none).all()
+    assert (np.abs(z - lse)[~none] <= 1e-4 + 1e-6 * np.abs(lse[~none])).all()
+
+
+# ---------------------------------------------------------------------------
+# router heads
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bs", [64, 48])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("shared", ["ids", "biases", "both", "neither", "ids_none"])
+def test_ids_and_biases_of_one_head_or_of_each(shared, dtype, bs):
+    """Ids and biases are per kv head each for itself: either may be one head
+    expanded over the others."""
+    t = make_tree(31, [9, 5], [800, 500], H=4, Hkv=2, bs=bs, window=1, K=5, index_heads=2)
+    idx, bias = t["idx"].copy(), t["bias"].copy()
+    if shared in ("ids", "both", "ids_none"):
+        idx[1] = idx[0]
+    if shared in ("biases", "both"):
+        bias[1] = bias[0]
+    gi, gb = torch.from_numpy(idx).cuda().to(dtype), torch.from_numpy(bias).cuda()
+    if shared in ("ids", "both", "ids_none"):
+        gi = gi[:1].expand(2, -1, -1)
+    if shared in ("biases", "both"):
+        gb = gb[:1].expand(2, -1, -1)
+    if shared == "ids_none":
+        gb = bias = None
+    close(t, attend(t, gi, gb), exact(t, idx, bias))

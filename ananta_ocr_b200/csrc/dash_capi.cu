@@ -630,7 +630,7 @@ int dash_pages_copy(const DashPagesCopyArgs* a, dash_stream_t stream) {
   if (rc || a->n == 0 || a->n_tensors == 0) return rc;
   if (!a->src || !a->dst) return set_error(DASH_ERR_INVALID, "null src/dst");
   if (a->check && !a->list) return set_error(DASH_ERR_INVALID, "a checked copy needs its list");
-  if (a->check && a->num_pages > (1 << 19))
+  if (a->check && a->num_pages > kPoolMaxPages)
     return set_error(DASH_ERR_UNSUPPORTED, "num_pages %lld > 2^19", (long long)a->num_pages);
   return launch_pages_copy(*a, (cudaStream_t)stream);
 }
@@ -640,8 +640,8 @@ static int check_pool(const DashPagePool& p) {
     return set_error(DASH_ERR_INVALID, "null pool tensor");
   if (p.num_pages <= 0 || p.max_rows <= 0 || p.bt_width <= 0 || p.block_size <= 0 || p.bt_stride < p.bt_width)
     return set_error(DASH_ERR_INVALID, "pool sizes must be > 0 and table rows must not overlap");
-  if (p.num_pages > (1 << 19)) return set_error(DASH_ERR_UNSUPPORTED, "num_pages %d > 2^19", p.num_pages);
-  if (p.max_rows > 8192) return set_error(DASH_ERR_UNSUPPORTED, "max_rows %d > 8192", p.max_rows);
+  if (p.num_pages > kPoolMaxPages) return set_error(DASH_ERR_UNSUPPORTED, "num_pages %d > 2^19", p.num_pages);
+  if (p.max_rows > kPoolMaxRows) return set_error(DASH_ERR_UNSUPPORTED, "max_rows %d > 8192", p.max_rows);
   return DASH_OK;
 }
 

@@ -51,6 +51,8 @@ int launch_tree_attn(const DashTreeAttnArgs& a, cudaStream_t st);
 bool tree_tc_supported(const DashTreeAttnArgs& a);
 int launch_tree_tc(const DashTreeAttnArgs& a, cudaStream_t st);
 int launch_verify(const DashVerifyArgs& a, cudaStream_t st);
+// the largest page pool (dash_pool.cu: its bit sets lie in shared memory)
+constexpr int kPoolMaxPages = 1 << 19, kPoolMaxRows = 8192;
 int launch_draft_commit(const DashCommitArgs& a, cudaStream_t st);
 int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st);
 int launch_pages_reserve(const DashPagesArgs& a, cudaStream_t st);

@@ -584,19 +584,23 @@ static int copy_pages(const DashCacheTensor* t, int n_tensors, const int32_t* sr
   return DASH_OK;
 }
 
-// shared memory above the default limit (48 KB with a kernel's static part)
+// Shared memory above the default limit (48 KB with a kernel's static part).  The
+// limit belongs to the kernel, not to the call: it is set to what the largest pool
+// needs, because a call that set its own need would take the limit from under a
+// larger one that another thread is about to launch.
+constexpr size_t kMaxRows = kPoolMaxRows, kMaxPageWords = kPoolMaxPages / 32;
 template <typename K>
-static int allow_smem(K kernel, size_t bytes, const char* name) {
+static int allow_smem(K kernel, size_t bytes, size_t most, const char* name) {
   if (bytes > 24 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess)
-    return set_error(DASH_ERR_CUDA, "%s: %zu bytes of shared memory refused", name, bytes);
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess)
+    return set_error(DASH_ERR_CUDA, "%s: %zu bytes of shared memory refused", name, most);
   return DASH_OK;
 }
 
 int launch_pages_copy(const DashPagesCopyArgs& a, cudaStream_t st) {
   if (!a.check) return copy_pages(a.tensors, a.n_tensors, a.src, a.dst, a.n, a.count, a.num_pages, TableMap{}, st);
   const size_t smem = (size_t)((a.num_pages + 31) / 32) * 3 * 4;
-  int rc = allow_smem(pages_check_kernel, smem, "pages_check_kernel");
+  int rc = allow_smem(pages_check_kernel, smem, kMaxPageWords * 3 * 4, "pages_check_kernel");
   if (rc) return rc;
   pages_check_kernel<<<1, kPoolThreads, smem, st>>>(a.src, a.dst, a.n, a.count, (int)a.num_pages, a.list,
                                                     a.device_error);
@@ -623,7 +627,7 @@ int launch_draft_commit(const DashCommitArgs& a, cudaStream_t st) {
 
 int launch_pages_reserve(const DashPagesArgs& a, cudaStream_t st) {
   const size_t smem = (size_t)a.pool.max_rows * 4;
-  const int rc = allow_smem(pages_reserve_kernel, smem, "pages_reserve_kernel");
+  const int rc = allow_smem(pages_reserve_kernel, smem, kMaxRows * 4, "pages_reserve_kernel");
   if (rc) return rc;
   pages_reserve_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();
@@ -632,7 +636,7 @@ int launch_pages_reserve(const DashPagesArgs& a, cudaStream_t st) {
 
 int launch_pages_fork(const DashPagesArgs& a, cudaStream_t st) {
   const size_t smem = (size_t)a.pool.max_rows * 4;
-  const int rc = allow_smem(pages_fork_kernel, smem, "pages_fork_kernel");
+  const int rc = allow_smem(pages_fork_kernel, smem, kMaxRows * 4, "pages_fork_kernel");
   if (rc) return rc;
   pages_fork_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();
@@ -645,7 +649,7 @@ int launch_pages_fork(const DashPagesArgs& a, cudaStream_t st) {
 int launch_pages_free(const DashPagesArgs& a, cudaStream_t st) {
   const size_t words = (size_t)(a.pool.num_pages + 31) / 32;
   const size_t smem = ((size_t)a.pool.max_rows + 2 * words + 1) * 4;
-  const int rc = allow_smem(pages_free_kernel, smem, "pages_free_kernel");
+  const int rc = allow_smem(pages_free_kernel, smem, (kMaxRows + 2 * kMaxPageWords + 1) * 4, "pages_free_kernel");
   if (rc) return rc;
   pages_free_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();
@@ -655,7 +659,7 @@ int launch_pages_free(const DashPagesArgs& a, cudaStream_t st) {
 int launch_pages_compact(const DashPagesArgs& a, cudaStream_t st) {
   const size_t words = (size_t)(a.pool.num_pages + 31) / 32;
   const size_t smem = (2 * words + 1) * 4;
-  const int rc = allow_smem(pages_compact_kernel, smem, "pages_compact_kernel");
+  const int rc = allow_smem(pages_compact_kernel, smem, (2 * kMaxPageWords + 1) * 4, "pages_compact_kernel");
   if (rc) return rc;
   pages_compact_kernel<<<1, kPoolThreads, smem, st>>>(a);
   count_launch();

@@ -27,7 +27,9 @@ def _routes_from(topk_idx, blk_bias, num_kv_heads):
     idx = topk_idx if topk_idx.dtype == torch.int32 else topk_idx.to(torch.int32)
     if idx.stride(2) != 1:
         idx = idx.contiguous()
-    nih = 1 if idx.stride(0) == 0 or idx.shape[0] == 1 else num_kv_heads
+    # one router head for all kv heads: ids and biases both
+    one = idx.shape[0] == 1 or (idx.stride(0) == 0 and (blk_bias is None or blk_bias.stride(0) == 0))
+    nih = 1 if one else num_kv_heads
     bias = None
     if blk_bias is not None:
         assert blk_bias.shape == topk_idx.shape, (blk_bias.shape, topk_idx.shape)

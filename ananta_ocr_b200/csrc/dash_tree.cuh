@@ -4,9 +4,11 @@
 // is not finite reached their sums (dash_tree_tc.cu).
 //
 // A warp is 4 groups of 8 lanes; group g takes keys g, g + 4, ... of a range,
-// lane `sub` 16 of the 128 dims.  Every group keeps a running maximum and sum in
-// the exp2 domain; the groups are merged at the end.  Only keys that the row
-// attends are read, so what lies in other rows of a page cannot reach it.
+// lane `sub` 16 of the 128 dims.  Every group keeps a running maximum and sum;
+// the groups are merged at the end.  Logits and maximum are in natural units,
+// where every bias of the type has its place: times log2(e) the lowest ones
+// would be -inf.  Only keys that the row attends are read, so what lies in
+// other rows of a page cannot reach it.
 #pragma once
 #include "dash_common.cuh"
 #include "dash_internal.h"
@@ -63,8 +65,8 @@ __device__ __forceinline__ void tree_unpack8(const uint4 w, float* x, __half* t)
 }
 
 // Attention of packed row r (token of sequence s) and query head hq; the whole
-// warp calls it.  On return every lane holds the row's maximum m (exp2 domain,
-// -inf without a key), sum l and dims [16 sub, 16 sub + 16) of the unscaled
+// warp calls it.  On return every lane holds the row's maximum m (-inf without a
+// key), sum l and dims [16 sub, 16 sub + 16) of the unscaled
 // output, the same in all four groups.
 template <typename T>
 __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, int s, int64_t r, int hq, float& m,
@@ -82,9 +84,8 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
                                                      (int64_t)hq * a.qo.q_stride_head + sub * 16);
     tree_unpack8(__ldg(qp), q, (T*)nullptr);
     tree_unpack8(__ldg(qp + 1), q + 8, (T*)nullptr);
-    const float sl2 = a.scale * kTreeLog2e;
 #pragma unroll
-    for (int c = 0; c < 16; ++c) q[c] *= sl2;
+    for (int c = 0; c < 16; ++c) q[c] *= a.scale;
   }
   m = -INFINITY;
   l = 0.0f;
@@ -97,7 +98,7 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
     if (lane == 0) record_error(a.device_error, DASH_DEV_BAD_PAGE, 70, p);
     return -1;
   };
-  // keys [t0, t1) of block b with the additive term b2; vis != null: only
+  // keys [t0, t1) of block b with the bias b2; vis != null: only
   // the drafted tokens whose bit is set there (token u is key sq.ctx + u)
   auto block = [&](int b, int t0, int t1, float b2, const uint32_t* vis) {
     if (t1 <= t0) return;
@@ -131,8 +132,8 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
         sc += b2;
         const float mn = fmaxf(m, sc);
         if (mn != -INFINITY || sc != sc) {
-          const float al = m == -INFINITY ? 0.0f : fast_exp2(m - mn);
-          const float p = fast_exp2(sc - mn);
+          const float al = m == -INFINITY ? 0.0f : fast_exp2((m - mn) * kTreeLog2e);
+          const float p = fast_exp2((sc - mn) * kTreeLog2e);
           l = l * al + p;
 #pragma unroll
           for (int c = 0; c < 16; ++c) o[c] = fmaf(p, v[c], o[c] * al);
@@ -155,7 +156,7 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
     bool again = false;                                                      // the first occurrence counts
     for (int u = lane; u < j; u += 32) again |= a.routes.idx[roff + u] == b;
     if (__any_sync(0xffffffffu, again)) continue;
-    const float b2 = a.routes.bias ? a.routes.bias[roff + j] * kTreeLog2e : 0.0f;
+    const float b2 = a.routes.bias ? a.routes.bias[roff + j] : 0.0f;
     const int t0 = (int)min((int64_t)b * bs, (int64_t)lstart);
     block(b, t0, (int)min((int64_t)(b + 1) * bs, (int64_t)lstart), b2, nullptr);
   }
@@ -175,8 +176,8 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
   for (int off = 8; off < 32; off <<= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, off), l2 = __shfl_xor_sync(0xffffffffu, l, off);
     const float mn = fmaxf(m, m2);
-    const float fa = m == -INFINITY ? (l == l ? 0.0f : 1.0f) : fast_exp2(m - mn);
-    const float fb = m2 == -INFINITY ? (l2 == l2 ? 0.0f : 1.0f) : fast_exp2(m2 - mn);
+    const float fa = m == -INFINITY ? (l == l ? 0.0f : 1.0f) : fast_exp2((m - mn) * kTreeLog2e);
+    const float fb = m2 == -INFINITY ? (l2 == l2 ? 0.0f : 1.0f) : fast_exp2((m2 - mn) * kTreeLog2e);
     l = l * fa + l2 * fb;
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
@@ -203,7 +204,7 @@ __device__ __forceinline__ void tree_row_store(const DashTreeAttnArgs& a, int64_
   *reinterpret_cast<uint4*>(op + 8) = make_uint4(w[4], w[5], w[6], w[7]);
   if (lane == 0 && a.qo.lse)
     a.qo.lse[r * a.qo.lse_stride_tok + (int64_t)hq * a.qo.lse_stride_head] =
-        none ? -INFINITY : (m + log2f(l)) * kTreeLn2;
+        none ? -INFINITY : m + log2f(l) * kTreeLn2;
 }
 
 }  // namespace dash

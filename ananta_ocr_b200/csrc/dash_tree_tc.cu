@@ -42,10 +42,14 @@
 // A masked key has P = 0, and 0 * v is 0 only for finite v.  V rows behind the last
 // drafted token are zeroed; a row whose joined output is not finite for any
 // other reason (a bad value in a key that some other row attends, or in its own)
-// is computed again from its own keys only (tree_row_attend), so no row
-// depends on keys that it does not attend.
+// is computed again from its own keys only (tree_row_attend), so no row's
+// result depends on keys that it does not attend, except in its last bits: there
+// the weights are not rounded to the caches' type.  Computed again is also a row
+// that has no key but in blocks of the lowest biases (below -1e30, where a bias
+// times log2(e) may leave the type's range and the logit is lost beside it).
 #include <cooperative_groups.h>
 #include <cudaTypedefs.h>
+#include <cfloat>
 #include "dash_tree.cuh"
 
 namespace cg = cooperative_groups;
@@ -61,6 +65,7 @@ constexpr int kMaxCluster = 16;
 constexpr int kMaxWords = 256;                   // 8192 granules of a sequence
 constexpr uint32_t kTmemCols = 256;              // S0 | S1 | O
 constexpr float kGrow = 8.0f;                    // O is rescaled when a row's maximum grows by 2^8
+constexpr float kFar = -1e30f;                   // below it a row's maximum is one of the lowest biases'
 
 // QR: rows of Q that are kept (32, 64 or 128)
 template <int QR>
@@ -530,8 +535,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       auto bias_of = [&](int e) {
         const int slot = e & ((1 << pad) - 1);
-        return a.routes.bias && e < entries && slot < K
-                   ? __ldg(a.routes.bias + rbase + (int64_t)(e >> pad) * a.routes.row_stride + slot) * kTreeLog2e : 0.0f;
+        const float b = a.routes.bias && e < entries && slot < K
+                            ? __ldg(a.routes.bias + rbase + (int64_t)(e >> pad) * a.routes.row_stride + slot) : 0.0f;
+        // a finite bias stays finite: its block has keys, if far ones (see kFar)
+        return b >= -FLT_MAX ? fmaxf(b * kTreeLog2e, -FLT_MAX) : b;
       };
       float next = bias_of(entry(0));
 #pragma unroll 1
@@ -753,7 +760,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           a.qo.lse[r * a.qo.lse_stride_tok + (int64_t)hq * a.qo.lse_stride_head] =
               l_run > 0.0f ? (m_run + log2f(l_run)) * kTreeLn2 : -INFINITY;
         __syncwarp();                            // these stores come before those of redo_row
-        for (uint32_t bad = __ballot_sync(0xffffffffu, row_ok && !(chk == 0.0f)); bad; bad &= bad - 1)
+        const bool far = m_run < kFar && m_run != -INFINITY;
+        for (uint32_t bad = __ballot_sync(0xffffffffu, row_ok && (!(chk == 0.0f) || far)); bad; bad &= bad - 1)
           redo_row<T>(a, sq, s, r0, warp * 32 + __ffs(bad) - 1, G, hk);
       } else {
         S.m[m] = m_run;
@@ -808,7 +816,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
     }
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-    const bool fine = (O.x + O.y + O.z + O.w + L) * 0.0f == 0.0f;
+    const bool fine = (O.x + O.y + O.z + O.w + L) * 0.0f == 0.0f && !(M < kFar && M != -INFINITY);
     if (!__all_sync(0xffffffffu, fine)) {
       redo_row<T>(a, sq, s, r0, m, G, hk);
       continue;

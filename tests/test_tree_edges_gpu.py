@@ -1,5 +1,5 @@
-"""Draft-tree attention at its edges: router heads shared in part.
-"""
+"""Draft-tree attention at its edges: router heads shared in part, biases of the
+type's lowest value."""
 import numpy as np
 import pytest
 import torch
@@ -35,7 +35,7 @@ def close(t, got, want, rows=slice(None)):
     assert (np.abs(out - ref) <= attention_tolerance(ref, A, t["dtype"])).all()
     none = np.isneginf(lse)
     assert (np.isneginf(z) == none).all()
-    assert (np.abs(z - lse)[~none] <= 1e-4 + 1e-6 * np.abs(lse[~none])).all()
+    assert (np.abs(z[~none] - lse[~none]) <= 1e-4 + 1e-6 * np.abs(lse[~none])).all()
 
 
 # ---------------------------------------------------------------------------
@@ -61,3 +61,36 @@ def test_ids_and_biases_of_one_head_or_of_each(shared, dtype, bs):
     if shared == "ids_none":
         gb = bias = None
     close(t, attend(t, gi, gb), exact(t, idx, bias))
+
+
+# ---------------------------------------------------------------------------
+# biases
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("bs", [64, 32, 48])
+def test_lowest_biases_alone(bs, splits):
+    """Rows whose only keys lie in blocks of lowest biases: in the sum of logit and
+    bias the logit vanishes (in 32 bits as in 64), so the keys of the largest bias
+    share the weight equally; lse is that bias.  Beside another key they add
+    nothing.  Biases: the lowest value, values whose product with log2(e) is past
+    the type's range, one just inside it, -1e35, and -inf (no key at all)."""
+    n = 8
+    t = make_tree(32, [n], [6 * bs], H=2, Hkv=2, bs=bs, window=0, K=3)
+    t["idx"][0] = np.array([[0, 2, 5]] * n)
+    t["vis"][:] = False
+    t["t_mask"].zero_()
+    b = t["bias"][0]
+    b[0] = LOW
+    b[1] = [LOW, -3.0e38, LOW]
+    b[2] = [-2.5e38, -2.4e38, -2.4e38]
+    b[3] = [-2.3e38, LOW, -2.3e38]
+    b[4] = [-1e35, -1e35, LOW]
+    b[5] = [-np.inf, LOW, -np.inf]
+    b[6] = -np.inf
+    b[7] = [LOW, 1.0, -np.inf]
+    t["idx"][0, 5] = [4, -1, 4]                            # the repeated id: the first, -inf, counts
+    b[5] = [-np.inf, 0.0, LOW]
+    want = exact(t, t["idx"], t["bias"])
+    assert np.isneginf(want[1][5:7]).all()
+    gi, gb = torch.from_numpy(t["idx"]).cuda().expand(2, -1, -1), torch.from_numpy(t["bias"]).cuda().expand(2, -1, -1)
+    close(t, attend(t, gi, gb, splits=splits), want)

@@ -157,6 +157,7 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
     for (int u = lane; u < j; u += 32) again |= a.routes.idx[roff + u] == b;
     if (__any_sync(0xffffffffu, again)) continue;
     const float b2 = a.routes.bias ? a.routes.bias[roff + j] : 0.0f;
+    if (b2 == -INFINITY) continue;                                           // masked: nothing in it counts
     const int t0 = (int)min((int64_t)b * bs, (int64_t)lstart);
     block(b, t0, (int)min((int64_t)(b + 1) * bs, (int64_t)lstart), b2, nullptr);
   }

@@ -854,7 +854,8 @@ int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
  *                            scale*<q,k_j> + bias of that slot
  *   drafted keys ctx + u, u < n:  bit u of the row's mask set: scale*<q,k>
  * out = softmax @ V; a row without a key gets 0 and lse -inf.  Ids repeated
- * in a row count once (first occurrence), -1 slots are unused.  Keys on a page
+ * in a row count once (first occurrence), -1 slots are unused, and a slot with a
+ * bias of -inf masks its block whatever lies in it.  Keys on a page
  * outside [0, num_pages) are left out and recorded.  K/V, q and out are bf16
  * or fp16, paged (block_table set), head_dim 128, page size == block_size;
  * block_size 16, 32 and multiples of 64 up to 256 run on the tensor cores

@@ -1,5 +1,5 @@
 """Draft-tree attention at its edges: router heads shared in part, biases of the
-type's lowest value."""
+type's lowest value and of -inf."""
 import numpy as np
 import pytest
 import torch
@@ -92,5 +92,24 @@ def test_lowest_biases_alone(bs, splits):
     b[5] = [-np.inf, 0.0, LOW]
     want = exact(t, t["idx"], t["bias"])
     assert np.isneginf(want[1][5:7]).all()
+    gi, gb = torch.from_numpy(t["idx"]).cuda().expand(2, -1, -1), torch.from_numpy(t["bias"]).cuda().expand(2, -1, -1)
+    close(t, attend(t, gi, gb, splits=splits), want)
+
+
+@pytest.mark.parametrize("splits", [0, 1, 3])
+@pytest.mark.parametrize("bs", [64, 32, 48])
+def test_what_a_bias_of_minus_infinity_masks_may_hold_anything(bs, splits):
+    """A bias of -inf masks a block: NaN and infinities in it stay out."""
+    n = 6
+    t = make_tree(33, [n], [6 * bs], H=2, Hkv=2, bs=bs, window=1, K=3)
+    t["idx"][0] = np.array([[0, 2, 3]] * n)
+    t["bias"][0, :, 1] = -np.inf
+    t["bias"][0, 4] = -np.inf                             # only the drafts are left
+    page = int(t["bt"][0, 2])
+    want = exact(t, t["idx"], t["bias"])
+    t["kc"][page, 3, :, 5] = float("nan")
+    t["kc"][page, 4] = float("inf")
+    t["vc"][page, 5:9] = float("nan")
+    t["vc"][page, 9, :, ::2] = -float("inf")
     gi, gb = torch.from_numpy(t["idx"]).cuda().expand(2, -1, -1), torch.from_numpy(t["bias"]).cuda().expand(2, -1, -1)
     close(t, attend(t, gi, gb, splits=splits), want)

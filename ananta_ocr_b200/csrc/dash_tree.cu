@@ -72,8 +72,11 @@ __global__ void __launch_bounds__(kTreeRowWarps * 32) tree_rows_kernel(const __g
   const int s = tree_seq_of_row(a.seqs.q_start, a.seqs.n_seq, r);
   const TreeSeq sq = tree_seq(a.seqs.q_start, a.ctx_len, a.seqs.q_len_fixed, a.seqs.max_q_len, s);
   if (r - sq.row0 >= sq.n) return;
-  float m, l, o[16];
-  tree_row_attend<T>(a, sq, s, r, hq, m, l, o);
+  const uint4* qp = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.qo.q) + r * a.qo.q_stride_tok +
+                                                   (int64_t)hq * a.qo.q_stride_head + (threadIdx.x & 7) * 16);
+  float q[16], m, l, o[16];
+  tree_load_q<T>(qp[0], qp[1], q);
+  tree_row_attend<T>(a, sq, s, r, hq, q, a.scale, m, l, o);
   tree_row_store<T>(a, r, hq, m, l, o);
 }
 

@@ -64,13 +64,20 @@ __device__ __forceinline__ void tree_unpack8(const uint4 w, float* x, __half* t)
   }
 }
 
-// Attention of packed row r (token of sequence s) and query head hq; the whole
-// warp calls it.  On return every lane holds the row's maximum m (-inf without a
-// key), sum l and dims [16 sub, 16 sub + 16) of the unscaled
-// output, the same in all four groups.
+// A lane's 16 dims of a query row, from its first dim's 16-byte piece and the next.
 template <typename T>
-__device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, int s, int64_t r, int hq, float& m,
-                                float& l, float (&o)[16]) {
+__device__ __forceinline__ void tree_load_q(const uint4& lo, const uint4& hi, float (&q)[16]) {
+  tree_unpack8(lo, q, (T*)nullptr);
+  tree_unpack8(hi, q + 8, (T*)nullptr);
+}
+
+// Attention of packed row r (token of sequence s) and query head hq, whose dims
+// [16 sub, 16 sub + 16) the caller has read into q; the whole warp calls it.  On
+// return every lane holds the row's maximum m (-inf without a key), sum l and its
+// dims of the unscaled output, the same in all four groups.
+template <typename T>
+__device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, int s, int64_t r, int hq,
+                                float (&q)[16], float scale, float& m, float& l, float (&o)[16]) {
   const int lane = threadIdx.x & 31, grp = lane >> 3, sub = lane & 7;
   const int H = a.qo.n_heads, hk = hq / (H / a.kv.n_kv_heads), bs = a.block_size;
   const int nih = a.routes.n_index_heads > 0 ? a.routes.n_index_heads : 1;
@@ -78,15 +85,8 @@ __device__ void tree_row_attend(const DashTreeAttnArgs& a, const TreeSeq& sq, in
   const T* kp = reinterpret_cast<const T*>(a.kv.k) + (int64_t)hk * a.kv.stride_head + sub * 16;
   const T* vp = reinterpret_cast<const T*>(a.kv.v) + (int64_t)hk * a.kv.stride_head + sub * 16;
   const int32_t* bt = a.kv.block_table + (int64_t)s * a.kv.bt_stride;
-  float q[16];
-  {
-    const uint4* qp = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.qo.q) + r * a.qo.q_stride_tok +
-                                                     (int64_t)hq * a.qo.q_stride_head + sub * 16);
-    tree_unpack8(__ldg(qp), q, (T*)nullptr);
-    tree_unpack8(__ldg(qp + 1), q + 8, (T*)nullptr);
 #pragma unroll
-    for (int c = 0; c < 16; ++c) q[c] *= a.scale;
-  }
+  for (int c = 0; c < 16; ++c) q[c] *= scale;
   m = -INFINITY;
   l = 0.0f;
 #pragma unroll

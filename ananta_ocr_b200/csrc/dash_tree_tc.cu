@@ -97,13 +97,19 @@ constexpr bool fits() {
 }
 static_assert(fits<32>() && fits<64>() && fits<128>(), "shared memory of a CTA");
 
-// Row m of a unit from its own keys only (the whole warp).
+// Row m of a unit from its own keys only (the whole warp).  Its query comes from the
+// operand tile sq_q (halves of `half` bytes), because the output may lie on q.
 template <typename T>
 __device__ __noinline__ void redo_row(const DashTreeAttnArgs& a, TreeSeq sq, int s, int64_t r0, int m, int G,
-                                      int hk) {
+                                      int hk, const uint8_t* sq_q, int half) {
   const int node = m / G, hq = hk * G + m - node * G;
-  float ms, ls, os[16];
-  tree_row_attend<T>(a, sq, s, r0 + node, hq, ms, ls, os);
+  const int c0 = 2 * (threadIdx.x & 7), c1 = c0 + 1;             // the lane's 16-byte pieces
+  auto piece = [&](int c) {
+    return *reinterpret_cast<const uint4*>(sq_q + (c >> 3) * half + m * 128 + (((c & 7) ^ (m & 7)) << 4));
+  };
+  float q[16], ms, ls, os[16];
+  tree_load_q<T>(piece(c0), piece(c1), q);
+  tree_row_attend<T>(a, sq, s, r0 + node, hq, q, fabsf(a.scale), ms, ls, os);     // (its sign is in the tile)
   tree_row_store<T>(a, r0 + node, hq, ms, ls, os);
 }
 
@@ -342,6 +348,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int share = (n_tile + nsp - 1) / nsp;
   const int first = min(n_tile, split * share), tiles = min(n_tile, first + share) - first;
   const int rank0 = first * NG;
+  uint32_t redo = 0;                             // rows of this warp to be computed again
 
   if (warp >= 4) {
     // Q has come (requested at the start)
@@ -759,10 +766,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (row_ok && a.qo.lse)
           a.qo.lse[r * a.qo.lse_stride_tok + (int64_t)hq * a.qo.lse_stride_head] =
               l_run > 0.0f ? (m_run + log2f(l_run)) * kTreeLn2 : -INFINITY;
-        __syncwarp();                            // these stores come before those of redo_row
         const bool far = m_run < kFar && m_run != -INFINITY;
-        for (uint32_t bad = __ballot_sync(0xffffffffu, row_ok && (!(chk == 0.0f) || far)); bad; bad &= bad - 1)
-          redo_row<T>(a, sq, s, r0, warp * 32 + __ffs(bad) - 1, G, hk);
+        redo = __ballot_sync(0xffffffffu, row_ok && (!(chk == 0.0f) || far));
       } else {
         S.m[m] = m_run;
         S.l[m] = tiles > 0 ? l_run : -1.0f;      // -1: this CTA had no tile
@@ -774,6 +779,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   tc_fence_after();
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
   if (nsp == 1) {
+    // (the stores above come before these, and Q is in place for every thread)
+    for (; redo; redo &= redo - 1) redo_row<T>(a, sq, s, r0, warp * 32 + __ffs(redo) - 1, G, hk, S.q, QR * 128);
     after_first();
     return;
   }
@@ -818,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     const bool fine = (O.x + O.y + O.z + O.w + L) * 0.0f == 0.0f && !(M < kFar && M != -INFINITY);
     if (!__all_sync(0xffffffffu, fine)) {
-      redo_row<T>(a, sq, s, r0, m, G, hk);
+      redo_row<T>(a, sq, s, r0, m, G, hk, S.q, QR * 128);
       continue;
     }
     T* op = reinterpret_cast<T*>(a.qo.out) + r * a.qo.o_stride_tok + (int64_t)hq * a.qo.o_stride_head + lane * 4;

@@ -91,8 +91,9 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     [rows, words] as ``tree_plan`` makes them.  A row attends its window of
     ``local_blocks * sparse_block_size`` committed tokens, its routed blocks
     (with their biases) before it, and the drafted tokens of its mask.  Rows
-    from ``cu_seqlens_q[-1]`` on are left as they were.  lse [rows, H] fp32:
-    natural-log sums.  num_splits: CTAs per sequence and kv head (0 = automatic)."""
+    from ``cu_seqlens_q[-1]`` on are left as they were.  output may be q itself.
+    lse [rows, H] fp32: natural-log sums.  num_splits: CTAs per sequence and kv head
+    (0 = automatic)."""
     index, dt = q.get_device(), q.dtype
     qs, ks, ts, ms = q.shape, k_cache.shape, topk_idx.shape, tree_mask.shape
     qst, kst, ist = q.stride(), k_cache.stride(), topk_idx.stride()

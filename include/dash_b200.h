@@ -853,7 +853,8 @@ int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
  *                            else, block j/block_size routed for the row:
  *                            scale*<q,k_j> + bias of that slot
  *   drafted keys ctx + u, u < n:  bit u of the row's mask set: scale*<q,k>
- * out = softmax @ V; a row without a key gets 0 and lse -inf.  Ids repeated
+ * out = softmax @ V; a row without a key gets 0 and lse -inf.  out may be q
+ * itself (same address and strides).  Ids repeated
  * in a row count once (first occurrence), -1 slots are unused, and a slot with a
  * bias of -inf masks its block whatever lies in it.  Keys on a page
  * outside [0, num_pages) are left out and recorded.  K/V, q and out are bf16

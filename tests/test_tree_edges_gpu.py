@@ -1,5 +1,5 @@
 """Draft-tree attention at its edges: router heads shared in part, biases of the
-type's lowest value and of -inf."""
+type's lowest value and of -inf, an output that lies on q."""
 import numpy as np
 import pytest
 import torch
@@ -113,3 +113,28 @@ def test_what_a_bias_of_minus_infinity_masks_may_hold_anything(bs, splits):
     t["vc"][page, 9, :, ::2] = -float("inf")
     gi, gb = torch.from_numpy(t["idx"]).cuda().expand(2, -1, -1), torch.from_numpy(t["bias"]).cuda().expand(2, -1, -1)
     close(t, attend(t, gi, gb, splits=splits), want)
+
+
+# ---------------------------------------------------------------------------
+# an output that lies on q
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("scale", [SCALE, -SCALE])
+@pytest.mark.parametrize("splits", [1, 0, 3])
+@pytest.mark.parametrize("bs", [64, 48])
+def test_output_in_place_of_q(bs, splits, scale):
+    """The result may be written over q; also for the rows that are computed again
+    because a neighbour attends a NaN (rows of token 0 do, all others must not)."""
+    n = 9
+    t = make_tree(34, [n], [6 * bs], H=4, Hkv=2, bs=bs, window=1, K=3)
+    t["idx"][0] = np.array([[0, -1, 3]] * n)
+    t["idx"][0, 0, 1] = 2
+    want = exact(t, t["idx"], t["bias"], scale)
+    t["vc"][int(t["bt"][0, 2]), 5] = float("nan")
+    gi, gb = torch.from_numpy(t["idx"]).cuda().expand(2, -1, -1), torch.from_numpy(t["bias"]).cuda().expand(2, -1, -1)
+    got = attend(t, gi, gb, splits=splits, scale=scale)
+    close(t, got, want, slice(1, None))
+    q = t["q"].cuda()
+    here = attend(t, gi, gb, splits=splits, scale=scale, q=q, out=q)
+    assert here[0] is q and torch.isnan(q[0]).any()
+    close(t, here, want, slice(1, None))
+    assert torch.equal(here[0][1:], got[0][1:]) and torch.equal(here[1][1:], got[1][1:])

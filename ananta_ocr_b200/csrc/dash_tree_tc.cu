@@ -542,10 +542,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       auto bias_of = [&](int e) {
         const int slot = e & ((1 << pad) - 1);
-        const float b = a.routes.bias && e < entries && slot < K
-                            ? __ldg(a.routes.bias + rbase + (int64_t)(e >> pad) * a.routes.row_stride + slot) : 0.0f;
-        // a finite bias stays finite: its block has keys, if far ones (see kFar)
-        return b >= -FLT_MAX ? fmaxf(b * kTreeLog2e, -FLT_MAX) : b;
+        return a.routes.bias && e < entries && slot < K
+                   ? __ldg(a.routes.bias + rbase + (int64_t)(e >> pad) * a.routes.row_stride + slot) : 0.0f;
       };
       float next = bias_of(entry(0));
 #pragma unroll 1
@@ -561,9 +559,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int rk1 = min(rk + (int)(v & 7u), c1);
         rk = max(rk, c0);
         const uint32_t same = __match_any_sync(0xffffffffu, v << 5 | (uint32_t)(lane >> lp));
-        if (__ffs(same) - 1 == lane)
+        if (__ffs(same) - 1 == lane) {
+          // a finite bias stays finite: its block has keys, if far ones (see kFar)
+          const float term = bias >= -FLT_MAX ? fmaxf(bias * kTreeLog2e, -FLT_MAX) : bias;
 #pragma unroll 1
-          for (float* c = S.cell + (rk - c0) * nt + nd; rk < rk1; ++rk, c += nt) *c = bias;
+          for (float* c = S.cell + (rk - c0) * nt + nd; rk < rk1; ++rk, c += nt) *c = term;
+        }
         __syncwarp();
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");

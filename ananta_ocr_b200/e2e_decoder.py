@@ -397,6 +397,14 @@ class DashDecoder:
             raise ValueError(f"{n - 1} drafts reach past the local window's whole blocks "
                              f"({(c.local_blocks - 1) * c.block_size} tokens)")
         T = B * n
+        # refused before anything is written
+        if drafted.shape[0] != B or (parents is not None and parents.numel() != T):
+            raise ValueError(f"drafted must be [{B}, n - 1] and parents [{B}, n]")
+        if temperature > 0:
+            if u_accept is None or u_sample is None or u_accept.shape != (T,) or u_sample.shape != (B,):
+                raise ValueError(f"a temperature needs u_accept [{T}] and u_sample [{B}]")
+            if draft_probs is not None and (draft_probs.shape != (T, c.vocab) or draft_probs.dtype != torch.float32):
+                raise ValueError(f"draft_probs must be fp32 [{T}, {c.vocab}]")
         tokens = torch.cat([self.tok[:, None], drafted], 1).reshape(T)
         if parents is not None:
             parents = parents.to(torch.int32).reshape(T)

@@ -135,3 +135,22 @@ def test_a_prefill_longer_than_the_tables():
     d = make(max_len=64)
     with pytest.raises(ValueError, match="do not fit"):
         d.prefill(d.embed[ids_of(65, 6)])
+
+
+def test_refused_calls_change_nothing():
+    """What draft_step refuses it refuses before it takes pages or writes."""
+    d = started(ids_of(64, 7), [64, 64], 8)
+    good = dict(temperature=1.0, u_accept=torch.zeros(8, device="cuda"), u_sample=torch.zeros(2, device="cuda"))
+    x = ids_of(3, 8)
+    before = [t.clone() for t in (*d.kc, *d.ic, d.pool.block_table, d.pool.n_free, d.seq_lens, d.tok)]
+    for args, kw in (((x,), dict(good, u_accept=None)), ((x,), dict(good, u_sample=None)),
+                     ((x,), dict(good, u_accept=torch.zeros(7, device="cuda"))),
+                     ((x,), dict(good, draft_probs=torch.zeros(8, 999, device="cuda"))),
+                     ((x,), dict(good, draft_probs=torch.zeros(8, 1000, device="cuda").half())),
+                     ((x[:1],), {}),
+                     ((x, torch.zeros(2, 3, dtype=torch.int32, device="cuda")), {})):
+        with pytest.raises(ValueError):
+            d.draft_step(*args, **kw)
+    for a, b in zip(before, (*d.kc, *d.ic, d.pool.block_table, d.pool.n_free, d.seq_lens, d.tok)):
+        assert torch.equal(a, b)
+    d.draft_step(x, **good)

@@ -125,13 +125,15 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     if n_seq == 0:
         return
     idx = bias = 0
+    bst = ist
     if blk_bias is not None:
         if blk_bias.shape != ts or blk_bias.dtype is not torch.float32 or blk_bias.get_device() != index:
             raise ValueError(f"blk_bias must be fp32 of topk_idx's shape on cuda:{index}")
+        bst = blk_bias.stride()
     # a router head that all kv heads share: ids and biases both
-    one = num_kv_heads == 1 or ist[0] == 0 and (blk_bias is None or blk_bias.stride(0) == 0)
+    one = ist[0] == 0 == bst[0] or num_kv_heads == 1
     if K:
-        if topk_idx.dtype is not torch.int32 or ist[2] != 1 or (blk_bias is not None and blk_bias.stride() != ist):
+        if topk_idx.dtype is not torch.int32 or ist[2] != 1 or bst != ist:
             # one layout for both; a shared router head is kept once
             topk_idx = (topk_idx[:1] if one else topk_idx).to(torch.int32).contiguous()
             if blk_bias is not None:

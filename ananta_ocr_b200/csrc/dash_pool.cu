@@ -156,7 +156,9 @@ __global__ void __launch_bounds__(kCopyThreads) pages_copy_kernel(const __grid_c
 }
 
 // The pairs that may run at the same time: no destination is another pair's
-// source or destination.  One CTA; three bit sets over the pages (destination
+// source or destination.  Of two pairs a -> b, b -> c both are left out: the second
+// reads what the first was to write, and which of them was meant to come first is
+// not known.  One CTA; three bit sets over the pages (destination
 // once, destination more than once, source) in shared memory.
 __global__ void __launch_bounds__(kPoolThreads) pages_check_kernel(const int32_t* src, const int32_t* dst, int n,
                                                                    const int32_t* count, int num_pages, int32_t* list,

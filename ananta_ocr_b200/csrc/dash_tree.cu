@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(kTreeRowWarps * 32) tree_rows_kernel(const __g
 }
 
 // The tensor cores wherever the block size lets a 64-key tile be made of granules: the
-// CUDA-core form reads every key once per row and head, and took 474 us where the
-// other takes 78 (32 sequences of one token on 27,556), 280 / 47 (16 trees of 16), 100 / 20.5
+// CUDA-core form reads every key once per row and head, and took five times as long or
+// more: 474 us where the other takes 78 (32 sequences of one token on 27,556), 280 / 47 (16 trees of 16), 100 / 20.5
 // (8 of 17), 83 / 14.5 (one of 8), 618 / 33 (four of 64).
 int launch_tree_attn(const DashTreeAttnArgs& a, cudaStream_t st) {
   if (tree_tc_supported(a)) return launch_tree_tc(a, st);

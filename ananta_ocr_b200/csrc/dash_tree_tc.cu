@@ -699,8 +699,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (grow) m_run = mx;
         const float mu = m_run == -INFINITY ? 0.0f : m_run;
         // P is rounded to the caches' type for the matrix product (half a unit
-        // in the last place per weight); the sum keeps the unrounded weights
-        // because lse is an fp32 result
+        // in the last place per weight): outputs are off by 0.0023 in bf16 where
+        // the rounded output alone gives 0.0017 (relative 2-norms).  A second
+        // product with what the rounding leaves would close the gap and was not
+        // taken: 82 -> 89 us (32 x 1 token), 47 -> 56 (16 x 16), 33 -> 35 (4 x 64).
+        // The sum keeps the unrounded weights because lse is an fp32 result
         uint64_t ls = f2_pack(0.0f, 0.0f);
         const uint64_t slv = f2_pack(sl, sl);
         uint32_t pk[kKeys / 2];
@@ -895,10 +898,12 @@ struct TreeCut {
 // 100 / 96 / 100 / 152, as 296 whole ones and 24 of 8 CTAs 78; 640 of 24 148 / 157 / 185 /
 // 309, as 592 whole ones and 48 of 6 135.)
 // More than 8 CTAs, which leave gaps in the GPU's processing clusters, only where most of
-// the GPU stays empty otherwise (4 units of some 250 tiles 33 -> 29 with 16 CTAs; 20
-// units of 20 tiles 17 -> 27 with 14).
-// The number of tiles is not known here; the drafted tokens of a sequence route similar
-// blocks: twice K are assumed.
+// the GPU stays empty otherwise: 10 units of 16 CTAs and 4 units of some 250 tiles (33 ->
+// 29 with 16 CTAs) are inside the bound of 160 CTAs, 20 units of 20 tiles (280 CTAs, 17 ->
+// 27 with 14) are outside; nothing between the two was measured.
+// The number of tiles is not known here.  The union of a tree's routed blocks is taken as
+// twice K, which is what the measured trees have (each token K of 2 K blocks); a router
+// whose tokens agree more or less shifts the choice, not the result.
 static TreeCut tree_cut(const DashTreeAttnArgs& a, int64_t units) {
   if (a.num_splits) return {0, a.num_splits};
   int64_t keys = (int64_t)(a.seqs.max_q_len == 1 ? 1 : 2) * a.routes.K * a.block_size + a.local_window + a.seqs.max_q_len;

@@ -22,9 +22,13 @@
 // token's probability.
 //
 // Measured (CUDA graph, vocabulary 129,280): 64 sequences of 16 fp32 rows, drawn
-// drafts, 33 us (set-up 3, then two passes of 9 us, each at memory rate, over the
-// rows that the walks reach); one sequence of 4 rows 12.4 us, greedy 16 of 8 18.6 us,
-// both bound by the latency of a pass (3 us) and the launch.
+// drafts, 33 us.  By the global timer: set-up 2.3; a first pass that all 512 CTAs
+// make at once, at memory rate, to 10-14 (66 MB), its exchange to 16; a second by
+// half of the sequences to 24 and a third by a third of them to 30; the search for
+// the token's place 0.7, and up to 10 where many CTAs still read.  One sequence of 4
+// rows 12.4 us, greedy 16 of 8 18.6 us (up to four passes of 3-4 us, one after the
+// other).  Certain drafts 18.5 us (1 x 4) and 43 (64 x 16): one pass, in which every
+// element is compared with the rejected tokens.
 #include <cooperative_groups.h>
 #include "dash_tree.cuh"
 

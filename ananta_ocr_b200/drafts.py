@@ -90,7 +90,9 @@ def dash_sparse_attn_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     [n_seq + 1]; ctx_lens [n_seq] committed tokens; row_pos [rows] and tree_mask
     [rows, words] as ``tree_plan`` makes them.  A row attends its window of
     ``local_blocks * sparse_block_size`` committed tokens, its routed blocks
-    (with their biases) before it, and the drafted tokens of its mask.  Rows
+    (with their biases) before it, and the drafted tokens of its mask, however far
+    back: the keys are those of decoding the path token by token as long as no
+    token lies ``local_blocks * sparse_block_size`` or more below the root.  Rows
     from ``cu_seqlens_q[-1]`` on are left as they were.  output may be q itself.
     lse [rows, H] fp32: natural-log sums.  num_splits: CTAs per sequence and kv head
     (0 = automatic)."""

@@ -102,8 +102,9 @@ def copy_pages(caches: Layers, src: torch.Tensor, dst: torch.Tensor,
                device_error: Optional[DeviceErrorWord] = None) -> None:
     """Page ``src[i]`` -> page ``dst[i]`` in every cache tensor (int32 vectors; a
     negative id skips the pair).  The pairs run at the same time: one whose
-    destination is another pair's source or destination is left out and
-    recorded, as is one with an id past the last page."""
+    destination is another pair's source or destination, or whose source is another
+    pair's destination, is left out and recorded, as is one with an id past the
+    last page."""
     layers = _layers(caches)
     src = _ints(src, "src", layers.index)
     n = src.numel()

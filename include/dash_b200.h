@@ -862,7 +862,11 @@ int dash_tree_plan(const DashTreePlanArgs* args, dash_stream_t stream);
  * block_size 16, 32 and multiples of 64 up to 256 run on the tensor cores
  * with up to 128 query heads per kv head and tables of up to 8,192 granules of
  * min(block_size, 64) tokens; other calls run on the CUDA cores (same results
- * within rounding, six and more times slower).
+ * within rounding, five and more times slower).
+ * The window bounds committed keys only: a row attends its drafted ancestors
+ * however far back they are.  Decoding the same path token by token gives the same
+ * keys as long as no row is local_window or more tokens below the root; from
+ * there on it would see the oldest ancestors only where their block is routed.
  * seqs: n_seq, q_start, q_len_fixed = rows, max_q_len = most drafted tokens of
  * a sequence (<= 256); pos0 and kv_len are not read.  num_splits 0: automatic
  * (1..16 CTAs share a sequence's keys and join their parts over the cluster's
@@ -956,9 +960,9 @@ typedef struct {
 int dash_draft_commit(const DashCommitArgs* args, dash_stream_t stream);
 
 /* dash_pages_copy -- page src[i] -> page dst[i] in every tensor, i < n (a pair
- * with a negative id or src == dst is skipped).  check != 0: pairs whose dst is
- * another pair's source or dst are left out and recorded (DASH_DEV_BAD_ROW), as are
- * ids >= num_pages; list (device, [2 n] scratch) receives the pairs that run.
+ * with a negative id or src == dst is skipped).  check != 0: a pair whose dst is
+ * another pair's source or dst, or whose source is another pair's dst, is left out
+ * and recorded (DASH_DEV_BAD_ROW), as is one with an id >= num_pages; list (device, [2 n] scratch) receives the pairs that run.
  * check == 0: the caller knows that no such pair exists.                    */
 typedef struct {
   const DashCacheTensor* tensors;   /* host */

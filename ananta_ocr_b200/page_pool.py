@@ -190,7 +190,9 @@ class PagePool:
              device_error: Optional[DeviceErrorWord] = None) -> None:
         """The empty row ``dst[i]`` becomes a copy of the first ``lens[i]`` tokens
         of row ``src[i]``: full pages are shared, a partly filled last one is
-        copied to a page of its own in every tensor of ``caches``."""
+        copied to a page of its own in every tensor of ``caches``.  Nothing is copied
+        later: a row that goes back behind tokens of a shared page must not write
+        there (fork it anew at the shorter length)."""
         layers = self._own(caches)
         src = _ints(src, "src", self.index)
         n = src.numel()
@@ -203,19 +205,27 @@ class PagePool:
                                             at + 4 * n), self.index)
 
     def compact(self, caches: Layers, into: Optional["PagePool"] = None,
-                device_error: Optional[DeviceErrorWord] = None) -> torch.Tensor:
+                device_error: Optional[DeviceErrorWord] = None,
+                new_ids: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Moves the held pages to the lowest ids.  With ``into`` (a pool of the
         same sizes) the new tables go there and this pool keeps the old ones,
         which stay usable until a page is handed out again: no page that they
-        name is overwritten.  Returns the number of moved pages (int32 [1],
-        on the GPU)."""
+        name is overwritten.  Whatever else is kept by page either is among
+        ``caches`` or follows ``new_ids`` (int32 [num_pages]), which receives every
+        page's new id (its own where it stays or is not held).  Returns the number of
+        moved pages (int32 [1], on the GPU)."""
         layers, to = self._own(caches), self if into is None else into
         if to.device != self.device or to.block_size != self.block_size:
             raise ValueError("`into` must be a pool of the same device and block size")
         P = self.c.num_pages
         half = P // 2
-        buf = torch.empty(2 * half + P + 1, dtype=torch.int32, device=self.device)
+        if new_ids is None:
+            new_ids = torch.empty(P, dtype=torch.int32, device=self.device)
+        elif new_ids.shape != (P,) or new_ids.dtype is not torch.int32 or new_ids.device != self.device or \
+                not new_ids.is_contiguous():
+            raise ValueError(f"new_ids must be contiguous int32 [{P}] on {self.device}")
+        buf = torch.empty(2 * half + 1, dtype=torch.int32, device=self.device)
         at = buf.data_ptr()
         _call("dash_pages_compact", self._args(device_error, layers=layers, copy_src=at, copy_dst=at + 4 * half,
-                                               new_id=at + 8 * half, n_moves=at + 8 * half + 4 * P, into=to), self.index)
-        return buf[2 * half + P:]
+                                               new_id=new_ids.data_ptr(), n_moves=at + 8 * half, into=to), self.index)
+        return buf[2 * half:]

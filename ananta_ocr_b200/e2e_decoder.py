@@ -385,8 +385,8 @@ class DashDecoder:
         drafts were drawn from).  The kept tokens' cache entries are moved
         together, the k-bar rows of their pages refreshed, ``self.seq_lens``
         advanced by the kept tokens and the root, and ``self.tok`` becomes the
-        next token.  A draft without a page (the row is full, the pool is empty) is
-        not kept.  Returns (drafts.Verified, logits [B, n, vocab])."""
+        next token.  A draft without a page (the row is full, the pool is empty) or
+        with an id outside the vocabulary (-1: no draft) is not kept.  Returns (drafts.Verified, logits [B, n, vocab])."""
         c = self.cfg
         if self.pst is not None:
             raise NotImplementedError("draft_step has no page-aware candidates (page state has no rewind)")
@@ -420,7 +420,8 @@ class DashDecoder:
         cos, sin = self.rope_tables(plan.row_pos)
         table = self.block_table.index_select(0, plan.row_seq)          # a row per token, for the router
         sl = (plan.row_pos + 1).clamp_(max=self.capacity)
-        x = self.embed[tokens]
+        # (an id outside the vocabulary is no draft: the verification passes it over)
+        x = self.embed[tokens.clamp(0, c.vocab - 1)]
         oi = torch.empty(T, c.slots, dtype=torch.int32, device=dev)
         ob = torch.empty(T, c.slots, dtype=torch.float32, device=dev)
         attn = torch.empty(T, c.heads, c.head_dim, dtype=torch.bfloat16, device=dev)

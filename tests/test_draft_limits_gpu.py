@@ -154,3 +154,20 @@ def test_refused_calls_change_nothing():
     for a, b in zip(before, (*d.kc, *d.ic, d.pool.block_table, d.pool.n_free, d.seq_lens, d.tok)):
         assert torch.equal(a, b)
     d.draft_step(x, **good)
+
+
+def test_ids_outside_the_vocabulary_are_no_drafts():
+    """Rows may draft fewer tokens than others: ids outside the vocabulary are passed
+    over, and the other tokens' logits are what they are without them."""
+    ids, n = ids_of(60, 9), 6
+    a, b = started(ids, [60, 60], 0), started(ids, [60, 60], 0)
+    x = ids_of(n - 1, 10)
+    y = x.clone()
+    y[0, 3:] = torch.tensor([-1, 1000], device="cuda")
+    y[1, 2:] = torch.tensor([-2 ** 40, 2 ** 40, -1001], device="cuda")
+    _, la = a.draft_step(x)
+    kept, lb = b.draft_step(y)
+    assert torch.equal(la[0, :4], lb[0, :4]) and torch.equal(la[1, :3], lb[1, :3])
+    root = torch.full((2, 1), 5, device="cuda")
+    tokens = torch.cat([root, y], 1)
+    verified(kept, lb, tokens, (tokens >= 0) & (tokens < 1000))

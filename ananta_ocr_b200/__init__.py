@@ -20,8 +20,14 @@ Speculative decoding on the paged cache (no counterpart in the reference):
   ananta_ocr_b200.drafts                     tree_plan, dash_sparse_attn_tree,
                                              verify_drafts, commit_drafts
   ananta_ocr_b200.page_pool                  PagePool, CacheLayers, copy_pages
+
+What a step does around its attention (no counterpart in the reference's kernels):
+
+  ananta_ocr_b200.norms                      rms_norm, add_rms_norm (with gradients)
+  ananta_ocr_b200.moe                        MoeWeights, moe_layer (a few tokens)
+  ananta_ocr_b200.sampling                   sample, probs
 """
 from . import _lib  # noqa: F401
 
 __all__ = ["ops", "sparse_gather_e2e_triton", "sparse_gather_triton", "modeling_deepseekv2",
-           "unlimited_dash_ops", "sharding", "drafts", "page_pool"]
+           "unlimited_dash_ops", "sharding", "drafts", "page_pool", "norms", "moe", "sampling"]

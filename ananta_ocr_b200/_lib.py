@@ -280,6 +280,37 @@ class DashPagesArgs(C.Structure):
                 ("copy_dst", _p), ("n_moves", _p), ("new_id", _p), ("device_error", _p)]
 
 
+class DashNormArgs(C.Structure):
+    _fields_ = [("y", _p), ("y_stride", _i64), ("residual", _p), ("residual_stride", _i64),
+                ("weight", _p), ("post", _p), ("gate", _p), ("gate_stride", _i64), ("stream", _p),
+                ("stream_stride", _i64), ("normed", _p), ("normed_stride", _i64), ("rows", _i64),
+                ("group_rows", _i64), ("hidden", _i32), ("dtype", _i32), ("weight_f32", _i32),
+                ("post_f32", _i32), ("gate_f32", _i32), ("eps", _f32), ("scale", _f32), ("pad0", _i32)]
+
+
+class DashNormBwdArgs(C.Structure):
+    _fields_ = [("fwd", DashNormArgs), ("dstream", _p), ("dstream_stride", _i64), ("dnormed", _p),
+                ("dnormed_stride", _i64), ("dy", _p), ("dy_stride", _i64), ("dresidual", _p),
+                ("dresidual_stride", _i64), ("dweight", _p), ("dpost", _p), ("dgate", _p),
+                ("workspace", _p), ("workspace_bytes", C.c_size_t)]
+
+
+class DashSampleArgs(C.Structure):
+    _fields_ = [("logits", _p), ("logits_stride", _i64), ("u", _p), ("temperature", _p), ("top_k", _p),
+                ("top_p", _p), ("min_p", _p), ("temperature_all", _f32), ("top_k_all", _i32),
+                ("top_p_all", _f32), ("min_p_all", _f32), ("rows", _i32), ("vocab", _i32),
+                ("dtype", _i32), ("pad0", _i32), ("tokens", _p), ("probs", _p), ("probs_stride", _i64)]
+
+
+class DashMoeArgs(C.Structure):
+    _fields_ = [("x", _p), ("x_stride", _i64), ("gate", _p), ("gate_up", _p), ("down", _p),
+                ("shared_gate_up", _p), ("shared_down", _p), ("residual", _p), ("residual_stride", _i64),
+                ("out", _p), ("out_stride", _i64), ("ids", _p), ("weights", _p), ("tokens", _i32),
+                ("hidden", _i32), ("ffn", _i32), ("experts", _i32), ("topk", _i32), ("shared_ffn", _i32),
+                ("dtype", _i32), ("gate_f32", _i32), ("renorm", _i32), ("scale", _f32), ("workspace", _p),
+                ("workspace_bytes", C.c_size_t), ("device_error", _p)]
+
+
 ABI_ORDER = [DashSeqs, DashKV, DashRoutes, DashQO, DashKbarArgs, DashRouteArgs,
              DashBlockMaxArgs, DashPrefillArgs, DashDecodeArgs, DashDeviceError,
              DashPageIdsArgs, DashPageStateArgs, DashPageAllowArgs, DashPageDecodeArgs,
@@ -287,7 +318,7 @@ ABI_ORDER = [DashSeqs, DashKV, DashRoutes, DashQO, DashKbarArgs, DashRouteArgs,
              DashAttnBwdArgs, DashEntmaxArgs, DashServingPlanArgs, DashPeerHandle,
              DashPageCoordArgs, DashCosSin2DArgs, DashTreePlanArgs, DashTreeAttnArgs,
              DashVerifyArgs, DashCacheTensor, DashCommitArgs, DashPagesCopyArgs, DashPagePool,
-             DashPagesArgs]
+             DashPagesArgs, DashNormArgs, DashNormBwdArgs, DashSampleArgs, DashMoeArgs]
 
 # every function the header declares
 EXPORTS = [
@@ -302,7 +333,8 @@ EXPORTS = [
     "dash_page_coords", "dash_cos_sin_2d", "dash_route_refresh",
     "dash_tree_plan", "dash_tree_attn", "dash_draft_verify", "dash_draft_commit",
     "dash_pages_copy", "dash_pages_reserve", "dash_pages_free", "dash_pages_fork",
-    "dash_pages_compact",
+    "dash_pages_compact", "dash_add_norm", "dash_add_norm_bwd", "dash_add_norm_bwd_workspace_size",
+    "dash_sample", "dash_moe", "dash_moe_workspace_size",
 ]
 
 
@@ -354,12 +386,20 @@ def load(path: str = LIB_PATH):
         ("dash_pages_free", [C.POINTER(DashPagesArgs), _p]),
         ("dash_pages_fork", [C.POINTER(DashPagesArgs), _p]),
         ("dash_pages_compact", [C.POINTER(DashPagesArgs), _p]),
+        ("dash_add_norm", [C.POINTER(DashNormArgs), _p]),
+        ("dash_add_norm_bwd", [C.POINTER(DashNormBwdArgs), _p]),
+        ("dash_sample", [C.POINTER(DashSampleArgs), _p]),
+        ("dash_moe", [C.POINTER(DashMoeArgs), _p]),
     ]:
         f = getattr(L, name)
         f.argtypes = args
         f.restype = C.c_int
     L.dash_route_refresh.argtypes = [C.POINTER(DashRouteArgs), C.POINTER(DashKbarArgs), _p]
     L.dash_route_refresh.restype = C.c_int
+    L.dash_add_norm_bwd_workspace_size.argtypes = [C.POINTER(DashNormBwdArgs)]
+    L.dash_add_norm_bwd_workspace_size.restype = C.c_size_t
+    L.dash_moe_workspace_size.argtypes = [C.POINTER(DashMoeArgs)]
+    L.dash_moe_workspace_size.restype = C.c_size_t
     L.dash_prefill_workspace_size.argtypes = [C.POINTER(DashPrefillArgs)]
     L.dash_prefill_workspace_size.restype = C.c_size_t
     L.dash_decode_workspace_size.argtypes = [C.POINTER(DashDecodeArgs)]

@@ -134,7 +134,7 @@ int dash_count_launches(int reset) {
 }
 
 int dash_abi_sizes(int64_t* out, int n) {
-  const int64_t s[32] = {(int64_t)sizeof(DashSeqs),           (int64_t)sizeof(DashKV),
+  const int64_t s[36] = {(int64_t)sizeof(DashSeqs),           (int64_t)sizeof(DashKV),
                          (int64_t)sizeof(DashRoutes),         (int64_t)sizeof(DashQO),
                          (int64_t)sizeof(DashKbarArgs),       (int64_t)sizeof(DashRouteArgs),
                          (int64_t)sizeof(DashBlockMaxArgs),   (int64_t)sizeof(DashPrefillArgs),
@@ -149,9 +149,11 @@ int dash_abi_sizes(int64_t* out, int n) {
                          (int64_t)sizeof(DashTreePlanArgs),   (int64_t)sizeof(DashTreeAttnArgs),
                          (int64_t)sizeof(DashVerifyArgs),     (int64_t)sizeof(DashCacheTensor),
                          (int64_t)sizeof(DashCommitArgs),     (int64_t)sizeof(DashPagesCopyArgs),
-                         (int64_t)sizeof(DashPagePool),       (int64_t)sizeof(DashPagesArgs)};
-  for (int i = 0; i < n && i < 32; ++i) out[i] = s[i];
-  return 32;
+                         (int64_t)sizeof(DashPagePool),       (int64_t)sizeof(DashPagesArgs),
+                         (int64_t)sizeof(DashNormArgs),       (int64_t)sizeof(DashNormBwdArgs),
+                         (int64_t)sizeof(DashSampleArgs),     (int64_t)sizeof(DashMoeArgs)};
+  for (int i = 0; i < n && i < 36; ++i) out[i] = s[i];
+  return 36;
 }
 
 static int validate_kbar(const DashKbarArgs* a) {
@@ -685,6 +687,104 @@ int dash_pages_compact(const DashPagesArgs* a, dash_stream_t stream) {
   rc = check_tensors(a->tensors, a->n_tensors, 0);
   if (rc) return rc;
   return launch_pages_compact(*a, (cudaStream_t)stream);
+}
+
+static bool known_dtype(int d) { return d == DASH_DTYPE_F32 || d == DASH_DTYPE_BF16 || d == DASH_DTYPE_F16; }
+
+static int check_norm(const DashNormArgs& a, bool out) {
+  if (!known_dtype(a.dtype)) return set_error(DASH_ERR_UNSUPPORTED, "rows must be fp32, bf16 or fp16");
+  if (a.rows < 0 || a.rows > INT_MAX) return set_error(DASH_ERR_INVALID, "rows %lld not in [0, 2^31)", (long long)a.rows);
+  if (a.hidden <= 0) return set_error(DASH_ERR_INVALID, "hidden must be > 0");
+  if (a.hidden > norm_max_hidden()) return set_error(DASH_ERR_UNSUPPORTED, "hidden %d > %d", a.hidden, norm_max_hidden());
+  if (a.rows == 0) return DASH_OK;
+  if (a.group_rows <= 0 || a.rows % a.group_rows)
+    return set_error(DASH_ERR_INVALID, "rows must be a multiple of group_rows (> 0)");
+  if (!a.y || !a.weight || (out && !a.normed)) return set_error(DASH_ERR_INVALID, "null y/weight/normed");
+  // (rows that are only read may be one row)
+  if (a.y_stride < 0 || a.residual_stride < 0 || a.gate_stride < 0) return set_error(DASH_ERR_INVALID, "negative stride");
+  if (out && a.rows > 1 && (a.normed_stride < a.hidden || (a.stream && a.stream_stride < a.hidden)))
+    return set_error(DASH_ERR_INVALID, "rows overlap");
+  return DASH_OK;
+}
+
+int dash_add_norm(const DashNormArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  const int rc = check_norm(*a, true);
+  return rc || a->rows == 0 ? rc : launch_add_norm(*a, (cudaStream_t)stream);
+}
+
+size_t dash_add_norm_bwd_workspace_size(const DashNormBwdArgs* a) {
+  return !a || check_norm(a->fwd, false) || a->fwd.rows == 0 ? 0 : add_norm_bwd_workspace(*a);
+}
+
+int dash_add_norm_bwd(const DashNormBwdArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  const int rc = check_norm(a->fwd, false);
+  if (rc || a->fwd.rows == 0) return rc;
+  if (!a->dnormed) return set_error(DASH_ERR_INVALID, "null dnormed");
+  if ((a->dpost && !a->fwd.post) || (a->dgate && !a->fwd.gate))
+    return set_error(DASH_ERR_INVALID, "a gradient of a weight that is not there");
+  const int64_t h = a->fwd.hidden;
+  if (a->dstream_stride < 0 || a->dnormed_stride < 0) return set_error(DASH_ERR_INVALID, "negative stride");
+  if (a->fwd.rows > 1 && ((a->dy && a->dy_stride < h) || (a->dresidual && a->dresidual_stride < h)))
+    return set_error(DASH_ERR_INVALID, "rows overlap");
+  const size_t need = add_norm_bwd_workspace(*a);
+  if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+    return set_error(DASH_ERR_WORKSPACE, "workspace of %zu bytes needed (16-byte aligned)", need);
+  return launch_add_norm_bwd(*a, (cudaStream_t)stream);
+}
+
+int dash_sample(const DashSampleArgs* a, dash_stream_t stream) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  if (!known_dtype(a->dtype)) return set_error(DASH_ERR_UNSUPPORTED, "logits must be fp32, bf16 or fp16");
+  if (a->rows < 0) return set_error(DASH_ERR_INVALID, "rows < 0");
+  if (a->rows > (1 << 24)) return set_error(DASH_ERR_UNSUPPORTED, "rows %d > 2^24", a->rows);
+  if (a->vocab <= 0) return set_error(DASH_ERR_INVALID, "vocab must be > 0");
+  if (a->vocab > (1 << 20)) return set_error(DASH_ERR_UNSUPPORTED, "vocab %d > 2^20", a->vocab);
+  if (a->rows == 0) return DASH_OK;
+  if (!a->logits) return set_error(DASH_ERR_INVALID, "null logits");
+  if (!a->tokens && !a->probs) return set_error(DASH_ERR_INVALID, "neither tokens nor probs");
+  if (a->tokens && !a->u) return set_error(DASH_ERR_INVALID, "tokens need u");
+  if (a->rows > 1 && (a->logits_stride < 0 || (a->probs && a->probs_stride < a->vocab)))   // rows may be one row
+    return set_error(DASH_ERR_INVALID, "probs rows shorter than vocab or a negative stride");
+  return launch_sample(*a, (cudaStream_t)stream);
+}
+
+static int check_moe(const DashMoeArgs* a) {
+  if (!a) return set_error(DASH_ERR_INVALID, "null args");
+  if (a->dtype != DASH_DTYPE_BF16 && a->dtype != DASH_DTYPE_F16)
+    return set_error(DASH_ERR_UNSUPPORTED, "the layer's type must be bf16 or fp16");
+  if (a->tokens < 0) return set_error(DASH_ERR_INVALID, "tokens < 0");
+  if (a->tokens > kMoeMaxTokens) return set_error(DASH_ERR_UNSUPPORTED, "tokens %d > %d", a->tokens, kMoeMaxTokens);
+  if (a->hidden <= 0 || a->ffn <= 0 || a->shared_ffn < 0 || a->hidden % 8 || a->ffn % 8 || a->shared_ffn % 8)
+    return set_error(DASH_ERR_UNSUPPORTED, "hidden, ffn and shared_ffn must be multiples of 8");
+  if (a->hidden > kMoeMaxWidth || a->ffn > kMoeMaxWidth || a->shared_ffn > kMoeMaxWidth)
+    return set_error(DASH_ERR_UNSUPPORTED, "hidden, ffn and shared_ffn must be at most %d", kMoeMaxWidth);
+  if (a->experts <= 0 || a->experts > kMoeMaxExperts)
+    return set_error(DASH_ERR_UNSUPPORTED, "experts %d not in [1, %d]", a->experts, kMoeMaxExperts);
+  if (a->topk <= 0 || a->topk > kMoeMaxTopk || a->topk > a->experts)
+    return set_error(DASH_ERR_UNSUPPORTED, "topk %d not in [1, min(%d, experts)]", a->topk, kMoeMaxTopk);
+  return DASH_OK;
+}
+
+size_t dash_moe_workspace_size(const DashMoeArgs* a) { return check_moe(a) ? 0 : moe_workspace(*a); }
+
+int dash_moe(const DashMoeArgs* a, dash_stream_t stream) {
+  const int rc = check_moe(a);
+  if (rc || a->tokens == 0) return rc;
+  if (!a->x || !a->gate || !a->gate_up || !a->down || !a->out || !a->ids || !a->weights)
+    return set_error(DASH_ERR_INVALID, "null pointer");
+  if (a->shared_ffn && (!a->shared_gate_up || !a->shared_down)) return set_error(DASH_ERR_INVALID, "null shared expert");
+  for (const void* p : {a->x, a->gate, a->gate_up, a->down, a->shared_gate_up, a->shared_down, a->residual, (const void*)a->out})
+    if (!aligned16(p)) return set_error(DASH_ERR_INVALID, "all rows must be 16-byte aligned");
+  if (a->x_stride % 8 || a->out_stride % 8 || (a->residual && a->residual_stride % 8))
+    return set_error(DASH_ERR_INVALID, "row strides must be multiples of 8 elements");
+  if (a->tokens > 1 && (a->x_stride < a->hidden || a->out_stride < a->hidden || (a->residual && a->residual_stride < a->hidden)))
+    return set_error(DASH_ERR_INVALID, "rows overlap");
+  const size_t need = moe_workspace(*a);
+  if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+    return set_error(DASH_ERR_WORKSPACE, "workspace of %zu bytes needed (16-byte aligned)", need);
+  return launch_moe(*a, (cudaStream_t)stream);
 }
 
 int dash_entmax15_fwd(const DashEntmaxArgs* a, dash_stream_t stream) {

@@ -59,5 +59,14 @@ int launch_pages_reserve(const DashPagesArgs& a, cudaStream_t st);
 int launch_pages_free(const DashPagesArgs& a, cudaStream_t st);
 int launch_pages_fork(const DashPagesArgs& a, cudaStream_t st);
 int launch_pages_compact(const DashPagesArgs& a, cudaStream_t st);
+int norm_max_hidden();
+int launch_add_norm(const DashNormArgs& a, cudaStream_t st);
+size_t add_norm_bwd_workspace(const DashNormBwdArgs& a);
+int launch_add_norm_bwd(const DashNormBwdArgs& a, cudaStream_t st);
+int launch_sample(const DashSampleArgs& a, cudaStream_t st);
+// a few tokens' mixture-of-experts layer (dash_moe.cu)
+constexpr int kMoeMaxTokens = 256, kMoeMaxExperts = 256, kMoeMaxTopk = 16, kMoeMaxWidth = 1 << 16;
+size_t moe_workspace(const DashMoeArgs& a);
+int launch_moe(const DashMoeArgs& a, cudaStream_t st);
 
 }  // namespace dash

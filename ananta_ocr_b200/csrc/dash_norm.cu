@@ -1,0 +1,520 @@
+// dash_norm.cu -- the residual sum behind a block, with the block's own norm, its
+// gate and scale, and the norm before the next block; forward and gradients.
+//
+//   z = y * r1 * post            r1 = 1 / sqrt(mean(y^2) + eps)   (post given; else z = y)
+//   s = residual + scale * gate * z
+//   h = s * r2 * weight          r2 = 1 / sqrt(mean(s^2) + eps)
+//
+// All arithmetic is fp32; s and h are rounded once each (h is made of the unrounded
+// s).  The gradients make s again from y and the residual, so that nothing but the
+// inputs is kept, and no rounded s enters the weights' gradients.
+//
+// Bound by memory: y and residual in, s and h out (forward); those two and the
+// gradients of s and h in, those of y and residual out (backward).
+#include "dash_common.cuh"
+#include "dash_internal.h"
+
+namespace dash {
+
+namespace {
+
+constexpr int kNormMaxHidden = 8192;
+
+// E consecutive elements as fp32
+template <typename T, int E>
+struct Row;
+template <typename T>
+struct Row<T, 1> {
+  T v;
+  __device__ __forceinline__ void read(const T* p) { v = *p; }
+  __device__ __forceinline__ void get(float (&x)[1]) const { x[0] = (float)v; }
+  __device__ __forceinline__ void put(const float (&x)[1]) { v = (T)x[0]; }
+  __device__ __forceinline__ void write(T* p) const { *p = v; }
+};
+template <typename T>
+struct Row<T, 8> {            // 16-bit types
+  uint4 v;
+  __device__ __forceinline__ void read(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2(w[i], (T*)nullptr);
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  }
+  __device__ __forceinline__ void put(const float (&x)[8]) {
+    v = make_uint4(pack2(x[0], x[1], (T*)nullptr), pack2(x[2], x[3], (T*)nullptr), pack2(x[4], x[5], (T*)nullptr),
+                   pack2(x[6], x[7], (T*)nullptr));
+  }
+  __device__ __forceinline__ void write(T* p) const { *reinterpret_cast<uint4*>(p) = v; }
+};
+template <>
+struct Row<float, 4> {
+  float4 v;
+  __device__ __forceinline__ void read(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void get(float (&x)[4]) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+  __device__ __forceinline__ void put(const float (&x)[4]) { v = make_float4(x[0], x[1], x[2], x[3]); }
+  __device__ __forceinline__ void write(float* p) const { *reinterpret_cast<float4*>(p) = v; }
+};
+
+// E elements of a weight that is fp32 or of the rows' type
+template <typename T, int E>
+__device__ __forceinline__ void read_weight(const void* p, int64_t at, bool f32, float (&x)[E]) {
+  if (f32) {
+    const float* w = static_cast<const float*>(p) + at;
+    if constexpr (E == 1) {
+      x[0] = *w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(w + i);
+        x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+      }
+    }
+  } else {
+    Row<T, E> r;
+    r.read(static_cast<const T*>(p) + at);
+    r.get(x);
+  }
+}
+
+// Sums of N values over a row's threads, the same in all of them: a warp's by
+// shuffles, then the warps' in their order.  `buf` alternates between two halves, so
+// that one barrier per call is enough.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int warps, int warp, int lane, float* buf, int& half) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  if (warps == 1) return;
+  float* b = buf + half * 32 * 5;
+  half ^= 1;
+  if (lane == 0)
+#pragma unroll
+    for (int n = 0; n < N; ++n) b[n * 32 + warp] = v[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float s = 0.0f;
+    for (int w = 0; w < warps; ++w) s += b[n * 32 + w];
+    v[n] = s;
+  }
+}
+
+template <typename T, int E, int NV>
+__global__ void __launch_bounds__(512) add_norm_kernel(const DashNormArgs a, int warps) {
+  __shared__ float buf[2 * 32 * 5];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // one warp per row, several rows per CTA; or the whole CTA on one row
+  const int64_t row = warps == 1 ? (int64_t)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
+  if (row >= a.rows) return;
+  const int t = warps == 1 ? lane : (int)threadIdx.x, step = warps * 32 * E;
+  int half = 0;
+  const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+  Row<T, E> ry[NV], rr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+    if (c < a.hidden) ry[i].read(y + c);
+    if (res && c < a.hidden) rr[i].read(res + c);
+  }
+  const float inv = 1.0f / (float)a.hidden;
+  float r1 = 1.0f;
+  if (a.post) {
+    float q[1] = {0.0f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t * E + i * step < a.hidden) {
+        float x[E];
+        ry[i].get(x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) q[0] = fmaf(x[e], x[e], q[0]);
+      }
+    row_sum(q, warps, warp, lane, buf, half);
+    r1 = rsqrtf(q[0] * inv + a.eps);
+  }
+  const int64_t group = a.gate ? row / a.group_rows : 0;
+  float s[NV][E], q[1] = {0.0f};
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+    if (c < a.hidden) {
+      ry[i].get(s[i]);
+      if (a.post) {
+        float p[E];
+        read_weight<T, E>(a.post, c, a.post_f32, p);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i][e] *= r1 * p[e];
+      }
+      if (a.gate) {
+        float g[E];
+        read_weight<T, E>(a.gate, group * a.gate_stride + c, a.gate_f32, g);
+#pragma unroll
+        for (int e = 0; e < E; ++e) s[i][e] *= g[e];
+      }
+      float r[E] = {};
+      if (res) rr[i].get(r);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s[i][e] = fmaf(s[i][e], a.scale, r[e]);
+        q[0] = fmaf(s[i][e], s[i][e], q[0]);
+      }
+    }
+  }
+  row_sum(q, warps, warp, lane, buf, half);
+  const float r2 = rsqrtf(q[0] * inv + a.eps);
+  T* so = a.stream ? static_cast<T*>(a.stream) + row * a.stream_stride : nullptr;
+  T* ho = static_cast<T*>(a.normed) + row * a.normed_stride;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+    if (c < a.hidden) {
+      Row<T, E> o;
+      if (so) {
+        o.put(s[i]);
+        o.write(so + c);
+      }
+      float w[E];
+      read_weight<T, E>(a.weight, c, a.weight_f32, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) w[e] *= s[i][e] * r2;
+      o.put(w);
+      o.write(ho + c);
+    }
+  }
+}
+
+// Gradients.  With a = dh * weight and sh = s * r2,
+//   ds_total = ds + r2 * (a - sh * mean(a * sh))         (the residual's gradient)
+//   dweight  = sum over rows of dh * sh
+//   dz       = scale * gate * ds_total,  dgate = sum over the group's rows of scale * z * ds_total
+//   dy       = dz;  with post, b = dz * post and yh = y * r1:  dy = r1 * (b - yh * mean(b * yh)),
+//              dpost = sum over rows of dz * yh
+// mean(b * yh) = r1 / n * sum(q * ds_total) with q = scale * gate * post * y, which splits into the
+// sums of q * ds, q * a and q * s: one exchange between the warps per row (two with post).
+//
+// A CTA takes whole rows, a thread the same columns of each, so the column sums stay in
+// registers; rows go to CTAs in chunks that lie within one gate's group.  Column sums of
+// a CTA (dweight, dpost) and of a chunk (dgate) are written to the workspace and added
+// in their order by norm_columns_kernel: no atomics.
+template <typename T, int E, int NV>
+__global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs b, int64_t chunk, int64_t chunks_per_group, int64_t chunks,
+                                    float* part_w, float* part_p, float* part_g) {
+  const DashNormArgs& a = b.fwd;
+  __shared__ float buf[2 * 32 * 5];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int t = threadIdx.x, step = (int)blockDim.x * E;
+  int half = 0;
+  const float inv = 1.0f / (float)a.hidden;
+  float dw[NV][E] = {}, dp[NV][E] = {};
+  for (int64_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+    const int64_t group = k / chunks_per_group, piece = k % chunks_per_group;
+    const int64_t end = min((group + 1) * a.group_rows, group * a.group_rows + (piece + 1) * chunk);
+    float dg[NV][E] = {};
+    for (int64_t row = group * a.group_rows + piece * chunk; row < end; ++row) {
+      const T* y = static_cast<const T*>(a.y) + row * a.y_stride;
+      const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+      const T* gs = b.dstream ? static_cast<const T*>(b.dstream) + row * b.dstream_stride : nullptr;
+      const T* gh = static_cast<const T*>(b.dnormed) + row * b.dnormed_stride;
+      Row<T, E> ry[NV], rr[NV], rs[NV], rh[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden) {
+          ry[i].read(y + c);
+          if (res) rr[i].read(res + c);
+          if (gs) rs[i].read(gs + c);
+          rh[i].read(gh + c);
+        }
+      }
+      float r1 = 1.0f;
+      if (a.post) {
+        float q[1] = {0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (t * E + i * step < a.hidden) {
+            float x[E];
+            ry[i].get(x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) q[0] = fmaf(x[e], x[e], q[0]);
+          }
+        row_sum(q, warps, warp, lane, buf, half);
+        r1 = rsqrtf(q[0] * inv + a.eps);
+      }
+      // f = scale * gate, q = f * post * y: s = residual + q * r1
+      float f[NV][E], p[NV][E], s[NV][E], ga[NV][E];
+      float sum[5] = {};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden) {
+          float x[E], r[E] = {}, d[E] = {};
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[i][e] = 1.0f, p[i][e] = 1.0f;
+          if (a.gate) read_weight<T, E>(a.gate, group * a.gate_stride + c, a.gate_f32, f[i]);
+          if (a.post) read_weight<T, E>(a.post, c, a.post_f32, p[i]);
+          read_weight<T, E>(a.weight, c, a.weight_f32, ga[i]);
+          ry[i].get(x);
+          if (res) rr[i].get(r);
+          rh[i].get(s[i]);
+          if (gs) rs[i].get(d);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            f[i][e] *= a.scale;
+            ga[i][e] *= s[i][e];
+            const float q = f[i][e] * p[i][e] * x[e];
+            s[i][e] = fmaf(q, r1, r[e]);
+            sum[0] = fmaf(s[i][e], s[i][e], sum[0]);
+            sum[1] = fmaf(ga[i][e], s[i][e], sum[1]);
+            sum[2] = fmaf(q, d[e], sum[2]);
+            sum[3] = fmaf(q, ga[i][e], sum[3]);
+            sum[4] = fmaf(q, s[i][e], sum[4]);
+          }
+        }
+      }
+      if (a.post) {
+        row_sum(sum, warps, warp, lane, buf, half);
+      } else {
+        float two[2] = {sum[0], sum[1]};
+        row_sum(two, warps, warp, lane, buf, half);
+        sum[0] = two[0], sum[1] = two[1];
+      }
+      const float r2 = rsqrtf(sum[0] * inv + a.eps);
+      const float m = r2 * r2 * r2 * sum[1] * inv;              // ds_total = ds + r2 * a - m * s
+      const float mb = r1 * r1 * r1 * inv * (sum[2] + r2 * sum[3] - m * sum[4]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden) {
+          float x[E], d[E] = {}, hh[E], o[E];
+          ry[i].get(x);
+          if (gs) rs[i].get(d);
+          rh[i].get(hh);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            d[e] = fmaf(r2, ga[i][e], d[e]) - m * s[i][e];
+            dw[i][e] = fmaf(hh[e], s[i][e] * r2, dw[i][e]);
+            const float dz = d[e] * f[i][e], yh = x[e] * r1;
+            dg[i][e] = fmaf(d[e], a.scale * yh * p[i][e], dg[i][e]);
+            dp[i][e] = fmaf(dz, yh, dp[i][e]);
+            o[e] = a.post ? fmaf(r1, dz * p[i][e], -mb * x[e]) : dz;
+          }
+          Row<T, E> w;
+          if (b.dresidual) {
+            w.put(d);
+            w.write(static_cast<T*>(b.dresidual) + row * b.dresidual_stride + c);
+          }
+          if (b.dy) {
+            w.put(o);
+            w.write(static_cast<T*>(b.dy) + row * b.dy_stride + c);
+          }
+        }
+      }
+    }
+    if (part_g) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden)
+#pragma unroll
+          for (int e = 0; e < E; ++e) part_g[k * a.hidden + c + e] = dg[i][e];
+      }
+    } else if (b.dgate) {                       // the chunk is a whole group
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (a.gate_f32) static_cast<float*>(b.dgate)[k * a.hidden + c + e] = dg[i][e];
+            else static_cast<T*>(b.dgate)[k * a.hidden + c + e] = (T)dg[i][e];
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+    if (c < a.hidden)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        part_w[(int64_t)blockIdx.x * a.hidden + c + e] = dw[i][e];
+        if (part_p) part_p[(int64_t)blockIdx.x * a.hidden + c + e] = dp[i][e];
+      }
+  }
+}
+
+// out[g][c] = sum over j of part[g * n + j][c], in that order: 32 columns per CTA, the
+// parts dealt to its warps
+template <typename T>
+__device__ __forceinline__ void columns(const float* part, int64_t n, int hidden, int64_t g, void* out, bool f32) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float v = 0.0f;
+  if (c < hidden)
+    for (int64_t j = warp; j < n; j += 32) v += part[(g * n + j) * hidden + c];
+  s[warp][lane] = v;
+  __syncthreads();
+  v = s[lane][warp];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int oc = blockIdx.x * 32 + warp;
+  if (lane == 0 && oc < hidden) {
+    if (f32) static_cast<float*>(out)[g * hidden + oc] = v;
+    else static_cast<T*>(out)[g * hidden + oc] = (T)v;
+  }
+}
+
+// blockIdx.y: 0 dweight, 1 dpost, then the gate's groups
+template <typename T>
+__global__ void __launch_bounds__(1024) norm_columns_kernel(const DashNormBwdArgs b, const float* part_w,
+                                                           const float* part_p, const float* part_g, int ctas,
+                                                           int64_t chunks_per_group) {
+  const DashNormArgs& a = b.fwd;
+  const int64_t first = part_p ? 2 : 1;
+  if (blockIdx.y == 0) {
+    if (b.dweight) columns<T>(part_w, ctas, a.hidden, 0, b.dweight, a.weight_f32);
+  } else if (blockIdx.y < first) {
+    if (b.dpost) columns<T>(part_p, ctas, a.hidden, 0, b.dpost, a.post_f32);
+  } else {
+    for (int64_t g = blockIdx.y - first; g < a.rows / a.group_rows; g += gridDim.y - first) {
+      columns<T>(part_g, chunks_per_group, a.hidden, g, b.dgate, a.gate_f32);
+      __syncthreads();
+    }
+  }
+}
+
+template <typename T, int E>
+bool wide(const DashNormArgs& a) {
+  const auto ok = [](const void* p, int64_t stride, int64_t unit) {
+    return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % unit == 0);
+  };
+  return a.hidden % E == 0 && ok(a.y, a.y_stride, E) && ok(a.residual, a.residual_stride, E) &&
+         ok(a.stream, a.stream_stride, E) && ok(a.normed, a.normed_stride, E) && ok(a.weight, 0, 1) &&
+         ok(a.post, 0, 1) && ok(a.gate, a.gate_stride, E);
+}
+
+template <typename T, int E>
+int launch_fwd_e(const DashNormArgs& a, cudaStream_t st) {
+  const int vecs = (a.hidden + E - 1) / E;
+  // A warp holds a row of up to 8 vectors per lane (no barrier); longer rows get the
+  // whole CTA.
+  const int warps = vecs <= 256 ? 1 : min(16, (vecs + 127) / 128);
+  const int nv = (vecs + warps * 32 - 1) / (warps * 32);
+  const int threads = warps == 1 ? 128 : warps * 32;
+  const unsigned grid = (unsigned)(warps == 1 ? (a.rows + 3) / 4 : a.rows);
+  if (nv <= 2) add_norm_kernel<T, E, 2><<<grid, threads, 0, st>>>(a, warps);
+  else if (nv <= 4) add_norm_kernel<T, E, 4><<<grid, threads, 0, st>>>(a, warps);
+  else if (nv <= 8) add_norm_kernel<T, E, 8><<<grid, threads, 0, st>>>(a, warps);
+  else if constexpr (E == 1) add_norm_kernel<T, E, 16><<<grid, threads, 0, st>>>(a, warps);
+  count_launch();
+  return check_launch("add_norm_kernel");
+}
+
+// How the rows of a backward call are dealt out
+struct NormCut {
+  int threads, nv, ctas;
+  int64_t chunk, per_group, chunks;
+};
+
+NormCut norm_cut(const DashNormArgs& a, int E) {
+  NormCut c;
+  const int vecs = (a.hidden + E - 1) / E;
+  // One vector per thread up to 256 of them; more vectors per thread, then 512
+  // threads, for longer rows (the column sums live in registers).
+  c.nv = 1;
+  int warps = (vecs + 31) / 32;
+  for (const int most : {8, 16})
+    while (warps > most && c.nv < (E == 1 ? (most == 8 ? 8 : 16) : most == 8 ? 8 / E : 16 / E))
+      c.nv *= 2, warps = (vecs + 32 * c.nv - 1) / (32 * c.nv);
+  c.threads = warps * 32;
+  const int most = 148 * max(1, min(8, 1024 / c.threads));
+  // chunks of at least 4 rows where there are enough rows for all CTAs
+  const int64_t groups = a.rows / a.group_rows;
+  const int64_t want = (a.rows + most - 1) / most;
+  c.chunk = min((int64_t)a.group_rows, max((int64_t)1, want));
+  c.per_group = (a.group_rows + c.chunk - 1) / c.chunk;
+  c.chunks = groups * c.per_group;
+  c.ctas = (int)min((int64_t)most, c.chunks);
+  return c;
+}
+
+template <typename T, int E>
+int launch_bwd_e(const DashNormBwdArgs& b, cudaStream_t st) {
+  const DashNormArgs& a = b.fwd;
+  const NormCut c = norm_cut(a, E);
+  float* part_w = static_cast<float*>(b.workspace);
+  float* part_p = a.post ? part_w + (int64_t)c.ctas * a.hidden : nullptr;
+  float* part_g = b.dgate && c.per_group > 1 ? part_w + (int64_t)c.ctas * a.hidden * (a.post ? 2 : 1) : nullptr;
+#define DASH_NORM_BWD(NV)                                                                                         \
+  add_norm_bwd_kernel<T, E, NV><<<c.ctas, c.threads, 0, st>>>(b, c.chunk, c.per_group, c.chunks, part_w, part_p, part_g)
+  if (c.nv == 1) DASH_NORM_BWD(1);
+  else if (c.nv == 2) DASH_NORM_BWD(2);
+  else if constexpr (E <= 4) {
+    if (c.nv == 4) DASH_NORM_BWD(4);
+    else if constexpr (E == 1) {
+      if (c.nv == 8) DASH_NORM_BWD(8);
+      else DASH_NORM_BWD(16);
+    }
+  }
+#undef DASH_NORM_BWD
+  count_launch();
+  int rc = check_launch("add_norm_bwd_kernel");
+  if (rc) return rc;
+  const int64_t groups = part_g ? a.rows / a.group_rows : 0;
+  const dim3 grid((a.hidden + 31) / 32, (unsigned)((a.post ? 2 : 1) + min(groups, (int64_t)4096)));
+  norm_columns_kernel<T><<<grid, 1024, 0, st>>>(b, part_w, part_p, part_g, c.ctas, c.per_group);
+  count_launch();
+  return check_launch("norm_columns_kernel");
+}
+
+bool norm_bwd_wide(const DashNormBwdArgs& b, int E) {
+  const auto ok = [E](const void* p, int64_t stride) {
+    return !p || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride % E == 0);
+  };
+  return ok(b.dstream, b.dstream_stride) && ok(b.dnormed, b.dnormed_stride) && ok(b.dy, b.dy_stride) &&
+         ok(b.dresidual, b.dresidual_stride);
+}
+
+}  // namespace
+
+int launch_add_norm(const DashNormArgs& a, cudaStream_t st) {
+  if (a.dtype == DASH_DTYPE_F32) return wide<float, 4>(a) ? launch_fwd_e<float, 4>(a, st) : launch_fwd_e<float, 1>(a, st);
+  if (a.dtype == DASH_DTYPE_BF16)
+    return wide<__nv_bfloat16, 8>(a) ? launch_fwd_e<__nv_bfloat16, 8>(a, st) : launch_fwd_e<__nv_bfloat16, 1>(a, st);
+  return wide<__half, 8>(a) ? launch_fwd_e<__half, 8>(a, st) : launch_fwd_e<__half, 1>(a, st);
+}
+
+static bool bwd_is_wide(const DashNormBwdArgs& b) {
+  if (b.fwd.dtype == DASH_DTYPE_F32) return wide<float, 4>(b.fwd) && norm_bwd_wide(b, 4);
+  return wide<__half, 8>(b.fwd) && norm_bwd_wide(b, 8);
+}
+
+size_t add_norm_bwd_workspace(const DashNormBwdArgs& b) {
+  const DashNormArgs& a = b.fwd;
+  // whichever vector width the pointers allow
+  size_t most = 0;
+  for (const int E : {1, a.dtype == DASH_DTYPE_F32 ? 4 : 8}) {
+    const NormCut c = norm_cut(a, E);
+    const size_t n = (size_t)a.hidden * ((size_t)c.ctas * (a.post ? 2 : 1) + (a.gate && c.per_group > 1 ? (size_t)c.chunks : 0));
+    if (n > most) most = n;
+  }
+  return most * sizeof(float);
+}
+
+int launch_add_norm_bwd(const DashNormBwdArgs& b, cudaStream_t st) {
+  const bool w = bwd_is_wide(b);
+  if (b.fwd.dtype == DASH_DTYPE_F32) return w ? launch_bwd_e<float, 4>(b, st) : launch_bwd_e<float, 1>(b, st);
+  if (b.fwd.dtype == DASH_DTYPE_BF16)
+    return w ? launch_bwd_e<__nv_bfloat16, 8>(b, st) : launch_bwd_e<__nv_bfloat16, 1>(b, st);
+  return w ? launch_bwd_e<__half, 8>(b, st) : launch_bwd_e<__half, 1>(b, st);
+}
+
+int norm_max_hidden() { return kNormMaxHidden; }
+
+}  // namespace dash

@@ -1,0 +1,510 @@
+// dash_sample.cu -- the next token of a row of logits from a given random number, with
+// temperature, top-k, top-p and min-p, or the distribution that it is drawn from.
+//
+// A cluster of CTAs takes a row; each CTA owns a contiguous slice of the vocabulary
+// and each warp a contiguous part of the slice, so running sums follow the
+// vocabulary's order.  The slice is read once and kept in shared memory.
+//
+// The tokens in descending order, lowest index first among equals, are cut off at one
+// place by all three filters.  It is found as a key (the logit as an ordered 32-bit
+// number) and a number of tokens of that key, by a radix descent in three
+// digits (11, 11 and 10 bits): histograms of counts (top-k) or of weights (top-p) in
+// shared memory, added over the cluster, then a search for the digit in which the
+// count or the share is reached.
+//
+// Weights exp((z - max) / t) are whole numbers of 2^-43 of the largest: sums do not
+// depend on the order of adding, so atomics and any split give the same token.  They
+// are made in 64-bit floating point: with 10^5 tokens of shares around 10^-5, errors of a 32-bit
+// exponential alone would move the borders between tokens by a share of 10^-8 or more, which
+// picks another token in one row of a thousand.
+#include <cooperative_groups.h>
+
+#include "dash_common.cuh"
+#include "dash_internal.h"
+
+namespace cg = cooperative_groups;
+
+namespace dash {
+
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kBins = 2048;
+constexpr int kTable = 64;                       // 2^(j / 64)
+// (the slice lies behind Shared, whose size is a multiple of its alignment)
+constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
+
+struct alignas(16) Shared {
+  uint32_t lo[kBins], hi[kBins];                 // this CTA's histogram: counts (lo), or 64-bit weights
+  uint64_t tot[kBins];                           // the cluster's
+  double table[kTable];
+  uint64_t warp_sum[kWarps];
+  uint32_t warp_cnt[kWarps];
+  uint32_t top[kMaxCluster];                     // each CTA's largest key
+  uint64_t cta_sum[kMaxCluster];
+  uint32_t cta_cnt[kMaxCluster];
+  uint64_t scan[kWarps];
+  uint64_t found_before, found_here;             // of the digit that was looked for
+  uint32_t found;
+  int32_t last;                                  // cutoff index, exchanged
+  int32_t any[kMaxCluster];
+};
+
+// -inf and NaN: 0 (out); otherwise in the order of the values, -0 as 0
+__device__ __forceinline__ uint32_t key_of(float z) {
+  z += 0.0f;
+  if (!(z > -INFINITY)) return 0u;
+  const uint32_t b = __float_as_uint(z);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// exp(x) for x <= 0, relative error below 1e-13: x = (64 k + j) ln2 / 64 + r, |r| <= ln2 / 128,
+// 2^k * 2^(j/64) * (1 + r + r^2/2 + r^3/6 + r^4/24) (the next term is 4e-14).  0 below -60, where
+// the weight is below 2^-43.
+__device__ __forceinline__ double exp64(double x, const double* table) {
+  if (!(x > -60.0)) return 0.0;
+  constexpr double kShift = 6755399441055744.0;                 // 1.5 * 2^52
+  const double t = fma(x, 92.332482616893656877, kShift);       // 64 / ln 2
+  const int n = (int)__double_as_longlong(t);
+  const double r = fma(t - kShift, -0.010830424696249145264, x);
+  double p = fma(r, 1.0 / 24, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0) * table[n & (kTable - 1)];
+  return __longlong_as_double(__double_as_longlong(p) + ((long long)(n >> 6) << 52));
+}
+
+struct Weight {
+  double top, inv;                               // largest logit, 1 / temperature
+  const double* table;
+  __device__ __forceinline__ double e(float z) const {
+    if ((double)z == top) return 1.0;            // an infinite one, too
+    return exp64(((double)z - top) * inv, table);
+  }
+  // in units of 2^-43 of the largest, rounded
+  __device__ __forceinline__ uint64_t units(float z) const {
+    const double v = fma(e(z), 8796093022208.0, 4503599627370496.0);     // 2^43, 2^52
+    return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
+  }
+};
+
+// a row's slice: in shared memory, or in global memory where it is too long
+template <typename T, int E>
+struct Slice {
+  const T* kept;                                 // shared memory or null
+  const T* row;                                  // the slice's first element in global memory
+  int have;                                      // elements of the row in the slice (may be <= 0)
+  bool vec;
+  // elements at .. at + E - 1 of the slice; behind its end -inf
+  __device__ __forceinline__ void read(int at, float (&z)[E]) const {
+    union {
+      uint4 v;
+      T t[E];
+    } u;
+    if (kept) {
+      u.v = *reinterpret_cast<const uint4*>(kept + at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = (float)u.t[e];
+    } else {
+      global(at, z);
+    }
+  }
+  __device__ __forceinline__ void global(int at, float (&z)[E]) const {
+    if (vec && at + E <= have) {
+      union {
+        uint4 v;
+        T t[E];
+      } u;
+      u.v = *reinterpret_cast<const uint4*>(row + at);
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = (float)u.t[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = at + e < have ? (float)row[at + e] : -INFINITY;
+    }
+  }
+};
+
+// adds w to the 64-bit number in (lo, hi)
+__device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
+  const uint32_t l = (uint32_t)w;
+  const uint32_t old = atomicAdd(lo, l);
+  const uint32_t h = (uint32_t)(w >> 32) + (old + l < old ? 1u : 0u);
+  if (h) atomicAdd(hi, h);
+}
+
+// The cluster's histogram into everybody's `tot`, then the largest digit d whose bins above it
+// hold less than `want` in sum, and those down to d at least `want`: S.found, with the
+// sum above it and its own.
+__device__ void find_digit(Shared& S, cg::cluster_group& cl, int C, int rank, bool counts, uint64_t want) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cl.sync();
+  const int per = kBins / C;
+  for (int i = tid; i < per; i += kThreads) {
+    const int b = rank * per + i;
+    uint64_t s = 0;
+    for (int c = 0; c < C; ++c) {
+      const Shared* o = cl.map_shared_rank(&S, c);
+      s += counts ? (uint64_t)o->lo[b] : ((uint64_t)o->hi[b] << 32) + o->lo[b];
+    }
+    for (int c = 0; c < C; ++c) cl.map_shared_rank(&S, c)->tot[b] = s;
+  }
+  cl.sync();
+  // thread t: the four bins from 4 t down, counted from the top
+  constexpr int PER = kBins / kThreads;
+  uint64_t v[PER], own = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    v[i] = S.tot[kBins - 1 - (tid * PER + i)];
+    own += v[i];
+  }
+  uint64_t incl = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) S.scan[warp] = incl;
+  __syncthreads();
+  uint64_t before = incl - own;
+  for (int w = 0; w < warp; ++w) before += S.scan[w];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (before < want && before + v[i] >= want) {
+      S.found = kBins - 1 - (tid * PER + i);
+      S.found_before = before;
+      S.found_here = v[i];
+    }
+    before += v[i];
+  }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a, int chunk, int keep_slice) {
+  constexpr int E = 16 / sizeof(T);
+  extern __shared__ __align__(16) unsigned char raw[];
+  Shared& S = *reinterpret_cast<Shared*>(raw);
+  T* kept = reinterpret_cast<T*>(raw + sizeof(Shared));
+  cg::cluster_group cl = cg::this_cluster();
+  const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  auto started = cl.barrier_arrive();            // no CTA is written into before it has started
+  const int row = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slice = chunk * kWarps, first = rank * slice;
+
+  const float temp = a.temperature ? a.temperature[row] : a.temperature_all;
+  const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
+  const float top_p = a.top_p ? a.top_p[row] : a.top_p_all, 
+              min_p = fminf(a.min_p ? a.min_p[row] : a.min_p_all, 1.0f);
+
+  Slice<T, E> sl;
+  sl.row = static_cast<const T*>(a.logits) + (int64_t)row * a.logits_stride + first;
+  sl.have = a.vocab - first;
+  sl.kept = nullptr;
+  sl.vec = (reinterpret_cast<uintptr_t>(sl.row) & 15) == 0;
+
+  if (tid < kTable) S.table[tid] = exp2((double)tid / kTable);
+
+  // ---- the largest logit; the slice into shared memory ----
+  uint32_t top = 0;
+  for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
+    float z[E];
+    sl.global(at, z);
+    if (keep_slice) {
+      union {
+        uint4 v;
+        T t[E];
+      } u;
+#pragma unroll
+      for (int e = 0; e < E; ++e) u.t[e] = (T)z[e];
+      *reinterpret_cast<uint4*>(kept + at) = u.v;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) top = max(top, key_of(z[e]));
+  }
+  if (keep_slice) sl.kept = kept;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) S.warp_cnt[warp] = top;
+  cl.barrier_wait(std::move(started));
+  __syncthreads();
+  if (tid < C) {
+    for (int w = 0; w < kWarps; ++w) top = max(top, S.warp_cnt[w]);
+    cl.map_shared_rank(&S, tid)->top[rank] = top;
+  }
+  cl.sync();
+  top = 0;
+  for (int c = 0; c < C; ++c) top = max(top, S.top[c]);
+
+  Weight wt;
+  wt.table = S.table;
+  wt.top = (double)value_of(top);
+  wt.inv = 1.0 / (double)temp;
+
+  // kept: key > cut, or key == cut and one of the first `ties` tokens of that key
+  uint32_t cut = 1u, ties = 0xffffffffu, equals = 0;
+  // each element of the slice, as f(index in the slice, logit, key)
+  const auto each = [&](auto&& f) {
+    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
+      float z[E];
+      sl.read(at, z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) f(at + e, z[e], key_of(z[e]));
+    }
+  };
+  const auto clear = [&] {
+    for (int i = tid; i < kBins; i += kThreads) S.lo[i] = S.hi[i] = 0;
+    __syncthreads();
+  };
+
+  const bool greedy = !(temp > 0.0f);
+  if (top == 0) {
+    cut = 0xffffffffu, ties = 0;                 // nothing is left of the row
+  } else if (greedy || (top_k <= 0 || top_k >= a.vocab ? false : top_k == 1)) {
+    cut = top, ties = 1;
+  } else {
+    if (top_k > 0 && top_k < a.vocab) {
+      uint64_t want = (uint64_t)top_k;
+      uint32_t prefix = 0;
+      bool all = false;
+#pragma unroll 1
+      for (int level = 0; level < 3 && !all; ++level) {
+        const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+        clear();
+        each([&](int, float, uint32_t k) {
+          if (k && (level == 0 || k >> (shift + bits) == prefix)) atomicAdd(&S.lo[(k >> shift) & ((1u << bits) - 1)], 1u);
+        });
+        if (tid == 0) S.found = 0xffffffffu;
+        find_digit(S, cl, C, rank, true, want);
+        if (S.found == 0xffffffffu) {            // fewer tokens than top_k
+          all = true;
+        } else {
+          want -= S.found_before;
+          prefix = (prefix << bits) | S.found;
+          equals = (uint32_t)S.found_here;
+        }
+      }
+      if (!all) cut = prefix, ties = (uint32_t)want;
+    }
+    if (top_p < 1.0f) {
+      // the weights' total over what top-k left, and the share of it
+      uint64_t want = 0;
+      uint32_t prefix = 0;
+      const uint32_t floor_key = cut;
+#pragma unroll 1
+      for (int level = 0; level < 3; ++level) {
+        const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+        clear();
+        each([&](int, float z, uint32_t k) {
+          if (k >= floor_key && (level == 0 || k >> (shift + bits) == prefix)) {
+            const uint64_t w = wt.units(z);
+            const uint32_t b = (k >> shift) & ((1u << bits) - 1);
+            if (w) add64(&S.lo[b], &S.hi[b], w);
+          }
+        });
+        if (level == 0) {
+          // the total first: the same two exchanges, then a sum over the bins
+          find_digit(S, cl, C, rank, false, ~0ull);
+          uint64_t s = 0;
+          for (int i = tid; i < kBins; i += kThreads) s += S.tot[i];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (lane == 0) S.warp_sum[warp] = s;
+          __syncthreads();
+          s = 0;
+          for (int w = 0; w < kWarps; ++w) s += S.warp_sum[w];
+          if (ties < equals) s -= (uint64_t)(equals - ties) * wt.units(value_of(cut));
+          const double share = (double)fmaxf(top_p, 0.0f) * (double)s;
+          want = max((uint64_t)1, (uint64_t)ceil(share));
+        }
+        find_digit(S, cl, C, rank, false, want);
+        want -= S.found_before;
+        prefix = (prefix << bits) | S.found;
+      }
+      const uint64_t w = wt.units(value_of(prefix));
+      const uint64_t n = w ? (want + w - 1) / w : 1;
+      const uint32_t had = prefix == cut ? ties : 0xffffffffu;
+      cut = prefix;
+      ties = n < had ? (uint32_t)n : had;
+    }
+  }
+
+  // ---- the index behind which tokens of the cutoff's key are left out ----
+  int last = 0x7fffffff;                         // in the row
+  if (ties != 0xffffffffu && ties) {
+    uint32_t n = 0;
+    each([&](int, float, uint32_t k) { n += k == cut; });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) S.warp_cnt[warp] = n;
+    __syncthreads();
+    if (tid < C) {
+      uint32_t s = 0;
+      for (int w = 0; w < kWarps; ++w) s += S.warp_cnt[w];
+      cl.map_shared_rank(&S, tid)->cta_cnt[rank] = s;
+    }
+    cl.sync();
+    uint32_t before = 0, total = 0;
+    for (int c = 0; c < C; ++c) {
+      if (c < rank) before += S.cta_cnt[c];
+      total += S.cta_cnt[c];
+    }
+    if (total > ties) {
+      for (int w = 0; w < warp; ++w) before += S.warp_cnt[w];
+      if (before < ties && before + S.warp_cnt[warp] >= ties) {
+        // this warp holds the last one: by its 32 * E elements at a time
+        for (int at = warp * chunk + lane * E; at - lane * E < (warp + 1) * chunk; at += 32 * E) {
+          float z[E];
+          sl.read(at, z);
+          uint32_t own = 0;
+#pragma unroll
+          for (int e = 0; e < E; ++e) own += key_of(z[e]) == cut;
+          uint32_t incl = own;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+          }
+          uint32_t b = before + incl - own;
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (key_of(z[e]) == cut && ++b == ties)
+              for (int c = 0; c < C; ++c) cl.map_shared_rank(&S, c)->last = first + at + e;
+          before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+      }
+      cl.sync();
+      last = S.last;
+    }
+  }
+  const auto is_kept = [&](int i, uint32_t k) { return k > cut || (k == cut && ties && first + i <= last); };
+  // a greedy row has one token, of weight 1
+  const auto weight = [&](float z) -> double {
+    if (greedy) return 1.0;
+    const double e = wt.e(z);
+    return e >= (double)min_p ? e : 0.0;
+  };
+  const auto units = [&](double e) {
+    return (uint64_t)__double_as_longlong(fma(e, 8796093022208.0, 4503599627370496.0)) & 0xfffffffffffffull;
+  };
+
+  // ---- the kept sum ----
+  uint64_t sum = 0;
+  each([&](int i, float z, uint32_t k) {
+    if (is_kept(i, k)) sum += units(weight(z));
+  });
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  __syncthreads();
+  if (lane == 0) S.warp_sum[warp] = sum;
+  __syncthreads();
+  if (tid < C) {
+    uint64_t s = 0;
+    for (int w = 0; w < kWarps; ++w) s += S.warp_sum[w];
+    cl.map_shared_rank(&S, tid)->cta_sum[rank] = s;
+  }
+  cl.sync();
+  uint64_t before = 0, total = 0;
+  for (int c = 0; c < C; ++c) {
+    if (c < rank) before += S.cta_sum[c];
+    total += S.cta_sum[c];
+  }
+
+  if (a.probs) {
+    const double inv = total ? 8796093022208.0 / (double)total : 0.0;
+    float* out = a.probs + (int64_t)row * a.probs_stride + first;
+    const bool ov = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
+      float z[E], p[E];
+      sl.read(at, z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, key_of(z[e])) ? (float)(weight(z[e]) * inv) : 0.0f;
+      if (ov && at + E <= sl.have) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(out + at + e) = make_float4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at + e < sl.have) out[at + e] = p[e];
+      }
+    }
+  }
+  if (a.tokens) {
+    if (total == 0) {
+      if (rank == 0 && tid == 0) a.tokens[row] = -1;
+      return;
+    }
+    // the first token whose running sum exceeds u * total
+    uint64_t at_sum = (uint64_t)((double)a.u[row] * (double)total);
+    if (at_sum >= total) at_sum = total - 1;
+    for (int w = 0; w < warp; ++w) before += S.warp_sum[w];
+    if (before <= at_sum && before + S.warp_sum[warp] > at_sum) {
+      for (int at = warp * chunk + lane * E; at - lane * E < (warp + 1) * chunk; at += 32 * E) {
+        float z[E];
+        sl.read(at, z);
+        uint64_t w[E], own = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          w[e] = is_kept(at + e, key_of(z[e])) ? units(weight(z[e])) : 0;
+          own += w[e];
+        }
+        uint64_t incl = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        uint64_t b = before + incl - own;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (b <= at_sum && b + w[e] > at_sum) a.tokens[row] = first + at + e;
+          b += w[e];
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_sample_t(const DashSampleArgs& a, cudaStream_t st) {
+  constexpr int E = 16 / sizeof(T);
+  // as many CTAs per row as leave each some work and the GPU's slots filled about once
+  int C = kMaxCluster;
+  while (C > 1 && a.vocab <= (C / 2) * kWarps * 32 * E) C >>= 1;
+  const int parts = C * kWarps;
+  const int chunk = ((a.vocab + parts - 1) / parts + 32 * E - 1) / (32 * E) * (32 * E);
+  const int64_t bytes = (int64_t)chunk * kWarps * sizeof(T);
+  const int keep = bytes <= kSliceMost;
+  static const cudaError_t set =
+      cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared) + kSliceMost);
+  if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(set));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows * C);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared) + (keep ? (size_t)bytes : 0);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, chunk, keep);
+  if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "sample_kernel launch failed: %s", cudaGetErrorString(e));
+  count_launch();
+  return check_launch("sample_kernel");
+}
+
+}  // namespace
+
+int launch_sample(const DashSampleArgs& a, cudaStream_t st) {
+  if (a.dtype == DASH_DTYPE_F32) return launch_sample_t<float>(a, st);
+  if (a.dtype == DASH_DTYPE_BF16) return launch_sample_t<__nv_bfloat16>(a, st);
+  return launch_sample_t<__half>(a, st);
+}
+
+}  // namespace dash

@@ -18,6 +18,9 @@
  *   dash_tree_attn,     speculative decoding over that cache: attention of a tree
  *   dash_draft_verify,  of drafted tokens, their verification, and the pages
  *   dash_pages_*        themselves (copied, forked, compacted, freed)
+ *   dash_add_norm(_bwd) residual sums with their norms, dash_moe a mixture-of-experts
+ *   dash_moe            layer for a few tokens, dash_sample the next token from
+ *   dash_sample         logits and random numbers
  *
  * Conventions
  *  - All pointers are DEVICE pointers unless stated; strides are in ELEMENTS.
@@ -1037,6 +1040,116 @@ int dash_pages_fork(const DashPagesArgs* args, dash_stream_t stream);
 int dash_pages_compact(const DashPagesArgs* args, dash_stream_t stream);
 
 /* ---------------------------------------------------------------------- */
+/* What a decoding or training step does around its attention (no counterpart in
+ * the reference's kernels; its decoder makes these of torch operations).  */
+
+/* dash_add_norm -- the residual sum behind a block and the norm before the next:
+ *   z = post ? y / sqrt(mean(y^2) + eps) * post : y
+ *   stream = residual + scale * gate * z
+ *   normed = stream / sqrt(mean(stream^2) + eps) * weight    (of the unrounded stream)
+ * row by row, in fp32, each output rounded once.  residual NULL: 0 (with stream NULL, a
+ * plain norm).  gate: one row per group of group_rows consecutive rows (rows is a
+ * multiple of it); NULL: 1.  weight, post and gate are fp32 where their flag says so, else
+ * of the rows' type; the inner stride is 1.  stream may lie on residual or y, and normed on
+ * y, if their strides agree.  hidden <= 8192.  */
+typedef struct {
+  const void* y;        int64_t y_stride;
+  const void* residual; int64_t residual_stride;
+  const void* weight;                          /* [hidden] */
+  const void* post;                            /* [hidden] or NULL */
+  const void* gate;     int64_t gate_stride;   /* [rows / group_rows, hidden] or NULL */
+  void* stream;         int64_t stream_stride; /* NULL: not written */
+  void* normed;         int64_t normed_stride;
+  int64_t rows, group_rows;
+  int32_t hidden;
+  int32_t dtype;                               /* DASH_DTYPE_* of the rows */
+  int32_t weight_f32, post_f32, gate_f32;
+  float eps, scale;
+  int32_t pad0;
+} DashNormArgs;
+int dash_add_norm(const DashNormArgs* args, dash_stream_t stream);
+
+/* dash_add_norm_bwd -- its gradients from those of stream (NULL: 0) and normed.
+ * fwd: the forward's arguments (stream and normed are not read).  dy and dresidual are
+ * rows of the rows' type, the weights' gradients contiguous and of their weight's
+ * type; NULL: not wanted.  workspace: dash_add_norm_bwd_workspace_size bytes.  Sums over rows
+ * are fp32 in a fixed order.  */
+typedef struct {
+  DashNormArgs fwd;
+  const void* dstream;  int64_t dstream_stride;
+  const void* dnormed;  int64_t dnormed_stride;
+  void* dy;             int64_t dy_stride;
+  void* dresidual;      int64_t dresidual_stride;
+  void* dweight;
+  void* dpost;
+  void* dgate;
+  void* workspace;
+  size_t workspace_bytes;
+} DashNormBwdArgs;
+size_t dash_add_norm_bwd_workspace_size(const DashNormBwdArgs* args);
+int dash_add_norm_bwd(const DashNormBwdArgs* args, dash_stream_t stream);
+
+/* dash_sample -- the next token of each row of logits, from given random numbers, or
+ * the distribution that it is drawn from.  Row by row, with t, k, p, m the row's
+ * temperature, top_k, top_p and min_p:
+ *   e_i = exp((z_i - max z) / t); tokens with z = -inf or NaN are out
+ *   kept: of the tokens in descending z (lowest index first among equals) the first k
+ *   (k <= 0: all), of those the shortest head that holds the share p of their sum of e
+ *   (p >= 1: all; always the first), of those the ones with e >= m
+ *   tokens: the first kept i whose running sum of e, in the vocabulary's order, exceeds u
+ *   times the kept sum; probs: e_i / kept sum for kept tokens, else 0
+ * t <= 0: the largest z alone.  A row that nothing is left of gives -1 and zeros.  Sums are
+ * whole numbers of 2^-43 of the largest e, so that no order of adding changes them.  Either
+ * of tokens and probs may be NULL.  vocab <= 2^20.  */
+typedef struct {
+  const void* logits;   int64_t logits_stride; /* [rows, vocab] */
+  const float* u;                              /* [rows], in [0, 1); tokens */
+  const float* temperature;                    /* [rows] or NULL: temperature_all, and so on */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+  int32_t rows, vocab;
+  int32_t dtype;                               /* DASH_DTYPE_* of the logits */
+  int32_t pad0;
+  int64_t* tokens;                             /* [rows] or NULL */
+  float* probs;         int64_t probs_stride;  /* [rows, vocab] or NULL */
+} DashSampleArgs;
+int dash_sample(const DashSampleArgs* args, dash_stream_t stream);
+
+/* dash_moe -- a whole mixture-of-experts layer for a few tokens (tokens <= 256):
+ *   score = x gate^T; ids = the topk largest (lowest index among equals; NaN is the
+ *   smallest), in that order; w = softmax(score)[ids] (renorm: over their sum) * scale
+ *   out = residual + sum_j w_j down[ids_j] act_j + shared_down act_s
+ *   act = silu(g) * u of gate_up x, whose first half of rows is g, its second u
+ * x, the experts and out are of one 16-bit type.  Scores are exact to 64 bits, act is kept
+ * as the sum of two 16-bit numbers (with fp16, beyond its range it is infinite), everything else is
+ * fp32, rounded once.  hidden, ffn and shared_ffn are multiples of 8; all rows and pointers
+ * 16-byte aligned.  out may lie on residual.  workspace: dash_moe_workspace_size bytes.  */
+typedef struct {
+  const void* x;          int64_t x_stride;         /* [tokens, hidden] */
+  const void* gate;                                 /* [experts, hidden], fp32 or of x's type */
+  const void* gate_up;                              /* [experts, 2 * ffn, hidden] */
+  const void* down;                                 /* [experts, hidden, ffn] */
+  const void* shared_gate_up;                       /* [2 * shared_ffn, hidden] or NULL */
+  const void* shared_down;                          /* [hidden, shared_ffn] or NULL */
+  const void* residual;   int64_t residual_stride;  /* [tokens, hidden] or NULL: 0 */
+  void* out;              int64_t out_stride;       /* [tokens, hidden] */
+  int32_t* ids;                                     /* [tokens, topk] */
+  float* weights;                                   /* [tokens, topk] */
+  int32_t tokens, hidden, ffn, experts, topk, shared_ffn;
+  int32_t dtype, gate_f32, renorm;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+  DashDeviceError* device_error;
+} DashMoeArgs;
+size_t dash_moe_workspace_size(const DashMoeArgs* args);
+int dash_moe(const DashMoeArgs* args, dash_stream_t stream);
+
+/* ---------------------------------------------------------------------- */
 /* Diagnostics */
 int dash_last_error(char* buf, int len);     /* copies the last host-side error message */
 int dash_library_version(void);              /* (major << 16) | minor */
@@ -1048,7 +1161,8 @@ int dash_count_launches(int reset);          /* kernels launched by this library
  * DashIndexProjArgs, DashRopeKVArgs, DashAttnBwdArgs, DashEntmaxArgs,
  * DashServingPlanArgs, DashPeerHandle, DashPageCoordArgs, DashCosSin2DArgs,
  * DashTreePlanArgs, DashTreeAttnArgs, DashVerifyArgs, DashCacheTensor,
- * DashCommitArgs, DashPagesCopyArgs, DashPagePool, DashPagesArgs.
+ * DashCommitArgs, DashPagesCopyArgs, DashPagePool, DashPagesArgs, DashNormArgs,
+ * DashNormBwdArgs, DashSampleArgs, DashMoeArgs.
  * Lets a binding
  * verify its struct layouts; returns the number of sizes available. */
 int dash_abi_sizes(int64_t* out, int n);

@@ -208,3 +208,72 @@ def test_entmax_rejects_bad_arguments():
     assert _call_status("dash_entmax15_bwd", a) == L.DASH_ERR_INVALID
     a.rows = 0
     assert _call_status("dash_entmax15_fwd", a) == 0
+
+
+def test_norm_rejects_bad_arguments():
+    a = L.DashNormArgs()
+    a.rows, a.group_rows, a.hidden, a.dtype = 4, 4, 64, L.DTYPE_BF16
+    assert _call_status("dash_add_norm", a) == L.DASH_ERR_INVALID and "null" in L.last_error()
+    a.y = a.weight = a.normed = 1 << 20
+    a.y_stride = a.normed_stride = 64
+    for field, bad in (("dtype", 7), ("rows", -1), ("hidden", 0), ("hidden", 8193), ("group_rows", 3), ("group_rows", 0),
+                       ("normed_stride", 63), ("y_stride", -1)):
+        old = getattr(a, field)
+        setattr(a, field, bad)
+        assert _call_status("dash_add_norm", a) in (L.DASH_ERR_INVALID, L.DASH_ERR_UNSUPPORTED), field
+        setattr(a, field, old)
+    b = L.DashNormBwdArgs()
+    b.fwd = a
+    assert _call_status("dash_add_norm_bwd", b) == L.DASH_ERR_INVALID            # null dnormed
+    b.dnormed, b.dnormed_stride = 1 << 20, 64
+    assert L.load().dash_add_norm_bwd_workspace_size(C.byref(b)) >= 4 * 64
+    assert _call_status("dash_add_norm_bwd", b) == L.DASH_ERR_WORKSPACE
+    b.dgate = 1 << 20
+    assert _call_status("dash_add_norm_bwd", b) == L.DASH_ERR_INVALID            # no gate
+    b.fwd.rows = 0
+    assert _call_status("dash_add_norm_bwd", b) == L.DASH_OK
+
+
+def test_sample_rejects_bad_arguments():
+    a = L.DashSampleArgs()
+    a.rows, a.vocab, a.logits_stride = 2, 100, 100
+    assert _call_status("dash_sample", a) == L.DASH_ERR_INVALID and "null" in L.last_error()
+    a.logits = 1 << 20
+    assert _call_status("dash_sample", a) == L.DASH_ERR_INVALID                  # neither output
+    a.tokens = 1 << 20
+    assert _call_status("dash_sample", a) == L.DASH_ERR_INVALID                  # no u
+    a.u = 1 << 20
+    for field, bad in (("dtype", 5), ("rows", -1), ("rows", (1 << 24) + 1), ("vocab", 0), ("vocab", (1 << 20) + 1),
+                       ("logits_stride", -1)):
+        old = getattr(a, field)
+        setattr(a, field, bad)
+        assert _call_status("dash_sample", a) in (L.DASH_ERR_INVALID, L.DASH_ERR_UNSUPPORTED), field
+        setattr(a, field, old)
+    a.probs, a.probs_stride = 1 << 20, 99
+    assert _call_status("dash_sample", a) == L.DASH_ERR_INVALID
+
+
+def test_moe_rejects_bad_arguments():
+    a = L.DashMoeArgs()
+    a.tokens, a.hidden, a.ffn, a.experts, a.topk, a.dtype = 4, 64, 32, 8, 2, L.DTYPE_BF16
+    need = L.load().dash_moe_workspace_size(C.byref(a))
+    assert need > 0
+    assert _call_status("dash_moe", a) == L.DASH_ERR_INVALID and "null" in L.last_error()
+    for field in ("x", "gate", "gate_up", "down", "out", "ids", "weights"):
+        setattr(a, field, 1 << 20)
+    a.x_stride = a.out_stride = 64
+    assert _call_status("dash_moe", a) == L.DASH_ERR_WORKSPACE
+    a.workspace, a.workspace_bytes = 1 << 20, need - 1
+    assert _call_status("dash_moe", a) == L.DASH_ERR_WORKSPACE
+    a.workspace_bytes = need
+    for field, bad in (("dtype", L.DTYPE_F32), ("tokens", -1), ("tokens", 257), ("hidden", 60), ("hidden", 0), ("ffn", 12),
+                       ("shared_ffn", -8), ("shared_ffn", 16), ("experts", 0), ("experts", 257), ("topk", 0), ("topk", 9),
+                       ("x", (1 << 20) + 2), ("x_stride", 68), ("x_stride", 56), ("out_stride", 8)):
+        old = getattr(a, field)
+        setattr(a, field, bad)
+        assert _call_status("dash_moe", a) in (L.DASH_ERR_INVALID, L.DASH_ERR_UNSUPPORTED), (field, bad)
+        if field not in ("x", "x_stride", "out_stride", "shared_ffn"):
+            assert L.load().dash_moe_workspace_size(C.byref(a)) == 0, (field, bad)
+        setattr(a, field, old)
+    a.tokens = 0
+    assert _call_status("dash_moe", a) == L.DASH_OK

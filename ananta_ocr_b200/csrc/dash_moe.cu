@@ -1,8 +1,26 @@
 // dash_moe.cu -- a whole mixture-of-experts layer for a few tokens.
 //
-// Four kernels: the router (scores exact to 64 bits, the picks, their weights), gate_up
-// and SwiGLU of every pick and of the shared expert, down, and the weighted sum in the
-// picks' order.  Bound by the weights of the experts that the tokens picked.
+// Bound by memory: the weights of the experts that the tokens picked cross the bus
+// once, 3 * ffn * hidden numbers each, for a handful of tokens each.  So the weights
+// are the M side of the products (128 rows of an expert's matrix per tile, straight from
+// TMA into shared memory and from there into tcgen05.mma) and the tokens the N side (16 to
+// 64 columns, gathered by row).
+//
+//   moe_route_kernel    scores to 64 bits, the picks and their weights
+//   moe_up_kernel       act = silu(g) * u of every pick and of the shared expert
+//   moe_down_kernel     down * act, by tile of 128 rows and by part of the ffn
+//   moe_combine_kernel  the weighted sum in the picks' order, and the residual
+//
+// Each kernel is launched while the one before it runs and waits for its results on the
+// GPU: gate_up's CTAs bring the shared expert's weights into L2 while the router
+// works, and down's CTAs (a second CTA on each SM) fill their rings with weights while gate_up's
+// last tiles are under way.
+//
+// act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
+// are far from bound by the tensor cores, and the layer's error stays the rounding of its output
+// (with one number it would be 0.0020 instead of 0.0017 of the output, bf16).
+#include <cudaTypedefs.h>
+
 #include "dash_common.cuh"
 #include "dash_internal.h"
 
@@ -10,125 +28,701 @@ namespace dash {
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float load(const void* p, int64_t i) { return (float)static_cast<const T*>(p)[i]; }
+constexpr int kThreads = 192;               // 4 epilogue warps, TMA, MMA
+constexpr int kTile = 128;                  // weight rows of a tile
+constexpr int kStep = 64;                   // k elements of a stage (128 bytes)
+constexpr int kABytes = kTile * 128;
+constexpr int kMaxStages = 8;
+constexpr int kExchange = 2 * 16 * 64 * 4;  // gate_up: accumulators that change warps
+constexpr int kSmem = 113 * 1024;           // two CTAs per SM
 
-// one CTA per token
+// How a call is cut up: the same for equal sizes, whatever the tokens pick, so that a
+// token's sums do not depend on the other tokens.
+struct Cut {
+  int nt;                                   // tokens of a tile at most
+  int ksteps, kshared;                      // 64-element steps of a part of down's k
+  int splits, shared_splits;                // such parts of ffn and of shared_ffn
+};
+
+struct Buffers {                            // workspace
+  size_t hi, lo, shi, slo, part, bytes;
+};
+
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+Cut cut_of(const DashMoeArgs& a) {
+  Cut c;
+  c.nt = a.tokens <= 16 ? 16 : a.tokens <= 128 ? 32 : 64;
+  // parts of down's k: enough items for two rounds of 148 CTAs where few experts are
+  // picked, but no less than four steps each
+  const int picked = min(a.experts, a.tokens * a.topk), tiles = ceil_div(a.hidden, kTile);
+  const int steps = ceil_div(a.ffn, kStep), sh = ceil_div(a.shared_ffn, kStep);
+  int k = max(steps, 1);
+  while (k > 4 && (int64_t)(picked * ceil_div(steps, k) + ceil_div(sh, k)) * tiles < 296) k = ceil_div(k, 2);
+  c.ksteps = k;
+  c.splits = ceil_div(steps, k);
+  c.kshared = k;
+  c.shared_splits = ceil_div(sh, k);
+  return c;
+}
+
+Buffers buffers_of(const DashMoeArgs& a, const Cut& c) {
+  Buffers b;
+  size_t at = 0;
+  const auto take = [&](size_t n) {
+    const size_t here = at;
+    at += (n + 255) & ~(size_t)255;
+    return here;
+  };
+  const size_t picks = (size_t)a.tokens * a.topk;
+  b.hi = take(picks * a.ffn * 2);
+  b.lo = take(picks * a.ffn * 2);
+  b.shi = take((size_t)a.tokens * a.shared_ffn * 2);
+  b.slo = take((size_t)a.tokens * a.shared_ffn * 2);
+  b.part = take((picks * c.splits + (size_t)a.tokens * c.shared_splits) * a.hidden * 4);
+  b.bytes = at + 256;
+  return b;
+}
+
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// router: a cluster of CTAs per token, a warp per expert
+// ---------------------------------------------------------------------------
+constexpr int kRouteThreads = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(256) moe_route_kernel(const DashMoeArgs a) {
-  __shared__ double score[kMoeMaxExperts];
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = warp; e < a.experts; e += 8) {
-    double s = 0.0;
-    for (int i = lane; i < a.hidden; i += 32) {
-      const double g = a.gate_f32 ? (double)static_cast<const float*>(a.gate)[(int64_t)e * a.hidden + i]
-                                  : (double)load<T>(a.gate, (int64_t)e * a.hidden + i);
-      s = fma((double)load<T>(a.x, t * a.x_stride + i), g, s);
-    }
+__device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at, bool f32, int n, int lane) {
+  double s = 0.0;
+  for (int i = lane * 8; i < n; i += 256) {
+    const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
+    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+    if (f32) {
+      const float* g = static_cast<const float*>(gate) + at + i;
+      const float4 a = *reinterpret_cast<const float4*>(g), b = *reinterpret_cast<const float4*>(g + 4);
+      const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) score[e] = s;
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2(xw[j], (T*)nullptr);
+        s = fma((double)f.x, (double)w[2 * j], s);
+        s = fma((double)f.y, (double)w[2 * j + 1], s);
+      }
+    } else {
+      const uint4 gv = *reinterpret_cast<const uint4*>(static_cast<const T*>(gate) + at + i);
+      const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // products of two 16-bit numbers are exact in fp32
+        const float2 f = unpack2(xw[j], (T*)nullptr), w = unpack2(gw[j], (T*)nullptr);
+        s += (double)(f.x * w.x);
+        s += (double)(f.y * w.y);
+      }
+    }
   }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %cluster_nctaid.x;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t n;
+  asm("mov.u32 %0, %cluster_ctarank;" : "=r"(n));
+  return n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+template <typename T>
+__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const DashMoeArgs a) {
+  __shared__ double score[kMoeMaxExperts];
+  __shared__ double red[kRouteThreads / 32], red2[kRouteThreads / 32];
+  __shared__ double best[kMoeMaxTopk];
+  __shared__ int id[kMoeMaxTopk];
+  launch_next();
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int t = blockIdx.x / C, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  cluster_arrive();
+  const T* x = static_cast<const T*>(a.x) + t * a.x_stride;
+  bool waited = false;
+  for (int e = rank * 8 + warp; e - warp < a.experts; e += 8 * C) {
+    double s = 0.0;
+    if (e < a.experts) s = dot64(x, a.gate, (int64_t)e * a.hidden, a.gate_f32, a.hidden, lane);
+    if (!waited) cluster_wait();                 // the first CTA has started
+    waited = true;
+    if (e < a.experts && lane == 0) {
+      uint32_t to;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(score + e)), "r"(0));
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(s) : "memory");
+    }
+  }
+  if (!waited) cluster_wait();
+  cluster_arrive();
+  cluster_wait();
+  if (rank) return;
+  // a thread per expert; its place among all of them decides
+  const double mine = tid < a.experts ? score[tid] : 0.0;
+  const bool nan = mine != mine;
+  double top = tid < a.experts && !nan ? mine : -INFINITY;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) red[warp] = top;
   __syncthreads();
-  if (warp) return;
-  double top = -INFINITY, sum = 0.0;
-  for (int e = 0; e < a.experts; ++e) top = fmax(top, score[e]);
-  for (int e = lane; e < a.experts; e += 32) sum += exp(score[e] - top);
+  for (int w = 0; w < kRouteThreads / 32; ++w) top = fmax(top, red[w]);
+  // (a NaN score makes the sum NaN)
+  const double e = tid < a.experts ? (mine == top ? 1.0 : exp(mine - top)) : 0.0;
+  double sum = e;
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  double mine = 0.0, picked = 0.0;
-  int id = 0;
-  uint32_t used = 0;                         // this lane's experts that are taken
-  for (int j = 0; j < a.topk; ++j) {
-    double best = 0.0;
-    int at = -1;
-    for (int e = lane, i = 0; e < a.experts; e += 32, ++i) {
-      const double s = score[e] == score[e] ? score[e] : -INFINITY;
-      if (!(used >> i & 1u) && (at < 0 || s > best)) best = s, at = e;
+  if (lane == 0) red2[warp] = sum;
+  if (tid < a.experts) {
+    const double m = nan ? -INFINITY : mine;
+    int before = 0;
+    for (int j = 0; j < a.experts; ++j) {
+      const double s = score[j] != score[j] ? -INFINITY : score[j];
+      before += s > m || (s == m && j < tid);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const double s = __shfl_xor_sync(0xffffffffu, best, o);
-      const int e = __shfl_xor_sync(0xffffffffu, at, o);
-      if (e >= 0 && (at < 0 || s > best || (s == best && e < at))) best = s, at = e;
-    }
-    if ((at & 31) == lane) used |= 1u << (at >> 5);
-    const double p = exp(score[at] - top) / sum;
-    if (lane == j) mine = p, id = at;
-    picked += p;
+    if (before < a.topk) best[before] = e, id[before] = tid;
   }
-  if (lane < a.topk) {
-    a.ids[t * a.topk + lane] = id;
-    a.weights[t * a.topk + lane] = (float)(mine / (a.renorm ? picked : 1.0) * (double)a.scale);
+  __syncthreads();
+  if (tid < a.topk) {
+    double total = 0.0, picked = 0.0;
+    for (int w = 0; w < kRouteThreads / 32; ++w) total += red2[w];
+    for (int j = 0; j < a.topk; ++j) picked += best[j];
+    a.ids[(int64_t)t * a.topk + tid] = id[tid];
+    a.weights[(int64_t)t * a.topk + tid] = (float)(best[tid] / (a.renorm ? picked + 0.0 * total : total) * (double)a.scale);
   }
 }
 
-// act[row][f]: a warp per feature; rows: the picks, then the tokens' shared expert
+// ---------------------------------------------------------------------------
+// gate_up and down
+// ---------------------------------------------------------------------------
+struct Maps {
+  CUtensorMap w, sw;                        // an expert's matrix, the shared one
+  CUtensorMap b, sb;                        // gate_up: x (both); down: hi of act, of the shared act
+  CUtensorMap lo, slo;                      // down: lo of act
+};
+
+__host__ __device__ constexpr int counts_bytes(int experts) {
+  return 2 * ((experts + 4) & ~3) * 4 + ((kThreads / 32 * experts + 3) & ~3) * 4;
+}
+
+struct Layout {                             // dynamic shared memory behind the ring
+  int stage, stages, bars, exchange, counts, list, bytes;
+};
+
+template <bool DOWN>
+__host__ __device__ inline Layout layout_of(int nt, int experts, int picks) {
+  Layout l;
+  l.stage = kABytes + nt * 128 * (DOWN ? 2 : 1);
+  const int control = 512 + (DOWN ? 0 : kExchange) + counts_bytes(experts) + ((picks * 2 + 15) & ~15);
+  l.stages = (kSmem - 1024 - control) / l.stage;
+  if (l.stages > kMaxStages) l.stages = kMaxStages;
+  l.bars = l.stages * l.stage;
+  l.exchange = l.bars + 512;
+  l.counts = l.exchange + (DOWN ? 0 : kExchange);
+  l.list = l.counts + counts_bytes(experts);
+  l.bytes = l.list + ((picks * 2 + 15) & ~15) + 1024;
+  return l;
+}
+
+// One tile of work: n tokens from `first` (of the expert's list, or the tokens
+// themselves) times rows mt * 128 .. of a matrix, k steps k0 .. k1
+struct Item {
+  bool shared;
+  int expert, first, n, mt, part, k0, k1;
+};
+
+template <bool DOWN>
+struct Tiles {
+  const int *base, *units;                  // per expert: its picks' start in the list, its tiles' start
+  int experts, nt, tokens, mt, smt, k, sk, kpart, parts, sparts, shared, total;
+
+  __device__ __forceinline__ Item at(int i) const {
+    Item it;
+    it.shared = i < shared;
+    if (!it.shared) i -= shared;
+    const int tiles = it.shared ? smt : mt, np = it.shared ? sparts : parts;
+    it.mt = i % tiles;
+    i /= tiles;
+    it.part = i % np;
+    i /= np;
+    if (it.shared) {
+      it.expert = 0;
+      it.first = i * nt;
+      it.n = min(nt, tokens - it.first);
+    } else {
+      int lo = 0, hi = experts;             // units[lo] <= i < units[hi]
+      while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (units[m] <= i) lo = m;
+        else hi = m;
+      }
+      it.expert = lo;
+      it.first = base[lo] + (i - units[lo]) * nt;
+      it.n = min(nt, base[lo + 1] - it.first);
+    }
+    it.k0 = it.part * kpart;
+    it.k1 = min(it.shared ? sk : k, it.k0 + kpart);
+    return it;
+  }
+};
+
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+
+// whether `ok` holds in all of the four epilogue warps (a barrier of theirs)
+__device__ __forceinline__ bool all_warps(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)ok)
+      : "memory");
+  return r != 0;
+}
+
+template <typename T, bool DOWN>
+__global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant__ Maps maps, const DashMoeArgs a, const Cut cut,
+                                                           const Buffers buf) {
+  extern __shared__ __align__(1024) uint8_t raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int picks = a.tokens * a.topk;
+  const Layout lay = layout_of<DOWN>(cut.nt, a.experts, picks);
+  const int NS = lay.stages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm + lay.bars);      // [stages] TMA -> MMA
+  uint64_t* empty = full + kMaxStages;                              // [stages] MMA -> TMA
+  uint64_t* acc_full = empty + kMaxStages;                          // [2] MMA -> epilogue
+  uint64_t* acc_empty = acc_full + 2;                               // [2] epilogue -> MMA
+  uint32_t* holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
+  int* base = reinterpret_cast<int*>(sm + lay.counts);              // [experts + 1]
+  int* units = base + ((a.experts + 4) & ~3);                       // [experts + 1]
+  int* cursor = units + ((a.experts + 4) & ~3);                     // [warps][experts]
+  uint16_t* list = reinterpret_cast<uint16_t*>(sm + lay.list);      // picks, by expert
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  DeviceError* derr = a.device_error;
+  const int cols = max(32, cut.nt);                                 // TMEM columns of an accumulator
+
+  if (tid == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(full + i, 1);
+      mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + i, 1);
+      mbar_init(acc_empty + i, 128);
+    }
+    *abort_flag = 0;
+    mbar_init_fence();
+  }
+  if (warp == 5) {
+    tmem_alloc(holder, 2 * cols);
+    tmem_relinquish();
+  }
+  for (int e = tid; e < a.experts * (kThreads / 32); e += kThreads) cursor[e] = 0;
+  if (!DOWN && a.shared_ffn) {
+    // the shared expert's weights into L2, while the router works
+    const int64_t bytes = (int64_t)a.shared_ffn * a.hidden * 2, piece = 4096;
+    for (int64_t at = ((int64_t)blockIdx.x * kThreads + tid) * piece; at < 3 * bytes; at += (int64_t)gridDim.x * kThreads * piece) {
+      const bool up = at < 2 * bytes;
+      const char* p = up ? static_cast<const char*>(a.shared_gate_up) + at : static_cast<const char*>(a.shared_down) + (at - 2 * bytes);
+      const int64_t n = min(piece, (up ? 2 * bytes : 3 * bytes) - at);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)n) : "memory");
+    }
+  }
+  // gate_up waits for the router here.  down starts when every CTA of gate_up has done so:
+  // the picks are there, act is not.
+  if (!DOWN) wait_previous();
+  launch_next();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *holder;
+
+  // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
+  // the same tiles): each warp counts and then places a sixth of them ----
+  constexpr int W = kThreads / 32;
+  const int seg = ceil_div(ceil_div(picks, W), 32) * 32, p0 = warp * seg, p1 = min(picks, p0 + seg);
+  for (int p = p0 + lane; p < p1; p += 32) atomicAdd(cursor + warp * a.experts + __ldcg(a.ids + p), 1);
+  __syncthreads();
+  if (warp == 0) {
+    int run = 0, urun = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const int e = e0 + lane;
+      int n = 0;
+      if (e < a.experts)
+        for (int w = 0; w < W; ++w) n += cursor[w * a.experts + e];
+      const int u0 = ceil_div(n, cut.nt);
+      int s = n, u = u0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, s, o), z = __shfl_up_sync(0xffffffffu, u, o);
+        if (lane >= o) s += y, u += z;
+      }
+      if (e < a.experts) {
+        int at = run + s - n;
+        base[e] = at;
+        units[e] = urun + u - u0;
+        for (int w = 0; w < W; ++w) {
+          const int c = cursor[w * a.experts + e];
+          cursor[w * a.experts + e] = at;
+          at += c;
+        }
+      }
+      run += __shfl_sync(0xffffffffu, s, 31);
+      urun += __shfl_sync(0xffffffffu, u, 31);
+    }
+    if (lane == 0) base[a.experts] = run, units[a.experts] = urun;
+  }
+  __syncthreads();
+  for (int p = p0; p < p1; p += 32) {
+    const bool in = p + lane < p1;
+    const int e = in ? __ldcg(a.ids + p + lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    int at = 0;
+    if (in) at = cursor[warp * a.experts + e] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (in) {
+      list[at] = (uint16_t)(p + lane);
+      if (lane == 31 - __clz(same)) cursor[warp * a.experts + e] = at + 1;
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+
+  Tiles<DOWN> tiles;
+  tiles.base = base;
+  tiles.units = units;
+  tiles.experts = a.experts;
+  tiles.nt = cut.nt;
+  tiles.tokens = a.tokens;
+  tiles.mt = ceil_div(DOWN ? a.hidden : a.ffn, DOWN ? kTile : kTile / 2);
+  tiles.smt = a.shared_ffn ? ceil_div(DOWN ? a.hidden : a.shared_ffn, DOWN ? kTile : kTile / 2) : 1;
+  tiles.k = ceil_div(DOWN ? a.ffn : a.hidden, kStep);
+  tiles.sk = ceil_div(DOWN ? a.shared_ffn : a.hidden, kStep);
+  tiles.kpart = DOWN ? cut.ksteps : tiles.k;
+  tiles.parts = DOWN ? cut.splits : 1;
+  tiles.sparts = DOWN ? max(1, cut.shared_splits) : 1;
+  tiles.shared = a.shared_ffn ? ceil_div(a.tokens, cut.nt) * tiles.smt * tiles.sparts : 0;
+  tiles.total = tiles.shared + units[a.experts] * tiles.mt * tiles.parts;
+
+  if (warp == 4) {
+    // =================== TMA: weights by lane 0, four token rows per lane ===================
+    if (lane == 0) {
+      prefetch_tmap(&maps.w);
+      prefetch_tmap(&maps.b);
+    }
+    int s = 0;                                    // steps so far
+    bool ok = true;
+    // down: the weights of the first stages go ahead of the wait for act
+    int ahead = 0;
+    if (DOWN) {
+      for (int i = blockIdx.x; i < tiles.total && ahead < NS; i += gridDim.x) {
+        const Item it = tiles.at(i);
+        const uint32_t bytes = kABytes + (uint32_t)((it.n + 15) & ~15) * 256;
+        for (int k = it.k0; k < it.k1 && ahead < NS; ++k, ++ahead)
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full + ahead, bytes);
+            tma_load_4d(sm + ahead * lay.stage, it.shared ? &maps.sw : &maps.w, full + ahead, k * kStep, it.mt * kTile, it.expert, 0);
+          }
+      }
+      wait_previous();
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+    }
+    for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x) {
+      const Item it = tiles.at(i);
+      const int groups = (it.n + 15) / 16 * 4;    // of four rows
+      const int g = DOWN ? lane & 15 : lane;
+      const CUtensorMap* bm = DOWN && lane >= 16 ? (it.shared ? &maps.slo : &maps.lo) : it.shared ? &maps.sb : &maps.b;
+      int r[4] = {0, 0, 0, 0};
+      if (g < groups && (DOWN || lane < 16))
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = it.first + min(g * 4 + j, it.n - 1);     // columns behind the last: its copies
+          r[j] = it.shared ? at : DOWN ? list[at] : list[at] / a.topk;
+        }
+      const uint32_t half = (uint32_t)groups * 512;               // bytes of the tokens' rows
+      for (int k = it.k0; k < it.k1; ++k, ++s) {
+        const int st = s % NS;
+        if (s >= NS && !mbar_wait_warp(empty + st, ((s / NS) - 1) & 1, abort_flag, derr, 90)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = sm + st * lay.stage;
+        if (s >= ahead) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(full + st, kABytes + half * (DOWN ? 2 : 1));
+            if (DOWN) {
+              tma_load_4d(dst, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, it.mt * kTile, it.expert, 0);
+            } else {
+              // 64 gate rows, then their up rows
+              const int f = it.mt * (kTile / 2), n = it.shared ? a.shared_ffn : a.ffn;
+              tma_load_4d(dst, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, f, it.expert, 0);
+              tma_load_4d(dst + kABytes / 2, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, n + f, it.expert, 0);
+            }
+          }
+          __syncwarp();
+        }
+        if (g < groups && (DOWN || lane < 16))
+          tma_gather4(dst + kABytes + (lane >= 16 ? half : 0) + g * 512, bm, full + st, k * kStep, r[0], r[1], r[2], r[3]);
+      }
+    }
+    // never leave with copies in flight
+    if (!ok && s < ahead) s = ahead;
+    for (int k = max(0, s - NS); k < s; ++k) {
+      volatile int no_abort = 0;
+      mbar_wait_warp(full + (k % NS), (k / NS) & 1, &no_abort, nullptr, 91);
+    }
+  } else if (warp == 5) {
+    // =================== MMA ===================
+    if (lane == 0) {
+      int s = 0, n_item = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x, ++n_item) {
+        const Item it = tiles.at(i);
+        const uint32_t n16 = (uint32_t)((it.n + 15) & ~15);
+        const uint32_t idesc = make_idesc(DType<T>::fmt, 0, 0, kTile, n16);
+        const int b = n_item & 1;
+        if (n_item >= 2 && !mbar_wait(acc_empty + b, ((n_item >> 1) - 1) & 1, abort_flag, derr, 92)) break;
+        tc_fence_after();
+        for (int k = it.k0; k < it.k1; ++k, ++s) {
+          const int st = s % NS;
+          if (!mbar_wait(full + st, (s / NS) & 1, abort_flag, derr, 93)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sA = smem_u32(sm + st * lay.stage), sB = sA + kABytes;
+#pragma unroll
+          for (int kk = 0; kk < kStep / 16; ++kk) {
+            const uint64_t ad = sw128_desc(sA + kk * 32, 16, 1024);
+            umma_ss(tmem + b * cols, ad, sw128_desc(sB + kk * 32, 16, 1024), idesc, k > it.k0 || kk > 0);
+            if (DOWN) umma_ss(tmem + b * cols, ad, sw128_desc(sB + n16 * 128 + kk * 32, 16, 1024), idesc, 1);
+          }
+          umma_commit(empty + st);
+        }
+        umma_commit(acc_full + b);
+      }
+      // what was issued is done before TMEM goes back
+      for (int k = max(0, n_item - 2); k < n_item; ++k) {
+        volatile int no_abort = 0;
+        mbar_wait(acc_full + (k & 1), (k >> 1) & 1, &no_abort, nullptr, 94);
+      }
+    }
+  } else {
+    // =================== epilogue: thread = weight row = TMEM lane ===================
+    if (DOWN) wait_previous();
+    float* xs = reinterpret_cast<float*>(sm + lay.exchange);        // [2][16][64]
+    T* hi = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.hi);
+    T* lo = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.lo);
+    T* shi = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.shi);
+    T* slo = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.slo);
+    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + buf.part);
+    int n_item = 0;
+    for (int i = blockIdx.x; i < tiles.total; i += gridDim.x, ++n_item) {
+      const Item it = tiles.at(i);
+      const int b = n_item & 1;
+      bool ok = mbar_wait_warp(acc_full + b, (n_item >> 1) & 1, abort_flag, derr, 95);
+      if (!DOWN) ok = all_warps(ok);              // none goes on to an exchange that another has left
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t tm = tmem + b * cols + ((uint32_t)(warp * 32) << 16);
+      for (int c0 = 0; c0 < it.n; c0 += 32) {
+        float v[32];
+        tmem_ld32f(tm + c0, v);
+        tmem_ld_wait();
+        if (c0 + 32 >= it.n) {
+          tc_fence_before();
+          mbar_arrive(acc_empty + b);
+        }
+        if (DOWN) {
+          const int h = it.mt * kTile + warp * 32 + lane;
+          if (h < a.hidden)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c0 + c < it.n) {
+                const int at = it.first + c0 + c;
+                const int64_t row = it.shared ? (int64_t)picks * cut.splits + (int64_t)at * cut.shared_splits + it.part
+                                              : (int64_t)list[at] * cut.splits + it.part;
+                __stcg(part + row * a.hidden + h, v[c]);
+              }
+        } else {
+          // warps 0, 1 hold g and take columns 0..15, warps 2, 3 hold u and take the others
+          const int f = (warp & 1) * 32 + lane, upper = warp >> 1;
+          if (c0) asm volatile("bar.sync 1, 128;" ::: "memory");    // the last exchange has been read
+#pragma unroll
+          for (int c = 0; c < 16; ++c) xs[(upper * 16 + c) * 64 + f] = upper ? v[c] : v[16 + c];
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const int width = it.shared ? a.shared_ffn : a.ffn, col = it.mt * (kTile / 2) + f;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const int n = c0 + upper * 16 + c;
+            if (n < it.n && col < width) {
+              const float other = xs[((1 - upper) * 16 + c) * 64 + f];
+              const float g = upper ? other : v[c], u = upper ? v[16 + c] : other;
+              const float x = silu(g) * u;
+              const T h = (T)x;
+              // (beyond the type's range: infinite, and no infinity less infinity)
+              const T l = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
+              const int64_t at = (int64_t)(it.shared ? it.first + n : list[it.first + n]) * width + col;
+              (it.shared ? shi : hi)[at] = h;
+              (it.shared ? slo : lo)[at] = l;
+            }
+          }
+        }
+      }
+    }
+  }
+  if (DOWN && warp == 5) wait_previous();         // every CTA of this grid has seen the last one's end
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, 2 * cols);
+}
+
+// ---------------------------------------------------------------------------
+// the sum: a thread per four columns of a token
+// ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) moe_up_kernel(const DashMoeArgs a, float* act) {
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(128) moe_combine_kernel(const DashMoeArgs a, const Cut cut, const Buffers buf) {
+  const int t = blockIdx.y, h = ((int)blockIdx.x * 128 + threadIdx.x) * 4;
+  const float* part = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + buf.part);
+  wait_previous();
+  if (h >= a.hidden) return;
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (a.residual) {
+    const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.residual) + t * a.residual_stride + h);
+    const float2 x = unpack2(r.x, (T*)nullptr), y = unpack2(r.y, (T*)nullptr);
+    s = make_float4(x.x, x.y, y.x, y.y);
+  }
   const int64_t picks = (int64_t)a.tokens * a.topk;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const bool shared = w >= picks * a.ffn;
-  const int64_t v = shared ? w - picks * a.ffn : w;
-  const int n = shared ? a.shared_ffn : a.ffn;
-  if (n == 0 || v >= (shared ? (int64_t)a.tokens : picks) * n) return;
-  const int64_t r = v / n;
-  const int f = (int)(v % n);
-  const int64_t t = shared ? r : r / a.topk;
-  const T* g = shared ? static_cast<const T*>(a.shared_gate_up)
-                      : static_cast<const T*>(a.gate_up) + (int64_t)a.ids[r] * 2 * a.ffn * a.hidden;
-  float x = 0.0f, y = 0.0f;
-  for (int i = lane; i < a.hidden; i += 32) {
-    const float h = load<T>(a.x, t * a.x_stride + i);
-    x = fmaf(h, (float)g[(int64_t)f * a.hidden + i], x);
-    y = fmaf(h, (float)g[(int64_t)(n + f) * a.hidden + i], y);
+  const auto rows = [&](int64_t row, int n, float w) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < n; ++i) {
+      const float4 p = __ldcg(reinterpret_cast<const float4*>(part + (row + i) * a.hidden + h));
+      v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
+    }
+    s.x = fmaf(w, v.x, s.x), s.y = fmaf(w, v.y, s.y), s.z = fmaf(w, v.z, s.z), s.w = fmaf(w, v.w, s.w);
+  };
+#pragma unroll 4
+  for (int j = 0; j < a.topk; ++j) {
+    const int64_t p = (int64_t)t * a.topk + j;
+    rows(p * cut.splits, cut.splits, __ldcg(a.weights + p));
   }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o), y += __shfl_xor_sync(0xffffffffu, y, o);
-  if (lane == 0) act[w] = x / (1.0f + expf(-x)) * y;
+  rows(picks * cut.splits + (int64_t)t * cut.shared_splits, cut.shared_splits, 1.0f);
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + t * a.out_stride + h) =
+      make_uint2(pack2(s.x, s.y, (T*)nullptr), pack2(s.z, s.w, (T*)nullptr));
 }
 
-// out: a warp per (token, feature)
-template <typename T>
-__global__ void __launch_bounds__(256) moe_down_kernel(const DashMoeArgs a, const float* act) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (w >= (int64_t)a.tokens * a.hidden) return;
-  const int64_t t = w / a.hidden, h = w % a.hidden;
-  float s = a.residual ? load<T>(a.residual, t * a.residual_stride + h) : 0.0f;
-  for (int j = 0; j <= a.topk; ++j) {
-    const bool shared = j == a.topk;
-    const int n = shared ? a.shared_ffn : a.ffn;
-    const int64_t r = t * a.topk + j;
-    const float* x = shared ? act + (int64_t)a.tokens * a.topk * a.ffn + t * n : act + r * n;
-    const T* d = shared ? static_cast<const T*>(a.shared_down)
-                        : static_cast<const T*>(a.down) + (int64_t)a.ids[r] * a.hidden * n;
-    float y = 0.0f;
-    for (int i = lane; i < n; i += 32) y = fmaf(x[i], (float)d[h * n + i], y);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (n) s = fmaf(y, shared ? 1.0f : a.weights[r], s);
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// [outer, rows, cols] of 16-bit numbers, boxes of box_rows rows and 64 columns, 128-byte swizzle;
+// box_rows 1: a plain [rows, cols] whose rows are gathered
+int encode(CUtensorMap* m, const void* p, bool bf16, int64_t cols, int64_t rows, int64_t stride, int64_t outer, int box_rows) {
+  const auto fn = encoder();
+  if (!fn) return set_error(DASH_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  const bool gather = box_rows == 1;
+  const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)outer, 1};
+  const cuuint64_t strides[3] = {(cuuint64_t)stride * 2, (cuuint64_t)(stride * rows) * 2, (cuuint64_t)(stride * rows * outer) * 2};
+  const cuuint32_t box[4] = {kStep, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, gather ? 2 : 4,
+                        const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? DASH_OK : set_error(DASH_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+}
+
+template <typename... P, typename... A>
+int launch(const char* name, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, bool early, int cluster, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  if (early) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (lane == 0) static_cast<T*>(a.out)[t * a.out_stride + h] = (T)s;
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = at;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+  if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "%s launch failed: %s", name, cudaGetErrorString(e));
+  count_launch();
+  return check_launch(name);
 }
 
 template <typename T>
 int launch_moe_t(const DashMoeArgs& a, cudaStream_t st) {
-  float* act = static_cast<float*>(a.workspace);
-  moe_route_kernel<T><<<a.tokens, 256, 0, st>>>(a);
-  const int64_t rows = (int64_t)a.tokens * ((int64_t)a.topk * a.ffn + a.shared_ffn);
-  moe_up_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(a, act);
-  moe_down_kernel<T><<<(unsigned)(((int64_t)a.tokens * a.hidden + 7) / 8), 256, 0, st>>>(a, act);
-  for (int i = 0; i < 3; ++i) count_launch();
-  return check_launch("moe kernels");
+  constexpr bool kBf16 = DType<T>::fmt == 1;
+  const Cut cut = cut_of(a);
+  const Buffers buf = buffers_of(a, cut);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  const int64_t picks = (int64_t)a.tokens * a.topk;
+  static const cudaError_t set = [] {
+    const cudaError_t e = cudaFuncSetAttribute(moe_ffn_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(moe_ffn_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  }();
+  if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "moe_ffn_kernel: %s", cudaGetErrorString(set));
+  Maps up, down;
+  const int64_t xs = a.tokens > 1 ? a.x_stride : a.hidden;
+  int rc = encode(&up.w, a.gate_up, kBf16, a.hidden, 2 * a.ffn, a.hidden, a.experts, kTile / 2);
+  if (!rc) rc = encode(&up.b, a.x, kBf16, a.hidden, a.tokens, xs, 1, 1);
+  up.sb = up.lo = up.slo = up.b;
+  up.sw = up.w;
+  if (!rc) rc = encode(&down.w, a.down, kBf16, a.ffn, a.hidden, a.ffn, a.experts, kTile);
+  if (!rc) rc = encode(&down.b, ws + buf.hi, kBf16, a.ffn, picks, a.ffn, 1, 1);
+  if (!rc) rc = encode(&down.lo, ws + buf.lo, kBf16, a.ffn, picks, a.ffn, 1, 1);
+  down.sw = down.w, down.sb = down.b, down.slo = down.lo;
+  if (a.shared_ffn) {
+    if (!rc) rc = encode(&up.sw, a.shared_gate_up, kBf16, a.hidden, 2 * a.shared_ffn, a.hidden, 1, kTile / 2);
+    if (!rc) rc = encode(&down.sw, a.shared_down, kBf16, a.shared_ffn, a.hidden, a.shared_ffn, 1, kTile);
+    if (!rc) rc = encode(&down.sb, ws + buf.shi, kBf16, a.shared_ffn, a.tokens, a.shared_ffn, 1, 1);
+    if (!rc) rc = encode(&down.slo, ws + buf.slo, kBf16, a.shared_ffn, a.tokens, a.shared_ffn, 1, 1);
+  }
+  if (rc) return rc;
+  int cluster = 8;
+  while (cluster > 1 && a.experts <= 4 * cluster) cluster >>= 1;
+  rc = launch("moe_route_kernel", moe_route_kernel<T>, dim3((unsigned)(a.tokens * cluster)), kRouteThreads, 0, st, false, cluster, a);
+  const Layout lu = layout_of<false>(cut.nt, a.experts, (int)picks), ld = layout_of<true>(cut.nt, a.experts, (int)picks);
+  if (!rc) rc = launch("moe_up_kernel", moe_ffn_kernel<T, false>, dim3(148), kThreads, lu.bytes, st, true, 1, up, a, cut, buf);
+  if (!rc) rc = launch("moe_down_kernel", moe_ffn_kernel<T, true>, dim3(148), kThreads, ld.bytes, st, true, 1, down, a, cut, buf);
+  const dim3 grid((unsigned)ceil_div(a.hidden, 512), (unsigned)a.tokens);
+  if (!rc) rc = launch("moe_combine_kernel", moe_combine_kernel<T>, grid, 128, 0, st, true, 1, a, cut, buf);
+  return rc;
 }
 
 }  // namespace
 
-size_t moe_workspace(const DashMoeArgs& a) {
-  return (size_t)a.tokens * ((size_t)a.topk * a.ffn + a.shared_ffn) * sizeof(float) + 16;
-}
+size_t moe_workspace(const DashMoeArgs& a) { return buffers_of(a, cut_of(a)).bytes; }
 
 int launch_moe(const DashMoeArgs& a, cudaStream_t st) {
   return a.dtype == DASH_DTYPE_BF16 ? launch_moe_t<__nv_bfloat16>(a, st) : launch_moe_t<__half>(a, st);

@@ -13,8 +13,8 @@
 //
 // Each kernel is launched while the one before it runs and waits for its results on the
 // GPU: gate_up's CTAs bring the shared expert's weights into L2 while the router
-// works, and down's CTAs (a second CTA on each SM) fill their rings with weights while gate_up's
-// last tiles are under way.
+// works, and down's CTAs take the places of gate_up's as they end and fill their rings with
+// weights while its last tiles are under way.
 //
 // act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
 // are far from bound by the tensor cores, and the layer's error stays the rounding of its output
@@ -28,24 +28,26 @@ namespace dash {
 
 namespace {
 
-constexpr int kThreads = 192;               // 4 epilogue warps, TMA, MMA
+constexpr int kThreads = 224;               // 4 epilogue warps, weights, MMA, tokens
 constexpr int kTile = 128;                  // weight rows of a tile
 constexpr int kStep = 64;                   // k elements of a stage (128 bytes)
 constexpr int kABytes = kTile * 128;
 constexpr int kMaxStages = 8;
 constexpr int kExchange = 2 * 16 * 64 * 4;  // gate_up: accumulators that change warps
 constexpr int kSmem = 113 * 1024;           // two CTAs per SM
+constexpr int kCtas = 2 * 148;
 
 // How a call is cut up: the same for equal sizes, whatever the tokens pick, so that a
 // token's sums do not depend on the other tokens.
 struct Cut {
   int nt;                                   // tokens of a tile at most
+  int rows;                                 // gate_up: gate rows of a tile (and as many up rows), 64 or 32
   int ksteps, kshared;                      // 64-element steps of a part of down's k
   int splits, shared_splits;                // such parts of ffn and of shared_ffn
 };
 
 struct Buffers {                            // workspace
-  size_t hi, lo, shi, slo, part, bytes;
+  size_t act, sact, part, bytes;            // act: [2][picks by expert][ffn], both parts of the numbers
 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -53,12 +55,15 @@ __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; 
 Cut cut_of(const DashMoeArgs& a) {
   Cut c;
   c.nt = a.tokens <= 16 ? 16 : a.tokens <= 128 ? 32 : 64;
-  // parts of down's k: enough items for two rounds of 148 CTAs where few experts are
-  // picked, but no less than four steps each
+  // narrow tiles where the wide ones would leave CTAs without work
+  const int chosen = min(a.experts, a.tokens * a.topk);
+  c.rows = (int64_t)chosen * ceil_div(a.ffn, 64) + ceil_div(a.shared_ffn, 64) * ceil_div(a.tokens, c.nt) < kCtas ? 32 : 64;
+  // parts of down's k: an item for every CTA where few experts are picked, but no less
+  // than four steps each
   const int picked = min(a.experts, a.tokens * a.topk), tiles = ceil_div(a.hidden, kTile);
   const int steps = ceil_div(a.ffn, kStep), sh = ceil_div(a.shared_ffn, kStep);
   int k = max(steps, 1);
-  while (k > 4 && (int64_t)(picked * ceil_div(steps, k) + ceil_div(sh, k)) * tiles < 296) k = ceil_div(k, 2);
+  while (k > 4 && (int64_t)(picked * ceil_div(steps, k) + ceil_div(sh, k)) * tiles < kCtas) k = ceil_div(k, 2);
   c.ksteps = k;
   c.splits = ceil_div(steps, k);
   c.kshared = k;
@@ -75,10 +80,8 @@ Buffers buffers_of(const DashMoeArgs& a, const Cut& c) {
     return here;
   };
   const size_t picks = (size_t)a.tokens * a.topk;
-  b.hi = take(picks * a.ffn * 2);
-  b.lo = take(picks * a.ffn * 2);
-  b.shi = take((size_t)a.tokens * a.shared_ffn * 2);
-  b.slo = take((size_t)a.tokens * a.shared_ffn * 2);
+  b.act = take(2 * picks * a.ffn * 2);
+  b.sact = take(2 * (size_t)a.tokens * a.shared_ffn * 2);
   b.part = take((picks * c.splits + (size_t)a.tokens * c.shared_splits) * a.hidden * 4);
   b.bytes = at + 256;
   return b;
@@ -203,9 +206,8 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const DashMoeA
 // gate_up and down
 // ---------------------------------------------------------------------------
 struct Maps {
-  CUtensorMap w, sw;                        // an expert's matrix, the shared one
-  CUtensorMap b, sb;                        // gate_up: x (both); down: hi of act, of the shared act
-  CUtensorMap lo, slo;                      // down: lo of act
+  CUtensorMap w, sw;                        // the experts' matrices, the shared one
+  CUtensorMap b, sb;                        // gate_up: x by rows, x by 16 rows; down: act, the shared act
 };
 
 __host__ __device__ constexpr int counts_bytes(int experts) {
@@ -217,9 +219,9 @@ struct Layout {                             // dynamic shared memory behind the 
 };
 
 template <bool DOWN>
-__host__ __device__ inline Layout layout_of(int nt, int experts, int picks) {
+__host__ __device__ inline Layout layout_of(int nt, int rows, int experts, int picks) {
   Layout l;
-  l.stage = kABytes + nt * 128 * (DOWN ? 2 : 1);
+  l.stage = (DOWN ? kABytes : 2 * rows * 128) + nt * 128 * (DOWN ? 2 : 1);
   const int control = 512 + (DOWN ? 0 : kExchange) + counts_bytes(experts) + ((picks * 2 + 15) & ~15);
   l.stages = (kSmem - 1024 - control) / l.stage;
   if (l.stages > kMaxStages) l.stages = kMaxStages;
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int picks = a.tokens * a.topk;
-  const Layout lay = layout_of<DOWN>(cut.nt, a.experts, picks);
+  const Layout lay = layout_of<DOWN>(cut.nt, cut.rows, a.experts, picks);
   const int NS = lay.stages;
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + lay.bars);      // [stages] TMA -> MMA
   uint64_t* empty = full + kMaxStages;                              // [stages] MMA -> TMA
@@ -310,11 +312,11 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   DeviceError* derr = a.device_error;
-  const int cols = max(32, cut.nt);                                 // TMEM columns of an accumulator
+  const int cols = DOWN ? 2 * cut.nt : max(32, cut.nt);             // TMEM columns of an accumulator
 
   if (tid == 0) {
     for (int i = 0; i < NS; ++i) {
-      mbar_init(full + i, 1);
+      mbar_init(full + i, 2);                     // weights and tokens
       mbar_init(empty + i, 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -405,8 +407,8 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   tiles.experts = a.experts;
   tiles.nt = cut.nt;
   tiles.tokens = a.tokens;
-  tiles.mt = ceil_div(DOWN ? a.hidden : a.ffn, DOWN ? kTile : kTile / 2);
-  tiles.smt = a.shared_ffn ? ceil_div(DOWN ? a.hidden : a.shared_ffn, DOWN ? kTile : kTile / 2) : 1;
+  tiles.mt = ceil_div(DOWN ? a.hidden : a.ffn, DOWN ? kTile : cut.rows);
+  tiles.smt = a.shared_ffn ? ceil_div(DOWN ? a.hidden : a.shared_ffn, DOWN ? kTile : cut.rows) : 1;
   tiles.k = ceil_div(DOWN ? a.ffn : a.hidden, kStep);
   tiles.sk = ceil_div(DOWN ? a.shared_ffn : a.hidden, kStep);
   tiles.kpart = DOWN ? cut.ksteps : tiles.k;
@@ -415,175 +417,215 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   tiles.shared = a.shared_ffn ? ceil_div(a.tokens, cut.nt) * tiles.smt * tiles.sparts : 0;
   tiles.total = tiles.shared + units[a.experts] * tiles.mt * tiles.parts;
 
+  const int a_bytes = DOWN ? kABytes : 2 * cut.rows * 128;
   if (warp == 4) {
-    // =================== TMA: weights by lane 0, four token rows per lane ===================
+    // =================== weights ===================
     if (lane == 0) {
       prefetch_tmap(&maps.w);
-      prefetch_tmap(&maps.b);
-    }
-    int s = 0;                                    // steps so far
-    bool ok = true;
-    // down: the weights of the first stages go ahead of the wait for act
-    int ahead = 0;
-    if (DOWN) {
-      for (int i = blockIdx.x; i < tiles.total && ahead < NS; i += gridDim.x) {
+      int st = 0, round = 0, s = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x) {
         const Item it = tiles.at(i);
-        const uint32_t bytes = kABytes + (uint32_t)((it.n + 15) & ~15) * 256;
-        for (int k = it.k0; k < it.k1 && ahead < NS; ++k, ++ahead)
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full + ahead, bytes);
-            tma_load_4d(sm + ahead * lay.stage, it.shared ? &maps.sw : &maps.w, full + ahead, k * kStep, it.mt * kTile, it.expert, 0);
+        const CUtensorMap* m = it.shared ? &maps.sw : &maps.w;
+        const int row = it.mt * (DOWN ? kTile : cut.rows);
+        for (int k = it.k0; k < it.k1; ++k, ++s) {
+          if (round && !mbar_wait(empty + st, (round - 1) & 1, abort_flag, derr, 90)) {
+            ok = false;
+            break;
           }
+          mbar_arrive_expect_tx(full + st, a_bytes);
+          // gate_up: gate rows, then their up rows
+          tma_load_4d(sm + st * lay.stage, m, full + st, k * kStep, row, DOWN ? it.expert : 0, DOWN ? 0 : it.expert);
+          if (++st == NS) st = 0, ++round;
+        }
       }
-      wait_previous();
+      // never leave with copies in flight
+      for (int n = min(s, NS); n > 0; --n) {
+        if (--st < 0) st = NS - 1, --round;
+        volatile int no_abort = 0;
+        mbar_wait(full + st, round & 1, &no_abort, nullptr, 91);
+      }
+    }
+  } else if (warp == 6) {
+    // =================== tokens ===================
+    int st = 0, round = 0, s = 0;
+    bool ok = true;
+    if (DOWN) {
+      wait_previous();                            // for act
       asm volatile("fence.proxy.async;" ::: "memory");
       __syncwarp();
     }
+    const bool gather = !DOWN && a.tokens > 16;
+    if (lane == 0) prefetch_tmap(gather ? &maps.b : &maps.sb);
     for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x) {
       const Item it = tiles.at(i);
-      const int groups = (it.n + 15) / 16 * 4;    // of four rows
-      const int g = DOWN ? lane & 15 : lane;
-      const CUtensorMap* bm = DOWN && lane >= 16 ? (it.shared ? &maps.slo : &maps.lo) : it.shared ? &maps.sb : &maps.b;
+      const int n16 = (it.n + 15) & ~15;
       int r[4] = {0, 0, 0, 0};
-      if (g < groups && (DOWN || lane < 16))
+      if (gather && lane < n16 / 4)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int at = it.first + min(g * 4 + j, it.n - 1);     // columns behind the last: its copies
-          r[j] = it.shared ? at : DOWN ? list[at] : list[at] / a.topk;
+          const int at = it.first + min(lane * 4 + j, it.n - 1);    // columns behind the last: its copies
+          r[j] = it.shared ? at : list[at] / a.topk;
         }
-      const uint32_t half = (uint32_t)groups * 512;               // bytes of the tokens' rows
+      const CUtensorMap* m = DOWN ? (it.shared ? &maps.sb : &maps.b) : &maps.sb;
       for (int k = it.k0; k < it.k1; ++k, ++s) {
-        const int st = s % NS;
-        if (s >= NS && !mbar_wait_warp(empty + st, ((s / NS) - 1) & 1, abort_flag, derr, 90)) {
+        if (round && !mbar_wait_warp(empty + st, (round - 1) & 1, abort_flag, derr, 92)) {
           ok = false;
           break;
         }
-        uint8_t* dst = sm + st * lay.stage;
-        if (s >= ahead) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full + st, kABytes + half * (DOWN ? 2 : 1));
-            if (DOWN) {
-              tma_load_4d(dst, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, it.mt * kTile, it.expert, 0);
-            } else {
-              // 64 gate rows, then their up rows
-              const int f = it.mt * (kTile / 2), n = it.shared ? a.shared_ffn : a.ffn;
-              tma_load_4d(dst, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, f, it.expert, 0);
-              tma_load_4d(dst + kABytes / 2, it.shared ? &maps.sw : &maps.w, full + st, k * kStep, n + f, it.expert, 0);
-            }
-          }
-          __syncwarp();
+        uint8_t* dst = sm + st * lay.stage + a_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(full + st, (DOWN ? n16 * 2 : n16) * 128);
+        __syncwarp();
+        if (DOWN) {
+          // 16 rows of the first parts, then of the second
+          if (lane < n16 / 16) tma_load_4d(dst + lane * 4096, m, full + st, k * kStep, it.first + lane * 16, 0, 0);
+        } else if (gather) {
+          if (lane < n16 / 4) tma_gather4(dst + lane * 512, &maps.b, full + st, k * kStep, r[0], r[1], r[2], r[3]);
+        } else if (lane == 0) {
+          tma_load_4d(dst, m, full + st, k * kStep, 0, 0, 0);        // all tokens
         }
-        if (g < groups && (DOWN || lane < 16))
-          tma_gather4(dst + kABytes + (lane >= 16 ? half : 0) + g * 512, bm, full + st, k * kStep, r[0], r[1], r[2], r[3]);
+        if (++st == NS) st = 0, ++round;
       }
     }
-    // never leave with copies in flight
-    if (!ok && s < ahead) s = ahead;
-    for (int k = max(0, s - NS); k < s; ++k) {
+    for (int n = min(s, NS); n > 0; --n) {
+      if (--st < 0) st = NS - 1, --round;
       volatile int no_abort = 0;
-      mbar_wait_warp(full + (k % NS), (k / NS) & 1, &no_abort, nullptr, 91);
+      mbar_wait_warp(full + st, round & 1, &no_abort, nullptr, 91);
     }
   } else if (warp == 5) {
     // =================== MMA ===================
     if (lane == 0) {
-      int s = 0, n_item = 0;
+      int st = 0, round = 0, n_item = 0;
       bool ok = true;
       for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x, ++n_item) {
         const Item it = tiles.at(i);
         const uint32_t n16 = (uint32_t)((it.n + 15) & ~15);
-        const uint32_t idesc = make_idesc(DType<T>::fmt, 0, 0, kTile, n16);
+        const uint32_t idesc = make_idesc(DType<T>::fmt, 0, 0, kTile, DOWN ? 2 * n16 : n16);
         const int b = n_item & 1;
-        if (n_item >= 2 && !mbar_wait(acc_empty + b, ((n_item >> 1) - 1) & 1, abort_flag, derr, 92)) break;
+        if (n_item >= 2 && !mbar_wait(acc_empty + b, ((n_item >> 1) - 1) & 1, abort_flag, derr, 93)) break;
         tc_fence_after();
-        for (int k = it.k0; k < it.k1; ++k, ++s) {
-          const int st = s % NS;
-          if (!mbar_wait(full + st, (s / NS) & 1, abort_flag, derr, 93)) {
+        for (int k = it.k0; k < it.k1; ++k) {
+          if (!mbar_wait(full + st, round & 1, abort_flag, derr, 94)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sA = smem_u32(sm + st * lay.stage), sB = sA + kABytes;
+          // (gate_up with narrow tiles: rows 64 and up are whatever lies behind, and nobody reads them)
+          const uint32_t sA = smem_u32(sm + st * lay.stage), sB = sA + a_bytes;
+          const uint64_t ad = sw128_desc(sA, 16, 1024), bd = sw128_desc(sB, 16, 1024);
 #pragma unroll
-          for (int kk = 0; kk < kStep / 16; ++kk) {
-            const uint64_t ad = sw128_desc(sA + kk * 32, 16, 1024);
-            umma_ss(tmem + b * cols, ad, sw128_desc(sB + kk * 32, 16, 1024), idesc, k > it.k0 || kk > 0);
-            if (DOWN) umma_ss(tmem + b * cols, ad, sw128_desc(sB + n16 * 128 + kk * 32, 16, 1024), idesc, 1);
-          }
+          for (int kk = 0; kk < kStep / 16; ++kk) umma_ss(tmem + b * cols, ad + kk * 2, bd + kk * 2, idesc, k > it.k0 || kk > 0);
           umma_commit(empty + st);
+          if (++st == NS) st = 0, ++round;
         }
         umma_commit(acc_full + b);
       }
       // what was issued is done before TMEM goes back
       for (int k = max(0, n_item - 2); k < n_item; ++k) {
         volatile int no_abort = 0;
-        mbar_wait(acc_full + (k & 1), (k >> 1) & 1, &no_abort, nullptr, 94);
+        mbar_wait(acc_full + (k & 1), (k >> 1) & 1, &no_abort, nullptr, 95);
       }
     }
   } else {
     // =================== epilogue: thread = weight row = TMEM lane ===================
     if (DOWN) wait_previous();
-    float* xs = reinterpret_cast<float*>(sm + lay.exchange);        // [2][16][64]
-    T* hi = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.hi);
-    T* lo = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.lo);
-    T* shi = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.shi);
-    T* slo = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.slo);
+    float* xs = reinterpret_cast<float*>(sm + lay.exchange);        // [2][16][rows]
+    T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.act);
+    T* sact = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.sact);
     float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + buf.part);
     int n_item = 0;
     for (int i = blockIdx.x; i < tiles.total; i += gridDim.x, ++n_item) {
       const Item it = tiles.at(i);
       const int b = n_item & 1;
-      bool ok = mbar_wait_warp(acc_full + b, (n_item >> 1) & 1, abort_flag, derr, 95);
+      bool ok = mbar_wait_warp(acc_full + b, (n_item >> 1) & 1, abort_flag, derr, 96);
       if (!DOWN) ok = all_warps(ok);              // none goes on to an exchange that another has left
       if (!ok) break;
       tc_fence_after();
       const uint32_t tm = tmem + b * cols + ((uint32_t)(warp * 32) << 16);
-      for (int c0 = 0; c0 < it.n; c0 += 32) {
-        float v[32];
-        tmem_ld32f(tm + c0, v);
-        tmem_ld_wait();
-        if (c0 + 32 >= it.n) {
-          tc_fence_before();
-          mbar_arrive(acc_empty + b);
-        }
-        if (DOWN) {
+      if (DOWN) {
+        // 16 tokens at a time: columns of the first parts, then of the second
+        for (int c0 = 0; c0 < it.n; c0 += 16) {
+          float v[32];
+          tmem_ld32f(tm + 2 * c0, v);
+          tmem_ld_wait();
+          if (c0 + 16 >= it.n) {
+            tc_fence_before();
+            mbar_arrive(acc_empty + b);
+          }
           const int h = it.mt * kTile + warp * 32 + lane;
           if (h < a.hidden)
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
+            for (int c = 0; c < 16; ++c)
               if (c0 + c < it.n) {
                 const int at = it.first + c0 + c;
                 const int64_t row = it.shared ? (int64_t)picks * cut.splits + (int64_t)at * cut.shared_splits + it.part
                                               : (int64_t)list[at] * cut.splits + it.part;
-                __stcg(part + row * a.hidden + h, v[c]);
+                __stcg(part + row * a.hidden + h, v[c] + v[16 + c]);
               }
-        } else {
-          // warps 0, 1 hold g and take columns 0..15, warps 2, 3 hold u and take the others
-          const int f = (warp & 1) * 32 + lane, upper = warp >> 1;
-          if (c0) asm volatile("bar.sync 1, 128;" ::: "memory");    // the last exchange has been read
+        }
+      } else {
+        // 32 columns at a time: the warps with g take the first 16, those with u the others
+        const bool wide = cut.rows == 64, upper = wide ? warp >= 2 : warp == 1;
+        const int f = wide ? (warp & 1) * 32 + lane : lane, mine = upper ? 16 : 0;
+        const bool live = wide || warp < 2;
+        const int width = it.shared ? a.shared_ffn : a.ffn, col = it.mt * cut.rows + f;
+        const int64_t rows = it.shared ? a.tokens : picks;
+        T* out = it.shared ? sact : act;
+        const auto put = [&](int64_t at, int c, float g, float u) {
+          const float x = silu(g) * u;
+          const T h = (T)x;
+          out[at * width + c] = h;
+          // (beyond the type's range: infinite, and no infinity less infinity)
+          out[(rows + at) * width + c] = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
+        };
+        if (!it.shared && a.tokens <= 16) {
+          // columns are tokens: all of them are exchanged, and the picks share out the threads
+          float v[32];
+          tmem_ld32f(tm, v);
+          tmem_ld_wait();
+          tc_fence_before();
+          mbar_arrive(acc_empty + b);
+          if (live)
 #pragma unroll
-          for (int c = 0; c < 16; ++c) xs[(upper * 16 + c) * 64 + f] = upper ? v[c] : v[16 + c];
+            for (int c = 0; c < 16; ++c) xs[(mine + c) * 64 + f] = v[c];
           asm volatile("bar.sync 1, 128;" ::: "memory");
-          const int width = it.shared ? a.shared_ffn : a.ffn, col = it.mt * (kTile / 2) + f;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const int n = c0 + upper * 16 + c;
-            if (n < it.n && col < width) {
-              const float other = xs[((1 - upper) * 16 + c) * 64 + f];
-              const float g = upper ? other : v[c], u = upper ? v[16 + c] : other;
-              const float x = silu(g) * u;
-              const T h = (T)x;
-              // (beyond the type's range: infinite, and no infinity less infinity)
-              const T l = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
-              const int64_t at = (int64_t)(it.shared ? it.first + n : list[it.first + n]) * width + col;
-              (it.shared ? shi : hi)[at] = h;
-              (it.shared ? slo : lo)[at] = l;
-            }
+          const int per = wide ? 64 : 32, fc = tid & (per - 1), c = it.mt * cut.rows + fc;
+          for (int q = tid / per; q < it.n; q += 128 / per) {
+            const int at = it.first + q, n = list[at] / a.topk;
+            if (c < width) put(at, c, xs[n * 64 + fc], xs[(16 + n) * 64 + fc]);
           }
+          continue;
+        }
+        for (int c0 = 0; c0 < it.n; c0 += 32) {
+          float v[32];
+          tmem_ld32f(tm + c0, v);
+          tmem_ld_wait();
+          if (c0 + 32 >= it.n) {
+            tc_fence_before();
+            mbar_arrive(acc_empty + b);
+          }
+          // of up to 16 columns the halves have eight each
+          const bool few = it.n - c0 <= 16;
+          const int take = few ? 8 : 16;
+          if (c0) asm volatile("bar.sync 1, 128;" ::: "memory");    // the last exchange has been read
+          if (live)
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+              if (c < take) xs[(mine + c) * 64 + f] = few ? (upper ? v[c & 7] : v[8 + (c & 7)]) : (upper ? v[c] : v[16 + c]);
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (live && col < width)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              const int n = c0 + (upper ? take : 0) + c;            // the accumulator's column
+              if (c >= take || n >= it.n) continue;
+              const float other = xs[((upper ? 0 : 16) + c) * 64 + f];
+              const float own = few ? (upper ? v[8 + (c & 7)] : v[c & 7]) : (upper ? v[16 + c] : v[c]);
+              put(it.first + n, col, upper ? other : own, upper ? own : other);
+            }
         }
       }
     }
   }
-  if (DOWN && warp == 5) wait_previous();         // every CTA of this grid has seen the last one's end
   __syncwarp();
   tc_fence_before();
   __syncthreads();
@@ -640,16 +682,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
   return fn;
 }
 
-// [outer, rows, cols] of 16-bit numbers, boxes of box_rows rows and 64 columns, 128-byte swizzle;
-// box_rows 1: a plain [rows, cols] whose rows are gathered
-int encode(CUtensorMap* m, const void* p, bool bf16, int64_t cols, int64_t rows, int64_t stride, int64_t outer, int box_rows) {
+// [outer, planes, rows, cols] of 16-bit numbers, packed behind rows of `stride`; boxes of 64 columns (128-byte
+// swizzle), box_rows rows and box_planes planes.  box_rows 1: a plain [rows, cols] whose rows are gathered
+int encode(CUtensorMap* m, const void* p, bool bf16, int64_t cols, int64_t rows, int64_t stride, int64_t planes, int64_t outer,
+           int box_rows, int box_planes) {
   const auto fn = encoder();
   if (!fn) return set_error(DASH_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
-  const bool gather = box_rows == 1;
-  const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)outer, 1};
-  const cuuint64_t strides[3] = {(cuuint64_t)stride * 2, (cuuint64_t)(stride * rows) * 2, (cuuint64_t)(stride * rows * outer) * 2};
-  const cuuint32_t box[4] = {kStep, (cuuint32_t)box_rows, 1, 1}, one[4] = {1, 1, 1, 1};
-  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, gather ? 2 : 4,
+  const cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes, (cuuint64_t)outer};
+  const cuuint64_t strides[3] = {(cuuint64_t)stride * 2, (cuuint64_t)(stride * rows) * 2, (cuuint64_t)(stride * rows * planes) * 2};
+  const cuuint32_t box[4] = {kStep, (cuuint32_t)box_rows, (cuuint32_t)box_planes, 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, box_rows == 1 ? 2 : 4,
                         const_cast<void*>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? DASH_OK : set_error(DASH_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
@@ -694,27 +736,27 @@ int launch_moe_t(const DashMoeArgs& a, cudaStream_t st) {
   if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "moe_ffn_kernel: %s", cudaGetErrorString(set));
   Maps up, down;
   const int64_t xs = a.tokens > 1 ? a.x_stride : a.hidden;
-  int rc = encode(&up.w, a.gate_up, kBf16, a.hidden, 2 * a.ffn, a.hidden, a.experts, kTile / 2);
-  if (!rc) rc = encode(&up.b, a.x, kBf16, a.hidden, a.tokens, xs, 1, 1);
-  up.sb = up.lo = up.slo = up.b;
+  // an expert's gate rows and up rows are two planes of one box
+  int rc = encode(&up.w, a.gate_up, kBf16, a.hidden, a.ffn, a.hidden, 2, a.experts, cut.rows, 2);
+  if (!rc) rc = encode(&up.b, a.x, kBf16, a.hidden, a.tokens, xs, 1, 1, 1, 1);
+  if (!rc) rc = encode(&up.sb, a.x, kBf16, a.hidden, a.tokens, xs, 1, 1, 16, 1);
   up.sw = up.w;
-  if (!rc) rc = encode(&down.w, a.down, kBf16, a.ffn, a.hidden, a.ffn, a.experts, kTile);
-  if (!rc) rc = encode(&down.b, ws + buf.hi, kBf16, a.ffn, picks, a.ffn, 1, 1);
-  if (!rc) rc = encode(&down.lo, ws + buf.lo, kBf16, a.ffn, picks, a.ffn, 1, 1);
-  down.sw = down.w, down.sb = down.b, down.slo = down.lo;
+  if (!rc) rc = encode(&down.w, a.down, kBf16, a.ffn, a.hidden, a.ffn, a.experts, 1, kTile, 1);
+  if (!rc) rc = encode(&down.b, ws + buf.act, kBf16, a.ffn, picks, a.ffn, 2, 1, 16, 2);
+  down.sw = down.w, down.sb = down.b;
   if (a.shared_ffn) {
-    if (!rc) rc = encode(&up.sw, a.shared_gate_up, kBf16, a.hidden, 2 * a.shared_ffn, a.hidden, 1, kTile / 2);
-    if (!rc) rc = encode(&down.sw, a.shared_down, kBf16, a.shared_ffn, a.hidden, a.shared_ffn, 1, kTile);
-    if (!rc) rc = encode(&down.sb, ws + buf.shi, kBf16, a.shared_ffn, a.tokens, a.shared_ffn, 1, 1);
-    if (!rc) rc = encode(&down.slo, ws + buf.slo, kBf16, a.shared_ffn, a.tokens, a.shared_ffn, 1, 1);
+    if (!rc) rc = encode(&up.sw, a.shared_gate_up, kBf16, a.hidden, a.shared_ffn, a.hidden, 2, 1, cut.rows, 2);
+    if (!rc) rc = encode(&down.sw, a.shared_down, kBf16, a.shared_ffn, a.hidden, a.shared_ffn, 1, 1, kTile, 1);
+    if (!rc) rc = encode(&down.sb, ws + buf.sact, kBf16, a.shared_ffn, a.tokens, a.shared_ffn, 2, 1, 16, 2);
   }
   if (rc) return rc;
   int cluster = 8;
   while (cluster > 1 && a.experts <= 4 * cluster) cluster >>= 1;
   rc = launch("moe_route_kernel", moe_route_kernel<T>, dim3((unsigned)(a.tokens * cluster)), kRouteThreads, 0, st, false, cluster, a);
-  const Layout lu = layout_of<false>(cut.nt, a.experts, (int)picks), ld = layout_of<true>(cut.nt, a.experts, (int)picks);
-  if (!rc) rc = launch("moe_up_kernel", moe_ffn_kernel<T, false>, dim3(148), kThreads, lu.bytes, st, true, 1, up, a, cut, buf);
-  if (!rc) rc = launch("moe_down_kernel", moe_ffn_kernel<T, true>, dim3(148), kThreads, ld.bytes, st, true, 1, down, a, cut, buf);
+  const Layout lu = layout_of<false>(cut.nt, cut.rows, a.experts, (int)picks),
+               ld = layout_of<true>(cut.nt, cut.rows, a.experts, (int)picks);
+  if (!rc) rc = launch("moe_up_kernel", moe_ffn_kernel<T, false>, dim3(kCtas), kThreads, lu.bytes, st, true, 1, up, a, cut, buf);
+  if (!rc) rc = launch("moe_down_kernel", moe_ffn_kernel<T, true>, dim3(kCtas), kThreads, ld.bytes, st, true, 1, down, a, cut, buf);
   const dim3 grid((unsigned)ceil_div(a.hidden, 512), (unsigned)a.tokens);
   if (!rc) rc = launch("moe_combine_kernel", moe_combine_kernel<T>, grid, 128, 0, st, true, 1, a, cut, buf);
   return rc;

@@ -34,7 +34,7 @@ constexpr int kStep = 64;                   // k elements of a stage (128 bytes)
 constexpr int kABytes = kTile * 128;
 constexpr int kMaxStages = 8;
 constexpr int kExchange = 2 * 16 * 64 * 4;  // gate_up: accumulators that change warps
-constexpr int kSmem = 113 * 1024;           // two CTAs per SM
+constexpr int kSmem = 75 * 1024;            // three CTAs per SM: two of a kernel, one of the next
 constexpr int kCtas = 2 * 148;
 
 // How a call is cut up: the same for equal sizes, whatever the tokens pick, so that a
@@ -54,7 +54,7 @@ __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; 
 
 Cut cut_of(const DashMoeArgs& a) {
   Cut c;
-  c.nt = a.tokens <= 16 ? 16 : a.tokens <= 128 ? 32 : 64;
+  c.nt = a.tokens <= 16 ? 16 : 32;
   // narrow tiles where the wide ones would leave CTAs without work
   const int chosen = min(a.experts, a.tokens * a.topk);
   c.rows = (int64_t)chosen * ceil_div(a.ffn, 64) + ceil_div(a.shared_ffn, 64) * ceil_div(a.tokens, c.nt) < kCtas ? 32 : 64;
@@ -95,31 +95,39 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 256;
 
-template <typename T>
-__device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at, bool f32, int n, int lane) {
+// lane's share of x . gate[at ..], 8 elements per 256; U such pieces in flight
+template <typename T, bool F32, int U>
+__device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at, int n, int lane) {
   double s = 0.0;
-  for (int i = lane * 8; i < n; i += 256) {
-    const uint4 xv = *reinterpret_cast<const uint4*>(x + i);
-    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
-    if (f32) {
-      const float* g = static_cast<const float*>(gate) + at + i;
-      const float4 a = *reinterpret_cast<const float4*>(g), b = *reinterpret_cast<const float4*>(g + 4);
-      const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  for (int i0 = lane * 8; i0 < n; i0 += 256 * U) {
+    uint4 xv[U], gv[U], hv[F32 ? U : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 256 * u;
+      xv[u] = gv[u] = hv[F32 ? u : 0] = make_uint4(0, 0, 0, 0);
+      if (i < n) {
+        xv[u] = *reinterpret_cast<const uint4*>(x + i);
+        const uint4* g = reinterpret_cast<const uint4*>(static_cast<const char*>(gate) + (at + i) * (F32 ? 4 : 2));
+        gv[u] = g[0];
+        if (F32) hv[F32 ? u : 0] = g[1];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t xw[4] = {xv[u].x, xv[u].y, xv[u].z, xv[u].w};
+      const uint32_t gw[8] = {gv[u].x, gv[u].y, gv[u].z, gv[u].w, hv[F32 ? u : 0].x, hv[F32 ? u : 0].y, hv[F32 ? u : 0].z, hv[F32 ? u : 0].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 f = unpack2(xw[j], (T*)nullptr);
-        s = fma((double)f.x, (double)w[2 * j], s);
-        s = fma((double)f.y, (double)w[2 * j + 1], s);
-      }
-    } else {
-      const uint4 gv = *reinterpret_cast<const uint4*>(static_cast<const T*>(gate) + at + i);
-      const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // products of two 16-bit numbers are exact in fp32
-        const float2 f = unpack2(xw[j], (T*)nullptr), w = unpack2(gw[j], (T*)nullptr);
-        s += (double)(f.x * w.x);
-        s += (double)(f.y * w.y);
+        if (F32) {
+          s = fma((double)f.x, (double)__uint_as_float(gw[2 * j]), s);
+          s = fma((double)f.y, (double)__uint_as_float(gw[2 * j + 1]), s);
+        } else {
+          // products of two 16-bit numbers are exact in fp32
+          const float2 w = unpack2(gw[j], (T*)nullptr);
+          s += (double)(f.x * w.x);
+          s += (double)(f.y * w.y);
+        }
       }
     }
   }
@@ -141,11 +149,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-template <typename T>
-__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const DashMoeArgs a) {
+template <typename T, bool F32>
+__global__ void __launch_bounds__(kRouteThreads, 4) moe_route_kernel(const DashMoeArgs a) {
   __shared__ double score[kMoeMaxExperts];
   __shared__ double red[kRouteThreads / 32], red2[kRouteThreads / 32];
-  __shared__ double best[kMoeMaxTopk];
+  __shared__ double value[kRouteThreads], best[kMoeMaxTopk];
   __shared__ int id[kMoeMaxTopk];
   launch_next();
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const DashMoeA
   bool waited = false;
   for (int e = rank * 8 + warp; e - warp < a.experts; e += 8 * C) {
     double s = 0.0;
-    if (e < a.experts) s = dot64(x, a.gate, (int64_t)e * a.hidden, a.gate_f32, a.hidden, lane);
+    if (e < a.experts) s = dot64<T, F32, F32 ? 2 : 5>(x, a.gate, (int64_t)e * a.hidden, a.hidden, lane);
     if (!waited) cluster_wait();                 // the first CTA has started
     waited = true;
     if (e < a.experts && lane == 0) {
@@ -183,14 +191,22 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const DashMoeA
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) red2[warp] = sum;
-  if (tid < a.experts) {
-    const double m = nan ? -INFINITY : mine;
+  // an expert's place: `share` threads count the experts before it
+  value[tid] = tid < a.experts ? e : 0.0;
+  __syncthreads();
+  int share = 1;
+  while (share < 32 && a.experts * share * 2 <= kRouteThreads) share *= 2;
+  for (int x0 = tid / share; x0 - tid / share < a.experts; x0 += kRouteThreads / share) {
     int before = 0;
-    for (int j = 0; j < a.experts; ++j) {
-      const double s = score[j] != score[j] ? -INFINITY : score[j];
-      before += s > m || (s == m && j < tid);
+    if (x0 < a.experts) {
+      const double m = score[x0] != score[x0] ? -INFINITY : score[x0];
+      for (int j = tid % share; j < a.experts; j += share) {
+        const double v = score[j] != score[j] ? -INFINITY : score[j];
+        before += v > m || (v == m && j < x0);
+      }
     }
-    if (before < a.topk) best[before] = e, id[before] = tid;
+    for (int o = 1; o < share; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (x0 < a.experts && tid % share == 0 && before < a.topk) best[before] = value[x0], id[before] = x0;
   }
   __syncthreads();
   if (tid < a.topk) {
@@ -210,26 +226,29 @@ struct Maps {
   CUtensorMap b, sb;                        // gate_up: x by rows, x by 16 rows; down: act, the shared act
 };
 
-__host__ __device__ constexpr int counts_bytes(int experts) {
-  return 2 * ((experts + 4) & ~3) * 4 + ((kThreads / 32 * experts + 3) & ~3) * 4;
-}
-
 struct Layout {                             // dynamic shared memory behind the ring
-  int stage, stages, bars, exchange, counts, list, bytes;
+  int stage, stages, bars, exchange, base, units, list, bytes;
 };
+
+// groups of up to nt picks of one expert
+__host__ __device__ constexpr int most_units(int nt, int experts, int picks) {
+  return picks < experts + picks / nt ? picks : experts + picks / nt;
+}
 
 template <bool DOWN>
 __host__ __device__ inline Layout layout_of(int nt, int rows, int experts, int picks) {
   Layout l;
+  const auto up16 = [](int n) { return (n + 15) & ~15; };
+  const int sizes[4] = {DOWN ? 0 : kExchange, up16((experts + 1) * 4), up16(most_units(nt, experts, picks) * 4), up16(picks * 2)};
   l.stage = (DOWN ? kABytes : 2 * rows * 128) + nt * 128 * (DOWN ? 2 : 1);
-  const int control = 512 + (DOWN ? 0 : kExchange) + counts_bytes(experts) + ((picks * 2 + 15) & ~15);
-  l.stages = (kSmem - 1024 - control) / l.stage;
+  l.stages = (kSmem - 1024 - 512 - sizes[0] - sizes[1] - sizes[2] - sizes[3]) / l.stage;
   if (l.stages > kMaxStages) l.stages = kMaxStages;
   l.bars = l.stages * l.stage;
   l.exchange = l.bars + 512;
-  l.counts = l.exchange + (DOWN ? 0 : kExchange);
-  l.list = l.counts + counts_bytes(experts);
-  l.bytes = l.list + ((picks * 2 + 15) & ~15) + 1024;
+  l.base = l.exchange + sizes[0];
+  l.units = l.base + sizes[1];
+  l.list = l.units + sizes[2];
+  l.bytes = l.list + sizes[3] + 1024;
   return l;
 }
 
@@ -242,8 +261,9 @@ struct Item {
 
 template <bool DOWN>
 struct Tiles {
-  const int *base, *units;                  // per expert: its picks' start in the list, its tiles' start
-  int experts, nt, tokens, mt, smt, k, sk, kpart, parts, sparts, shared, total;
+  const int* base;                          // per expert: its picks' start in the list
+  const uint32_t* units;                    // groups: expert << 16 | first pick
+  int nt, tokens, mt, smt, k, sk, kpart, parts, sparts, shared, total;
 
   __device__ __forceinline__ Item at(int i) const {
     Item it;
@@ -259,15 +279,10 @@ struct Tiles {
       it.first = i * nt;
       it.n = min(nt, tokens - it.first);
     } else {
-      int lo = 0, hi = experts;             // units[lo] <= i < units[hi]
-      while (hi - lo > 1) {
-        const int m = (lo + hi) >> 1;
-        if (units[m] <= i) lo = m;
-        else hi = m;
-      }
-      it.expert = lo;
-      it.first = base[lo] + (i - units[lo]) * nt;
-      it.n = min(nt, base[lo + 1] - it.first);
+      const uint32_t u = units[i];
+      it.expert = (int)(u >> 16);
+      it.first = (int)(u & 0xffffu);
+      it.n = min(nt, base[it.expert + 1] - it.first);
     }
     it.k0 = it.part * kpart;
     it.k1 = min(it.shared ? sk : k, it.k0 + kpart);
@@ -291,8 +306,9 @@ __device__ __forceinline__ bool all_warps(bool ok) {
   return r != 0;
 }
 
+// (bounds of 256 threads: 80 registers, with which three CTAs fit each quarter of an SM)
 template <typename T, bool DOWN>
-__global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant__ Maps maps, const DashMoeArgs a, const Cut cut,
+__global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__ Maps maps, const DashMoeArgs a, const Cut cut,
                                                            const Buffers buf) {
   extern __shared__ __align__(1024) uint8_t raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -305,9 +321,9 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   uint64_t* acc_empty = acc_full + 2;                               // [2] epilogue -> MMA
   uint32_t* holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
-  int* base = reinterpret_cast<int*>(sm + lay.counts);              // [experts + 1]
-  int* units = base + ((a.experts + 4) & ~3);                       // [experts + 1]
-  int* cursor = units + ((a.experts + 4) & ~3);                     // [warps][experts]
+  int* n_groups = reinterpret_cast<int*>(holder + 2);
+  int* base = reinterpret_cast<int*>(sm + lay.base);                // [experts + 1]
+  uint32_t* units = reinterpret_cast<uint32_t*>(sm + lay.units);    // groups of picks
   uint16_t* list = reinterpret_cast<uint16_t*>(sm + lay.list);      // picks, by expert
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -330,7 +346,17 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
     tmem_alloc(holder, 2 * cols);
     tmem_relinquish();
   }
-  for (int e = tid; e < a.experts * (kThreads / 32); e += kThreads) cursor[e] = 0;
+  // (in the ring, which is not in use yet)
+  uint32_t* tokens = reinterpret_cast<uint32_t*>(sm);               // [experts][words]: who picked it
+  const int words = ceil_div(a.tokens, 32);
+  uint16_t* expert_of = reinterpret_cast<uint16_t*>(tokens + a.experts * words);
+  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
+  if (tid == 32) {
+    prefetch_tmap(&maps.w);
+    prefetch_tmap(&maps.b);
+    prefetch_tmap(&maps.sb);
+    prefetch_tmap(&maps.sw);
+  }
   if (!DOWN && a.shared_ffn) {
     // the shared expert's weights into L2, while the router works
     const int64_t bytes = (int64_t)a.shared_ffn * a.hidden * 2, piece = 4096;
@@ -351,60 +377,52 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   const uint32_t tmem = *holder;
 
   // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
-  // the same tiles): each warp counts and then places a sixth of them ----
-  constexpr int W = kThreads / 32;
-  const int seg = ceil_div(ceil_div(picks, W), 32) * 32, p0 = warp * seg, p1 = min(picks, p0 + seg);
-  for (int p = p0 + lane; p < p1; p += 32) atomicAdd(cursor + warp * a.experts + __ldcg(a.ids + p), 1);
+  // the same groups): a bit per token and expert ----
+  for (int p = tid; p < picks; p += kThreads) {
+    const int e = __ldcg(a.ids + p), t = p / a.topk;
+    expert_of[p] = (uint16_t)e;
+    atomicOr(tokens + e * words + (t >> 5), 1u << (t & 31));
+  }
   __syncthreads();
   if (warp == 0) {
-    int run = 0, urun = 0;
+    int run = 0, groups = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
       const int e = e0 + lane;
       int n = 0;
       if (e < a.experts)
-        for (int w = 0; w < W; ++w) n += cursor[w * a.experts + e];
-      const int u0 = ceil_div(n, cut.nt);
-      int s = n, u = u0;
+        for (int w = 0; w < words; ++w) n += __popc(tokens[e * words + w]);
+      const int own = ceil_div(n, cut.nt);
+      int both = n << 16 | own;                   // sums of both at once: picks < 2^13, groups < 2^13
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, s, o), z = __shfl_up_sync(0xffffffffu, u, o);
-        if (lane >= o) s += y, u += z;
+        const int y = __shfl_up_sync(0xffffffffu, both, o);
+        if (lane >= o) both += y;
       }
+      const int at = run + (both >> 16) - n, g = groups + (both & 0xffff) - own;
       if (e < a.experts) {
-        int at = run + s - n;
         base[e] = at;
-        units[e] = urun + u - u0;
-        for (int w = 0; w < W; ++w) {
-          const int c = cursor[w * a.experts + e];
-          cursor[w * a.experts + e] = at;
-          at += c;
-        }
+        for (int i = 0; i < own; ++i) units[g + i] = (uint32_t)e << 16 | (uint32_t)(at + i * cut.nt);
       }
-      run += __shfl_sync(0xffffffffu, s, 31);
-      urun += __shfl_sync(0xffffffffu, u, 31);
+      both = __shfl_sync(0xffffffffu, both, 31);
+      run += both >> 16;
+      groups += both & 0xffff;
     }
-    if (lane == 0) base[a.experts] = run, units[a.experts] = urun;
+    if (lane == 0) base[a.experts] = run, *n_groups = groups;
   }
   __syncthreads();
-  for (int p = p0; p < p1; p += 32) {
-    const bool in = p + lane < p1;
-    const int e = in ? __ldcg(a.ids + p + lane) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, e);
-    int at = 0;
-    if (in) at = cursor[warp * a.experts + e] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (in) {
-      list[at] = (uint16_t)(p + lane);
-      if (lane == 31 - __clz(same)) cursor[warp * a.experts + e] = at + 1;
-    }
-    __syncwarp();
+  for (int p = tid; p < picks; p += kThreads) {
+    const int e = expert_of[p], t = p / a.topk;
+    int at = base[e] + __popc(tokens[e * words + (t >> 5)] & ((1u << (t & 31)) - 1));
+    for (int w = 0; w < t >> 5; ++w) at += __popc(tokens[e * words + w]);
+    list[at] = (uint16_t)p;
   }
+  // the ring's first writer is the TMA unit
+  fence_proxy_async_smem();
   __syncthreads();
 
   Tiles<DOWN> tiles;
   tiles.base = base;
   tiles.units = units;
-  tiles.experts = a.experts;
   tiles.nt = cut.nt;
   tiles.tokens = a.tokens;
   tiles.mt = ceil_div(DOWN ? a.hidden : a.ffn, DOWN ? kTile : cut.rows);
@@ -415,13 +433,12 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
   tiles.parts = DOWN ? cut.splits : 1;
   tiles.sparts = DOWN ? max(1, cut.shared_splits) : 1;
   tiles.shared = a.shared_ffn ? ceil_div(a.tokens, cut.nt) * tiles.smt * tiles.sparts : 0;
-  tiles.total = tiles.shared + units[a.experts] * tiles.mt * tiles.parts;
+  tiles.total = tiles.shared + *n_groups * tiles.mt * tiles.parts;
 
   const int a_bytes = DOWN ? kABytes : 2 * cut.rows * 128;
   if (warp == 4) {
     // =================== weights ===================
     if (lane == 0) {
-      prefetch_tmap(&maps.w);
       int st = 0, round = 0, s = 0;
       bool ok = true;
       for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x) {
@@ -456,7 +473,6 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
       __syncwarp();
     }
     const bool gather = !DOWN && a.tokens > 16;
-    if (lane == 0) prefetch_tmap(gather ? &maps.b : &maps.sb);
     for (int i = blockIdx.x; i < tiles.total && ok; i += gridDim.x) {
       const Item it = tiles.at(i);
       const int n16 = (it.n + 15) & ~15;
@@ -634,35 +650,39 @@ __global__ void __launch_bounds__(kThreads) moe_ffn_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------------------
-// the sum: a thread per four columns of a token
+// the sum: a CTA per 128 columns of a token, its warps take the parts in turn (little code
+// and few loads one after the other: this kernel runs for a microsecond or two)
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(128) moe_combine_kernel(const DashMoeArgs a, const Cut cut, const Buffers buf) {
-  const int t = blockIdx.y, h = ((int)blockIdx.x * 128 + threadIdx.x) * 4;
+__global__ void __launch_bounds__(256) moe_combine_kernel(const DashMoeArgs a, const Cut cut, const Buffers buf) {
+  __shared__ float4 sum[8][32];
+  const int t = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = ((int)blockIdx.x * 32 + lane) * 4;
   const float* part = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.workspace) + buf.part);
+  const int routed = a.topk * cut.splits, total = routed + cut.shared_splits;
   wait_previous();
-  if (h >= a.hidden) return;
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (h < a.hidden)
+#pragma unroll 4
+    for (int i = warp; i < total; i += 8) {
+      const int64_t row = i < routed ? (int64_t)t * routed + i : (int64_t)a.tokens * routed + (int64_t)t * cut.shared_splits + i - routed;
+      const float4 p = __ldcg(reinterpret_cast<const float4*>(part + row * a.hidden + h));
+      const float w = i < routed ? __ldcg(a.weights + (int64_t)t * a.topk + i / cut.splits) : 1.0f;
+      s.x = fmaf(w, p.x, s.x), s.y = fmaf(w, p.y, s.y), s.z = fmaf(w, p.z, s.z), s.w = fmaf(w, p.w, s.w);
+    }
+  sum[warp][lane] = s;
+  __syncthreads();
+  if (warp || h >= a.hidden) return;
+  s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (a.residual) {
     const uint2 r = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.residual) + t * a.residual_stride + h);
     const float2 x = unpack2(r.x, (T*)nullptr), y = unpack2(r.y, (T*)nullptr);
     s = make_float4(x.x, x.y, y.x, y.y);
   }
-  const int64_t picks = (int64_t)a.tokens * a.topk;
-  const auto rows = [&](int64_t row, int n, float w) {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i = 0; i < n; ++i) {
-      const float4 p = __ldcg(reinterpret_cast<const float4*>(part + (row + i) * a.hidden + h));
-      v.x += p.x, v.y += p.y, v.z += p.z, v.w += p.w;
-    }
-    s.x = fmaf(w, v.x, s.x), s.y = fmaf(w, v.y, s.y), s.z = fmaf(w, v.z, s.z), s.w = fmaf(w, v.w, s.w);
-  };
-#pragma unroll 4
-  for (int j = 0; j < a.topk; ++j) {
-    const int64_t p = (int64_t)t * a.topk + j;
-    rows(p * cut.splits, cut.splits, __ldcg(a.weights + p));
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float4 p = sum[w][lane];
+    s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
   }
-  rows(picks * cut.splits + (int64_t)t * cut.shared_splits, cut.shared_splits, 1.0f);
   *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + t * a.out_stride + h) =
       make_uint2(pack2(s.x, s.y, (T*)nullptr), pack2(s.z, s.w, (T*)nullptr));
 }
@@ -730,8 +750,13 @@ int launch_moe_t(const DashMoeArgs& a, cudaStream_t st) {
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   const int64_t picks = (int64_t)a.tokens * a.topk;
   static const cudaError_t set = [] {
-    const cudaError_t e = cudaFuncSetAttribute(moe_ffn_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    return e != cudaSuccess ? e : cudaFuncSetAttribute(moe_ffn_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    cudaError_t e = cudaSuccess;
+    for (const auto k : {moe_ffn_kernel<T, false>, moe_ffn_kernel<T, true>}) {
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      // room for the next kernel's CTA beside this one's two
+      if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+    return e;
   }();
   if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "moe_ffn_kernel: %s", cudaGetErrorString(set));
   Maps up, down;
@@ -752,13 +777,13 @@ int launch_moe_t(const DashMoeArgs& a, cudaStream_t st) {
   if (rc) return rc;
   int cluster = 8;
   while (cluster > 1 && a.experts <= 4 * cluster) cluster >>= 1;
-  rc = launch("moe_route_kernel", moe_route_kernel<T>, dim3((unsigned)(a.tokens * cluster)), kRouteThreads, 0, st, false, cluster, a);
+  rc = launch("moe_route_kernel", a.gate_f32 ? moe_route_kernel<T, true> : moe_route_kernel<T, false>, dim3((unsigned)(a.tokens * cluster)), kRouteThreads, 0, st, false, cluster, a);
   const Layout lu = layout_of<false>(cut.nt, cut.rows, a.experts, (int)picks),
                ld = layout_of<true>(cut.nt, cut.rows, a.experts, (int)picks);
   if (!rc) rc = launch("moe_up_kernel", moe_ffn_kernel<T, false>, dim3(kCtas), kThreads, lu.bytes, st, true, 1, up, a, cut, buf);
   if (!rc) rc = launch("moe_down_kernel", moe_ffn_kernel<T, true>, dim3(kCtas), kThreads, ld.bytes, st, true, 1, down, a, cut, buf);
-  const dim3 grid((unsigned)ceil_div(a.hidden, 512), (unsigned)a.tokens);
-  if (!rc) rc = launch("moe_combine_kernel", moe_combine_kernel<T>, grid, 128, 0, st, true, 1, a, cut, buf);
+  const dim3 grid((unsigned)ceil_div(a.hidden, 128), (unsigned)a.tokens);
+  if (!rc) rc = launch("moe_combine_kernel", moe_combine_kernel<T>, grid, 256, 0, st, true, 1, a, cut, buf);
   return rc;
 }
 

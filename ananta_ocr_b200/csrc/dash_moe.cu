@@ -21,6 +21,9 @@
 // (with one number it would be 0.0020 instead of 0.0017 of the output, bf16).
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "dash_common.cuh"
 #include "dash_internal.h"
 
@@ -34,14 +37,16 @@ constexpr int kStep = 64;                   // k elements of a stage (128 bytes)
 constexpr int kABytes = kTile * 128;
 constexpr int kMaxStages = 8;
 constexpr int kExchange = 2 * 16 * 64 * 4;  // gate_up: accumulators that change warps
-constexpr int kSmem = 75 * 1024;            // three CTAs per SM: two of a kernel, one of the next
-constexpr int kCtas = 2 * 148;
+constexpr int kSmem = 75 * 1024;            // three CTAs per SM
+// Every place of every SM: with fewer CTAs than places some SMs get three and some none, as
+// they are dealt out while the kernel before is still there (131 of 148 SMs had work).
+constexpr int kCtas = 3 * 148;
 
 // How a call is cut up: the same for equal sizes, whatever the tokens pick, so that a
 // token's sums do not depend on the other tokens.
 struct Cut {
   int nt;                                   // tokens of a tile at most
-  int rows;                                 // gate_up: gate rows of a tile (and as many up rows), 64 or 32
+  int rows;                                 // gate_up: gate rows of a tile (and as many up rows), 32 .. 64
   int ksteps, kshared;                      // 64-element steps of a part of down's k
   int splits, shared_splits;                // such parts of ffn and of shared_ffn
 };
@@ -55,15 +60,29 @@ __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; 
 Cut cut_of(const DashMoeArgs& a) {
   Cut c;
   c.nt = a.tokens <= 16 ? 16 : 32;
-  // narrow tiles where the wide ones would leave CTAs without work
-  const int chosen = min(a.experts, a.tokens * a.topk);
-  c.rows = (int64_t)chosen * ceil_div(a.ffn, 64) + ceil_div(a.shared_ffn, 64) * ceil_div(a.tokens, c.nt) < kCtas ? 32 : 64;
-  // parts of down's k: an item for every CTA where few experts are picked, but no less
-  // than four steps each
-  const int picked = min(a.experts, a.tokens * a.topk), tiles = ceil_div(a.hidden, kTile);
-  const int steps = ceil_div(a.ffn, kStep), sh = ceil_div(a.shared_ffn, kStep);
-  int k = max(steps, 1);
-  while (k > 4 && (int64_t)(picked * ceil_div(steps, k) + ceil_div(sh, k)) * tiles < kCtas) k = ceil_div(k, 2);
+  // gate_up's tiles: as high as lets the CTAs finish together.  `groups`: of tokens of one
+  // expert, with a router that picks evenly, and some more.
+  const double active = a.experts * (1.0 - std::pow(1.0 - (double)a.topk / a.experts, a.tokens));
+  const double groups = 1.05 * std::max(active, (double)a.tokens * a.topk / c.nt);
+  const int chunks = ceil_div(a.tokens, c.nt);
+  double best = 0.0;
+  for (int rows = 64; rows >= 32; rows -= 8) {
+    const double tiles = groups * ceil_div(a.ffn, rows) + chunks * ceil_div(a.shared_ffn, rows);
+    const double time = std::ceil(tiles / kCtas) * rows;
+    if (rows == 64 || time < best) best = time, c.rows = rows;
+  }
+  // parts of down's k: as long as lets the CTAs finish together (a part costs two steps
+  // more than its own)
+  const int tiles = ceil_div(a.hidden, kTile), steps = ceil_div(a.ffn, kStep), sh = ceil_div(a.shared_ffn, kStep);
+  int k = std::max(steps, 1);
+  for (int n = 1; n <= steps; ++n) {
+    const int len = ceil_div(steps, n);
+    if (len < std::min(4, steps)) break;
+    const auto time = [&](int l) {
+      return std::ceil((groups * ceil_div(steps, l) + chunks * ceil_div(sh, l)) * tiles / kCtas) * (l + 2);
+    };
+    if (time(len) < time(k)) k = len;
+  }
   c.ksteps = k;
   c.splits = ceil_div(steps, k);
   c.kshared = k;
@@ -290,6 +309,15 @@ struct Tiles {
   }
 };
 
+// 32 lanes x 16 consecutive 32-bit columns
+__device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
+
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
 // whether `ok` holds in all of the four epilogue warps (a barrier of theirs)
@@ -350,7 +378,6 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   uint32_t* tokens = reinterpret_cast<uint32_t*>(sm);               // [experts][words]: who picked it
   const int words = ceil_div(a.tokens, 32);
   uint16_t* expert_of = reinterpret_cast<uint16_t*>(tokens + a.experts * words);
-  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
   if (tid == 32) {
     prefetch_tmap(&maps.w);
     prefetch_tmap(&maps.b);
@@ -360,7 +387,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   if (!DOWN && a.shared_ffn) {
     // the shared expert's weights into L2, while the router works
     const int64_t bytes = (int64_t)a.shared_ffn * a.hidden * 2, piece = 4096;
-    for (int64_t at = ((int64_t)blockIdx.x * kThreads + tid) * piece; at < 3 * bytes; at += (int64_t)gridDim.x * kThreads * piece) {
+    for (int64_t at = ((int64_t)tid * gridDim.x + blockIdx.x) * piece; at < 3 * bytes; at += (int64_t)gridDim.x * kThreads * piece) {
       const bool up = at < 2 * bytes;
       const char* p = up ? static_cast<const char*>(a.shared_gate_up) + at : static_cast<const char*>(a.shared_down) + (at - 2 * bytes);
       const int64_t n = min(piece, (up ? 2 * bytes : 3 * bytes) - at);
@@ -369,17 +396,25 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   }
   // gate_up waits for the router here.  down starts when every CTA of gate_up has done so:
   // the picks are there, act is not.
-  if (!DOWN) wait_previous();
-  launch_next();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *holder;
+  // (gate_up goes through the sorting once without the picks while it waits: code that runs
+  // for the first time waits for its own instructions)
+#pragma unroll 1
+  for (int dry = DOWN ? 0 : 1; dry >= 0; --dry) {
+  if (!dry) {
+    if (!DOWN) wait_previous();
+    launch_next();
+  }
+  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
+  __syncthreads();
 
   // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
   // the same groups): a bit per token and expert ----
   for (int p = tid; p < picks; p += kThreads) {
-    const int e = __ldcg(a.ids + p), t = p / a.topk;
+    const int e = dry ? 0 : __ldcg(a.ids + p), t = p / a.topk;
     expert_of[p] = (uint16_t)e;
     atomicOr(tokens + e * words + (t >> 5), 1u << (t & 31));
   }
@@ -416,7 +451,9 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
     for (int w = 0; w < t >> 5; ++w) at += __popc(tokens[e * words + w]);
     list[at] = (uint16_t)p;
   }
-  // the ring's first writer is the TMA unit
+  __syncthreads();
+  }
+  // the ring's next writer is the TMA unit
   fence_proxy_async_smem();
   __syncthreads();
 
@@ -580,64 +617,37 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
               }
         }
       } else {
-        // 32 columns at a time: the warps with g take the first 16, those with u the others
-        const bool wide = cut.rows == 64, upper = wide ? warp >= 2 : warp == 1;
-        const int f = wide ? (warp & 1) * 32 + lane : lane, mine = upper ? 16 : 0;
-        const bool live = wide || warp < 2;
-        const int width = it.shared ? a.shared_ffn : a.ffn, col = it.mt * cut.rows + f;
+        // 16 columns at a time are exchanged, so that a thread has g and u of a row
+        const int r = warp * 32 + lane, which = r >= cut.rows, f = r - which * cut.rows;
+        const int width = it.shared ? a.shared_ffn : a.ffn;
         const int64_t rows = it.shared ? a.tokens : picks;
         T* out = it.shared ? sact : act;
-        const auto put = [&](int64_t at, int c, float g, float u) {
-          const float x = silu(g) * u;
-          const T h = (T)x;
-          out[at * width + c] = h;
-          // (beyond the type's range: infinite, and no infinity less infinity)
-          out[(rows + at) * width + c] = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
-        };
-        if (!it.shared && a.tokens <= 16) {
-          // columns are tokens: all of them are exchanged, and the picks share out the threads
-          float v[32];
-          tmem_ld32f(tm, v);
+        const bool all = !it.shared && a.tokens <= 16;              // columns are the tokens, not the picks
+        const int step = kTile / cut.rows, q0 = tid / cut.rows, fc = tid - q0 * cut.rows, col = it.mt * cut.rows + fc;
+        for (int c0 = 0; c0 < it.n; c0 += 16) {
+          float v[16];
+          tmem_ld16f(tm + c0, v);
           tmem_ld_wait();
-          tc_fence_before();
-          mbar_arrive(acc_empty + b);
-          if (live)
-#pragma unroll
-            for (int c = 0; c < 16; ++c) xs[(mine + c) * 64 + f] = v[c];
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          const int per = wide ? 64 : 32, fc = tid & (per - 1), c = it.mt * cut.rows + fc;
-          for (int q = tid / per; q < it.n; q += 128 / per) {
-            const int at = it.first + q, n = list[at] / a.topk;
-            if (c < width) put(at, c, xs[n * 64 + fc], xs[(16 + n) * 64 + fc]);
-          }
-          continue;
-        }
-        for (int c0 = 0; c0 < it.n; c0 += 32) {
-          float v[32];
-          tmem_ld32f(tm + c0, v);
-          tmem_ld_wait();
-          if (c0 + 32 >= it.n) {
+          const bool end = all || c0 + 16 >= it.n;
+          if (end) {
             tc_fence_before();
             mbar_arrive(acc_empty + b);
           }
-          // of up to 16 columns the halves have eight each
-          const bool few = it.n - c0 <= 16;
-          const int take = few ? 8 : 16;
           if (c0) asm volatile("bar.sync 1, 128;" ::: "memory");    // the last exchange has been read
-          if (live)
+          if (f < cut.rows)
 #pragma unroll
-            for (int c = 0; c < 16; ++c)
-              if (c < take) xs[(mine + c) * 64 + f] = few ? (upper ? v[c & 7] : v[8 + (c & 7)]) : (upper ? v[c] : v[16 + c]);
+            for (int c = 0; c < 16; ++c) xs[(which * 16 + c) * 64 + f] = v[c];
           asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (live && col < width)
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const int n = c0 + (upper ? take : 0) + c;            // the accumulator's column
-              if (c >= take || n >= it.n) continue;
-              const float other = xs[((upper ? 0 : 16) + c) * 64 + f];
-              const float own = few ? (upper ? v[8 + (c & 7)] : v[c & 7]) : (upper ? v[16 + c] : v[c]);
-              put(it.first + n, col, upper ? other : own, upper ? own : other);
+          if (q0 < step && col < width)
+            for (int q = c0 + q0; q < it.n && (all || q < c0 + 16); q += step) {
+              const int at = it.first + q, n = all ? list[at] / a.topk : q - c0;
+              const float x = silu(xs[n * 64 + fc]) * xs[(16 + n) * 64 + fc];
+              const T h = (T)x;
+              out[(int64_t)at * width + col] = h;
+              // (beyond the type's range: infinite, and no infinity less infinity)
+              out[(rows + at) * width + col] = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
             }
+          if (end) break;
         }
       }
     }

@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(512) add_norm_kernel(const DashNormArgs a, int
 // A CTA takes whole rows, a thread the same columns of each, so the column sums stay in
 // registers; rows go to CTAs in chunks that lie within one gate's group.  Column sums of
 // a CTA (dweight, dpost) and of a chunk (dgate) are written to the workspace and added
-// in their order by norm_columns_kernel: no atomics.
+// in their order by norm_columns_kernel: no atomics.  This form is for rows that are not
+// aligned to 16 bytes, and for the longest fp32 rows.
 template <typename T, int E, int NV>
 __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs b, int64_t chunk, int64_t chunks_per_group, int64_t chunks,
                                     float* part_w, float* part_p, float* part_g) {
@@ -348,6 +349,310 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs
   }
 }
 
+// The same for aligned rows.  What bounded the form above at 36,992 rows of 1,280 (bf16, gate and
+// post: 234 us, memory takes 87) were instructions and the two exchanges per row, not
+// the loads, so here
+//  - two elements share an instruction (f32x2),
+//  - a row's exchange carries the sum of squares that the next row's r1 is made of,
+//  - sums are folded together before they are shuffled (9 shuffles for 6 sums, not 30),
+//  - the next rows are on their way into shared memory (cp.async; a thread fetches what it
+//    reads itself, so they need no barrier).
+template <int NV>
+constexpr int kAhead = NV == 1 ? 3 : 1;            // rows on their way: 128 KB of shared memory at most
+constexpr int kRingMost = 128 * 1024;
+
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t both(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ float add_up(uint64_t v) {
+  float x, y;
+  f2_unpack(v, x, y);
+  return x + y;
+}
+
+// 16 bytes as pairs of fp32, and back
+template <typename T>
+struct Pairs {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ uint64_t get(const uint4& v, int j) {
+    const uint32_t w = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
+    const float2 f = unpack2(w, (T*)nullptr);
+    return f2_pack(f.x, f.y);
+  }
+  static __device__ __forceinline__ void put(uint4& v, int j, uint64_t x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    const uint32_t w = pack2(a, b, (T*)nullptr);
+    (j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w) = w;
+  }
+};
+template <>
+struct Pairs<float> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ uint64_t get(const uint4& v, int j) {
+    return j ? f2_pack(__uint_as_float(v.z), __uint_as_float(v.w)) : f2_pack(__uint_as_float(v.x), __uint_as_float(v.y));
+  }
+  static __device__ __forceinline__ void put(uint4& v, int j, uint64_t x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    (j ? v.z : v.x) = __float_as_uint(a);
+    (j ? v.w : v.y) = __float_as_uint(b);
+  }
+};
+
+// Sums of N (2 or 8) values over a row's threads, the same in all of them.  At each step
+// the lanes send the half of the values that they will not keep.
+template <int N>
+__device__ __forceinline__ void fold(float (&v)[N], int warps, int warp, int lane, float* buf, int& half) {
+  float x = 0.0f;
+  int mine;
+  if constexpr (N == 2) {
+    const bool up = lane & 16;
+    x = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+    mine = 16;
+  } else {
+    float f[4], g[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = (lane & 16 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, lane & 16 ? v[i] : v[4 + i], 16);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      g[i] = (lane & 8 ? f[2 + i] : f[i]) + __shfl_xor_sync(0xffffffffu, lane & 8 ? f[i] : f[2 + i], 8);
+    x = (lane & 4 ? g[1] : g[0]) + __shfl_xor_sync(0xffffffffu, lane & 4 ? g[0] : g[1], 4);
+    mine = 4;
+  }
+  for (int o = mine / 2; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  float* b = buf + half * 16 * 8;
+  half ^= 1;
+  if ((lane & (mine - 1)) == 0) b[warp * 8 + lane / mine] = x;
+  if (warps > 1) __syncthreads();
+  else __syncwarp();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = 0.0f;
+  for (int w = 0; w < warps; ++w) {
+    if constexpr (N == 2) {
+      const float2 s = *reinterpret_cast<const float2*>(b + w * 8);
+      v[0] += s.x, v[1] += s.y;
+    } else {
+      const float4 s = *reinterpret_cast<const float4*>(b + w * 8), t = *reinterpret_cast<const float4*>(b + w * 8 + 4);
+      v[0] += s.x, v[1] += s.y, v[2] += s.z, v[3] += s.w;
+      v[4] += t.x, v[5] += t.y, v[6] += t.z, v[7] += t.w;
+    }
+  }
+}
+
+// FULL: with post, gate or both
+template <typename T, int NV, bool FULL>
+__global__ void __launch_bounds__(512) add_norm_bwd_wide_kernel(const DashNormBwdArgs b, int64_t chunk, int64_t chunks_per_group,
+                                                                int64_t chunks, float* part_w, float* part_p, float* part_g) {
+  constexpr int E = 16 / sizeof(T), P = Pairs<T>::N, AHEAD = kAhead<NV>, F = FULL ? NV : 1;
+  const DashNormArgs& a = b.fwd;
+  __shared__ __align__(16) float buf[2 * 16 * 8];
+  extern __shared__ uint4 ring[];                // [AHEAD + 1][4][NV][threads]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int t = threadIdx.x, step = (int)blockDim.x * E, plane = NV * (int)blockDim.x;
+  const bool post = FULL && a.post, gate = FULL && a.gate;
+  int half = 0;
+  const float inv = 1.0f / (float)a.hidden;
+  uint64_t dw[NV][P] = {}, dp[F][P] = {}, dg[F][P], w[NV][P], p[F][P], g[F][P];
+  const auto pairs_of = [&](const void* from, int64_t at, bool f32, uint64_t (&to)[P]) {
+    float x[E];
+    read_weight<T, E>(from, at, f32, x);
+#pragma unroll
+    for (int j = 0; j < P; ++j) to[j] = f2_pack(x[2 * j], x[2 * j + 1]);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      w[i][j] = 0;
+      if (FULL) p[FULL ? i : 0][j] = both(1.0f);
+    }
+    if (c < a.hidden) {
+      pairs_of(a.weight, c, a.weight_f32, w[i]);
+      if (post) pairs_of(a.post, c, a.post_f32, p[FULL ? i : 0]);
+    }
+  }
+  // the row to be fetched next, in this CTA's order
+  int64_t fk = blockIdx.x, frow = 0, fend = 0;
+  const auto open = [&](int64_t k, int64_t& row, int64_t& end) {
+    const int64_t group = k / chunks_per_group;
+    row = group * a.group_rows + (k - group * chunks_per_group) * chunk;
+    end = min((group + 1) * a.group_rows, row + chunk);
+  };
+  const auto fetch = [&](int slot) {
+    if (fk < chunks) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        const uint32_t to = smem_u32(ring + (slot * 4 * NV + i) * (int)blockDim.x + t);
+        const auto copy = [&](int n, const void* from, int64_t stride) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n * plane * 16),
+                       "l"(static_cast<const T*>(from) + frow * stride + c)
+                       : "memory");
+        };
+        if (c < a.hidden) {
+          copy(0, a.y, a.y_stride);
+          if (a.residual) copy(1, a.residual, a.residual_stride);
+          if (b.dstream) copy(2, b.dstream, b.dstream_stride);
+          copy(3, b.dnormed, b.dnormed_stride);
+        }
+      }
+      if (++frow == fend && (fk += gridDim.x) < chunks) open(fk, frow, fend);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  open(fk, frow, fend);
+  for (int n = 0; n < AHEAD; ++n) fetch(n);
+  // what lies behind the row's end, or has no tensor, counts as 0
+  const auto read = [&](int slot, int n, int i, bool on) {
+    return on && t * E + i * step < a.hidden ? ring[(slot * 4 + n) * plane + i * (int)blockDim.x + t] : make_uint4(0, 0, 0, 0);
+  };
+  const auto squares = [&](int slot) {           // of this thread's part of y
+    uint64_t q = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint4 v = read(slot, 0, i, true);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const uint64_t x = Pairs<T>::get(v, j);
+        q = ffma2(x, x, q);
+      }
+    }
+    return add_up(q);
+  };
+  int at = 0;                                    // the ring's row in use
+  float next = 0.0f;                             // sum of squares of the row that comes next
+  bool known = false;
+  for (int64_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+    int64_t row, end;
+    open(k, row, end);
+    if (FULL) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        constexpr int I = FULL ? 1 : 0;
+        const int c = t * E + i * step;
+#pragma unroll
+        for (int j = 0; j < P; ++j) g[I * i][j] = both(1.0f), dg[I * i][j] = 0;
+        if (gate && c < a.hidden) pairs_of(a.gate, k / chunks_per_group * a.gate_stride + c, a.gate_f32, g[I * i]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) g[I * i][j] = fmul2(g[I * i][j], both(a.scale));
+      }
+    }
+    for (; row < end; ++row) {
+      // this row is there, and with three rows on their way the next one too
+      asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD >= 3 ? AHEAD - 2 : AHEAD - 1) : "memory");
+      const int after = at == AHEAD ? 0 : at + 1;
+      if (post && !(AHEAD >= 3 && known)) {
+        float q[2] = {squares(at), 0.0f};
+        fold(q, warps, warp, lane, buf, half);
+        next = q[0];
+        known = true;
+      }
+      const float r1 = post ? rsqrtf(next * inv + a.eps) : 1.0f;
+      uint4 ry[NV], rs[NV], rh[NV];
+      uint64_t s[NV][P], sum[5] = {};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        constexpr int I = FULL ? 1 : 0;
+        ry[i] = read(at, 0, i, true);
+        rs[i] = read(at, 2, i, b.dstream);
+        rh[i] = read(at, 3, i, true);
+        const uint4 rr = read(at, 1, i, a.residual);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const uint64_t ga = fmul2(w[i][j], Pairs<T>::get(rh[i], j));
+          const uint64_t q = fmul2(FULL ? fmul2(g[I * i][j], p[I * i][j]) : both(a.scale), Pairs<T>::get(ry[i], j));
+          s[i][j] = ffma2(q, both(r1), Pairs<T>::get(rr, j));
+          sum[0] = ffma2(s[i][j], s[i][j], sum[0]);
+          sum[1] = ffma2(ga, s[i][j], sum[1]);
+          if (FULL) {
+            sum[2] = ffma2(q, Pairs<T>::get(rs[i], j), sum[2]);
+            sum[3] = ffma2(q, ga, sum[3]);
+            sum[4] = ffma2(q, s[i][j], sum[4]);
+          }
+        }
+      }
+      float v[8] = {add_up(sum[0]), add_up(sum[1])};
+      if (post) {
+        v[2] = add_up(sum[2]), v[3] = add_up(sum[3]), v[4] = add_up(sum[4]);
+        if (AHEAD >= 3) v[5] = squares(after);
+        fold(v, warps, warp, lane, buf, half);
+        next = v[5];
+      } else {
+        float two[2] = {v[0], v[1]};
+        fold(two, warps, warp, lane, buf, half);
+        v[0] = two[0], v[1] = two[1];
+      }
+      // (the slot that is filled now was read before the exchange)
+      fetch(at == 0 ? AHEAD : at - 1);
+      at = after;
+      const float r2 = rsqrtf(v[0] * inv + a.eps);
+      const float m = r2 * r2 * r2 * v[1] * inv;                // ds_total = ds + r2 * ga - m * s
+      const float mb = r1 * r1 * r1 * inv * (v[2] + r2 * v[3] - m * v[4]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        constexpr int I = FULL ? 1 : 0;
+        const int c = t * E + i * step;
+        uint4 od, oy;
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+          const uint64_t h = fmul2(Pairs<T>::get(rh[i], j), both(r2));
+          uint64_t d = ffma2(w[i][j], h, Pairs<T>::get(rs[i], j));
+          d = ffma2(both(-m), s[i][j], d);
+          dw[i][j] = ffma2(h, s[i][j], dw[i][j]);
+          Pairs<T>::put(od, j, d);
+          if (FULL) {
+            const uint64_t x = Pairs<T>::get(ry[i], j), yh = fmul2(x, both(r1)), dz = fmul2(d, g[I * i][j]);
+            dg[I * i][j] = ffma2(d, fmul2(yh, p[I * i][j]), dg[I * i][j]);
+            dp[I * i][j] = ffma2(dz, yh, dp[I * i][j]);
+            Pairs<T>::put(oy, j, post ? ffma2(fmul2(dz, p[I * i][j]), both(r1), fmul2(x, both(-mb))) : dz);
+          } else {
+            Pairs<T>::put(oy, j, fmul2(d, both(a.scale)));
+          }
+        }
+        if (c < a.hidden) {
+          if (b.dresidual) *reinterpret_cast<uint4*>(static_cast<T*>(b.dresidual) + row * b.dresidual_stride + c) = od;
+          if (b.dy) *reinterpret_cast<uint4*>(static_cast<T*>(b.dy) + row * b.dy_stride + c) = oy;
+        }
+      }
+    }
+    if (FULL && b.dgate) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        if (c < a.hidden)
+#pragma unroll
+          for (int j = 0; j < P; ++j) {
+            float x[2];
+            f2_unpack(fmul2(dg[FULL ? i : 0][j], both(a.scale)), x[0], x[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int64_t o = k * a.hidden + c + 2 * j + e;
+              if (part_g) part_g[o] = x[e];
+              else if (a.gate_f32) static_cast<float*>(b.dgate)[o] = x[e];     // the chunk is a whole group
+              else static_cast<T*>(b.dgate)[o] = (T)x[e];
+            }
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+    if (c < a.hidden)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        *reinterpret_cast<uint64_t*>(part_w + (int64_t)blockIdx.x * a.hidden + c + 2 * j) = dw[i][j];
+        if (FULL && part_p) *reinterpret_cast<uint64_t*>(part_p + (int64_t)blockIdx.x * a.hidden + c + 2 * j) = dp[FULL ? i : 0][j];
+      }
+  }
+}
+
 // out[g][c] = sum over j of part[g * n + j][c], in that order: 32 columns per CTA, the
 // parts dealt to its warps
 template <typename T>
@@ -416,6 +721,8 @@ int launch_fwd_e(const DashNormArgs& a, cudaStream_t st) {
   return check_launch("add_norm_kernel");
 }
 
+constexpr int kNormThreads = 512;                  // of a backward call on an SM: 128 registers each
+
 // How the rows of a backward call are dealt out
 struct NormCut {
   int threads, nv, ctas;
@@ -433,7 +740,7 @@ NormCut norm_cut(const DashNormArgs& a, int E) {
     while (warps > most && c.nv < (E == 1 ? (most == 8 ? 8 : 16) : most == 8 ? 8 / E : 16 / E))
       c.nv *= 2, warps = (vecs + 32 * c.nv - 1) / (32 * c.nv);
   c.threads = warps * 32;
-  const int most = 148 * max(1, min(8, 1024 / c.threads));
+  const int most = 148 * max(1, min(8, kNormThreads / c.threads));
   // chunks of at least 4 rows where there are enough rows for all CTAs
   const int64_t groups = a.rows / a.group_rows;
   const int64_t want = (a.rows + most - 1) / most;
@@ -451,18 +758,31 @@ int launch_bwd_e(const DashNormBwdArgs& b, cudaStream_t st) {
   float* part_w = static_cast<float*>(b.workspace);
   float* part_p = a.post ? part_w + (int64_t)c.ctas * a.hidden : nullptr;
   float* part_g = b.dgate && c.per_group > 1 ? part_w + (int64_t)c.ctas * a.hidden * (a.post ? 2 : 1) : nullptr;
-#define DASH_NORM_BWD(NV)                                                                                         \
-  add_norm_bwd_kernel<T, E, NV><<<c.ctas, c.threads, 0, st>>>(b, c.chunk, c.per_group, c.chunks, part_w, part_p, part_g)
-  if (c.nv == 1) DASH_NORM_BWD(1);
-  else if (c.nv == 2) DASH_NORM_BWD(2);
-  else if constexpr (E <= 4) {
-    if (c.nv == 4) DASH_NORM_BWD(4);
-    else if constexpr (E == 1) {
-      if (c.nv == 8) DASH_NORM_BWD(8);
-      else DASH_NORM_BWD(16);
-    }
+  const auto go = [&](auto kernel, size_t ring) {
+    if (ring > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
+      return set_error(DASH_ERR_CUDA, "add_norm_bwd_kernel: no shared memory for the ring");
+    kernel<<<c.ctas, c.threads, ring, st>>>(b, c.chunk, c.per_group, c.chunks, part_w, part_p, part_g);
+    return (int)DASH_OK;
+  };
+  const size_t row = (size_t)4 * c.nv * c.threads * 16;
+  const bool full = a.post || a.gate;
+  int rr = DASH_OK;
+  if constexpr (E == 1) {
+    rr = c.nv == 1   ? go(add_norm_bwd_kernel<T, E, 1>, 0)
+         : c.nv == 2 ? go(add_norm_bwd_kernel<T, E, 2>, 0)
+         : c.nv == 4 ? go(add_norm_bwd_kernel<T, E, 4>, 0)
+         : c.nv == 8 ? go(add_norm_bwd_kernel<T, E, 8>, 0)
+                     : go(add_norm_bwd_kernel<T, E, 16>, 0);
+  } else if (c.nv == 1) {
+    const size_t ring = row * (kAhead<1> + 1);
+    rr = full ? go(add_norm_bwd_wide_kernel<T, 1, true>, ring) : go(add_norm_bwd_wide_kernel<T, 1, false>, ring);
+  } else if (c.nv == 2) {
+    const size_t ring = row * (kAhead<2> + 1);
+    rr = full ? go(add_norm_bwd_wide_kernel<T, 2, true>, ring) : go(add_norm_bwd_wide_kernel<T, 2, false>, ring);
+  } else if constexpr (E == 4) {
+    rr = go(add_norm_bwd_kernel<T, E, 4>, 0);
   }
-#undef DASH_NORM_BWD
+  if (rr) return rr;
   count_launch();
   int rc = check_launch("add_norm_bwd_kernel");
   if (rc) return rc;

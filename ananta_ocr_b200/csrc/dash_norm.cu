@@ -653,6 +653,138 @@ __global__ void __launch_bounds__(512) add_norm_bwd_wide_kernel(const DashNormBw
   }
 }
 
+// The forward with post or gate in the same manner, for many aligned rows: a CTA takes rows one after the other,
+// its weights stay in registers.
+template <typename T, int NV>
+__global__ void __launch_bounds__(512) add_norm_wide_kernel(const DashNormArgs a, int64_t per) {
+  constexpr int E = 16 / sizeof(T), P = Pairs<T>::N, AHEAD = kAhead<NV>;
+  __shared__ __align__(16) float buf[2 * 16 * 8];
+  extern __shared__ uint4 ring[];                // [AHEAD + 1][2][NV][threads]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int t = threadIdx.x, step = (int)blockDim.x * E, plane = NV * (int)blockDim.x;
+  const bool post = a.post, gate = a.gate;
+  const int64_t first = blockIdx.x * per, end = min(a.rows, first + per);
+  int half = 0;
+  const float inv = 1.0f / (float)a.hidden;
+  uint64_t w[NV][P], p[NV][P], g[NV][P];
+  const auto pairs_of = [&](const void* from, int64_t at, bool f32, uint64_t (&to)[P]) {
+    float x[E];
+    read_weight<T, E>(from, at, f32, x);
+#pragma unroll
+    for (int j = 0; j < P; ++j) to[j] = f2_pack(x[2 * j], x[2 * j + 1]);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = t * E + i * step;
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      w[i][j] = 0;
+      p[i][j] = both(1.0f);
+    }
+    if (c < a.hidden) {
+      pairs_of(a.weight, c, a.weight_f32, w[i]);
+      if (post) pairs_of(a.post, c, a.post_f32, p[i]);
+    }
+  }
+  int64_t frow = first;
+  const auto fetch = [&](int slot) {
+    if (frow < end) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+        const uint32_t to = smem_u32(ring + (slot * 2 * NV + i) * (int)blockDim.x + t);
+        const auto copy = [&](int n, const void* from, int64_t stride) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + n * plane * 16),
+                       "l"(static_cast<const T*>(from) + frow * stride + c)
+                       : "memory");
+        };
+        if (c < a.hidden) {
+          copy(0, a.y, a.y_stride);
+          if (a.residual) copy(1, a.residual, a.residual_stride);
+        }
+      }
+      ++frow;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int n = 0; n < AHEAD; ++n) fetch(n);
+  const auto read = [&](int slot, int n, int i, bool on) {
+    return on && t * E + i * step < a.hidden ? ring[(slot * 2 + n) * plane + i * (int)blockDim.x + t] : make_uint4(0, 0, 0, 0);
+  };
+  const auto squares = [&](int slot) {
+    uint64_t q = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint4 v = read(slot, 0, i, true);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const uint64_t x = Pairs<T>::get(v, j);
+        q = ffma2(x, x, q);
+      }
+    }
+    return add_up(q);
+  };
+  int at = 0;
+  float next = 0.0f;
+  bool known = false;
+  int64_t border = first;                        // the row at which another gate begins
+  for (int64_t row = first; row < end; ++row) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD >= 3 ? AHEAD - 2 : AHEAD - 1) : "memory");
+    const int after = at == AHEAD ? 0 : at + 1;
+    if (row == border) {
+      const int64_t group = row / a.group_rows;
+      border = (group + 1) * a.group_rows;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = t * E + i * step;
+#pragma unroll
+        for (int j = 0; j < P; ++j) g[i][j] = both(1.0f);
+        if (gate && c < a.hidden) pairs_of(a.gate, group * a.gate_stride + c, a.gate_f32, g[i]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) g[i][j] = fmul2(fmul2(g[i][j], p[i][j]), both(a.scale));
+      }
+    }
+    if (post && !(AHEAD >= 3 && known)) {
+      float q[2] = {squares(at), 0.0f};
+      fold(q, warps, warp, lane, buf, half);
+      next = q[0];
+      known = true;
+    }
+    const uint64_t r1 = both(post ? rsqrtf(next * inv + a.eps) : 1.0f);
+    uint64_t s[NV][P], sum = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const uint4 y = read(at, 0, i, true), r = read(at, 1, i, a.residual);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const uint64_t q = fmul2(g[i][j], Pairs<T>::get(y, j));
+        s[i][j] = ffma2(q, r1, Pairs<T>::get(r, j));
+        sum = ffma2(s[i][j], s[i][j], sum);
+      }
+    }
+    float v[2] = {add_up(sum), post && AHEAD >= 3 ? squares(after) : 0.0f};
+    fold(v, warps, warp, lane, buf, half);
+    next = v[1];
+    fetch(at == 0 ? AHEAD : at - 1);
+    at = after;
+    const uint64_t r2 = both(rsqrtf(v[0] * inv + a.eps));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = t * E + i * step;
+      uint4 os, oh;
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        Pairs<T>::put(os, j, s[i][j]);
+        Pairs<T>::put(oh, j, fmul2(fmul2(s[i][j], r2), w[i][j]));
+      }
+      if (c < a.hidden) {
+        if (a.stream) *reinterpret_cast<uint4*>(static_cast<T*>(a.stream) + row * a.stream_stride + c) = os;
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.normed) + row * a.normed_stride + c) = oh;
+      }
+    }
+  }
+}
+
 // out[g][c] = sum over j of part[g * n + j][c], in that order: 32 columns per CTA, the
 // parts dealt to its warps
 template <typename T>
@@ -704,9 +836,31 @@ bool wide(const DashNormArgs& a) {
          ok(a.post, 0, 1) && ok(a.gate, a.gate_stride, E);
 }
 
+// The forward with post or gate takes a CTA per row where each CTA has a few of them: 36,992
+// rows of 1,280 (bf16) 78 us, a warp per row 89.  Without them a warp per row takes 66
+// us, a CTA 68.
+constexpr int kFwdRows = 4, kFwdThreads = 1536;
+
 template <typename T, int E>
 int launch_fwd_e(const DashNormArgs& a, cudaStream_t st) {
   const int vecs = (a.hidden + E - 1) / E;
+  if constexpr (E > 1) {
+    const int nv = vecs <= 512 ? 1 : 2, threads = (vecs + 32 * nv - 1) / (32 * nv) * 32;
+    const int64_t ctas = 148 * max(1, min(12, kFwdThreads / threads));
+    if ((a.post || a.gate) && threads <= 512 && threads >= 64 && a.rows >= kFwdRows * ctas) {
+      const int64_t per = (a.rows + ctas - 1) / ctas;
+      const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+      const size_t ring = (size_t)(nv == 1 ? kAhead<1> + 1 : kAhead<2> + 1) * 2 * nv * threads * 16;
+      const auto go = [&](auto kernel) {
+        if (ring > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
+          return set_error(DASH_ERR_CUDA, "add_norm_kernel: no shared memory for the ring");
+        kernel<<<grid, threads, ring, st>>>(a, per);
+        count_launch();
+        return check_launch("add_norm_kernel");
+      };
+      return nv == 1 ? go(add_norm_wide_kernel<T, 1>) : go(add_norm_wide_kernel<T, 2>);
+    }
+  }
   // A warp holds a row of up to 8 vectors per lane (no barrier); longer rows get the
   // whole CTA.
   const int warps = vecs <= 256 ? 1 : min(16, (vecs + 127) / 128);

@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
+constexpr int kList = 1024;                      // tokens that one CTA sorts out by itself
 constexpr int kTable = 64;                       // 2^(j / 64)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
@@ -38,10 +39,13 @@ constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in sha
 struct alignas(16) Shared {
   uint32_t lo[kBins], hi[kBins];                 // this CTA's histogram: counts (lo), or 64-bit weights
   uint64_t tot[kBins];                           // the cluster's
+  uint64_t list[kList];                          // ~key << 32 | index: what may be kept
+  uint32_t n_list;
+  uint32_t floor_key;
   double table[kTable];
   uint64_t warp_sum[kWarps];
   uint32_t warp_cnt[kWarps];
-  uint32_t top[kMaxCluster];                     // each CTA's largest key
+  uint32_t top[kMaxCluster * kWarps];            // each warp's largest key
   uint64_t cta_sum[kMaxCluster];
   uint32_t cta_cnt[kMaxCluster];
   uint64_t scan[kWarps];
@@ -137,11 +141,9 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
   if (h) atomicAdd(hi, h);
 }
 
-// The cluster's histogram into everybody's `tot`, then the largest digit d whose bins above it
-// hold less than `want` in sum, and those down to d at least `want`: S.found, with the
-// sum above it and its own.
-__device__ void find_digit(Shared& S, cg::cluster_group& cl, int C, int rank, bool counts, uint64_t want) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// the cluster's histogram into everybody's `tot`
+__device__ void total_of(Shared& S, cg::cluster_group& cl, int C, int rank, bool counts) {
+  const int tid = threadIdx.x;
   cl.sync();
   const int per = kBins / C;
   for (int i = tid; i < per; i += kThreads) {
@@ -154,6 +156,12 @@ __device__ void find_digit(Shared& S, cg::cluster_group& cl, int C, int rank, bo
     for (int c = 0; c < C; ++c) cl.map_shared_rank(&S, c)->tot[b] = s;
   }
   cl.sync();
+}
+
+// The largest digit d whose bins above it hold less than `want` in sum, and those down to d
+// at least `want`: S.found, with the sum above it and its own.
+__device__ void digit_of(Shared& S, uint64_t want) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // thread t: the four bins from 4 t down, counted from the top
   constexpr int PER = kBins / kThreads;
   uint64_t v[PER], own = 0;
@@ -229,15 +237,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
   if (keep_slice) sl.kept = kept;
   top = __reduce_max_sync(0xffffffffu, top);
   if (lane == 0) S.warp_cnt[warp] = top;
+  if (tid == 0) S.n_list = 0;
   cl.barrier_wait(std::move(started));
   __syncthreads();
-  if (tid < C) {
-    for (int w = 0; w < kWarps; ++w) top = max(top, S.warp_cnt[w]);
-    cl.map_shared_rank(&S, tid)->top[rank] = top;
-  }
+  const int parts = C * kWarps;
+  if (tid < parts) cl.map_shared_rank(&S, tid / kWarps)->top[rank * kWarps + tid % kWarps] = S.warp_cnt[tid % kWarps];
   cl.sync();
   top = 0;
-  for (int c = 0; c < C; ++c) top = max(top, S.top[c]);
+  for (int i = lane; i < parts; i += 32) top = max(top, S.top[i]);
+  top = __reduce_max_sync(0xffffffffu, top);
 
   Weight wt;
   wt.table = S.table;
@@ -260,42 +268,180 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
     __syncthreads();
   };
 
-  const bool greedy = !(temp > 0.0f);
+  // Tokens with from <= key <= to into every CTA's list, in any order; their number
+  bool filled = false;
+  const auto gather = [&](uint32_t from, uint32_t to) {
+    if (filled) {                                // a list that was too long is given up
+      cl.sync();
+      if (tid == 0) S.n_list = 0;
+      cl.sync();
+    }
+    filled = true;
+    for (int at = warp * chunk + lane * E; at - lane * E < (warp + 1) * chunk; at += 32 * E) {
+      float z[E];
+      sl.read(at, z);
+      uint32_t mine = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t k = key_of(z[e]);
+        mine += k >= from && k <= to;
+      }
+      if (!__any_sync(0xffffffffu, mine)) continue;
+      uint32_t incl = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      const uint32_t n = __shfl_sync(0xffffffffu, incl, 31);
+      uint32_t start = 0;
+      if (lane < C) start = atomicAdd(&cl.map_shared_rank(&S, lane)->n_list, n);
+      for (int c = 0; c < C; ++c) {
+        uint32_t place = __shfl_sync(0xffffffffu, start, c) + incl - mine;
+        uint64_t* to_list = cl.map_shared_rank(&S, c)->list;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t k = key_of(z[e]);
+          if (k >= from && k <= to) {
+            if (place < kList) to_list[place] = (uint64_t)~k << 32 | (uint32_t)(first + at + e);
+            ++place;
+          }
+        }
+      }
+    }
+    cl.sync();
+    return S.n_list;
+  };
+  // The list's n tokens in descending order into `sorted`, with the weights' running sums
+  // in `cums` (both lie on the histogram)
+  uint64_t* sorted = reinterpret_cast<uint64_t*>(S.lo);
+  uint64_t* cums = reinterpret_cast<uint64_t*>(S.hi);
+  const auto sort = [&](int n) {
+    constexpr int PER = kList / kThreads;
+    uint64_t v[PER];
+    int place[PER] = {};
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = tid + i * kThreads < n ? S.list[tid + i * kThreads] : ~0ull;
+    for (int j = 0; j < n; ++j) {
+      const uint64_t o = S.list[j];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) place[i] += o < v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (tid + i * kThreads < n) {
+        sorted[place[i]] = v[i];
+        cums[place[i]] = wt.units(value_of(~(uint32_t)(v[i] >> 32)));
+      }
+    __syncthreads();
+    uint64_t w[PER], own = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      w[i] = tid * PER + i < n ? cums[tid * PER + i] : 0;
+      own += w[i];
+    }
+    uint64_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) S.scan[warp] = incl;
+    __syncthreads();
+    uint64_t run = incl - own;
+    for (int x = 0; x < warp; ++x) run += S.scan[x];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      run += w[i];
+      if (tid * PER + i < n) cums[tid * PER + i] = run;
+    }
+    __syncthreads();
+  };
+  // how many of the first n places have a sum before them that is below `want`
+  const auto count_below = [&](int n, uint64_t want) {
+    int mine = 0;
+    for (int i = tid; i < n; i += kThreads) mine += (i ? cums[i - 1] : 0) < want;
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) S.warp_cnt[warp] = (uint32_t)mine;
+    __syncthreads();
+    int s = 0;
+    for (int w = 0; w < kWarps; ++w) s += (int)S.warp_cnt[w];
+    __syncthreads();
+    return s;
+  };
+
+  const bool greedy = !(temp > 0.0f), k_on = top_k > 0 && top_k < a.vocab;
+  int last = 0x7fffffff;                         // the row's index behind which equals of the cutoff are left out
+  bool done = false;                             // cut and last are final
+  int n_kept = -1;                               // of the sorted list, if it holds all kept ones
+  const auto keep_first = [&](int k) {
+    cut = ~(uint32_t)(sorted[k - 1] >> 32);
+    ties = 1;
+    last = (int)(uint32_t)sorted[k - 1];
+    done = true;
+  };
+  // all that is kept is among the tokens of these keys
+  const auto by_list = [&](uint32_t from) {
+    const uint32_t n = gather(from, 0xffffffffu);
+    if (n > kList) return;
+    sort((int)n);
+    int k = k_on ? min((int)n, top_k) : (int)n;
+    if (top_p < 1.0f) k = count_below(k, max((uint64_t)1, (uint64_t)ceil((double)fmaxf(top_p, 0.0f) * (double)cums[k - 1])));
+    keep_first(k);
+    n_kept = k;
+  };
   if (top == 0) {
-    cut = 0xffffffffu, ties = 0;                 // nothing is left of the row
-  } else if (greedy || (top_k <= 0 || top_k >= a.vocab ? false : top_k == 1)) {
+    cut = 0xffffffffu, ties = 0, done = true;    // nothing is left of the row
+  } else if (greedy || top_k == 1) {
     cut = top, ties = 1;
   } else {
-    if (top_k > 0 && top_k < a.vocab) {
+    if (a.vocab <= kList) {
+      by_list(1u);
+    } else if (k_on && top_k <= parts / 4 * 3) {
+      // At least top_k tokens are as large as the top_k-th largest of the warps' largest,
+      // and not many more (1.4 times top_k at half the warps' number).
+      if (tid < parts) {
+        const uint32_t mine = S.top[tid];
+        int before = 0;
+        for (int j = 0; j < parts; ++j) before += S.top[j] > mine || (S.top[j] == mine && j < tid);
+        if (before == top_k - 1) S.floor_key = max(mine, 1u);
+      }
+      __syncthreads();
+      by_list(S.floor_key);
+    }
+    if (!done && k_on) {
       uint64_t want = (uint64_t)top_k;
       uint32_t prefix = 0;
       bool all = false;
 #pragma unroll 1
-      for (int level = 0; level < 3 && !all; ++level) {
+      for (int level = 0; level < 3 && !all && !done; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
         each([&](int, float, uint32_t k) {
           if (k && (level == 0 || k >> (shift + bits) == prefix)) atomicAdd(&S.lo[(k >> shift) & ((1u << bits) - 1)], 1u);
         });
         if (tid == 0) S.found = 0xffffffffu;
-        find_digit(S, cl, C, rank, true, want);
+        total_of(S, cl, C, rank, true);
+        digit_of(S, want);
         if (S.found == 0xffffffffu) {            // fewer tokens than top_k
           all = true;
         } else {
+          const uint64_t reach = S.found_before + S.found_here;
           want -= S.found_before;
           prefix = (prefix << bits) | S.found;
           equals = (uint32_t)S.found_here;
+          if (level == 0 && reach <= kList && !filled) by_list(max(prefix << shift, 1u));
         }
       }
-      if (!all) cut = prefix, ties = (uint32_t)want;
+      if (!all && !done) cut = prefix, ties = (uint32_t)want;
     }
-    if (top_p < 1.0f) {
+    if (!done && top_p < 1.0f) {
       // the weights' total over what top-k left, and the share of it
       uint64_t want = 0;
       uint32_t prefix = 0;
       const uint32_t floor_key = cut;
 #pragma unroll 1
-      for (int level = 0; level < 3; ++level) {
+      for (int level = 0; level < 3 && !done; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
         each([&](int, float z, uint32_t k) {
@@ -305,9 +451,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
             if (w) add64(&S.lo[b], &S.hi[b], w);
           }
         });
+        total_of(S, cl, C, rank, false);
         if (level == 0) {
-          // the total first: the same two exchanges, then a sum over the bins
-          find_digit(S, cl, C, rank, false, ~0ull);
           uint64_t s = 0;
           for (int i = tid; i < kBins; i += kThreads) s += S.tot[i];
 #pragma unroll
@@ -320,21 +465,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
           const double share = (double)fmaxf(top_p, 0.0f) * (double)s;
           want = max((uint64_t)1, (uint64_t)ceil(share));
         }
-        find_digit(S, cl, C, rank, false, want);
+        digit_of(S, want);
         want -= S.found_before;
         prefix = (prefix << bits) | S.found;
+        if (level == 0 && !k_on) {
+          // this digit's tokens decide the rest, if they are few
+          const uint32_t n = gather(max(prefix << shift, 1u), (prefix << shift) | ((1u << shift) - 1));
+          if (n <= kList) {
+            sort((int)n);
+            keep_first(max(1, count_below((int)n, want)));
+          }
+        }
       }
-      const uint64_t w = wt.units(value_of(prefix));
-      const uint64_t n = w ? (want + w - 1) / w : 1;
-      const uint32_t had = prefix == cut ? ties : 0xffffffffu;
-      cut = prefix;
-      ties = n < had ? (uint32_t)n : had;
+      if (!done) {
+        const uint64_t w = wt.units(value_of(prefix));
+        const uint64_t n = w ? (want + w - 1) / w : 1;
+        const uint32_t had = prefix == cut ? ties : 0xffffffffu;
+        cut = prefix;
+        ties = n < had ? (uint32_t)n : had;
+      }
     }
   }
 
   // ---- the index behind which tokens of the cutoff's key are left out ----
-  int last = 0x7fffffff;                         // in the row
-  if (ties != 0xffffffffu && ties) {
+  if (!done && ties != 0xffffffffu) {
     uint32_t n = 0;
     each([&](int, float, uint32_t k) { n += k == cut; });
     n = __reduce_add_sync(0xffffffffu, n);
@@ -390,6 +544,56 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
     return (uint64_t)__double_as_longlong(fma(e, 8796093022208.0, 4503599627370496.0)) & 0xfffffffffffffull;
   };
 
+  const auto put_probs = [&](uint64_t total) {
+    const double inv = total ? 8796093022208.0 / (double)total : 0.0;
+    float* out = a.probs + (int64_t)row * a.probs_stride + first;
+    const bool ov = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
+      float z[E], p[E];
+      sl.read(at, z);
+#pragma unroll
+      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, key_of(z[e])) ? (float)(weight(z[e]) * inv) : 0.0f;
+      if (ov && at + E <= sl.have) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(out + at + e) = make_float4(p[e], p[e + 1], p[e + 2], p[e + 3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at + e < sl.have) out[at + e] = p[e];
+      }
+    }
+  };
+
+  if (n_kept >= 0) {
+    // the list has all: its weights again, without those that min_p leaves out, and their sum
+    uint64_t sum = 0;
+    for (int i = tid; i < n_kept; i += kThreads) {
+      const uint64_t w = units(weight(value_of(~(uint32_t)(sorted[i] >> 32))));
+      cums[i] = w;
+      sum += w;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) S.warp_sum[warp] = sum;
+    __syncthreads();
+    uint64_t total = 0;
+    for (int w = 0; w < kWarps; ++w) total += S.warp_sum[w];
+    if (a.probs) put_probs(total);
+    if (a.tokens && rank == 0) {
+      uint64_t at_sum = (uint64_t)((double)a.u[row] * (double)total);
+      if (at_sum >= total) at_sum = total - 1;
+      for (int i = tid; i < n_kept; i += kThreads) {
+        const uint32_t mine = (uint32_t)sorted[i];
+        uint64_t before = 0;
+        for (int j = 0; j < n_kept; ++j)
+          if ((uint32_t)sorted[j] < mine) before += cums[j];
+        if (before <= at_sum && before + cums[i] > at_sum) a.tokens[row] = mine;
+      }
+    }
+    return;
+  }
+
   // ---- the kept sum ----
   uint64_t sum = 0;
   each([&](int i, float z, uint32_t k) {
@@ -412,26 +616,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
     total += S.cta_sum[c];
   }
 
-  if (a.probs) {
-    const double inv = total ? 8796093022208.0 / (double)total : 0.0;
-    float* out = a.probs + (int64_t)row * a.probs_stride + first;
-    const bool ov = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
-      float z[E], p[E];
-      sl.read(at, z);
-#pragma unroll
-      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, key_of(z[e])) ? (float)(weight(z[e]) * inv) : 0.0f;
-      if (ov && at + E <= sl.have) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<float4*>(out + at + e) = make_float4(p[e], p[e + 1], p[e + 2], p[e + 3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (at + e < sl.have) out[at + e] = p[e];
-      }
-    }
-  }
+  if (a.probs) put_probs(total);
   if (a.tokens) {
     if (total == 0) {
       if (rank == 0 && tid == 0) a.tokens[row] = -1;

@@ -28,27 +28,32 @@ namespace dash {
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
-constexpr int kList = 1024;                      // tokens that one CTA sorts out by itself
+constexpr int kList = 2048;                      // tokens that one CTA sorts out by itself
+constexpr int kDraw = 128;                       // of which it draws one by itself
 constexpr int kTable = 64;                       // 2^(j / 64)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
+constexpr int kSliceMany = 20 * 1024;            // the same with four CTAs on an SM
+constexpr int kFewRows = 36;                     // up to which a row gets eight CTAs of 512 threads
 
 struct alignas(16) Shared {
   uint32_t lo[kBins], hi[kBins];                 // this CTA's histogram: counts (lo), or 64-bit weights
-  uint64_t tot[kBins];                           // the cluster's
-  uint64_t list[kList];                          // ~key << 32 | index: what may be kept
+  union {
+    uint64_t tot[kBins];                         // the cluster's
+    uint64_t list[kList];                        // ~key << 32 | index: what may be kept
+  };
   uint32_t n_list;
   uint32_t floor_key;
   double table[kTable];
-  uint64_t warp_sum[kWarps];
-  uint32_t warp_cnt[kWarps];
-  uint32_t top[kMaxCluster * kWarps];            // each warp's largest key
+  uint64_t warp_sum[kMaxWarps];
+  uint32_t warp_cnt[2 * kMaxWarps];
+  uint32_t top[kMaxCluster * 2 * kMaxWarps];     // each half warp's largest key
   uint64_t cta_sum[kMaxCluster];
   uint32_t cta_cnt[kMaxCluster];
-  uint64_t scan[kWarps];
+  uint64_t scan[kMaxWarps];
   uint64_t found_before, found_here;             // of the digit that was looked for
   uint32_t found;
   int32_t last;                                  // cutoff index, exchanged
@@ -142,6 +147,7 @@ __device__ __forceinline__ void add64(uint32_t* lo, uint32_t* hi, uint64_t w) {
 }
 
 // the cluster's histogram into everybody's `tot`
+template <int kThreads>
 __device__ void total_of(Shared& S, cg::cluster_group& cl, int C, int rank, bool counts) {
   const int tid = threadIdx.x;
   cl.sync();
@@ -160,6 +166,7 @@ __device__ void total_of(Shared& S, cg::cluster_group& cl, int C, int rank, bool
 
 // The largest digit d whose bins above it hold less than `want` in sum, and those down to d
 // at least `want`: S.found, with the sum above it and its own.
+template <int kThreads>
 __device__ void digit_of(Shared& S, uint64_t want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // thread t: the four bins from 4 t down, counted from the top
@@ -192,9 +199,9 @@ __device__ void digit_of(Shared& S, uint64_t want) {
   __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a, int chunk, int keep_slice) {
-  constexpr int E = 16 / sizeof(T);
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const DashSampleArgs a, int chunk, int keep_slice) {
+  constexpr int E = 16 / sizeof(T), kWarps = kThreads / 32;
   extern __shared__ __align__(16) unsigned char raw[];
   Shared& S = *reinterpret_cast<Shared*>(raw);
   T* kept = reinterpret_cast<T*>(raw + sizeof(Shared));
@@ -219,29 +226,41 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
 
   // ---- the largest logit; the slice into shared memory ----
   uint32_t top = 0;
-  for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
-    float z[E];
-    sl.global(at, z);
-    if (keep_slice) {
-      union {
-        uint4 v;
-        T t[E];
-      } u;
+  const int w0 = warp * chunk + lane * E, w1 = (warp + 1) * chunk;
+  if (keep_slice) {
+    for (int at = w0; at < w1; at += 32 * E) {   // all on their way at once
+      if (sl.vec && at + E <= sl.have) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(kept + at)), "l"(sl.row + at) : "memory");
+      } else {
+        float z[E];
+        sl.global(at, z);
 #pragma unroll
-      for (int e = 0; e < E; ++e) u.t[e] = (T)z[e];
-      *reinterpret_cast<uint4*>(kept + at) = u.v;
+        for (int e = 0; e < E; ++e) kept[at + e] = (T)z[e];
+      }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) top = max(top, key_of(z[e]));
+    asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+    sl.kept = kept;                              // (a thread reads what it has written)
   }
-  if (keep_slice) sl.kept = kept;
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) S.warp_cnt[warp] = top;
+  for (int at = w0; at < w1; at += 4 * 32 * E) {
+    float z[4][E];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i * 32 * E < w1) sl.read(at + i * 32 * E, z[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (at + i * 32 * E < w1)
+#pragma unroll
+        for (int e = 0; e < E; ++e) top = max(top, key_of(z[i][e]));
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((lane & 15) == 0) S.warp_cnt[2 * warp + (lane >> 4)] = top;
   if (tid == 0) S.n_list = 0;
   cl.barrier_wait(std::move(started));
   __syncthreads();
-  const int parts = C * kWarps;
-  if (tid < parts) cl.map_shared_rank(&S, tid / kWarps)->top[rank * kWarps + tid % kWarps] = S.warp_cnt[tid % kWarps];
+  constexpr int OWN = 2 * kWarps;                // half warps
+  const int parts = C * OWN;
+  for (int i = tid; i < parts; i += kThreads) cl.map_shared_rank(&S, i / OWN)->top[rank * OWN + i % OWN] = S.warp_cnt[i % OWN];
   cl.sync();
   top = 0;
   for (int i = lane; i < parts; i += 32) top = max(top, S.top[i]);
@@ -252,6 +271,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
   wt.top = (double)value_of(top);
   wt.inv = 1.0 / (double)temp;
 
+  bool filled = false, counted = false;          // the list, the histogram have been used
   // kept: key > cut, or key == cut and one of the first `ties` tokens of that key
   uint32_t cut = 1u, ties = 0xffffffffu, equals = 0;
   // each element of the slice, as f(index in the slice, logit, key)
@@ -265,17 +285,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
   };
   const auto clear = [&] {
     for (int i = tid; i < kBins; i += kThreads) S.lo[i] = S.hi[i] = 0;
+    counted = true;
     __syncthreads();
   };
 
-  // Tokens with from <= key <= to into every CTA's list, in any order; their number
-  bool filled = false;
-  const auto gather = [&](uint32_t from, uint32_t to) {
+  // Tokens that `in` holds for (logit, key) into every CTA's list, in any order; their number
+  const auto gather = [&](auto&& in) {
     if (filled) {                                // a list that was too long is given up
       cl.sync();
       if (tid == 0) S.n_list = 0;
-      cl.sync();
     }
+    if (filled || counted) cl.sync();            // nobody reads `tot` any more
     filled = true;
     for (int at = warp * chunk + lane * E; at - lane * E < (warp + 1) * chunk; at += 32 * E) {
       float z[E];
@@ -284,7 +304,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t k = key_of(z[e]);
-        mine += k >= from && k <= to;
+        mine += k && in(z[e], k);
       }
       if (!__any_sync(0xffffffffu, mine)) continue;
       uint32_t incl = mine;
@@ -302,7 +322,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const uint32_t k = key_of(z[e]);
-          if (k >= from && k <= to) {
+          if (k && in(z[e], k)) {
             if (place < kList) to_list[place] = (uint64_t)~k << 32 | (uint32_t)(first + at + e);
             ++place;
           }
@@ -312,32 +332,40 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
     cl.sync();
     return S.n_list;
   };
-  // The list's n tokens in descending order into `sorted`, with the weights' running sums
-  // in `cums` (both lie on the histogram)
-  uint64_t* sorted = reinterpret_cast<uint64_t*>(S.lo);
-  uint64_t* cums = reinterpret_cast<uint64_t*>(S.hi);
+  // The list's n tokens in descending order (lowest index first among equals), and the weights'
+  // running sums in `cums` (on the histogram)
+  uint64_t* sorted = S.list;
+  uint64_t* cums = reinterpret_cast<uint64_t*>(S.lo);
   const auto sort = [&](int n) {
     constexpr int PER = kList / kThreads;
-    uint64_t v[PER];
-    int place[PER] = {};
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = tid + i * kThreads < n ? S.list[tid + i * kThreads] : ~0ull;
-    for (int j = 0; j < n; ++j) {
-      const uint64_t o = S.list[j];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) place[i] += o < v[i];
+    if (n <= 256) {
+      // by each one's place among all
+      uint64_t v = tid < n ? S.list[tid] : ~0ull;
+      int place = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) place += S.list[j] < v;
+      __syncthreads();
+      if (tid < n) sorted[place] = v;
+    } else {
+      int m = 512;
+      while (m < n) m *= 2;
+      for (int i = n + tid; i < m; i += kThreads) sorted[i] = ~0ull;
+      for (int size = 2; size <= m; size *= 2)
+        for (int d = size / 2; d; d /= 2) {
+          __syncthreads();
+          for (int x = tid; x < m / 2; x += kThreads) {
+            const int i = 2 * x - (x & (d - 1)), j = i + d;        // bitonic network
+            const uint64_t p = sorted[i], q = sorted[j];
+            if ((p > q) == ((i & size) == 0)) sorted[i] = q, sorted[j] = p;
+          }
+        }
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (tid + i * kThreads < n) {
-        sorted[place[i]] = v[i];
-        cums[place[i]] = wt.units(value_of(~(uint32_t)(v[i] >> 32)));
-      }
     __syncthreads();
     uint64_t w[PER], own = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      w[i] = tid * PER + i < n ? cums[tid * PER + i] : 0;
+      const int x = tid * PER + i;
+      w[i] = x < n ? wt.units(value_of(~(uint32_t)(sorted[x] >> 32))) : 0;
       own += w[i];
     }
     uint64_t incl = own;
@@ -380,57 +408,104 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
     last = (int)(uint32_t)sorted[k - 1];
     done = true;
   };
-  // all that is kept is among the tokens of these keys
-  const auto by_list = [&](uint32_t from) {
-    const uint32_t n = gather(from, 0xffffffffu);
+  // all that is kept is among the tokens that `in` holds for
+  const auto by_list = [&](auto&& in) {
+    const uint32_t n = gather(in);
     if (n > kList) return;
     sort((int)n);
     int k = k_on ? min((int)n, top_k) : (int)n;
     if (top_p < 1.0f) k = count_below(k, max((uint64_t)1, (uint64_t)ceil((double)fmaxf(top_p, 0.0f) * (double)cums[k - 1])));
     keep_first(k);
-    n_kept = k;
+    if (k <= kDraw) n_kept = k;
   };
+  // A bin per 1/50 of an exponent below the largest logit's (bins of the key's digits hold a
+  // tenth of the vocabulary each: atomics on few addresses); monotone, like each of its steps
+  const float top_f = value_of(top), scale = 50.0f / temp;
+  const auto bin = [&](float z) { return kBins - 1 - min(kBins - 1, (int)((top_f - z) * scale)); };
+  // the weights' total in `tot`
+  const auto total_weight = [&] {
+    uint64_t s = 0;
+    for (int i = tid; i < kBins; i += kThreads) s += S.tot[i];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (lane == 0) S.warp_sum[warp] = s;
+    __syncthreads();
+    s = 0;
+    for (int w = 0; w < kWarps; ++w) s += S.warp_sum[w];
+    return s;
+  };
+  const auto share_of = [&](uint64_t s) { return max((uint64_t)1, (uint64_t)ceil((double)fmaxf(top_p, 0.0f) * (double)s)); };
+
   if (top == 0) {
     cut = 0xffffffffu, ties = 0, done = true;    // nothing is left of the row
   } else if (greedy || top_k == 1) {
     cut = top, ties = 1;
   } else {
     if (a.vocab <= kList) {
-      by_list(1u);
+      by_list([](float, uint32_t) { return true; });
     } else if (k_on && top_k <= parts / 4 * 3) {
-      // At least top_k tokens are as large as the top_k-th largest of the warps' largest,
-      // and not many more (1.4 times top_k at half the warps' number).
-      if (tid < parts) {
-        const uint32_t mine = S.top[tid];
+      // At least top_k tokens are as large as the top_k-th largest of the half warps'
+      // largest, and not many more (1.4 times top_k at half their number).
+      for (int i = tid; i < parts; i += kThreads) {
+        const uint32_t mine = S.top[i];
         int before = 0;
-        for (int j = 0; j < parts; ++j) before += S.top[j] > mine || (S.top[j] == mine && j < tid);
-        if (before == top_k - 1) S.floor_key = max(mine, 1u);
+        for (int j = 0; j < parts; ++j) before += S.top[j] > mine || (S.top[j] == mine && j < i);
+        if (before == top_k - 1) S.floor_key = mine;
       }
       __syncthreads();
-      by_list(S.floor_key);
+      const uint32_t from = S.floor_key;
+      by_list([=](float, uint32_t k) { return k >= from; });
+    } else if (k_on) {
+      clear();
+      each([&](int, float z, uint32_t k) {
+        if (k) atomicAdd(&S.lo[bin(z)], 1u);
+      });
+      if (tid == 0) S.found = 0u, S.found_before = S.found_here = 0;      // fewer tokens than top_k: all
+      total_of<kThreads>(S, cl, C, rank, true);
+      digit_of<kThreads>(S, (uint64_t)top_k);
+      const int from = (int)S.found;
+      if (S.found_before + S.found_here <= kList) by_list([&](float z, uint32_t) { return bin(z) >= from; });
+    } else if (top_p < 1.0f) {
+      clear();
+      each([&](int, float z, uint32_t k) {
+        if (k) {
+          const uint64_t w = wt.units(z);
+          const int b = bin(z);
+          if (w) add64(&S.lo[b], &S.hi[b], w);
+        }
+      });
+      total_of<kThreads>(S, cl, C, rank, false);
+      const uint64_t want = share_of(total_weight());
+      digit_of<kThreads>(S, want);
+      const int at = (int)S.found;
+      const uint64_t left = want - S.found_before;
+      const uint32_t n = gather([&](float z, uint32_t) { return bin(z) == at; });
+      if (n <= kList) {
+        sort((int)n);
+        keep_first(max(1, count_below((int)n, left)));
+      }
     }
+    // what no list could hold: by the key's digits
     if (!done && k_on) {
       uint64_t want = (uint64_t)top_k;
       uint32_t prefix = 0;
       bool all = false;
 #pragma unroll 1
-      for (int level = 0; level < 3 && !all && !done; ++level) {
+      for (int level = 0; level < 3 && !all; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
         each([&](int, float, uint32_t k) {
           if (k && (level == 0 || k >> (shift + bits) == prefix)) atomicAdd(&S.lo[(k >> shift) & ((1u << bits) - 1)], 1u);
         });
         if (tid == 0) S.found = 0xffffffffu;
-        total_of(S, cl, C, rank, true);
-        digit_of(S, want);
+        total_of<kThreads>(S, cl, C, rank, true);
+        digit_of<kThreads>(S, want);
         if (S.found == 0xffffffffu) {            // fewer tokens than top_k
           all = true;
         } else {
-          const uint64_t reach = S.found_before + S.found_here;
           want -= S.found_before;
           prefix = (prefix << bits) | S.found;
           equals = (uint32_t)S.found_here;
-          if (level == 0 && reach <= kList && !filled) by_list(max(prefix << shift, 1u));
         }
       }
       if (!all && !done) cut = prefix, ties = (uint32_t)want;
@@ -441,7 +516,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
       uint32_t prefix = 0;
       const uint32_t floor_key = cut;
 #pragma unroll 1
-      for (int level = 0; level < 3 && !done; ++level) {
+      for (int level = 0; level < 3; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
         each([&](int, float z, uint32_t k) {
@@ -451,39 +526,21 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
             if (w) add64(&S.lo[b], &S.hi[b], w);
           }
         });
-        total_of(S, cl, C, rank, false);
+        total_of<kThreads>(S, cl, C, rank, false);
         if (level == 0) {
-          uint64_t s = 0;
-          for (int i = tid; i < kBins; i += kThreads) s += S.tot[i];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (lane == 0) S.warp_sum[warp] = s;
-          __syncthreads();
-          s = 0;
-          for (int w = 0; w < kWarps; ++w) s += S.warp_sum[w];
+          uint64_t s = total_weight();
           if (ties < equals) s -= (uint64_t)(equals - ties) * wt.units(value_of(cut));
-          const double share = (double)fmaxf(top_p, 0.0f) * (double)s;
-          want = max((uint64_t)1, (uint64_t)ceil(share));
+          want = share_of(s);
         }
-        digit_of(S, want);
+        digit_of<kThreads>(S, want);
         want -= S.found_before;
         prefix = (prefix << bits) | S.found;
-        if (level == 0 && !k_on) {
-          // this digit's tokens decide the rest, if they are few
-          const uint32_t n = gather(max(prefix << shift, 1u), (prefix << shift) | ((1u << shift) - 1));
-          if (n <= kList) {
-            sort((int)n);
-            keep_first(max(1, count_below((int)n, want)));
-          }
-        }
       }
-      if (!done) {
-        const uint64_t w = wt.units(value_of(prefix));
-        const uint64_t n = w ? (want + w - 1) / w : 1;
-        const uint32_t had = prefix == cut ? ties : 0xffffffffu;
-        cut = prefix;
-        ties = n < had ? (uint32_t)n : had;
-      }
+      const uint64_t w = wt.units(value_of(prefix));
+      const uint64_t n = w ? (want + w - 1) / w : 1;
+      const uint32_t had = prefix == cut ? ties : 0xffffffffu;
+      cut = prefix;
+      ties = n < had ? (uint32_t)n : had;
     }
   }
 
@@ -654,22 +711,22 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const DashSampleArgs a
   }
 }
 
-template <typename T>
+template <typename T, int THREADS>
 int launch_sample_t(const DashSampleArgs& a, cudaStream_t st) {
-  constexpr int E = 16 / sizeof(T);
-  // as many CTAs per row as leave each some work and the GPU's slots filled about once
+  constexpr int E = 16 / sizeof(T), WARPS = THREADS / 32;
+  // eight CTAs per row, as far as that leaves each warp some work
   int C = kMaxCluster;
-  while (C > 1 && a.vocab <= (C / 2) * kWarps * 32 * E) C >>= 1;
-  const int parts = C * kWarps;
+  while (C > 1 && a.vocab <= (C / 2) * WARPS * 32 * E) C >>= 1;
+  const int parts = C * WARPS;
   const int chunk = ((a.vocab + parts - 1) / parts + 32 * E - 1) / (32 * E) * (32 * E);
-  const int64_t bytes = (int64_t)chunk * kWarps * sizeof(T);
-  const int keep = bytes <= kSliceMost;
-  static const cudaError_t set =
-      cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared) + kSliceMost);
+  const int64_t bytes = (int64_t)chunk * WARPS * sizeof(T);
+  const int keep = bytes <= (THREADS == 512 ? kSliceMost : kSliceMany);
+  static const cudaError_t set = cudaFuncSetAttribute(sample_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (int)sizeof(Shared) + kSliceMost);
   if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(set));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * C);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = sizeof(Shared) + (keep ? (size_t)bytes : 0);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -678,18 +735,23 @@ int launch_sample_t(const DashSampleArgs& a, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, chunk, keep);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel<T, THREADS>, a, chunk, keep);
   if (e != cudaSuccess) return set_error(DASH_ERR_CUDA, "sample_kernel launch failed: %s", cudaGetErrorString(e));
   count_launch();
   return check_launch("sample_kernel");
 }
 
+template <typename T>
+int launch_sample_rows(const DashSampleArgs& a, cudaStream_t st) {
+  return a.rows <= kFewRows ? launch_sample_t<T, 512>(a, st) : launch_sample_t<T, 256>(a, st);
+}
+
 }  // namespace
 
 int launch_sample(const DashSampleArgs& a, cudaStream_t st) {
-  if (a.dtype == DASH_DTYPE_F32) return launch_sample_t<float>(a, st);
-  if (a.dtype == DASH_DTYPE_BF16) return launch_sample_t<__nv_bfloat16>(a, st);
-  return launch_sample_t<__half>(a, st);
+  if (a.dtype == DASH_DTYPE_F32) return launch_sample_rows<float>(a, st);
+  if (a.dtype == DASH_DTYPE_BF16) return launch_sample_rows<__nv_bfloat16>(a, st);
+  return launch_sample_rows<__half>(a, st);
 }
 
 }  // namespace dash

@@ -33,7 +33,7 @@ constexpr int kMaxCluster = 8;
 constexpr int kBins = 2048;
 constexpr int kList = 2048;                      // tokens that one CTA sorts out by itself
 constexpr int kDraw = 128;                       // of which it draws one by itself
-constexpr int kTable = 64;                       // 2^(j / 64)
+constexpr int kTable = 256;                      // 2^(j / 256)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
 constexpr int kSliceMany = 20 * 1024;            // the same with four CTAs on an SM
@@ -45,12 +45,12 @@ struct alignas(16) Shared {
     uint64_t tot[kBins];                         // the cluster's
     uint64_t list[kList];                        // ~key << 32 | index: what may be kept
   };
-  uint32_t n_list;
+  uint32_t n_own;
   uint32_t floor_key;
   double table[kTable];
   uint64_t warp_sum[kMaxWarps];
   uint32_t warp_cnt[2 * kMaxWarps];
-  uint32_t top[kMaxCluster * 2 * kMaxWarps];     // each half warp's largest key
+  alignas(16) uint32_t top[kMaxCluster * 2 * kMaxWarps];     // each half warp's largest key
   uint64_t cta_sum[kMaxCluster];
   uint32_t cta_cnt[kMaxCluster];
   uint64_t scan[kMaxWarps];
@@ -71,34 +71,44 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// exp(x) for x <= 0, relative error below 1e-13: x = (64 k + j) ln2 / 64 + r, |r| <= ln2 / 128,
-// 2^k * 2^(j/64) * (1 + r + r^2/2 + r^3/6 + r^4/24) (the next term is 4e-14).  0 below -60, where
-// the weight is below 2^-43.
-__device__ __forceinline__ double exp64(double x, const double* table) {
-  if (!(x > -60.0)) return 0.0;
-  constexpr double kShift = 6755399441055744.0;                 // 1.5 * 2^52
-  const double t = fma(x, 92.332482616893656877, kShift);       // 64 / ln 2
-  const int n = (int)__double_as_longlong(t);
-  const double r = fma(t - kShift, -0.010830424696249145264, x);
-  double p = fma(r, 1.0 / 24, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0) * table[n & (kTable - 1)];
-  return __longlong_as_double(__double_as_longlong(p) + ((long long)(n >> 6) << 52));
-}
-
+// exp((z - top) / t) in units of 2^-43, relative error below 3e-12: with y = (z - top) / (t ln 2) * 256
+// = 256 k + j + r, |r| <= 1, it is 2^k * 2^(j/256) * exp(r ln2 / 256), the last factor by its series
+// (the term behind the cubic one is 2.2e-12).  Eight 64-bit operations per weight; the
+// largest logit has 1 exactly, an infinite one, too.
 struct Weight {
-  double top, inv;                               // largest logit, 1 / temperature
-  const double* table;
+  float top;                                     // largest logit
+  double mul, add;                               // y = z * mul + add
+  const double* table;                           // 2^(j/256) * 2^43
+  static constexpr double kOne = 8796093022208.0;                                        // 2^43
+
+  __device__ __forceinline__ Weight(float t, float temperature, const double* tab) : top(t), table(tab) {
+    mul = 369.32993046757462271 / (double)temperature;                                   // 256 / ln 2
+    add = -(double)t * mul;
+  }
+  // a 32-bit number as a 64-bit one, without the conversion unit (0 becomes 2^-127)
+  static __device__ __forceinline__ double wide(float z) {
+    const uint32_t b = __float_as_uint(z);
+    return __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)), (int)(b << 29));
+  }
   __device__ __forceinline__ double e(float z) const {
-    if ((double)z == top) return 1.0;            // an infinite one, too
-    return exp64(((double)z - top) * inv, table);
+    if (z == top) return kOne;
+    constexpr double kShift = 6755399441055744.0;                                        // 1.5 * 2^52
+    const double w = wide(z), t = fma(w, mul, add + kShift);
+    const int n = __double2loint(t);
+    // (beyond 2^31 / 256 the whole part does not fit: 2^43 below 1 is far behind by then)
+    if (!((z - top) * (float)mul > -44.0f * 256.0f)) return 0.0;
+    const double r = fma(w, mul, add - (t - kShift));
+    double p = fma(r, 3.3083026805413711e-9, 3.6655755969101061e-6);                           // (ln2/256)^3 / 6, ^2 / 2
+    p = fma(p, r, 2.7076061740622863e-3);                                                // ln 2 / 256
+    p = fma(p, r, 1.0);
+    const double s = table[n & (kTable - 1)];
+    return p * __hiloint2double(__double2hiint(s) + (n >> 8) * (1 << 20), __double2loint(s));
   }
-  // in units of 2^-43 of the largest, rounded
-  __device__ __forceinline__ uint64_t units(float z) const {
-    const double v = fma(e(z), 8796093022208.0, 4503599627370496.0);     // 2^43, 2^52
-    return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffull;
+  // rounded to whole units
+  static __device__ __forceinline__ uint64_t whole(double e) {
+    return (uint64_t)__double_as_longlong(e + 4503599627370496.0) & 0xfffffffffffffull;  // 2^52
   }
+  __device__ __forceinline__ uint64_t units(float z) const { return whole(e(z)); }
 };
 
 // a row's slice: in shared memory, or in global memory where it is too long
@@ -222,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   sl.kept = nullptr;
   sl.vec = (reinterpret_cast<uintptr_t>(sl.row) & 15) == 0;
 
-  if (tid < kTable) S.table[tid] = exp2((double)tid / kTable);
+  if (tid < kTable) S.table[tid] = exp2(43.0 + (double)tid / kTable);
 
   // ---- the largest logit; the slice into shared memory ----
   uint32_t top = 0;
@@ -255,7 +265,6 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 #pragma unroll
   for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((lane & 15) == 0) S.warp_cnt[2 * warp + (lane >> 4)] = top;
-  if (tid == 0) S.n_list = 0;
   cl.barrier_wait(std::move(started));
   __syncthreads();
   constexpr int OWN = 2 * kWarps;                // half warps
@@ -266,12 +275,9 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   for (int i = lane; i < parts; i += 32) top = max(top, S.top[i]);
   top = __reduce_max_sync(0xffffffffu, top);
 
-  Weight wt;
-  wt.table = S.table;
-  wt.top = (double)value_of(top);
-  wt.inv = 1.0 / (double)temp;
+  const Weight wt(value_of(top), temp, S.table);
 
-  bool filled = false, counted = false;          // the list, the histogram have been used
+  bool counted = false;                          // the histogram has been used
   // kept: key > cut, or key == cut and one of the first `ties` tokens of that key
   uint32_t cut = 1u, ties = 0xffffffffu, equals = 0;
   // each element of the slice, as f(index in the slice, logit, key)
@@ -291,75 +297,67 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 
   // Tokens that `in` holds for (logit, key) into every CTA's list, in any order; their number
   const auto gather = [&](auto&& in) {
-    if (filled) {                                // a list that was too long is given up
-      cl.sync();
-      if (tid == 0) S.n_list = 0;
-    }
-    if (filled || counted) cl.sync();            // nobody reads `tot` any more
-    filled = true;
-    for (int at = warp * chunk + lane * E; at - lane * E < (warp + 1) * chunk; at += 32 * E) {
+    if (counted) cl.sync();                      // nobody reads `tot` any more
+    // this CTA's own first (on the histogram), then every CTA's behind those of the CTAs before it
+    uint64_t* own = reinterpret_cast<uint64_t*>(S.lo);
+    if (tid == 0) S.n_own = 0;
+    __syncthreads();
+    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
       float z[E];
       sl.read(at, z);
-      uint32_t mine = 0;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t k = key_of(z[e]);
-        mine += k && in(z[e], k);
-      }
-      if (!__any_sync(0xffffffffu, mine)) continue;
-      uint32_t incl = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      const uint32_t n = __shfl_sync(0xffffffffu, incl, 31);
-      uint32_t start = 0;
-      if (lane < C) start = atomicAdd(&cl.map_shared_rank(&S, lane)->n_list, n);
-      for (int c = 0; c < C; ++c) {
-        uint32_t place = __shfl_sync(0xffffffffu, start, c) + incl - mine;
-        uint64_t* to_list = cl.map_shared_rank(&S, c)->list;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t k = key_of(z[e]);
-          if (k && in(z[e], k)) {
-            if (place < kList) to_list[place] = (uint64_t)~k << 32 | (uint32_t)(first + at + e);
-            ++place;
-          }
+        if (k && in(z[e], k)) {
+          const uint32_t place = atomicAdd(&S.n_own, 1u);
+          if (place < kList) own[place] = (uint64_t)~k << 32 | (uint32_t)(first + at + e);
         }
       }
     }
+    __syncthreads();
+    if (tid < C) cl.map_shared_rank(&S, tid)->cta_cnt[rank] = S.n_own;
     cl.sync();
-    return S.n_list;
+    uint32_t start = 0, total = 0;
+    for (int c = 0; c < C; ++c) {
+      if (c < rank) start += S.cta_cnt[c];
+      total += S.cta_cnt[c];
+    }
+    if (total <= kList)
+      for (int c = 0; c < C; ++c) {
+        uint64_t* to = cl.map_shared_rank(&S, c)->list + start;
+        for (uint32_t i = tid; i < S.n_own; i += kThreads) to[i] = own[i];
+      }
+    cl.sync();
+    return total;
   };
   // The list's n tokens in descending order (lowest index first among equals), and the weights'
   // running sums in `cums` (on the histogram)
-  uint64_t* sorted = S.list;
-  uint64_t* cums = reinterpret_cast<uint64_t*>(S.lo);
+  uint64_t* sorted = reinterpret_cast<uint64_t*>(S.lo);
+  uint64_t* cums = S.list;
   const auto sort = [&](int n) {
     constexpr int PER = kList / kThreads;
-    if (n <= 256) {
-      // by each one's place among all
-      uint64_t v = tid < n ? S.list[tid] : ~0ull;
+    // Each one's place is the number before it.  A long list is shared out to the CTAs: eight
+    // threads count for one token.
+    const bool alone = n <= 128 || C == 1;
+    const int from = alone ? 0 : n * rank / C, to = alone ? n : n * (rank + 1) / C;
+    for (int i0 = from; i0 < to; i0 += kThreads / 8) {
+      const int i = i0 + tid / 8;
+      const uint64_t v = i < to ? S.list[i] : 0;
       int place = 0;
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) place += S.list[j] < v;
-      __syncthreads();
-      if (tid < n) sorted[place] = v;
-    } else {
-      int m = 512;
-      while (m < n) m *= 2;
-      for (int i = n + tid; i < m; i += kThreads) sorted[i] = ~0ull;
-      for (int size = 2; size <= m; size *= 2)
-        for (int d = size / 2; d; d /= 2) {
-          __syncthreads();
-          for (int x = tid; x < m / 2; x += kThreads) {
-            const int i = 2 * x - (x & (d - 1)), j = i + d;        // bitonic network
-            const uint64_t p = sorted[i], q = sorted[j];
-            if ((p > q) == ((i & size) == 0)) sorted[i] = q, sorted[j] = p;
-          }
+      for (int j = tid & 7; j < n; j += 8) place += S.list[j] < v;
+      place += __shfl_xor_sync(0xffffffffu, place, 1);
+      place += __shfl_xor_sync(0xffffffffu, place, 2);
+      place += __shfl_xor_sync(0xffffffffu, place, 4);
+      if (i < to) {
+        if (alone) {
+          if ((tid & 7) == 0) sorted[place] = v;
+        } else if ((tid & 7) < C) {
+          reinterpret_cast<uint64_t*>(cl.map_shared_rank(&S, tid & 7)->lo)[place] = v;
         }
+      }
     }
+    if (!alone) cl.sync();
     __syncthreads();
     uint64_t w[PER], own = 0;
 #pragma unroll
@@ -449,7 +447,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       for (int i = tid; i < parts; i += kThreads) {
         const uint32_t mine = S.top[i];
         int before = 0;
-        for (int j = 0; j < parts; ++j) before += S.top[j] > mine || (S.top[j] == mine && j < i);
+#pragma unroll 4
+        for (int j = 0; j < parts; j += 4) {
+          const uint4 o = *reinterpret_cast<const uint4*>(S.top + j);
+          before += (o.x > mine || (o.x == mine && j < i)) + (o.y > mine || (o.y == mine && j + 1 < i)) +
+                    (o.z > mine || (o.z == mine && j + 2 < i)) + (o.w > mine || (o.w == mine && j + 3 < i));
+        }
         if (before == top_k - 1) S.floor_key = mine;
       }
       __syncthreads();
@@ -592,17 +595,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   const auto is_kept = [&](int i, uint32_t k) { return k > cut || (k == cut && ties && first + i <= last); };
   // a greedy row has one token, of weight 1
+  const double least = (double)min_p * Weight::kOne;
   const auto weight = [&](float z) -> double {
-    if (greedy) return 1.0;
+    if (greedy) return Weight::kOne;
     const double e = wt.e(z);
-    return e >= (double)min_p ? e : 0.0;
+    return e >= least ? e : 0.0;
   };
-  const auto units = [&](double e) {
-    return (uint64_t)__double_as_longlong(fma(e, 8796093022208.0, 4503599627370496.0)) & 0xfffffffffffffull;
-  };
-
   const auto put_probs = [&](uint64_t total) {
-    const double inv = total ? 8796093022208.0 / (double)total : 0.0;
+    const double inv = total ? 1.0 / (double)total : 0.0;
     float* out = a.probs + (int64_t)row * a.probs_stride + first;
     const bool ov = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
     for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     // the list has all: its weights again, without those that min_p leaves out, and their sum
     uint64_t sum = 0;
     for (int i = tid; i < n_kept; i += kThreads) {
-      const uint64_t w = units(weight(value_of(~(uint32_t)(sorted[i] >> 32))));
+      const uint64_t w = Weight::whole(weight(value_of(~(uint32_t)(sorted[i] >> 32))));
       cums[i] = w;
       sum += w;
     }
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // ---- the kept sum ----
   uint64_t sum = 0;
   each([&](int i, float z, uint32_t k) {
-    if (is_kept(i, k)) sum += units(weight(z));
+    if (is_kept(i, k)) sum += Weight::whole(weight(z));
   });
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         uint64_t w[E], own = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          w[e] = is_kept(at + e, key_of(z[e])) ? units(weight(z[e])) : 0;
+          w[e] = is_kept(at + e, key_of(z[e])) ? Weight::whole(weight(z[e])) : 0;
           own += w[e];
         }
         uint64_t incl = own;

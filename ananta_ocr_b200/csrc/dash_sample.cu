@@ -37,7 +37,10 @@ constexpr int kTable = 256;                      // 2^(j / 256)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
 constexpr int kSliceMany = 20 * 1024;            // the same with four CTAs on an SM
-constexpr int kFewRows = 36;                     // up to which a row gets eight CTAs of 512 threads
+// Up to so many rows a CTA has 512 threads (two on an SM, slices in shared memory), above it 256
+// (four).  64 rows of 129,280 (fp32) with settings of their own 59 us, with 256 threads 78;
+// with top-k 20 alone 36 and 22.  128 rows (bf16), top-k 50: 88 and 63.
+constexpr int kFewRows = 64;
 
 struct alignas(16) Shared {
   uint32_t lo[kBins], hi[kBins];                 // this CTA's histogram: counts (lo), or 64-bit weights
@@ -45,6 +48,7 @@ struct alignas(16) Shared {
     uint64_t tot[kBins];                         // the cluster's
     uint64_t list[kList];                        // ~key << 32 | index: what may be kept
   };
+  uint32_t bucket[kBins + 1];                    // of the list's sorting
   uint32_t n_own;
   uint32_t floor_key;
   double table[kTable];
@@ -80,6 +84,7 @@ struct Weight {
   double mul, add;                               // y = z * mul + add
   const double* table;                           // 2^(j/256) * 2^43
   static constexpr double kOne = 8796093022208.0;                                        // 2^43
+  static constexpr double kShift = 6755399441055744.0;                                   // 1.5 * 2^52
 
   __device__ __forceinline__ Weight(float t, float temperature, const double* tab) : top(t), table(tab) {
     mul = 369.32993046757462271 / (double)temperature;                                   // 256 / ln 2
@@ -90,19 +95,18 @@ struct Weight {
     const uint32_t b = __float_as_uint(z);
     return __hiloint2double((int)((((b & 0x7fffffffu) >> 3) + 0x38000000u) | (b & 0x80000000u)), (int)(b << 29));
   }
+  // (without branches, so that the chains of several weights run side by side)
   __device__ __forceinline__ double e(float z) const {
-    if (z == top) return kOne;
-    constexpr double kShift = 6755399441055744.0;                                        // 1.5 * 2^52
     const double w = wide(z), t = fma(w, mul, add + kShift);
     const int n = __double2loint(t);
-    // (beyond 2^31 / 256 the whole part does not fit: 2^43 below 1 is far behind by then)
-    if (!((z - top) * (float)mul > -44.0f * 256.0f)) return 0.0;
     const double r = fma(w, mul, add - (t - kShift));
-    double p = fma(r, 3.3083026805413711e-9, 3.6655755969101061e-6);                           // (ln2/256)^3 / 6, ^2 / 2
+    double p = fma(r, 3.3083026805413711e-9, 3.6655755969101061e-6);                     // (ln2/256)^3 / 6, ^2 / 2
     p = fma(p, r, 2.7076061740622863e-3);                                                // ln 2 / 256
     p = fma(p, r, 1.0);
     const double s = table[n & (kTable - 1)];
-    return p * __hiloint2double(__double2hiint(s) + (n >> 8) * (1 << 20), __double2loint(s));
+    p *= __hiloint2double(__double2hiint(s) + (n >> 8) * (1 << 20), __double2loint(s));
+    // below 2^-44 nothing; further down the whole part does not fit
+    return z == top ? kOne : (z - top) * (float)mul > -44.0f * 256.0f ? p : 0.0;
   }
   // rounded to whole units
   static __device__ __forceinline__ uint64_t whole(double e) {
@@ -118,33 +122,35 @@ struct Slice {
   const T* row;                                  // the slice's first element in global memory
   int have;                                      // elements of the row in the slice (may be <= 0)
   bool vec;
-  // elements at .. at + E - 1 of the slice; behind its end -inf
-  __device__ __forceinline__ void read(int at, float (&z)[E]) const {
+  // elements at .. at + E - 1 of the slice as they are; behind its end -inf
+  __device__ __forceinline__ uint4 raw(int at) const { return kept ? *reinterpret_cast<const uint4*>(kept + at) : global(at); }
+  __device__ __forceinline__ uint4 global(int at) const {
+    if (vec && at + E <= have) return *reinterpret_cast<const uint4*>(row + at);
     union {
       uint4 v;
       T t[E];
     } u;
-    if (kept) {
-      u.v = *reinterpret_cast<const uint4*>(kept + at);
 #pragma unroll
-      for (int e = 0; e < E; ++e) z[e] = (float)u.t[e];
+    for (int e = 0; e < E; ++e) u.t[e] = at + e < have ? row[at + e] : (T)-INFINITY;
+    return u.v;
+  }
+  // half of them
+  static constexpr int H = E / 2;
+  static __device__ __forceinline__ void half(uint32_t x, uint32_t y, float (&z)[H]) {
+    if constexpr (E == 4) {
+      z[0] = __uint_as_float(x), z[1] = __uint_as_float(y);
     } else {
-      global(at, z);
+      const float2 a = unpack2(x, (T*)nullptr), b = unpack2(y, (T*)nullptr);
+      z[0] = a.x, z[1] = a.y, z[2] = b.x, z[3] = b.y;
     }
   }
-  __device__ __forceinline__ void global(int at, float (&z)[E]) const {
-    if (vec && at + E <= have) {
-      union {
-        uint4 v;
-        T t[E];
-      } u;
-      u.v = *reinterpret_cast<const uint4*>(row + at);
+  __device__ __forceinline__ void read(int at, float (&z)[E]) const {
+    const uint4 v = raw(at);
+    float a[H], b[H];
+    half(v.x, v.y, a);
+    half(v.z, v.w, b);
 #pragma unroll
-      for (int e = 0; e < E; ++e) z[e] = (float)u.t[e];
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) z[e] = at + e < have ? (float)row[at + e] : -INFINITY;
-    }
+    for (int e = 0; e < H; ++e) z[e] = a[e], z[H + e] = b[e];
   }
 };
 
@@ -235,33 +241,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (tid < kTable) S.table[tid] = exp2(43.0 + (double)tid / kTable);
 
   // ---- the largest logit; the slice into shared memory ----
-  uint32_t top = 0;
   const int w0 = warp * chunk + lane * E, w1 = (warp + 1) * chunk;
   if (keep_slice) {
     for (int at = w0; at < w1; at += 32 * E) {   // all on their way at once
       if (sl.vec && at + E <= sl.have) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(kept + at)), "l"(sl.row + at) : "memory");
       } else {
-        float z[E];
-        sl.global(at, z);
-#pragma unroll
-        for (int e = 0; e < E; ++e) kept[at + e] = (T)z[e];
+        *reinterpret_cast<uint4*>(kept + at) = sl.global(at);
       }
     }
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
     sl.kept = kept;                              // (a thread reads what it has written)
   }
-  for (int at = w0; at < w1; at += 4 * 32 * E) {
-    float z[4][E];
+  float most = -INFINITY;                        // (fmaxf leaves NaN out)
+#pragma unroll 4
+  for (int at = w0; at < w1; at += 32 * E) {
+    float z[E];
+    sl.read(at, z);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (at + i * 32 * E < w1) sl.read(at + i * 32 * E, z[i]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (at + i * 32 * E < w1)
-#pragma unroll
-        for (int e = 0; e < E; ++e) top = max(top, key_of(z[i][e]));
+    for (int e = 0; e < E; ++e) most = fmaxf(most, z[e]);
   }
+  uint32_t top = key_of(most);
 #pragma unroll
   for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((lane & 15) == 0) S.warp_cnt[2 * warp + (lane >> 4)] = top;
@@ -280,14 +280,27 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   bool counted = false;                          // the histogram has been used
   // kept: key > cut, or key == cut and one of the first `ties` tokens of that key
   uint32_t cut = 1u, ties = 0xffffffffu, equals = 0;
-  // each element of the slice, as f(index in the slice, logit, key)
-  const auto each = [&](auto&& f) {
-    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
-      float z[E];
-      sl.read(at, z);
-#pragma unroll
-      for (int e = 0; e < E; ++e) f(at + e, z[e], key_of(z[e]));
+  // The slice's elements, as f(index in the slice, H logits): two words of four at a time,
+  // as with few rows most of the time goes into fetching instructions, which a loop saves
+  constexpr int H = Slice<T, E>::H;
+  const auto halves = [&](auto&& f) {
+#pragma unroll 1
+    for (int at = w0; at < w1; at += 32 * E) {
+      uint4 v = sl.raw(at);
+#pragma unroll 1
+      for (int h = 0; h < E; h += H) {
+        float z[H];
+        Slice<T, E>::half(v.x, v.y, z);
+        f(at + h, z);
+        v.x = v.z, v.y = v.w;
+      }
     }
+  };
+  const auto each = [&](auto&& f) {
+    halves([&](int at, const float (&z)[H]) {
+#pragma unroll
+      for (int e = 0; e < H; ++e) f(at + e, z[e]);
+    });
   };
   const auto clear = [&] {
     for (int i = tid; i < kBins; i += kThreads) S.lo[i] = S.hi[i] = 0;
@@ -295,25 +308,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     __syncthreads();
   };
 
-  // Tokens that `in` holds for (logit, key) into every CTA's list, in any order; their number
+  // Tokens that `in` holds for into every CTA's list, in any order; their number
   const auto gather = [&](auto&& in) {
     if (counted) cl.sync();                      // nobody reads `tot` any more
     // this CTA's own first (on the histogram), then every CTA's behind those of the CTAs before it
     uint64_t* own = reinterpret_cast<uint64_t*>(S.lo);
     if (tid == 0) S.n_own = 0;
     __syncthreads();
-    for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
-      float z[E];
-      sl.read(at, z);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t k = key_of(z[e]);
-        if (k && in(z[e], k)) {
-          const uint32_t place = atomicAdd(&S.n_own, 1u);
-          if (place < kList) own[place] = (uint64_t)~k << 32 | (uint32_t)(first + at + e);
-        }
+    each([&](int i, float z) {
+      if (z > -INFINITY && in(z)) {
+        const uint32_t place = atomicAdd(&S.n_own, 1u);
+        if (place < kList) own[place] = (uint64_t)~key_of(z) << 32 | (uint32_t)(first + i);
       }
-    }
+    });
     __syncthreads();
     if (tid < C) cl.map_shared_rank(&S, tid)->cta_cnt[rank] = S.n_own;
     cl.sync();
@@ -332,32 +339,82 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   };
   // The list's n tokens in descending order (lowest index first among equals), and the weights'
   // running sums in `cums` (on the histogram)
-  uint64_t* sorted = reinterpret_cast<uint64_t*>(S.lo);
-  uint64_t* cums = S.list;
+  uint64_t* sorted = S.list;
+  uint64_t* cums = reinterpret_cast<uint64_t*>(S.lo);
   const auto sort = [&](int n) {
     constexpr int PER = kList / kThreads;
-    // Each one's place is the number before it.  A long list is shared out to the CTAs: eight
-    // threads count for one token.
-    const bool alone = n <= 128 || C == 1;
-    const int from = alone ? 0 : n * rank / C, to = alone ? n : n * (rank + 1) / C;
-    for (int i0 = from; i0 < to; i0 += kThreads / 8) {
-      const int i = i0 + tid / 8;
-      const uint64_t v = i < to ? S.list[i] : 0;
+    if (n <= 128) {
+      // each one's place is the number before it
+      const uint64_t v = tid < n ? S.list[tid] : ~0ull;
       int place = 0;
 #pragma unroll 4
-      for (int j = tid & 7; j < n; j += 8) place += S.list[j] < v;
-      place += __shfl_xor_sync(0xffffffffu, place, 1);
-      place += __shfl_xor_sync(0xffffffffu, place, 2);
-      place += __shfl_xor_sync(0xffffffffu, place, 4);
-      if (i < to) {
-        if (alone) {
-          if ((tid & 7) == 0) sorted[place] = v;
-        } else if ((tid & 7) < C) {
-          reinterpret_cast<uint64_t*>(cl.map_shared_rank(&S, tid & 7)->lo)[place] = v;
+      for (int j = 0; j < n; ++j) place += S.list[j] < v;
+      __syncthreads();
+      if (tid < n) sorted[place] = v;
+    } else {
+      // By buckets between the largest logit and the list's least (monotone), then by place
+      // within the bucket.  (1,100 tokens: comparing all with all takes 20 us, a bitonic
+      // network 17; it is what remains for many equal ones.)
+      uint64_t* dealt = reinterpret_cast<uint64_t*>(S.lo);
+      uint32_t far = 0;                          // ~key
+      for (int i = tid; i < n; i += kThreads) far = max(far, (uint32_t)(S.list[i] >> 32));
+      far = __reduce_max_sync(0xffffffffu, far);
+      if (lane == 0) S.warp_cnt[warp] = far;
+      for (int i = tid; i <= kBins; i += kThreads) S.bucket[i] = 0;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w) far = max(far, S.warp_cnt[w]);
+      const float t = value_of(top), step = (float)(kBins - 1) / (t - value_of(~far));
+      const auto of = [&](uint64_t v) { return min(kBins - 1, (int)((t - value_of(~(uint32_t)(v >> 32))) * step)); };
+      for (int i = tid; i < n; i += kThreads) atomicAdd(&S.bucket[of(S.list[i])], 1u);
+      __syncthreads();
+      constexpr int EACH = kBins / kThreads;
+      uint32_t c[EACH], own = 0, crowd = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) c[i] = S.bucket[tid * EACH + i], own += c[i], crowd = max(crowd, c[i]);
+      uint32_t incl = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) S.warp_cnt[warp] = incl;
+      const bool crowded = __syncthreads_or(crowd > 64);
+      uint32_t run = incl - own;
+      for (int w = 0; w < warp; ++w) run += S.warp_cnt[w];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) S.bucket[tid * EACH + i] = run, run += c[i];
+      __syncthreads();
+      if (!crowded) {
+        // (a bucket's entry becomes its end, which is the next one's start)
+        for (int i = tid; i < n; i += kThreads) {
+          const uint64_t v = S.list[i];
+          dealt[atomicAdd(&S.bucket[of(v)], 1u)] = v;
         }
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+          const uint64_t v = dealt[i];
+          const int b = of(v), from = b ? (int)S.bucket[b - 1] : 0, to = (int)S.bucket[b];
+          int place = from;
+          for (int j = from; j < to; ++j) place += dealt[j] < v;
+          sorted[place] = v;
+        }
+      } else {
+        int m = 256;
+        while (m < n) m *= 2;
+        for (int i = n + tid; i < m; i += kThreads) sorted[i] = ~0ull;
+#pragma unroll 1
+        for (int size = 2; size <= m; size *= 2)
+#pragma unroll 1
+          for (int d = size / 2; d; d /= 2) {
+            __syncthreads();
+            for (int x = tid; x < m / 2; x += kThreads) {
+              const int i = 2 * x - (x & (d - 1)), j = i + d;
+              const uint64_t p = sorted[i], q = sorted[j];
+              if ((p > q) == ((i & size) == 0)) sorted[i] = q, sorted[j] = p;
+            }
+          }
       }
     }
-    if (!alone) cl.sync();
     __syncthreads();
     uint64_t w[PER], own = 0;
 #pragma unroll
@@ -437,11 +494,19 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   if (top == 0) {
     cut = 0xffffffffu, ties = 0, done = true;    // nothing is left of the row
   } else if (greedy || top_k == 1) {
-    cut = top, ties = 1;
+    const float best = value_of(top);
+    const uint32_t n = gather([=](float z) { return z == best; });
+    if (n <= kList) {
+      sort((int)n);
+      keep_first(1);
+      n_kept = 1;
+    } else {
+      cut = top, ties = 1;
+    }
+  } else if (a.vocab <= kList) {
+    by_list([](float) { return true; });
   } else {
-    if (a.vocab <= kList) {
-      by_list([](float, uint32_t) { return true; });
-    } else if (k_on && top_k <= parts / 4 * 3) {
+    if (k_on && top_k <= parts / 4 * 3) {
       // At least top_k tokens are as large as the top_k-th largest of the half warps'
       // largest, and not many more (1.4 times top_k at half their number).
       for (int i = tid; i < parts; i += kThreads) {
@@ -456,33 +521,43 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         if (before == top_k - 1) S.floor_key = mine;
       }
       __syncthreads();
-      const uint32_t from = S.floor_key;
-      by_list([=](float, uint32_t k) { return k >= from; });
-    } else if (k_on) {
+      // (none, where a mask leaves most of them nothing)
+      const float from = value_of(S.floor_key);
+      if (S.floor_key) by_list([=](float z) { return z >= from; });
+    }
+    if (!done && k_on) {
       clear();
-      each([&](int, float z, uint32_t k) {
-        if (k) atomicAdd(&S.lo[bin(z)], 1u);
+      each([&](int, float z) {
+        if (z > -INFINITY) atomicAdd(&S.lo[bin(z)], 1u);
       });
       if (tid == 0) S.found = 0u, S.found_before = S.found_here = 0;      // fewer tokens than top_k: all
       total_of<kThreads>(S, cl, C, rank, true);
       digit_of<kThreads>(S, (uint64_t)top_k);
       const int from = (int)S.found;
-      if (S.found_before + S.found_here <= kList) by_list([&](float z, uint32_t) { return bin(z) >= from; });
-    } else if (top_p < 1.0f) {
+      if (S.found_before + S.found_here <= kList) by_list([&](float z) { return bin(z) >= from; });
+    } else if (!done && top_p < 1.0f) {
       clear();
-      each([&](int, float z, uint32_t k) {
-        if (k) {
-          const uint64_t w = wt.units(z);
-          const int b = bin(z);
-          if (w) add64(&S.lo[b], &S.hi[b], w);
-        }
+      halves([&](int, const float (&z)[H]) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < H; ++e) any |= z[e] > -INFINITY;
+        if (!__any_sync(0xffffffffu, any)) return;
+        uint64_t w[H];
+#pragma unroll
+        for (int e = 0; e < H; ++e) w[e] = wt.units(z[e]);
+#pragma unroll
+        for (int e = 0; e < H; ++e)
+          if (z[e] > -INFINITY && w[e]) {
+            const int b = bin(z[e]);
+            add64(&S.lo[b], &S.hi[b], w[e]);
+          }
       });
       total_of<kThreads>(S, cl, C, rank, false);
       const uint64_t want = share_of(total_weight());
       digit_of<kThreads>(S, want);
       const int at = (int)S.found;
       const uint64_t left = want - S.found_before;
-      const uint32_t n = gather([&](float z, uint32_t) { return bin(z) == at; });
+      const uint32_t n = gather([&](float z) { return bin(z) == at; });
       if (n <= kList) {
         sort((int)n);
         keep_first(max(1, count_below((int)n, left)));
@@ -497,7 +572,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       for (int level = 0; level < 3 && !all; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
-        each([&](int, float, uint32_t k) {
+        each([&](int, float z) {
+          const uint32_t k = key_of(z);
           if (k && (level == 0 || k >> (shift + bits) == prefix)) atomicAdd(&S.lo[(k >> shift) & ((1u << bits) - 1)], 1u);
         });
         if (tid == 0) S.found = 0xffffffffu;
@@ -522,7 +598,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       for (int level = 0; level < 3; ++level) {
         const int shift = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
         clear();
-        each([&](int, float z, uint32_t k) {
+        each([&](int, float z) {
+          const uint32_t k = key_of(z);
           if (k >= floor_key && (level == 0 || k >> (shift + bits) == prefix)) {
             const uint64_t w = wt.units(z);
             const uint32_t b = (k >> shift) & ((1u << bits) - 1);
@@ -550,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   // ---- the index behind which tokens of the cutoff's key are left out ----
   if (!done && ties != 0xffffffffu) {
     uint32_t n = 0;
-    each([&](int, float, uint32_t k) { n += k == cut; });
+    const float cut_z = value_of(cut);
+    each([&](int, float z) { n += z == cut_z; });
     n = __reduce_add_sync(0xffffffffu, n);
     if (lane == 0) S.warp_cnt[warp] = n;
     __syncthreads();
@@ -593,13 +671,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       last = S.last;
     }
   }
-  const auto is_kept = [&](int i, uint32_t k) { return k > cut || (k == cut && ties && first + i <= last); };
+  // by the values: above the cutoff, or equal to it and not behind `last` (without a cutoff above -inf)
+  const float cut_at = cut == 0xffffffffu ? INFINITY : cut == 1u ? -INFINITY : value_of(cut);
+  const int cut_last = ties && cut != 1u && cut != 0xffffffffu ? (last == 0x7fffffff ? last : last - first) : -1;
+  const auto is_kept = [&](int i, float z) { return z > cut_at || (z == cut_at && i <= cut_last); };
   // a greedy row has one token, of weight 1
   const double least = (double)min_p * Weight::kOne;
   const auto weight = [&](float z) -> double {
-    if (greedy) return Weight::kOne;
     const double e = wt.e(z);
-    return e >= least ? e : 0.0;
+    return greedy ? Weight::kOne : e >= least ? e : 0.0;
   };
   const auto put_probs = [&](uint64_t total) {
     const double inv = total ? 1.0 / (double)total : 0.0;
@@ -609,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
       float z[E], p[E];
       sl.read(at, z);
 #pragma unroll
-      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, key_of(z[e])) ? (float)(weight(z[e]) * inv) : 0.0f;
+      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, z[e]) ? (float)(weight(z[e]) * inv) : 0.0f;
       if (ov && at + E <= sl.have) {
 #pragma unroll
         for (int e = 0; e < E; e += 4)
@@ -653,8 +733,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 
   // ---- the kept sum ----
   uint64_t sum = 0;
-  each([&](int i, float z, uint32_t k) {
-    if (is_kept(i, k)) sum += Weight::whole(weight(z));
+  halves([&](int at, const float (&z)[H]) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < H; ++e) any |= is_kept(at + e, z[e]);
+    if (!__any_sync(0xffffffffu, any)) return;
+    uint64_t w[H];
+#pragma unroll
+    for (int e = 0; e < H; ++e) w[e] = Weight::whole(weight(z[e]));
+#pragma unroll
+    for (int e = 0; e < H; ++e) sum += is_kept(at + e, z[e]) ? w[e] : 0;
   });
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -690,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
         uint64_t w[E], own = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          w[e] = is_kept(at + e, key_of(z[e])) ? Weight::whole(weight(z[e])) : 0;
+          w[e] = is_kept(at + e, z[e]) ? Weight::whole(weight(z[e])) : 0;
           own += w[e];
         }
         uint64_t incl = own;

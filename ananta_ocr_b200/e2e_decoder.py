@@ -31,6 +31,11 @@ GPU: a token without a page (the pool is empty, the row is full) or a malformed
 tree is recorded in ``errors``.  A draft without a page is passed over, as if it
 had not been drafted.  A row whose next token has no page stays as long as its
 pages allow and its tokens mean nothing from there on; other rows are not touched.
+
+With ``fused_steps`` the steps take the residual sums with their norms and the MoE
+layers as kernels of this library (norms.py, moe.py: only the picked experts are
+read, gate scores are not rounded to bf16 as the default's are).  ``decode_step`` and
+``draft_step`` can draw tokens with top-k, top-p and min-p (sampling.py).
 """
 from __future__ import annotations
 
@@ -41,7 +46,7 @@ from typing import List, Optional, Sequence
 import torch
 import torch.nn.functional as F
 
-from . import drafts
+from . import drafts, moe, norms, sampling
 from .ops import DeviceErrorWord
 from .page_pool import CacheLayers, PagePool, copy_pages
 from .unlimited_dash_ops import attend_triton as AT
@@ -91,10 +96,11 @@ def rmsnorm(x, w, eps):
 class DashDecoder:
     """Random-init bf16 decoder with paged caches for ``batch`` sequences of
     up to ``max_len`` tokens.  ``pool_pages``: that many pages shared by the
-    sequences through a page pool (default: a fixed set for each)."""
+    sequences through a page pool (default: a fixed set for each).  ``fused_steps``:
+    decode and draft steps of up to 256 tokens with fused norms and MoE layers."""
 
     def __init__(self, cfg: DecoderConfig, batch: int, max_len: int, device, seed: int = 0,
-                 page_cfg=None, page_mask: bool = False, pool_pages: int = 0):
+                 page_cfg=None, page_mask: bool = False, pool_pages: int = 0, fused_steps: bool = False):
         self.cfg = c = cfg
         self.B = batch
         self.dev = device
@@ -128,7 +134,10 @@ class DashDecoder:
                 sf = c.shared * c.moe_ffn
                 L["sh_gu"] = rnd(2 * sf, H, std=1.0 / math.sqrt(H))
                 L["sh_d"] = rnd(H, sf, std=1.0 / math.sqrt(sf))
+            if fused_steps and "gate" in L:
+                L["moe"] = moe.MoeWeights(L["gate"], L["exp_gu"], L["exp_d"], L["sh_gu"], L["sh_d"])
             self.layers.append(L)
+        self.fused_steps = fused_steps
         # paged caches: one block of block_size tokens per page, random block table
         bs = c.block_size
         self.pps = -(-max_len // bs)
@@ -225,6 +234,26 @@ class DashDecoder:
         out += (y * gates.t()[:, None, :]).sum(0).t()
         return out.to(h.dtype)
 
+    def _step_norm(self, x, w):
+        """The norm before the first layer of a decode or draft step."""
+        return (norms.rms_norm if self.fused_steps else rmsnorm)(x, w, self.cfg.eps)
+
+    def _step_layer(self, li, x, attn):
+        """What a decode or draft step does between a layer's attention and the next
+        layer's: (x, the normed rows that the next layer, or the LM head, takes)."""
+        c, L = self.cfg, self.layers[li]
+        after = self.layers[li + 1]["ln1"] if li + 1 < c.layers else self.final_norm
+        out = F.linear(attn, L["wo"])
+        if not self.fused_steps:
+            x = x + out
+            x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
+            return x, rmsnorm(x, after, c.eps)
+        x, h = norms.add_rms_norm(out, x, L["ln2"], c.eps)
+        if "moe" in L and h.shape[0] <= moe.MAX_TOKENS:
+            x = moe.moe_layer(h, L["moe"], c.topk, residual=x, device_error=self.errors).out
+            return x, norms.rms_norm(x, after, c.eps)
+        return norms.add_rms_norm(self.ffn_decode(L, h), x, after, c.eps)
+
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
     def prefill(self, embeds: torch.Tensor, attn_events=None, token_ids=None, gen_start=None):
@@ -309,10 +338,13 @@ class DashDecoder:
 
     # ---------------------------------------------------------------- decode
     @torch.no_grad()
-    def decode_step(self):
+    def decode_step(self, u: Optional[torch.Tensor] = None, *, temperature: sampling.Setting = 1.0, top_k=0,
+                    top_p: sampling.Setting = 1.0, min_p: sampling.Setting = 0.0):
         """One token per sequence: ``self.tok`` at position ``self.seq_lens``;
-        returns logits [B, vocab], writes the greedy next token into
-        ``self.tok`` and advances ``self.seq_lens``."""
+        returns logits [B, vocab], writes the next token into ``self.tok`` and
+        advances ``self.seq_lens``.  The next token is the greedy one, or with
+        random numbers ``u`` [B] drawn as ``sampling.sample`` draws it (a setting can
+        be one number or one per sequence)."""
         c = self.cfg
         B, H = self.B, c.hidden
         dev = self.tok.device
@@ -340,8 +372,8 @@ class DashDecoder:
                                               q_page=q_page, seq_lens=sl, max_block=self.pps,
                                               num_blocks=self.num_pages, block_size=c.block_size)
                 domain = None
+        h = self._step_norm(x, self.layers[0]["ln1"])
         for li, L in enumerate(self.layers):
-            h = rmsnorm(x, L["ln1"], c.eps)
             qkv = F.linear(h, L["wqkv"])
             q, k, v = qkv[:, :H], qkv[:, H:2 * H], qkv[:, 2 * H:]
             IF.rope_and_store_kv(q, k, v, cos, sin, self.kc[li], self.vc[li], slots, c.head_dim)
@@ -363,10 +395,13 @@ class DashDecoder:
                                        sl, c.kv_heads, 1.0 / math.sqrt(c.head_dim), self.attn_out, 1,
                                        local_blocks=c.local_blocks, sparse_block_size=c.block_size,
                                        workspace=self.dec_ws)
-            x = x + F.linear(self.attn_out.view(B, H), L["wo"])
-            x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
-        logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
-        self.tok.copy_(logits.argmax(-1))
+            x, h = self._step_layer(li, x, self.attn_out.view(B, H))
+        logits = F.linear(h, self.lm_head)
+        if u is None:
+            self.tok.copy_(logits.argmax(-1))
+        else:
+            drawn = sampling.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            self.tok.copy_(drawn.clamp_(min=0))                         # (-1: logits that are no numbers)
         self.seq_lens.copy_(sl)
         return logits
 
@@ -374,7 +409,8 @@ class DashDecoder:
     @torch.no_grad()
     def draft_step(self, drafted: torch.Tensor, parents: Optional[torch.Tensor] = None, *,
                    temperature: float = 0.0, draft_probs: Optional[torch.Tensor] = None,
-                   u_accept: Optional[torch.Tensor] = None, u_sample: Optional[torch.Tensor] = None):
+                   u_accept: Optional[torch.Tensor] = None, u_sample: Optional[torch.Tensor] = None,
+                   top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
         """Checks drafted tokens [B, n - 1] (int64) behind ``self.tok`` at once.
 
         With the root ``self.tok`` as token 0, ``parents`` [B, n] int32 gives each
@@ -382,7 +418,8 @@ class DashDecoder:
         decoding would have chosen; otherwise the drafts are accepted against the
         softmax of logits / temperature with the random numbers ``u_accept`` [B * n]
         and ``u_sample`` [B] (``draft_probs`` [B * n, vocab]: the distributions that the
-        drafts were drawn from).  The kept tokens' cache entries are moved
+        drafts were drawn from; ``top_k``, ``top_p``, ``min_p``: the target is what
+        ``sampling.probs`` keeps of the softmax).  The kept tokens' cache entries are moved
         together, the k-bar rows of their pages refreshed, ``self.seq_lens``
         advanced by the kept tokens and the root, and ``self.tok`` becomes the
         next token.  A draft without a page (the row is full, the pool is empty) or
@@ -425,8 +462,8 @@ class DashDecoder:
         oi = torch.empty(T, c.slots, dtype=torch.int32, device=dev)
         ob = torch.empty(T, c.slots, dtype=torch.float32, device=dev)
         attn = torch.empty(T, c.heads, c.head_dim, dtype=torch.bfloat16, device=dev)
+        h = self._step_norm(x, self.layers[0]["ln1"])
         for li, L in enumerate(self.layers):
-            h = rmsnorm(x, L["ln1"], c.eps)
             qkv = F.linear(h, L["wqkv"])
             q, k, v = qkv[:, :H], qkv[:, H:2 * H], qkv[:, 2 * H:]
             IF.rope_and_store_kv(q, k, v, cos, sin, self.kc[li], self.vc[li], plan.slots, c.head_dim)
@@ -443,13 +480,15 @@ class DashDecoder:
                                          plan.row_pos, plan.mask, n, c.kv_heads, 1.0 / math.sqrt(c.head_dim), attn,
                                          local_blocks=c.local_blocks, sparse_block_size=c.block_size,
                                          device_error=self.errors)
-            x = x + F.linear(attn.view(T, H), L["wo"])
-            x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
-        logits = F.linear(rmsnorm(x, self.final_norm, c.eps), self.lm_head)
+            x, h = self._step_layer(li, x, attn.view(T, H))
+        logits = F.linear(h, self.lm_head)
         # a draft whose keys could not be stored is passed over
         tokens = tokens.masked_fill(plan.slots < 0, -1)
         if temperature > 0:
-            target = (logits.float() / temperature).softmax(-1)
+            if top_k > 0 or top_p < 1 or min_p > 0:
+                target = sampling.probs(logits, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            else:
+                target = (logits.float() / temperature).softmax(-1)
             kept = drafts.verify_drafts(tokens, parents, cu, target, max_nodes=n, draft=draft_probs,
                                         u_accept=u_accept, u_sample=u_sample, device_error=self.errors)
         else:

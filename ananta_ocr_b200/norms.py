@@ -72,86 +72,99 @@ def add_rms_norm_backward(dstream: Optional[torch.Tensor], dnormed: torch.Tensor
     return NormGrads(*_backward(dstream, dnormed, y, residual, weight, gate, post_weight, eps, scale))
 
 
-def _rows(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> torch.Tensor:
+def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
     """[rows, hidden] with a unit inner stride."""
-    if like is not None and (t.shape != like.shape or t.dtype is not like.dtype or t.device != like.device):
+    if t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device():
         _need_cuda(t)
         raise ValueError(f"{name} must be {tuple(like.shape)} {like.dtype} on {like.device}")
-    if t.dim() != 2:
+    if t.ndim != 2:
         t = t.reshape(-1, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _weight(w: Optional[torch.Tensor], name: str, y: torch.Tensor, shape) -> Tuple[Optional[torch.Tensor], int, int]:
-    """The tensor, its address and whether it is fp32."""
-    if w is None:
-        return None, 0, 0
-    if w.shape != shape or (w.dtype is not torch.float32 and w.dtype is not y.dtype) or w.device != y.device:
+def _weight(w: torch.Tensor, name: str, y: torch.Tensor, shape) -> torch.Tensor:
+    if w.shape != shape or (w.dtype is not torch.float32 and w.dtype is not y.dtype) or w.get_device() != y.get_device():
         _need_cuda(w)
         raise ValueError(f"{name} must be {tuple(shape)} in fp32 or {y.dtype} on {y.device}")
-    if w.stride(-1) != 1:
-        w = w.contiguous()
-    return w, w.data_ptr(), 1 if w.dtype is torch.float32 else 0
+    return w if w.stride(-1) == 1 else w.contiguous()
 
 
-def _inputs(y, residual, weight, gate, post):
-    """Checked rows and weights: (y2, residual2, w, p, g, rows, hidden, group_rows)."""
-    _need_cuda(y)
-    if y.dtype not in _DT or y.dim() < 1:
+def _fields(y, residual, weight, gate, post, eps, scale, stream=0, normed=0):
+    """(tensors to be kept alive, the fields of DashNormArgs in order)."""
+    shape, dt = y.shape, y.dtype
+    if y.get_device() < 0 or dt not in _DT or not shape:
+        _need_cuda(y)
         raise ValueError("y must be [..., hidden] in fp32, bf16 or fp16")
-    hidden = y.shape[-1]
-    y2 = _rows(y, "y")
-    r2 = None if residual is None else _rows(residual, "residual", y)
-    rows = y2.shape[0]
-    w, p = _weight(weight, "weight", y, (hidden,)), _weight(post, "post_weight", y, (hidden,))
-    if gate is not None and gate.dim() not in (1, 2):
-        raise ValueError("gate must be [hidden] or [groups, hidden]")
-    groups = 1 if gate is None or gate.dim() == 1 else gate.shape[0]
-    g = _weight(gate, "gate", y, (hidden,) if gate is None or gate.dim() == 1 else (groups, hidden))
-    if rows and (groups == 0 or rows % groups):
-        raise ValueError(f"{rows} rows do not divide into {groups} groups")
-    return y2, r2, w, p, g, rows, hidden, max(1, rows // max(1, groups))
-
-
-def _values(y2, r2, w, p, g, rows, hidden, group_rows, eps, scale, stream, normed):
-    """The fields of DashNormArgs in order."""
-    return (y2.data_ptr(), y2.stride(0), 0 if r2 is None else r2.data_ptr(), 0 if r2 is None else r2.stride(0),
-            w[1], p[1], g[1], g[0].stride(0) if g[0] is not None and g[0].dim() == 2 else hidden,
-            0 if stream is None else stream.data_ptr(), hidden, 0 if normed is None else normed.data_ptr(), hidden,
-            rows, group_rows, hidden, _DT[y2.dtype], w[2], p[2], g[2], eps, scale, 0)
+    hidden = shape[-1]
+    y2 = _rows(y, "y", y)
+    rows, f32 = y2.shape[0], torch.float32
+    w = _weight(weight, "weight", y, (hidden,))
+    keep = [y2, w]
+    res = res_stride = post_at = post_f32 = gate_at = gate_f32 = 0
+    gate_stride, group = hidden, rows
+    if residual is not None:
+        r2 = _rows(residual, "residual", y)
+        keep.append(r2)
+        res, res_stride = r2.data_ptr(), r2.stride(0)
+    if post is not None:
+        p = _weight(post, "post_weight", y, (hidden,))
+        keep.append(p)
+        post_at, post_f32 = p.data_ptr(), int(p.dtype is f32)
+    if gate is not None:
+        if gate.ndim not in (1, 2):
+            raise ValueError("gate must be [hidden] or [groups, hidden]")
+        groups = 1 if gate.ndim == 1 else gate.shape[0]
+        g = _weight(gate, "gate", y, (hidden,) if gate.ndim == 1 else (groups, hidden))
+        if rows and (groups == 0 or rows % groups):
+            raise ValueError(f"{rows} rows do not divide into {groups} groups")
+        keep.append(g)
+        gate_at, gate_f32 = g.data_ptr(), int(g.dtype is f32)
+        if g.ndim == 2:
+            gate_stride, group = g.stride(0), rows // max(1, groups)
+    return keep, (y2.data_ptr(), y2.stride(0), res, res_stride, w.data_ptr(), post_at, gate_at, gate_stride, stream, hidden,
+                  normed, hidden, rows, max(1, group), hidden, _DT[dt], int(w.dtype is f32), post_f32, gate_f32, eps, scale, 0)
 
 
 def _forward(y, residual, weight, gate, post, eps, scale):
-    y2, r2, w, p, g, rows, hidden, group_rows = _inputs(y, residual, weight, gate, post)
-    stream = None if r2 is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    # (not empty_like: that keeps the strides of a part of a wider tensor)
     normed = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    if rows:
-        _call("dash_add_norm", _NORM(*_values(y2, r2, w, p, g, rows, hidden, group_rows, eps, scale, stream, normed)),
-              y.get_device())
+    stream = None if residual is None else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    keep, values = _fields(y, residual, weight, gate, post, eps, scale, 0 if stream is None else stream.data_ptr(),
+                           normed.data_ptr())
+    if values[12]:
+        _call("dash_add_norm", _NORM(*values), y.get_device())
     return stream, normed
 
 
 def _backward(dstream, dnormed, y, residual, weight, gate, post, eps, scale, need=(True,) * 5):
-    y2, r2, w, p, g, rows, hidden, group_rows = _inputs(y, residual, weight, gate, post)
-    ds = None if dstream is None else _rows(dstream, "dstream", y)
+    keep, values = _fields(y, residual, weight, gate, post, eps, scale)
     dh = _rows(dnormed, "dnormed", y)
-    empty = lambda t, on: torch.empty(t.shape, dtype=t.dtype, device=t.device) if on else None  # noqa: E731
-    dy, dr = empty(y, need[0]), empty(y, need[1] and residual is not None)
-    dw = empty(weight, need[2])
-    dg, dp = empty(gate, need[3] and gate is not None), empty(post, need[4] and post is not None)
+    ds = None if dstream is None else _rows(dstream, "dstream", y)
+    device = y.device
+    dy = torch.empty(y.shape, dtype=y.dtype, device=device) if need[0] else None
+    dr = torch.empty(y.shape, dtype=y.dtype, device=device) if need[1] and residual is not None else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=device) if need[2] else None
+    dg = torch.empty(gate.shape, dtype=gate.dtype, device=device) if need[3] and gate is not None else None
+    dp = torch.empty(post.shape, dtype=post.dtype, device=device) if need[4] and post is not None else None
+    rows, hidden = values[12], values[14]
     if not rows:
         for t in (dw, dg, dp):
             if t is not None:
                 t.zero_()
         return dy, dr, dw, dg, dp
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    values = _values(y2, r2, w, p, g, rows, hidden, group_rows, eps, scale, None, None) + (
-        at(ds), 0 if ds is None else ds.stride(0), dh.data_ptr(), dh.stride(0), at(dy), hidden, at(dr), hidden,
-        at(dw), at(dp), at(dg))
-    size = L.load().dash_add_norm_bwd_workspace_size(_BWD(*values, 0, 0))
-    ws = torch.empty(size, dtype=torch.uint8, device=y.device)
-    _call("dash_add_norm_bwd", _BWD(*values, ws.data_ptr(), size), y.get_device())
+    # the workspace depends on sizes and on which weights there are
+    key = (rows, hidden, values[13], values[15], post is None, gate is None)
+    size = _SIZES.get(key)
+    if size is None:
+        size = _SIZES[key] = L.load().dash_add_norm_bwd_workspace_size(_BWD(*values, *(0,) * 13))
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    _call("dash_add_norm_bwd", _BWD(*values, at(ds), 0 if ds is None else ds.stride(0), dh.data_ptr(), dh.stride(0), at(dy),
+                                    hidden, at(dr), hidden, at(dw), at(dp), at(dg), ws.data_ptr(), size), y.get_device())
     return dy, dr, dw, dg, dp
+
+
+_SIZES = {}
 
 
 class _AddNorm(torch.autograd.Function):

@@ -93,12 +93,12 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
         raise ValueError("residual must have x's shape, type and device")
     x = _aligned(x)
     res = None if residual is None else _aligned(residual)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    ids = torch.empty(T, topk, dtype=torch.int32, device=x.device)
-    w = torch.empty(T, topk, dtype=torch.float32, device=x.device)
+    out = x.new_empty(x.shape)
+    ids = x.new_empty((T, topk), dtype=torch.int32)
+    w = x.new_empty((T, topk), dtype=torch.float32)
     if T:
         size = weights.workspace_bytes(T, topk)
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(size, dtype=torch.uint8)
         t = weights.tensors
         _call("dash_moe", _ARGS(
             x.data_ptr(), x.stride(0), t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(),

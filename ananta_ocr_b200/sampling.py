@@ -40,7 +40,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
     if u.shape != (rows,) or u.dtype is not torch.float32 or u.get_device() != logits.get_device():
         _need_cuda(u)
         raise ValueError(f"u must be fp32 [{rows}] on {logits.device}")
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    tokens = logits.new_empty(rows, dtype=torch.int64)
     _run(logits, rows, u.contiguous(), temperature, top_k, top_p, min_p, tokens, None)
     return tokens
 
@@ -50,7 +50,7 @@ def probs(logits: torch.Tensor, *, temperature: Setting = 1.0, top_k: Union[int,
     """fp32 [rows, vocab]: the kept tokens' probabilities, 0 for the others (a row that
     keeps nothing is all 0)."""
     rows = _check(logits)
-    out = torch.empty(logits.shape, dtype=torch.float32, device=logits.device)
+    out = logits.new_empty(logits.shape, dtype=torch.float32)
     _run(logits, rows, None, temperature, top_k, top_p, min_p, None, out)
     return out
 

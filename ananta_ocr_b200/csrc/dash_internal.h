@@ -2,6 +2,7 @@
 // libdash_b200.so (error reporting, launch accounting, kernel launchers).
 #pragma once
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include "../../include/dash_b200.h"
 
@@ -10,6 +11,18 @@ namespace dash {
 int set_error(int code, const char* fmt, ...);   // stores the message, returns code
 int check_launch(const char* kernel);            // cudaGetLastError -> status
 void count_launch();
+
+// A kernel's attributes are those of a device: `set` runs once on each that a call comes from
+template <typename F>
+cudaError_t once_per_device(std::atomic<uint64_t>& done, F&& set) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  const uint64_t bit = (uint64_t)1 << (device & 63);
+  if (e != cudaSuccess || (device < 64 && (done.load(std::memory_order_acquire) & bit))) return e;
+  e = set();
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 int launch_kbar(const DashKbarArgs& a, cudaStream_t st);
 int launch_route(const DashRouteArgs& a, int64_t n_rows, cudaStream_t st);

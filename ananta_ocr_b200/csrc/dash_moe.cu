@@ -759,15 +759,16 @@ int launch_moe_t(const DashMoeArgs& a, cudaStream_t st) {
   const Buffers buf = buffers_of(a, cut);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   const int64_t picks = (int64_t)a.tokens * a.topk;
-  static const cudaError_t set = [] {
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t set = once_per_device(done, [] {
     cudaError_t e = cudaSuccess;
     for (const auto k : {moe_ffn_kernel<T, false>, moe_ffn_kernel<T, true>}) {
       if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-      // room for the next kernel's CTA beside this one's two
+      // three CTAs, this kernel's or the next one's
       if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
     return e;
-  }();
+  });
   if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "moe_ffn_kernel: %s", cudaGetErrorString(set));
   Maps up, down;
   const int64_t xs = a.tokens > 1 ? a.x_stride : a.hidden;

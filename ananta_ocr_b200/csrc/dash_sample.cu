@@ -53,8 +53,8 @@ struct alignas(16) Shared {
   uint32_t floor_key;
   double table[kTable];
   uint64_t warp_sum[kMaxWarps];
-  uint32_t warp_cnt[2 * kMaxWarps];
-  alignas(16) uint32_t top[kMaxCluster * 2 * kMaxWarps];     // each half warp's largest key
+  uint32_t warp_cnt[2 * kMaxWarps];              // (512 threads: two groups per warp, 256: four)
+  alignas(16) uint32_t top[kMaxCluster * 2 * kMaxWarps];     // the largest key of each group of lanes
   uint64_t cta_sum[kMaxCluster];
   uint32_t cta_cnt[kMaxCluster];
   uint64_t scan[kMaxWarps];
@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
     sl.kept = kept;                              // (a thread reads what it has written)
   }
+  constexpr int GROUP = kThreads / 32;           // lanes: 32 groups in a CTA
   float most = -INFINITY;                        // (fmaxf leaves NaN out)
 #pragma unroll 4
   for (int at = w0; at < w1; at += 32 * E) {
@@ -263,11 +264,11 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   uint32_t top = key_of(most);
 #pragma unroll
-  for (int o = 8; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((lane & 15) == 0) S.warp_cnt[2 * warp + (lane >> 4)] = top;
+  for (int o = GROUP / 2; o; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane % GROUP == 0) S.warp_cnt[tid / GROUP] = top;
   cl.barrier_wait(std::move(started));
   __syncthreads();
-  constexpr int OWN = 2 * kWarps;                // half warps
+  constexpr int OWN = kThreads / GROUP;
   const int parts = C * OWN;
   for (int i = tid; i < parts; i += kThreads) cl.map_shared_rank(&S, i / OWN)->top[rank * OWN + i % OWN] = S.warp_cnt[i % OWN];
   cl.sync();
@@ -507,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     by_list([](float) { return true; });
   } else {
     if (k_on && top_k <= parts / 4 * 3) {
-      // At least top_k tokens are as large as the top_k-th largest of the half warps'
-      // largest, and not many more (1.4 times top_k at half their number).
+      // At least top_k tokens are as large as the top_k-th largest of the groups' largest,
+      // and not many more (1.4 times top_k at half their number).
       for (int i = tid; i < parts; i += kThreads) {
         const uint32_t mine = S.top[i];
         int before = 0;
@@ -688,8 +689,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     for (int at = warp * chunk + lane * E; at < (warp + 1) * chunk; at += 32 * E) {
       float z[E], p[E];
       sl.read(at, z);
+      bool any = false;
 #pragma unroll
-      for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, z[e]) ? (float)(weight(z[e]) * inv) : 0.0f;
+      for (int e = 0; e < E; ++e) any |= is_kept(at + e, z[e]), p[e] = 0.0f;
+      if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) p[e] = is_kept(at + e, z[e]) ? (float)(weight(z[e]) * inv) : 0.0f;
+      }
       if (ov && at + E <= sl.have) {
 #pragma unroll
         for (int e = 0; e < E; e += 4)
@@ -802,15 +808,20 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 template <typename T, int THREADS>
 int launch_sample_t(const DashSampleArgs& a, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T), WARPS = THREADS / 32;
-  // eight CTAs per row, as far as that leaves each warp some work
+  // eight CTAs per row, as far as that leaves each warp some work and, with many rows, all of
+  // them run at once
   int C = kMaxCluster;
+  while (THREADS == 256 && C > 1 && (int64_t)a.rows * C > 4 * 148) C >>= 1;
   while (C > 1 && a.vocab <= (C / 2) * WARPS * 32 * E) C >>= 1;
   const int parts = C * WARPS;
   const int chunk = ((a.vocab + parts - 1) / parts + 32 * E - 1) / (32 * E) * (32 * E);
   const int64_t bytes = (int64_t)chunk * WARPS * sizeof(T);
   const int keep = bytes <= (THREADS == 512 ? kSliceMost : kSliceMany);
-  static const cudaError_t set = cudaFuncSetAttribute(sample_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (int)sizeof(Shared) + kSliceMost);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t set = once_per_device(done, [] {
+    return cudaFuncSetAttribute(sample_kernel<T, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)sizeof(Shared) + kSliceMost);
+  });
   if (set != cudaSuccess) return set_error(DASH_ERR_CUDA, "sample_kernel: %s", cudaGetErrorString(set));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * C);

@@ -5,10 +5,10 @@
   add_rms_norm            residual + scale * gate * (norm of) y, and its norm
   add_rms_norm_backward   the gradients of both, as a plain call
 
-``rms_norm`` and ``add_rms_norm`` can be differentiated.  To capture a backward pass
-into a CUDA graph, call ``add_rms_norm_backward``, or make sure that no graph that was
-recorded outside of the capture still holds the leaves: torch's own accumulation
-nodes belong to the stream that they were made on, and ends the process otherwise.
+``rms_norm`` and ``add_rms_norm`` can be differentiated (once).  A backward pass that is
+captured into a CUDA graph should be a call of ``add_rms_norm_backward``: torch's own
+differentiation of leaves whose accumulation nodes were made outside of the capture
+(by an earlier graph that still lives) ends the process.
 CUDA tensors only; every non-zero library status raises.
 """
 from __future__ import annotations
@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .ops import _DT, _need_cuda
@@ -180,6 +181,7 @@ class _AddNorm(torch.autograd.Function):
         return normed if residual is None else (stream, normed)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         y, residual, weight, gate, post = ctx.saved_tensors
         dstream, dnormed = (None, grads[0]) if residual is None else grads

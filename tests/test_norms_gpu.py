@@ -141,6 +141,14 @@ def test_rms_norm_gradients():
     check_grads(t, None, dh, {"y": dy, "weight": dw}, 1e-6, 1.0)
 
 
+def test_second_derivatives_are_refused():
+    t, ds, dh = make(4, 64, "fp32", grad=True)
+    h = norms.rms_norm(t["y"], t["weight"], 1e-6)
+    (dy,) = torch.autograd.grad(h.square().sum(), [t["y"]], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dy.sum().backward()
+
+
 def test_only_one_output_is_used():
     t, ds, dh = make(4, 64, "fp32", grad=True)
     s, h = norms.add_rms_norm(t["y"], t["residual"], t["weight"], 1e-6)

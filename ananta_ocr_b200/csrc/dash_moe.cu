@@ -16,6 +16,12 @@
 // works, and down's CTAs take the places of gate_up's as they end and fill their rings with
 // weights while its last tiles are under way.
 //
+// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 26.7 / 54 / 87.6 us
+// for 1 / 8 / 64 tokens, where the weights at the copy rate take 8.4 / 38.7 / 69.2.  While gate_up
+// and down stream, they read at 7.1 TB/s; the rest is the order of things.  One token, by the
+// global timer: scores 2.5 us, picks 4.1, sorted by expert in every CTA 6.4, the first
+// weights 8.2, the last 15; act to down, 18-22; the sum 24-26.
+//
 // act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
 // are far from bound by the tensor cores, and the layer's error stays the rounding of its output
 // (with one number it would be 0.0020 instead of 0.0017 of the output, bf16).
@@ -31,13 +37,18 @@ namespace dash {
 
 namespace {
 
-constexpr int kThreads = 224;               // 4 epilogue warps, weights, MMA, tokens
+// 4 epilogue warps, and one each that issues the weights' loads, the products and the tokens'
+// loads: with one warp for both kinds of loads and one CTA per SM, issuing was the limit
+// (64 tokens: 148 us; 20 us less without the tokens' loads, 17 less without products).
+constexpr int kThreads = 224;
 constexpr int kTile = 128;                  // weight rows of a tile
 constexpr int kStep = 64;                   // k elements of a stage (128 bytes)
 constexpr int kABytes = kTile * 128;
 constexpr int kMaxStages = 8;
 constexpr int kExchange = 2 * 16 * 64 * 4;  // gate_up: accumulators that change warps
-constexpr int kSmem = 75 * 1024;            // three CTAs per SM
+// Three CTAs per SM.  Two with 113 KB each are as fast at 64 tokens (89 us) and slower at 8
+// (56); prefetching stages beyond the ring into L2 was slower (104 us with 4 of them, 131 with 16).
+constexpr int kSmem = 75 * 1024;
 // Every place of every SM: with fewer CTAs than places some SMs get three and some none, as
 // they are dealt out while the kernel before is still there (131 of 148 SMs had work).
 constexpr int kCtas = 3 * 148;
@@ -661,7 +672,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
 
 // ---------------------------------------------------------------------------
 // the sum: a CTA per 128 columns of a token, its warps take the parts in turn (little code
-// and few loads one after the other: this kernel runs for a microsecond or two)
+// and few loads one after the other: 2 us; a thread for all parts of its columns took 5)
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(256) moe_combine_kernel(const DashMoeArgs a, const Cut cut, const Buffers buf) {

@@ -3,7 +3,7 @@
 //
 // A cluster of CTAs takes a row; each CTA owns a contiguous slice of the vocabulary
 // and each warp a contiguous part of the slice, so running sums follow the
-// vocabulary's order.  The slice is read once and kept in shared memory.
+// vocabulary's order.  The slice is kept in shared memory where it fits.
 //
 // The tokens in descending order, lowest index first among equals, are cut off at one
 // place by all three filters.  It is found as a key (the logit as an ordered 32-bit
@@ -17,6 +17,19 @@
 // are made in 64-bit floating point: with 10^5 tokens of shares around 10^-5, errors of a 32-bit
 // exponential alone would move the borders between tokens by a share of 10^-8 or more, which
 // picks another token in one row of a thousand.
+//
+// The radix descent is what always works; most rows do not need it.  A small top_k is cut
+// out of the tokens that reach the top_k-th largest of the groups' largest logits; a large
+// one, and a share of all tokens, out of those in one of 2,048 linear bins.  Such a list
+// (up to 2,048 tokens) lies in every CTA, is sorted there and decides alone; up to 128
+// kept tokens are drawn from it, too.
+//
+// Measured (vocabulary 129,280, CUDA graph): one row 9 us greedy, 14 with top-k 50 and top-p,
+// 15 unfiltered, 28 with top-k 1,000 or top-p 0.9 alone.  One row's time is that of code
+// that runs once (half of the stalls are for instructions) and of four to seven cluster
+// barriers of 0.8 us.  64 rows (fp32): 25 greedy, 40 unfiltered (the weights: 25 instructions
+// each, 8 of them in 64 bits), 89 with top-p 0.9 (two atomics per token besides); memory
+// takes 5.
 #include <cooperative_groups.h>
 
 #include "dash_common.cuh"

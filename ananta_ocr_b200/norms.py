@@ -55,7 +55,8 @@ def add_rms_norm(y: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, 
 
 
 class NormGrads(NamedTuple):
-    """Gradients of ``add_rms_norm``'s inputs; None where there is no such input."""
+    """Gradients of ``add_rms_norm``'s inputs; None where there is no such input.  Without
+    gate, post_weight and scale those of y and residual are one tensor."""
     y: torch.Tensor
     residual: torch.Tensor
     weight: torch.Tensor
@@ -145,17 +146,20 @@ def _backward(dstream, dnormed, y, residual, weight, gate, post, eps, scale, nee
     keep, values = _fields(y, residual, weight, gate, post, eps, scale)
     dh = _rows(dnormed, "dnormed", y)
     ds = None if dstream is None else _rows(dstream, "dstream", y)
-    dy = _new(y) if need[0] else None
-    dr = _new(y) if need[1] and residual is not None else None
+    # of a plain sum both gradients are the same, and one tensor
+    same = residual is not None and gate is None and post is None and scale == 1.0
+    dy = _new(y) if need[0] and not same else None
+    dr = _new(y) if residual is not None and (need[1] or (same and need[0])) else None
     dw = _new(weight) if need[2] else None
     dg = _new(gate) if need[3] and gate is not None else None
     dp = _new(post) if need[4] and post is not None else None
     rows, hidden = values[12], values[14]
+    out = dr if same else dy, dr, dw, dg, dp
     if not rows:
         for t in (dw, dg, dp):
             if t is not None:
                 t.zero_()
-        return dy, dr, dw, dg, dp
+        return out
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     # the workspace depends on sizes and on which weights there are
     key = (rows, hidden, values[13], values[15], post is None, gate is None)
@@ -165,7 +169,7 @@ def _backward(dstream, dnormed, y, residual, weight, gate, post, eps, scale, nee
     ws = y.new_empty(size, dtype=torch.uint8)
     _call("dash_add_norm_bwd", _BWD(*values, at(ds), 0 if ds is None else ds.stride(0), dh.data_ptr(), dh.stride(0), at(dy),
                                     hidden, at(dr), hidden, at(dw), at(dp), at(dg), ws.data_ptr(), size), y.get_device())
-    return dy, dr, dw, dg, dp
+    return out
 
 
 _SIZES = {}

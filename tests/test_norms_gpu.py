@@ -141,6 +141,18 @@ def test_rms_norm_gradients():
     check_grads(t, None, dh, {"y": dy, "weight": dw}, 1e-6, 1.0)
 
 
+def test_leaves_keep_gradients_of_their_own():
+    """The plain sum's two gradients are one tensor; the leaves' are not."""
+    t, ds, dh = make(4, 64, "fp32", grad=True)
+    for _ in range(2):
+        s, h = norms.add_rms_norm(t["y"], t["residual"], t["weight"], 1e-6)
+        torch.autograd.backward([s, h], [ds, dh])
+    t["y"].grad.zero_()
+    check_grads({**t}, ds, dh, {"residual": t["residual"].grad / 2, "weight": t["weight"].grad / 2}, 1e-6, 1.0)
+    got = norms.add_rms_norm_backward(ds, dh, t["y"].detach(), t["residual"].detach(), t["weight"].detach(), 1e-6, scale=0.5)
+    check_grads(t, ds, dh, {"y": got.y, "residual": got.residual}, 1e-6, 0.5)
+
+
 def test_second_derivatives_are_refused():
     t, ds, dh = make(4, 64, "fp32", grad=True)
     h = norms.rms_norm(t["y"], t["weight"], 1e-6)

@@ -83,12 +83,13 @@ Cut cut_of(const DashMoeArgs& a) {
     if (rows == 64 || time < best) best = time, c.rows = rows;
   }
   // parts of down's k: as long as lets the CTAs finish together (a part costs two steps
-  // more than its own)
+  // more than its own), but seven steps at least: more items than CTAs that start beside
+  // gate_up's last ones wait for places (one token: 26.8 us with parts of 4, 25.9 with 7)
   const int tiles = ceil_div(a.hidden, kTile), steps = ceil_div(a.ffn, kStep), sh = ceil_div(a.shared_ffn, kStep);
   int k = std::max(steps, 1);
   for (int n = 1; n <= steps; ++n) {
     const int len = ceil_div(steps, n);
-    if (len < std::min(4, steps)) break;
+    if (len < std::min(7, steps)) break;
     const auto time = [&](int l) {
       return std::ceil((groups * ceil_div(steps, l) + chunks * ceil_div(sh, l)) * tiles / kCtas) * (l + 2);
     };
@@ -128,7 +129,7 @@ constexpr int kRouteThreads = 256;
 // lane's share of x . gate[at ..], 8 elements per 256; U such pieces in flight
 template <typename T, bool F32, int U>
 __device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at, int n, int lane) {
-  double s = 0.0;
+  double s[4] = {};                            // (sums of 64-bit numbers take 20 cycles each)
   for (int i0 = lane * 8; i0 < n; i0 += 256 * U) {
     uint4 xv[U], gv[U], hv[F32 ? U : 1];
 #pragma unroll
@@ -150,20 +151,21 @@ __device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at
       for (int j = 0; j < 4; ++j) {
         const float2 f = unpack2(xw[j], (T*)nullptr);
         if (F32) {
-          s = fma((double)f.x, (double)__uint_as_float(gw[2 * j]), s);
-          s = fma((double)f.y, (double)__uint_as_float(gw[2 * j + 1]), s);
+          s[j] = fma((double)f.x, (double)__uint_as_float(gw[2 * j]), s[j]);
+          s[j] = fma((double)f.y, (double)__uint_as_float(gw[2 * j + 1]), s[j]);
         } else {
           // products of two 16-bit numbers are exact in fp32
           const float2 w = unpack2(gw[j], (T*)nullptr);
-          s += (double)(f.x * w.x);
-          s += (double)(f.y * w.y);
+          s[j] += (double)(f.x * w.x);
+          s[j] += (double)(f.y * w.y);
         }
       }
     }
   }
+  double sum = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return s;
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
 }
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -182,8 +184,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 template <typename T, bool F32>
 __global__ void __launch_bounds__(kRouteThreads, 4) moe_route_kernel(const DashMoeArgs a) {
   __shared__ double score[kMoeMaxExperts];
-  __shared__ double red[kRouteThreads / 32], red2[kRouteThreads / 32];
-  __shared__ double value[kRouteThreads], best[kMoeMaxTopk];
+  __shared__ double red[kRouteThreads / 32], best[kMoeMaxTopk];
   __shared__ int id[kMoeMaxTopk];
   launch_next();
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
@@ -206,42 +207,35 @@ __global__ void __launch_bounds__(kRouteThreads, 4) moe_route_kernel(const DashM
   cluster_arrive();
   cluster_wait();
   if (rank) return;
-  // a thread per expert; its place among all of them decides
-  const double mine = tid < a.experts ? score[tid] : 0.0;
-  const bool nan = mine != mine;
-  double top = tid < a.experts && !nan ? mine : -INFINITY;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
-  for (int w = 0; w < kRouteThreads / 32; ++w) top = fmax(top, red[w]);
-  // (a NaN score makes the sum NaN)
-  const double e = tid < a.experts ? (mine == top ? 1.0 : exp(mine - top)) : 0.0;
-  double sum = e;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) red2[warp] = sum;
-  // an expert's place: `share` threads count the experts before it
-  value[tid] = tid < a.experts ? e : 0.0;
-  __syncthreads();
+  // an expert's place among all decides: `share` threads count the experts before it
+  const auto value = [&](int e) { return score[e] != score[e] ? -INFINITY : score[e]; };      // NaN: the smallest
   int share = 1;
   while (share < 32 && a.experts * share * 2 <= kRouteThreads) share *= 2;
   for (int x0 = tid / share; x0 - tid / share < a.experts; x0 += kRouteThreads / share) {
     int before = 0;
     if (x0 < a.experts) {
-      const double m = score[x0] != score[x0] ? -INFINITY : score[x0];
+      const double m = value(x0);
       for (int j = tid % share; j < a.experts; j += share) {
-        const double v = score[j] != score[j] ? -INFINITY : score[j];
+        const double v = value(j);
         before += v > m || (v == m && j < x0);
       }
     }
     for (int o = 1; o < share; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-    if (x0 < a.experts && tid % share == 0 && before < a.topk) best[before] = value[x0], id[before] = x0;
+    if (x0 < a.experts && tid % share == 0 && before < a.topk) id[before] = x0;
   }
+  __syncthreads();
+  const double top = value(id[0]);
+  const auto weight = [&](int e) { return score[e] == top ? 1.0 : exp(score[e] - top); };
+  // (a NaN score makes the sum NaN)
+  double sum = tid < a.experts ? weight(tid) : 0.0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp] = sum;
+  if (tid < a.topk) best[tid] = weight(id[tid]);
   __syncthreads();
   if (tid < a.topk) {
     double total = 0.0, picked = 0.0;
-    for (int w = 0; w < kRouteThreads / 32; ++w) total += red2[w];
+    for (int w = 0; w < kRouteThreads / 32; ++w) total += red[w];
     for (int j = 0; j < a.topk; ++j) picked += best[j];
     a.ids[(int64_t)t * a.topk + tid] = id[tid];
     a.weights[(int64_t)t * a.topk + tid] = (float)(best[tid] / (a.renorm ? picked + 0.0 * total : total) * (double)a.scale);
@@ -415,12 +409,12 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   // for the first time waits for its own instructions)
 #pragma unroll 1
   for (int dry = DOWN ? 0 : 1; dry >= 0; --dry) {
+  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
+  __syncthreads();
   if (!dry) {
     if (!DOWN) wait_previous();
     launch_next();
   }
-  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
-  __syncthreads();
 
   // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
   // the same groups): a bit per token and expert ----

@@ -16,11 +16,11 @@
 // works, and down's CTAs take the places of gate_up's as they end and fill their rings with
 // weights while its last tiles are under way.
 //
-// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 26.7 / 54 / 87.6 us
+// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 25.7 / 53.5 / 87.6 us
 // for 1 / 8 / 64 tokens, where the weights at the copy rate take 8.4 / 38.7 / 69.2.  While gate_up
 // and down stream, they read at 7.1 TB/s; the rest is the order of things.  One token, by the
-// global timer: scores 2.5 us, picks 4.1, sorted by expert in every CTA 6.4, the first
-// weights 8.2, the last 15; act to down, 18-22; the sum 24-26.
+// global timer: scores 2.5 us, picks 3.8, sorted by expert in every CTA 6.4, the first
+// weights 8.2, the last 15; act to down and its products, 18-22; the sum 23-25.
 //
 // act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
 // are far from bound by the tensor cores, and the layer's error stays the rounding of its output
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   tc_fence_after();
   const uint32_t tmem = *holder;
   // (gate_up goes through the sorting once without the picks while it waits: code that runs
-  // for the first time waits for its own instructions)
+  // for the first time waits for its own instructions; one token 26.6 -> 25.7 us)
 #pragma unroll 1
   for (int dry = DOWN ? 0 : 1; dry >= 0; --dry) {
   for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;

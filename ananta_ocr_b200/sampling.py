@@ -48,8 +48,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 def probs(logits: torch.Tensor, *, temperature: Setting = 1.0, top_k: Union[int, torch.Tensor] = 0, top_p: Setting = 1.0,
           min_p: Setting = 0.0) -> torch.Tensor:
     """fp32 [rows, vocab]: the kept tokens' probabilities, 0 for the others (a row that
-    keeps nothing is all 0)."""
+    keeps nothing is all 0).  No gradients: logits that ask for them are refused."""
     rows = _check(logits)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise NotImplementedError("probs has no gradients")
     out = logits.new_empty(logits.shape, dtype=torch.float32)
     _run(logits, rows, None, temperature, top_k, top_p, min_p, None, out)
     return out

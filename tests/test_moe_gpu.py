@@ -166,6 +166,10 @@ def test_empty_and_refusals():
     t, w = make(4, 64, 32, 6, 8)
     r = moe.moe_layer(t["x"][:0], w, 2)
     assert r.out.shape == (0, 64) and r.ids.shape == (0, 2)
+    with pytest.raises(NotImplementedError):
+        moe.moe_layer(t["x"].clone().requires_grad_(), w, 2)
+    with torch.no_grad():
+        moe.moe_layer(t["x"].clone().requires_grad_(), w, 2)
     with pytest.raises(ValueError):
         moe.moe_layer(t["x"][:, :56], w, 2)
     with pytest.raises(ValueError):

@@ -192,4 +192,7 @@ def test_empty_and_refusals():
             bad()
     with pytest.raises(RuntimeError):
         sampling.probs(z.cpu())
+    with pytest.raises(NotImplementedError):
+        sampling.probs(z.clone().requires_grad_())
+    assert sampling.sample(z.clone().requires_grad_(), u).shape == (3,)
     assert len(kept(z[0].double().cpu().numpy(), 1.0, 3, 1.0, 0.0)[0]) == 3

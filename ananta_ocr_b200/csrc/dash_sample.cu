@@ -29,7 +29,7 @@
 // that runs once (half of the stalls are for instructions) and of four to seven cluster
 // barriers of 0.8 us.  64 rows (fp32): 25 greedy, 40 unfiltered (the weights: 25 instructions
 // each, 8 of them in 64 bits), 89 with top-p 0.9 (two atomics per token besides); memory
-// takes 5.
+// takes 5.  In bf16, with four CTAs per row: 14, 37 and 87, and 16 with top-k 20.
 #include <cooperative_groups.h>
 
 #include "dash_common.cuh"
@@ -49,10 +49,11 @@ constexpr int kDraw = 128;                       // of which it draws one by its
 constexpr int kTable = 256;                      // 2^(j / 256)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
-constexpr int kSliceMany = 20 * 1024;            // the same with four CTAs on an SM
+constexpr int kSliceTwo = 68 * 1024;             // the same with two CTAs on an SM
+constexpr int kSliceMany = 20 * 1024;            // with four
 // Up to so many rows a CTA has 512 threads (two on an SM, slices in shared memory), above it 256
-// (four).  64 rows of 129,280 (fp32) with settings of their own 59 us, with 256 threads 78;
-// with top-k 20 alone 36 and 22.  128 rows (bf16), top-k 50: 88 and 63.
+// (four).  64 rows of 129,280 (fp32) with settings of their own 59 us, with 256 threads 78; with
+// top-k 20 alone 37 and 30.  Distributions of 128 rows (bf16), top-k 50: 88 and 52.
 constexpr int kFewRows = 64;
 
 struct alignas(16) Shared {
@@ -821,10 +822,14 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
 template <typename T, int THREADS>
 int launch_sample_t(const DashSampleArgs& a, cudaStream_t st) {
   constexpr int E = 16 / sizeof(T), WARPS = THREADS / 32;
-  // eight CTAs per row, as far as that leaves each warp some work and, with many rows, all of
-  // them run at once
+  // Eight CTAs per row, as far as that leaves each warp some work and, with many rows, all of
+  // them run at once (of 512 threads: while two slices fit an SM.  64 rows, bf16, top-k 20: 34
+  // us with 8 CTAs, 16 with 4; in fp32, where the slices of 4 do not fit, rows of several
+  // settings 59 with 8, 79 with 4).
   int C = kMaxCluster;
-  while (THREADS == 256 && C > 1 && (int64_t)a.rows * C > 4 * 148) C >>= 1;
+  while (C > 1 && (int64_t)a.rows * C > (THREADS == 256 ? 4 : 2) * 148 &&
+         (THREADS == 256 || (int64_t)a.vocab * sizeof(T) <= (int64_t)(C / 2) * kSliceTwo))
+    C >>= 1;
   while (C > 1 && a.vocab <= (C / 2) * WARPS * 32 * E) C >>= 1;
   const int parts = C * WARPS;
   const int chunk = ((a.vocab + parts - 1) / parts + 32 * E - 1) / (32 * E) * (32 * E);

@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs
 template <int NV>
 constexpr int kAhead = NV == 1 ? 3 : 1;            // rows on their way: 128 KB of shared memory at most
 constexpr int kRingMost = 128 * 1024;
+constexpr int kRingPlain = 46 * 1024;              // without asking for more: 48 KB with the static part
 
 __device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
   uint64_t d;
@@ -856,7 +857,7 @@ int launch_fwd_e(const DashNormArgs& a, cudaStream_t st) {
       const unsigned grid = (unsigned)((a.rows + per - 1) / per);
       const size_t ring = (size_t)(nv == 1 ? kAhead<1> + 1 : kAhead<2> + 1) * 2 * nv * threads * 16;
       const auto go = [&](auto kernel) {
-        if (ring > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
+        if (ring > kRingPlain && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
           return set_error(DASH_ERR_CUDA, "add_norm_kernel: no shared memory for the ring");
         kernel<<<grid, threads, ring, st>>>(a, per);
         count_launch();
@@ -917,7 +918,7 @@ int launch_bwd_e(const DashNormBwdArgs& b, cudaStream_t st) {
   float* part_p = a.post ? part_w + (int64_t)c.ctas * a.hidden : nullptr;
   float* part_g = b.dgate && c.per_group > 1 ? part_w + (int64_t)c.ctas * a.hidden * (a.post ? 2 : 1) : nullptr;
   const auto go = [&](auto kernel, size_t ring) {
-    if (ring > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
+    if (ring > kRingPlain && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingMost) != cudaSuccess)
       return set_error(DASH_ERR_CUDA, "add_norm_bwd_kernel: no shared memory for the ring");
     kernel<<<c.ctas, c.threads, ring, st>>>(b, c.chunk, c.per_group, c.chunks, part_w, part_p, part_g);
     return (int)DASH_OK;

@@ -109,6 +109,16 @@ def test_forward_of_many_rows(hidden, groups, post, dt):
                                          scale=0.5), 1e-6, 0.5)
 
 
+@pytest.mark.parametrize("hidden,dt", [(656, "fp32"), (768, "fp32"), (1536, "bf16"), (1544, "bf16"), (2048, "fp16")])
+def test_rings_around_48_kb(hidden, dt):
+    """The fetched rows and the static part together pass the default limit of shared memory."""
+    t, ds, dh = make(5, hidden, dt, 1, True, grad=True)
+    out = norms.add_rms_norm(t["y"], t["residual"], t["weight"], 1e-5, gate=t["gate"], post_weight=t["post"])
+    check_grads(t, ds, dh, dict(zip(t, torch.autograd.grad(out, list(t.values()), [ds, dh]))), 1e-5, 1.0)
+    t, _, _ = make(16000, hidden, dt, 1, True)
+    check_forward(t, *norms.add_rms_norm(t["y"], t["residual"], t["weight"], 1e-5, gate=t["gate"], post_weight=t["post"]), 1e-5, 1.0)
+
+
 def test_gradients_against_differences():
     """Along random directions: the 64-bit definition's central difference with a step of
     1e-6 is off by 1e-9 of the values here; the gradients are fp32."""

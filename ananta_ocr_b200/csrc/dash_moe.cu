@@ -13,14 +13,16 @@
 //
 // Each kernel is launched while the one before it runs and waits for its results on the
 // GPU: gate_up's CTAs bring the shared expert's weights into L2 while the router
-// works, and down's CTAs take the places of gate_up's as they end and fill their rings with
-// weights while its last tiles are under way.
+// works, and down's CTAs take the places of gate_up's as they end.  Each waits for all of the kernel before it
+// before it reads anything: down takes the sorted picks from gate_up, which waited for the router.  (Reading
+// the router's picks while gate_up's last tiles were under way, and filling the rings with weights, took 1
+// to 2.5 us less, but nothing promises that what the kernel before last has written is visible then.)
 //
-// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 25.7 / 53.5 / 87.6 us
+// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 27.2 / 56.3 / 90.1 us
 // for 1 / 8 / 64 tokens, where the weights at the copy rate take 8.4 / 38.7 / 69.2.  While gate_up
 // and down stream, they read at 7.1 TB/s; the rest is the order of things.  One token, by the
 // global timer: scores 2.5 us, picks 3.8, sorted by expert in every CTA 6.4, the first
-// weights 8.2, the last 15; act to down and its products, 18-22; the sum 23-25.
+// weights 8.2, the last 15; then down, and the sum.
 //
 // act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
 // are far from bound by the tensor cores, and the layer's error stays the rounding of its output
@@ -63,7 +65,9 @@ struct Cut {
 };
 
 struct Buffers {                            // workspace
-  size_t act, sact, part, bytes;            // act: [2][picks by expert][ffn], both parts of the numbers
+  size_t act, sact, part;                   // act: [2][picks by expert][ffn], both parts of the numbers
+  size_t sorted;                            // the picks by expert, as they lie in shared memory (Layout)
+  size_t bytes;
 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -102,6 +106,19 @@ Cut cut_of(const DashMoeArgs& a) {
   return c;
 }
 
+// groups of up to nt picks of one expert
+__host__ __device__ constexpr int most_units(int nt, int experts, int picks) {
+  return picks < experts + picks / nt ? picks : experts + picks / nt;
+}
+// the sorted picks: each expert's start in the list (one more is the end, and behind it the number of groups), the
+// groups, the list
+__host__ __device__ constexpr int up16(int n) { return (n + 15) & ~15; }
+__host__ __device__ constexpr int base_bytes(int experts) { return up16((experts + 2) * 4); }
+__host__ __device__ constexpr int units_bytes(int nt, int experts, int picks) { return up16(most_units(nt, experts, picks) * 4); }
+__host__ __device__ constexpr int sorted_bytes(int nt, int experts, int picks) {
+  return base_bytes(experts) + units_bytes(nt, experts, picks) + up16(picks * 2);
+}
+
 Buffers buffers_of(const DashMoeArgs& a, const Cut& c) {
   Buffers b;
   size_t at = 0;
@@ -114,6 +131,7 @@ Buffers buffers_of(const DashMoeArgs& a, const Cut& c) {
   b.act = take(2 * picks * a.ffn * 2);
   b.sact = take(2 * (size_t)a.tokens * a.shared_ffn * 2);
   b.part = take((picks * c.splits + (size_t)a.tokens * c.shared_splits) * a.hidden * 4);
+  b.sorted = take(sorted_bytes(c.nt, a.experts, (int)picks));
   b.bytes = at + 256;
   return b;
 }
@@ -254,25 +272,19 @@ struct Layout {                             // dynamic shared memory behind the 
   int stage, stages, bars, exchange, base, units, list, bytes;
 };
 
-// groups of up to nt picks of one expert
-__host__ __device__ constexpr int most_units(int nt, int experts, int picks) {
-  return picks < experts + picks / nt ? picks : experts + picks / nt;
-}
-
 template <bool DOWN>
 __host__ __device__ inline Layout layout_of(int nt, int rows, int experts, int picks) {
   Layout l;
-  const auto up16 = [](int n) { return (n + 15) & ~15; };
-  const int sizes[4] = {DOWN ? 0 : kExchange, up16((experts + 1) * 4), up16(most_units(nt, experts, picks) * 4), up16(picks * 2)};
+  const int exchange = DOWN ? 0 : kExchange, sorted = sorted_bytes(nt, experts, picks);
   l.stage = (DOWN ? kABytes : 2 * rows * 128) + nt * 128 * (DOWN ? 2 : 1);
-  l.stages = (kSmem - 1024 - 512 - sizes[0] - sizes[1] - sizes[2] - sizes[3]) / l.stage;
+  l.stages = (kSmem - 1024 - 512 - exchange - sorted) / l.stage;
   if (l.stages > kMaxStages) l.stages = kMaxStages;
   l.bars = l.stages * l.stage;
   l.exchange = l.bars + 512;
-  l.base = l.exchange + sizes[0];
-  l.units = l.base + sizes[1];
-  l.list = l.units + sizes[2];
-  l.bytes = l.list + sizes[3] + 1024;
+  l.base = l.exchange + exchange;
+  l.units = l.base + base_bytes(experts);
+  l.list = l.units + units_bytes(nt, experts, picks);
+  l.bytes = l.base + sorted + 1024;
   return l;
 }
 
@@ -354,8 +366,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   uint64_t* acc_empty = acc_full + 2;                               // [2] epilogue -> MMA
   uint32_t* holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(holder + 1);
-  int* n_groups = reinterpret_cast<int*>(holder + 2);
-  int* base = reinterpret_cast<int*>(sm + lay.base);                // [experts + 1]
+  int* base = reinterpret_cast<int*>(sm + lay.base);                // [experts + 1], the number of groups
   uint32_t* units = reinterpret_cast<uint32_t*>(sm + lay.units);    // groups of picks
   uint16_t* list = reinterpret_cast<uint16_t*>(sm + lay.list);      // picks, by expert
 
@@ -379,10 +390,6 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
     tmem_alloc(holder, 2 * cols);
     tmem_relinquish();
   }
-  // (in the ring, which is not in use yet)
-  uint32_t* tokens = reinterpret_cast<uint32_t*>(sm);               // [experts][words]: who picked it
-  const int words = ceil_div(a.tokens, 32);
-  uint16_t* expert_of = reinterpret_cast<uint16_t*>(tokens + a.experts * words);
   if (tid == 32) {
     prefetch_tmap(&maps.w);
     prefetch_tmap(&maps.b);
@@ -399,64 +406,82 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"((uint32_t)n) : "memory");
     }
   }
-  // gate_up waits for the router here.  down starts when every CTA of gate_up has done so:
-  // the picks are there, act is not.
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *holder;
-  // (gate_up goes through the sorting once without the picks while it waits: code that runs
-  // for the first time waits for its own instructions; one token 26.6 -> 25.7 us)
-#pragma unroll 1
-  for (int dry = DOWN ? 0 : 1; dry >= 0; --dry) {
-  for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
-  __syncthreads();
-  if (!dry) {
-    if (!DOWN) wait_previous();
+  // Each kernel waits here for the one before it: gate_up for the router's picks, down for
+  // the sorted picks and act.  (Nothing is read before this kernel's own wait: only what the kernel
+  // directly before has written, or itself waited for and passed on, is sure to be there.)
+  uint8_t* sorted = static_cast<uint8_t*>(a.workspace) + buf.sorted;
+  const int sorted_end = sorted_bytes(cut.nt, a.experts, picks);
+  if constexpr (DOWN) {
+    wait_previous();
     launch_next();
-  }
+    for (int i = tid * 16; i < sorted_end; i += kThreads * 16)
+      *reinterpret_cast<uint4*>(sm + lay.base + i) = __ldcg(reinterpret_cast<const uint4*>(sorted + i));
+  } else {
+    // (in the ring, which is not in use yet)
+    uint32_t* tokens = reinterpret_cast<uint32_t*>(sm);               // [experts][words]: who picked it
+    const int words = ceil_div(a.tokens, 32);
+    uint16_t* expert_of = reinterpret_cast<uint16_t*>(tokens + a.experts * words);
+    // (once without the picks while it waits: code that runs for the first time waits for its own
+    // instructions; one token 26.6 -> 25.7 us)
+#pragma unroll 1
+    for (int dry = 1; dry >= 0; --dry) {
+      for (int i = tid; i < a.experts * words; i += kThreads) tokens[i] = 0;
+      __syncthreads();
+      if (!dry) {
+        wait_previous();
+        launch_next();
+      }
 
-  // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
-  // the same groups): a bit per token and expert ----
-  for (int p = tid; p < picks; p += kThreads) {
-    const int e = dry ? 0 : __ldcg(a.ids + p), t = p / a.topk;
-    expert_of[p] = (uint16_t)e;
-    atomicOr(tokens + e * words + (t >> 5), 1u << (t & 31));
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int run = 0, groups = 0;
-    for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + lane;
-      int n = 0;
-      if (e < a.experts)
-        for (int w = 0; w < words; ++w) n += __popc(tokens[e * words + w]);
-      const int own = ceil_div(n, cut.nt);
-      int both = n << 16 | own;                   // sums of both at once: picks < 2^13, groups < 2^13
+      // ---- the picks by expert, in their order (every CTA has to cut an expert's picks into
+      // the same groups): a bit per token and expert ----
+      for (int p = tid; p < picks; p += kThreads) {
+        const int e = dry ? 0 : __ldcg(a.ids + p), t = p / a.topk;
+        expert_of[p] = (uint16_t)e;
+        atomicOr(tokens + e * words + (t >> 5), 1u << (t & 31));
+      }
+      __syncthreads();
+      if (warp == 0) {
+        int run = 0, groups = 0;
+        for (int e0 = 0; e0 < a.experts; e0 += 32) {
+          const int e = e0 + lane;
+          int n = 0;
+          if (e < a.experts)
+            for (int w = 0; w < words; ++w) n += __popc(tokens[e * words + w]);
+          const int own = ceil_div(n, cut.nt);
+          int both = n << 16 | own;                   // sums of both at once: picks < 2^13, groups < 2^13
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, both, o);
-        if (lane >= o) both += y;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, both, o);
+            if (lane >= o) both += y;
+          }
+          const int at = run + (both >> 16) - n, g = groups + (both & 0xffff) - own;
+          if (e < a.experts) {
+            base[e] = at;
+            for (int i = 0; i < own; ++i) units[g + i] = (uint32_t)e << 16 | (uint32_t)(at + i * cut.nt);
+          }
+          both = __shfl_sync(0xffffffffu, both, 31);
+          run += both >> 16;
+          groups += both & 0xffff;
+        }
+        if (lane == 0) base[a.experts] = run, base[a.experts + 1] = groups;
       }
-      const int at = run + (both >> 16) - n, g = groups + (both & 0xffff) - own;
-      if (e < a.experts) {
-        base[e] = at;
-        for (int i = 0; i < own; ++i) units[g + i] = (uint32_t)e << 16 | (uint32_t)(at + i * cut.nt);
+      __syncthreads();
+      for (int p = tid; p < picks; p += kThreads) {
+        const int e = expert_of[p], t = p / a.topk;
+        int at = base[e] + __popc(tokens[e * words + (t >> 5)] & ((1u << (t & 31)) - 1));
+        for (int w = 0; w < t >> 5; ++w) at += __popc(tokens[e * words + w]);
+        list[at] = (uint16_t)p;
       }
-      both = __shfl_sync(0xffffffffu, both, 31);
-      run += both >> 16;
-      groups += both & 0xffff;
+      __syncthreads();
     }
-    if (lane == 0) base[a.experts] = run, *n_groups = groups;
-  }
-  __syncthreads();
-  for (int p = tid; p < picks; p += kThreads) {
-    const int e = expert_of[p], t = p / a.topk;
-    int at = base[e] + __popc(tokens[e * words + (t >> 5)] & ((1u << (t & 31)) - 1));
-    for (int w = 0; w < t >> 5; ++w) at += __popc(tokens[e * words + w]);
-    list[at] = (uint16_t)p;
-  }
-  __syncthreads();
+    // for down: from the first CTA, as every CTA has the same
+    if (blockIdx.x == 0)
+      for (int i = tid * 16; i < sorted_end; i += kThreads * 16)
+        *reinterpret_cast<uint4*>(sorted + i) = *reinterpret_cast<const uint4*>(sm + lay.base + i);
   }
   // the ring's next writer is the TMA unit
   fence_proxy_async_smem();
@@ -475,7 +500,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   tiles.parts = DOWN ? cut.splits : 1;
   tiles.sparts = DOWN ? max(1, cut.shared_splits) : 1;
   tiles.shared = a.shared_ffn ? ceil_div(a.tokens, cut.nt) * tiles.smt * tiles.sparts : 0;
-  tiles.total = tiles.shared + *n_groups * tiles.mt * tiles.parts;
+  tiles.total = tiles.shared + base[a.experts + 1] * tiles.mt * tiles.parts;
 
   const int a_bytes = DOWN ? kABytes : 2 * cut.rows * 128;
   if (warp == 4) {
@@ -510,8 +535,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
     int st = 0, round = 0, s = 0;
     bool ok = true;
     if (DOWN) {
-      wait_previous();                            // for act
-      asm volatile("fence.proxy.async;" ::: "memory");
+      asm volatile("fence.proxy.async;" ::: "memory");             // act is read by the TMA unit
       __syncwarp();
     }
     const bool gather = !DOWN && a.tokens > 16;
@@ -586,7 +610,6 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
     }
   } else {
     // =================== epilogue: thread = weight row = TMEM lane ===================
-    if (DOWN) wait_previous();
     float* xs = reinterpret_cast<float*>(sm + lay.exchange);        // [2][16][rows]
     T* act = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.act);
     T* sact = reinterpret_cast<T*>(static_cast<uint8_t*>(a.workspace) + buf.sact);

@@ -1,0 +1,33 @@
+"""The few-token mixture-of-experts layer where calls follow one another, in odd layouts and
+with tensors that are trained."""
+import pytest
+import torch
+
+from ananta_ocr_b200 import moe
+from test_moe_gpu import make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("tokens,experts,topk", [(1, 32, 4), (9, 32, 4), (70, 12, 3)])
+def test_picks_of_an_earlier_call_are_not_used(tokens, experts, topk):
+    """Replays in a row on one workspace, each with other picks: every kernel has to wait for those of
+    its own call."""
+    n = 24
+    t, w = make(tokens, 128, 64, experts, 32)
+    xs = torch.stack([make(tokens, 128, 64, experts, 32, seed=s)[0]["x"] for s in range(n)])
+    want = [moe.moe_layer(x, w, topk, residual=t["residual"]) for x in xs]
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r = moe.moe_layer(t["x"], w, topk, residual=t["residual"])
+    outs, ids = torch.empty_like(xs), torch.empty(n, tokens, topk, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        for i in range(n):
+            t["x"].copy_(xs[i])
+            g.replay()
+            outs[i].copy_(r.out)
+            ids[i].copy_(r.ids)
+        for i in range(n):
+            assert torch.equal(outs[i], want[i].out) and torch.equal(ids[i], want[i].ids)
+    assert not torch.equal(ids[0], ids[1])

@@ -81,10 +81,10 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     index among equals), w their softmax over all experts (``renormalize``: over the
     picked ones) times ``scale``.
 
-    x, residual [tokens, hidden] of the weights' type, at most 256 tokens; no gradients (inputs
-    that ask for them are refused).  Scores are
-    computed to 64 bits, everything else in fp32 (the FFN's inner values as the sum of two
-    numbers of the weights' type), and rounded once."""
+    x, residual [tokens, hidden] of the weights' type, at most 256 tokens; no gradients (inputs and
+    weights that ask for them are refused).  Scores are computed to 64 bits, everything
+    else in fp32 (the FFN's inner values as the sum of two numbers of the weights' type), and
+    rounded once."""
     T = x.shape[0]
     if x.dim() != 2 or x.shape[1] != weights.hidden or x.dtype is not weights.dtype or x.get_device() != weights.index:
         _need_cuda(x)
@@ -92,8 +92,10 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     if residual is not None and (residual.shape != x.shape or residual.dtype is not x.dtype or
                                  residual.get_device() != weights.index):
         raise ValueError("residual must have x's shape, type and device")
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        raise NotImplementedError("moe_layer has no gradients")
+    if torch.is_grad_enabled():
+        for v in (x, residual, *weights.tensors):
+            if v is not None and v.requires_grad:
+                raise NotImplementedError("moe_layer has no gradients")
     x = _aligned(x)
     res = None if residual is None else _aligned(residual)
     out = x.new_empty(x.shape)

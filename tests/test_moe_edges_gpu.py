@@ -31,3 +31,17 @@ def test_picks_of_an_earlier_call_are_not_used(tokens, experts, topk):
         for i in range(n):
             assert torch.equal(outs[i], want[i].out) and torch.equal(ids[i], want[i].ids)
     assert not torch.equal(ids[0], ids[1])
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_weights_that_are_trained_are_refused(which):
+    """The flag can be set after the handle was made, and taken back."""
+    t, w = make(4, 64, 32, 6, 8)
+    want = moe.moe_layer(t["x"], w, 2).out
+    w.tensors[which].requires_grad_()
+    with pytest.raises(NotImplementedError):
+        moe.moe_layer(t["x"], w, 2)
+    with torch.no_grad():
+        assert torch.equal(moe.moe_layer(t["x"], w, 2).out, want)
+    w.tensors[which].requires_grad_(False)
+    assert torch.equal(moe.moe_layer(t["x"], w, 2).out, want)

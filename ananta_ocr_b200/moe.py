@@ -119,4 +119,5 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Rows of unit inner stride that start at 16-byte boundaries."""
     if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    # (clone and contiguous keep the stride of a dimension of one)
+    return t.new_empty(t.shape).copy_(t)

@@ -45,3 +45,16 @@ def test_weights_that_are_trained_are_refused(which):
         assert torch.equal(moe.moe_layer(t["x"], w, 2).out, want)
     w.tensors[which].requires_grad_(False)
     assert torch.equal(moe.moe_layer(t["x"], w, 2).out, want)
+
+
+@pytest.mark.parametrize("at", [0, 3, 8])
+def test_one_row_of_a_wider_tensor(at):
+    """torch leaves the stride of a dimension of one as it is, also in copies."""
+    t, w = make(1, 64, 32, 6, 8)
+    want = moe.moe_layer(t["x"], w, 2, residual=t["residual"])
+    x, res = (torch.zeros(1, 83, dtype=torch.bfloat16, device="cuda")[:, at:at + 64] for _ in range(2))
+    x.copy_(t["x"]), res.copy_(t["residual"])
+    assert x.stride(0) == 83
+    for a, b in ((x, t["residual"]), (t["x"], res), (x, res)):
+        got = moe.moe_layer(a, w, 2, residual=b)
+        assert torch.equal(got.out, want.out) and torch.equal(got.ids, want.ids)

@@ -15,7 +15,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib as L
-from .ops import _DT, DeviceErrorWord, _need_cuda
+from .ops import _DT, DeviceErrorWord, _need_cuda, _no_tangents
 from .page_pool import _call
 
 MAX_TOKENS = 256                  # of a call
@@ -82,7 +82,7 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     picked ones) times ``scale``.
 
     x, residual [tokens, hidden] of the weights' type, at most 256 tokens; no gradients (inputs and
-    weights that ask for them are refused).  Scores are computed to 64 bits, everything
+    weights that ask for them, or carry tangents, are refused).  Scores are computed to 64 bits, everything
     else in fp32 (the FFN's inner values as the sum of two numbers of the weights' type), and
     rounded once."""
     T = x.shape[0]
@@ -96,6 +96,7 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
         for v in (x, residual, *weights.tensors):
             if v is not None and v.requires_grad:
                 raise NotImplementedError("moe_layer has no gradients")
+    _no_tangents("moe_layer", x, residual, *weights.tensors)
     x = _aligned(x)
     res = None if residual is None else _aligned(residual)
     out = x.new_empty(x.shape)

@@ -5,7 +5,8 @@
   add_rms_norm            residual + scale * gate * (norm of) y, and its norm
   add_rms_norm_backward   the gradients of both, as a plain call
 
-``rms_norm`` and ``add_rms_norm`` can be differentiated (once).  A backward pass that is
+``rms_norm`` and ``add_rms_norm`` can be differentiated (once, in reverse; tensors with tangents
+are refused).  A backward pass that is
 captured into a CUDA graph should be a call of ``add_rms_norm_backward``: torch's own
 differentiation of leaves whose accumulation nodes were made outside of the capture
 (by an earlier graph that still lives) ends the process.
@@ -19,7 +20,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from .ops import _DT, _need_cuda
+from .ops import _DT, _need_cuda, _no_tangents
 from .page_pool import _call
 
 _NORM = L.packer(L.DashNormArgs)
@@ -93,6 +94,7 @@ def _weight(w: torch.Tensor, name: str, y: torch.Tensor, shape) -> torch.Tensor:
 
 def _fields(y, residual, weight, gate, post, eps, scale, stream=0, normed=0):
     """(tensors to be kept alive, the fields of DashNormArgs in order)."""
+    _no_tangents("the norm", y, residual, weight, gate, post)
     shape, dt = y.shape, y.dtype
     if y.get_device() < 0 or dt not in _DT or not shape:
         _need_cuda(y)
@@ -143,6 +145,7 @@ def _forward(y, residual, weight, gate, post, eps, scale):
 
 
 def _backward(dstream, dnormed, y, residual, weight, gate, post, eps, scale, need=(True,) * 5):
+    _no_tangents("the norm", dstream, dnormed)
     keep, values = _fields(y, residual, weight, gate, post, eps, scale)
     dh = _rows(dnormed, "dnormed", y)
     ds = None if dstream is None else _rows(dstream, "dstream", y)

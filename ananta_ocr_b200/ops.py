@@ -11,6 +11,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -25,6 +26,14 @@ def _need_cuda(*ts):
     for t in ts:
         if t is not None and not t.is_cuda:
             raise RuntimeError("DASH B200 kernels need CUDA tensors (no CPU fallback)")
+
+
+def _no_tangents(what: str, *ts):
+    """Forward-mode derivatives: dual tensors do not ask for gradients, and a kernel's outputs have no tangents."""
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if torch.is_tensor(t) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivatives")
 
 
 @dataclass

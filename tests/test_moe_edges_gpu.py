@@ -2,6 +2,7 @@
 with tensors that are trained."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from ananta_ocr_b200 import moe
 from test_moe_gpu import make
@@ -58,3 +59,18 @@ def test_one_row_of_a_wider_tensor(at):
     for a, b in ((x, t["residual"]), (t["x"], res), (x, res)):
         got = moe.moe_layer(a, w, 2, residual=b)
         assert torch.equal(got.out, want.out) and torch.equal(got.ids, want.ids)
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives: dual tensors do not ask for gradients."""
+    t, w = make(4, 64, 32, 6, 8)
+    one = torch.ones_like(t["x"])
+    with fwAD.dual_level():
+        want = moe.moe_layer(t["x"], w, 2, residual=t["residual"]).out
+        for x, res in ((fwAD.make_dual(t["x"], one), t["residual"]), (t["x"], fwAD.make_dual(t["residual"], one))):
+            with pytest.raises(NotImplementedError):
+                moe.moe_layer(x, w, 2, residual=res)
+        dual = moe.MoeWeights(fwAD.make_dual(t["gate"], torch.ones_like(t["gate"])), t["gu"], t["down"])
+        with pytest.raises(NotImplementedError):
+            moe.moe_layer(t["x"], dual, 2)
+    assert torch.equal(moe.moe_layer(t["x"], w, 2, residual=t["residual"]).out, want)

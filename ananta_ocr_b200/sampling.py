@@ -48,9 +48,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 def probs(logits: torch.Tensor, *, temperature: Setting = 1.0, top_k: Union[int, torch.Tensor] = 0, top_p: Setting = 1.0,
           min_p: Setting = 0.0) -> torch.Tensor:
     """fp32 [rows, vocab]: the kept tokens' probabilities, 0 for the others (a row that
-    keeps nothing is all 0).  No gradients: logits that ask for them, or carry tangents, are refused."""
+    keeps nothing is all 0).  No gradients: logits and settings that ask for them, or
+    carry tangents, are refused."""
     rows = _check(logits)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in (logits, temperature, top_p, min_p)):
         raise NotImplementedError("probs has no gradients")
     _no_tangents("probs", logits, temperature, top_p, min_p)
     out = logits.new_empty(logits.shape, dtype=torch.float32)

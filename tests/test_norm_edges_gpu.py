@@ -1,12 +1,18 @@
-"""Residual norms and their gradients: forward-mode derivatives."""
+"""Residual norms and their gradients: streams of any size, many rows for each CTA, forward-mode
+derivatives.  Tolerances are those of test_norms_gpu."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
 from ananta_ocr_b200 import norms
-from test_norms_gpu import make
+from test_norms_gpu import check_forward, check_grads, make
 
 pytestmark = pytest.mark.gpu
+
+
+def grads_of(t, ds, dh, eps, scale=1.0):
+    g = norms.add_rms_norm_backward(ds, dh, t["y"], t["residual"], t["weight"], eps, gate=t["gate"], post_weight=t["post"], scale=scale)
+    return dict(y=g.y, residual=g.residual, weight=g.weight, gate=g.gate, post=g.post_weight)
 
 
 def test_tangents_are_refused():

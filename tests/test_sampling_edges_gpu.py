@@ -1,10 +1,11 @@
-"""Sampling: forward-mode derivatives."""
+"""Sampling of more rows than a CTA of 512 threads is taken for, whole numbers of 64 bits, forward-mode
+derivatives: against the definition as in test_sampling_gpu."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
 from ananta_ocr_b200 import sampling
-from test_sampling_gpu import logits_of
+from test_sampling_gpu import SETTINGS, columns, logits_of, same
 
 pytestmark = pytest.mark.gpu
 
@@ -18,3 +19,14 @@ def test_tangents_are_refused():
         with pytest.raises(NotImplementedError):
             sampling.probs(z, temperature=fwAD.make_dual(u, u))
         sampling.probs(z)
+
+
+def test_settings_that_ask_for_gradients_are_refused():
+    z, u = (t.cuda() for t in logits_of(3, 10, "fp32", 1))
+    s = (u + 0.5).requires_grad_()
+    for name in ("temperature", "top_p", "min_p"):
+        with pytest.raises(NotImplementedError):
+            sampling.probs(z, **{name: s})
+        with torch.no_grad():
+            assert torch.equal(sampling.probs(z, **{name: s}), sampling.probs(z, **{name: s.detach()}))
+        assert sampling.sample(z, u, **{name: s}).shape == (3,)      # tokens have no derivatives

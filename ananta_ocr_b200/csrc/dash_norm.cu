@@ -289,8 +289,10 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs
         sum[0] = two[0], sum[1] = two[1];
       }
       const float r2 = rsqrtf(sum[0] * inv + a.eps);
-      const float m = r2 * r2 * r2 * sum[1] * inv;              // ds_total = ds + r2 * a - m * s
-      const float mb = r1 * r1 * r1 * inv * (sum[2] + r2 * sum[3] - m * sum[4]);
+      // ds_total = ds + r2 * a - m * s, dy = r1 * (b - mb * yh)   (multiplied in turn: r1 and r2 to the
+      // third power leave the range of fp32 where the rows are around 2^43 or 2^-43)
+      const float m = r2 * (r2 * (r2 * sum[1]) * inv);
+      const float mb = r1 * (sum[2] + r2 * sum[3] - m * sum[4]) * inv;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int c = t * E + i * step;
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(512) add_norm_bwd_kernel(const DashNormBwdArgs
             const float dz = d[e] * f[i][e], yh = x[e] * r1;
             dg[i][e] = fmaf(d[e], a.scale * yh * p[i][e], dg[i][e]);
             dp[i][e] = fmaf(dz, yh, dp[i][e]);
-            o[e] = a.post ? fmaf(r1, dz * p[i][e], -mb * x[e]) : dz;
+            o[e] = a.post ? r1 * fmaf(-mb, yh, dz * p[i][e]) : dz;
           }
           Row<T, E> w;
           if (b.dresidual) {
@@ -597,8 +599,8 @@ __global__ void __launch_bounds__(512) add_norm_bwd_wide_kernel(const DashNormBw
       fetch(at == 0 ? AHEAD : at - 1);
       at = after;
       const float r2 = rsqrtf(v[0] * inv + a.eps);
-      const float m = r2 * r2 * r2 * v[1] * inv;                // ds_total = ds + r2 * ga - m * s
-      const float mb = r1 * r1 * r1 * inv * (v[2] + r2 * v[3] - m * v[4]);
+      const float m = r2 * (r2 * (r2 * v[1]) * inv);            // ds_total = ds + r2 * ga - m * s (in turn, as above)
+      const float mb = r1 * (v[2] + r2 * v[3] - m * v[4]) * inv;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         constexpr int I = FULL ? 1 : 0;
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(512) add_norm_bwd_wide_kernel(const DashNormBw
             const uint64_t x = Pairs<T>::get(ry[i], j), yh = fmul2(x, both(r1)), dz = fmul2(d, g[I * i][j]);
             dg[I * i][j] = ffma2(d, fmul2(yh, p[I * i][j]), dg[I * i][j]);
             dp[I * i][j] = ffma2(dz, yh, dp[I * i][j]);
-            Pairs<T>::put(oy, j, post ? ffma2(fmul2(dz, p[I * i][j]), both(r1), fmul2(x, both(-mb))) : dz);
+            Pairs<T>::put(oy, j, post ? fmul2(ffma2(yh, both(-mb), fmul2(dz, p[I * i][j])), both(r1)) : dz);
           } else {
             Pairs<T>::put(oy, j, fmul2(d, both(a.scale)));
           }

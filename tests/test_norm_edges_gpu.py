@@ -31,3 +31,17 @@ def test_tangents_are_refused():
         for ds, dh in ((dual, t["y"]), (None, dual)):
             with pytest.raises(NotImplementedError):
                 norms.add_rms_norm_backward(ds, dh, t["y"], t["residual"], t["weight"], 1e-6)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("hidden", [136, 1280, 1283, 4104, 8192])
+@pytest.mark.parametrize("power,eps", [(45, 1e-6), (52, 1e-6), (-50, 0.0)])
+def test_gradients_of_streams_of_any_size(power, eps, hidden, dt):
+    """Values around 2^45, 2^52 and 2^-50: 1 / rms to the third power is no 32-bit number there."""
+    for groups, post in ((0, False), (1, True)):
+        t, _, dh = make(5, hidden, dt, groups, post)
+        t["y"].mul_(2.0 ** power), t["residual"].mul_(1.0 if post else 2.0 ** power)
+        check_grads(t, None, dh, grads_of(t, None, dh, eps), eps, 1.0)
+        if post:
+            t["residual"].mul_(2.0 ** power)
+            check_grads(t, None, dh, grads_of(t, None, dh, eps), eps, 1.0)

@@ -144,8 +144,9 @@ __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.w
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 256;
 
-// lane's share of x . gate[at ..], 8 elements per 256; U such pieces in flight
-template <typename T, bool F32, int U>
+// lane's share of x . gate[at ..], 8 elements per 256; U such pieces in flight.  A 16-bit gate's products are
+// made in fp32, or (WIDE) in 64 bits like those of an fp32 one
+template <typename T, bool F32, int U, bool WIDE = F32>
 __device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at, int n, int lane) {
   double s[4] = {};                            // (sums of 64-bit numbers take 20 cycles each)
   for (int i0 = lane * 8; i0 < n; i0 += 256 * U) {
@@ -172,10 +173,14 @@ __device__ __forceinline__ double dot64(const T* x, const void* gate, int64_t at
           s[j] = fma((double)f.x, (double)__uint_as_float(gw[2 * j]), s[j]);
           s[j] = fma((double)f.y, (double)__uint_as_float(gw[2 * j + 1]), s[j]);
         } else {
-          // products of two 16-bit numbers are exact in fp32
           const float2 w = unpack2(gw[j], (T*)nullptr);
-          s[j] += (double)(f.x * w.x);
-          s[j] += (double)(f.y * w.y);
+          if (WIDE) {
+            s[j] = fma((double)f.x, (double)w.x, s[j]);
+            s[j] = fma((double)f.y, (double)w.y, s[j]);
+          } else {
+            s[j] += (double)(f.x * w.x);
+            s[j] += (double)(f.y * w.y);
+          }
         }
       }
     }
@@ -212,7 +217,14 @@ __global__ void __launch_bounds__(kRouteThreads, 4) moe_route_kernel(const DashM
   bool waited = false;
   for (int e = rank * 8 + warp; e - warp < a.experts; e += 8 * C) {
     double s = 0.0;
-    if (e < a.experts) s = dot64<T, F32, F32 ? 2 : 5>(x, a.gate, (int64_t)e * a.hidden, a.hidden, lane);
+    if (e < a.experts) {
+      s = dot64<T, F32, F32 ? 2 : 5>(x, a.gate, (int64_t)e * a.hidden, a.hidden, lane);
+      // Products of two 16-bit numbers have digits for fp32, but those of bf16 can leave its range: above
+      // it the sum is no number, and below 2^-126 each is off by 2^-150 at most, which a sum of 2^16
+      // products above 2^-80 does not show in 53 bits.  (All in 64 bits: 64 tokens 1.5 us more.)
+      if (!F32 && DType<T>::fmt == 1 && !(fabs(s) >= 0x1p-80 && fabs(s) < INFINITY))
+        s = dot64<T, F32, 2, true>(x, a.gate, (int64_t)e * a.hidden, a.hidden, lane);
+    }
     if (!waited) cluster_wait();                 // the first CTA has started
     waited = true;
     if (e < a.experts && lane == 0) {

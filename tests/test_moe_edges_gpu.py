@@ -5,7 +5,8 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 from ananta_ocr_b200 import moe
-from test_moe_gpu import make
+from step_testutil import moe as definition
+from test_moe_gpu import check, make
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,18 @@ def test_tangents_are_refused():
         with pytest.raises(NotImplementedError):
             moe.moe_layer(t["x"], dual, 2)
     assert torch.equal(moe.moe_layer(t["x"], w, 2, residual=t["residual"]).out, want)
+
+
+@pytest.mark.parametrize("gate", ["same", "fp32"])
+@pytest.mark.parametrize("factor,other", [(2.0 ** 70, 0.0), (2.0 ** 70, -0.5), (2.0 ** -80, 0.0)])
+def test_scores_of_products_beyond_32_bits(factor, other, gate):
+    """2^140 and 2^-160 are numbers of a 64-bit score, and 2^140 - 2^139 is 2^139."""
+    t, w = make(3, 64, 32, 6, gate=gate)
+    t["gate"].zero_()
+    t["gu"][:, :, :2] = 0                         # (of the router alone)
+    t["x"][:, 0], t["x"][:, 1] = factor, other * factor
+    for e in range(6):
+        t["gate"][e, :2] = factor * (e + 1)
+    r = moe.moe_layer(t["x"], w, 3, residual=t["residual"])
+    assert r.ids.tolist() == [[5, 4, 3]] * 3
+    check(t, r, 3)

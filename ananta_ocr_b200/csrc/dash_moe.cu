@@ -26,7 +26,9 @@
 //
 // act is kept as the sum of two 16-bit numbers, each multiplied by itself: the products
 // are far from bound by the tensor cores, and the layer's error stays the rounding of its output
-// (with one number it would be 0.0020 instead of 0.0017 of the output, bf16).
+// (with one number it would be 0.0020 instead of 0.0017 of the output, bf16).  In fp16 the second one is kept
+// 2^11 times as large: what the first leaves is at most 2^-12 of it, and below 2^-14 that type has multiples
+// of 2^-24 only.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -347,6 +349,9 @@ __device__ __forceinline__ void tmem_ld16f(uint32_t taddr, float (&r)[16]) {
       : "r"(taddr));
 }
 
+template <typename T>
+constexpr float kLow = DType<T>::fmt == 0 ? 2048.0f : 1.0f;          // of act's second numbers
+
 __device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
 
 // whether `ok` holds in all of the four epilogue warps (a barrier of theirs)
@@ -653,7 +658,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
                 const int at = it.first + c0 + c;
                 const int64_t row = it.shared ? (int64_t)picks * cut.splits + (int64_t)at * cut.shared_splits + it.part
                                               : (int64_t)list[at] * cut.splits + it.part;
-                __stcg(part + row * a.hidden + h, v[c] + v[16 + c]);
+                __stcg(part + row * a.hidden + h, fmaf(v[16 + c], 1.0f / kLow<T>, v[c]));
               }
         }
       } else {
@@ -685,7 +690,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
               const T h = (T)x;
               out[(int64_t)at * width + col] = h;
               // (beyond the type's range: infinite, and no infinity less infinity)
-              out[(rows + at) * width + col] = isinf((float)h) ? (T)0.0f : (T)(x - (float)h);
+              out[(rows + at) * width + col] = isinf((float)h) ? (T)0.0f : (T)((x - (float)h) * kLow<T>);
             }
           if (end) break;
         }

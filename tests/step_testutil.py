@@ -102,7 +102,7 @@ def distribution(z, *setting):
 # ---------------------------------------------------------------------------
 # mixture of experts
 # ---------------------------------------------------------------------------
-def moe(x, gate, gu, down, sgu, sd, topk, renorm, scale, residual, dtype):
+def moe(x, gate, gu, down, sgu, sd, topk, renorm, scale, residual, dtype, least=2.0 ** -25):
     """64-bit tensors -> (out, ids, weights, tolerance).
 
     The tolerance counts: the output's rounding; each inner product of n terms in fp32,
@@ -119,7 +119,7 @@ def moe(x, gate, gu, down, sgu, sd, topk, renorm, scale, residual, dtype):
     w = w * scale
     out = torch.zeros_like(x) if residual is None else residual.clone()
     tol = out.abs() * U * (topk + 3)
-    two = half_step(dtype) ** 2 * 2 + 2.0 ** -20
+    two = half_step(dtype) ** 2 * 2 + 2.0 ** -20            # (`least`: the inner values' smallest error)
 
     def ffn(v, g, d, weight):
         n = d.shape[1]
@@ -127,7 +127,7 @@ def moe(x, gate, gu, down, sgu, sd, topk, renorm, scale, residual, dtype):
         a, b = h[:n], h[n:]
         act = a * torch.sigmoid(a) * b
         # |d silu| <= 1.1, |silu| <= |a|
-        at = 1.1 * ht[:n] * (b.abs() + ht[n:]) + a.abs() * ht[n:] + act.abs() * two + 2.0 ** -25
+        at = 1.1 * ht[:n] * (b.abs() + ht[n:]) + a.abs() * ht[n:] + act.abs() * two + least
         mag = d.abs() @ act.abs()
         return weight * (d @ act), abs(weight) * (d.abs() @ at + mag * (n + topk + 3) * U)
 

@@ -90,3 +90,19 @@ def test_scores_of_products_beyond_32_bits(factor, other, gate):
     r = moe.moe_layer(t["x"], w, 3, residual=t["residual"])
     assert r.ids.tolist() == [[5, 4, 3]] * 3
     check(t, r, 3)
+
+
+@pytest.mark.parametrize("tokens", [2, 20])
+def test_small_inner_values(tokens):
+    """fp16: inner values around 2^-21, where that type has multiples of 2^-24.  Their second number
+    holds what the first one leaves to 2^-36 (half a step of 2^-24, kept 2^11 times as large)."""
+    t, w = make(tokens, 64, 136, 6, 40, "fp16")
+    t["gu"].mul_(2.0 ** -10), t["sgu"].mul_(2.0 ** -10)
+    t["down"].mul_(8.0), t["sd"].mul_(8.0)
+    r = moe.moe_layer(t["x"], w, 4)
+    up = {k: v.double().cpu() for k, v in t.items()}
+    out, ids, _, tol = definition(up["x"], up["gate"], up["gu"], up["down"], up["sgu"], up["sd"], 4, False, 1.0, None,
+                                  torch.float16, least=2.0 ** -36)
+    assert torch.equal(r.ids.cpu(), ids)
+    off = (r.out.double().cpu() - out).abs()
+    assert (off <= tol).all(), (off / tol).max()

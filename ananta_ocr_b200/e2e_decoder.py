@@ -134,8 +134,6 @@ class DashDecoder:
                 sf = c.shared * c.moe_ffn
                 L["sh_gu"] = rnd(2 * sf, H, std=1.0 / math.sqrt(H))
                 L["sh_d"] = rnd(H, sf, std=1.0 / math.sqrt(sf))
-            if fused_steps and "gate" in L:
-                L["moe"] = moe.MoeWeights(L["gate"], L["exp_gu"], L["exp_d"], L["sh_gu"], L["sh_d"])
             self.layers.append(L)
         self.fused_steps = fused_steps
         # paged caches: one block of block_size tokens per page, random block table
@@ -234,6 +232,15 @@ class DashDecoder:
         out += (y * gates.t()[:, None, :]).sum(0).t()
         return out.to(h.dtype)
 
+    @staticmethod
+    def _moe_weights(L):
+        """The handle of a layer's tensors, made again when one of them is another tensor."""
+        t = [L[k] for k in ("gate", "exp_gu", "exp_d", "sh_gu", "sh_d")]
+        w = L.get("moe")
+        if w is None or any(a is not b for a, b in zip(w.tensors, t)):
+            w = L["moe"] = moe.MoeWeights(*t)
+        return w
+
     def _step_norm(self, x, w):
         """The norm before the first layer of a decode or draft step."""
         return (norms.rms_norm if self.fused_steps else rmsnorm)(x, w, self.cfg.eps)
@@ -249,8 +256,8 @@ class DashDecoder:
             x = x + self.ffn_decode(L, rmsnorm(x, L["ln2"], c.eps))
             return x, rmsnorm(x, after, c.eps)
         x, h = norms.add_rms_norm(out, x, L["ln2"], c.eps)
-        if "moe" in L and h.shape[0] <= moe.MAX_TOKENS:
-            x = moe.moe_layer(h, L["moe"], c.topk, residual=x, device_error=self.errors).out
+        if "gate" in L and h.shape[0] <= moe.MAX_TOKENS:
+            x = moe.moe_layer(h, self._moe_weights(L), c.topk, residual=x, device_error=self.errors).out
             return x, norms.rms_norm(x, after, c.eps)
         return norms.add_rms_norm(self.ffn_decode(L, h), x, after, c.eps)
 

@@ -87,7 +87,8 @@ def _run(logits, rows, u, temperature, top_k, top_p, min_p, tokens, out):
     p, pa = floats(top_p, "top_p")
     m, ma = floats(min_p, "min_p")
     if torch.is_tensor(top_k):
-        keep.append(_ints(top_k, "top_k", index, rows))
+        # (64-bit numbers do not wrap: those beyond the vocabulary keep all, as they are)
+        keep.append(_ints(top_k.clamp(0, V) if top_k.dtype is torch.int64 else top_k, "top_k", index, rows))
         k, ka = keep[-1].data_ptr(), 0
     else:
         k, ka = 0, max(0, min(int(top_k), V))

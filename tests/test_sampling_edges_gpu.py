@@ -30,3 +30,11 @@ def test_settings_that_ask_for_gradients_are_refused():
         with torch.no_grad():
             assert torch.equal(sampling.probs(z, **{name: s}), sampling.probs(z, **{name: s.detach()}))
         assert sampling.sample(z, u, **{name: s}).shape == (3,)      # tokens have no derivatives
+
+
+def test_top_k_of_64_bits():
+    """Numbers beyond 32 bits are beyond the vocabulary, or below zero: all tokens."""
+    z, u = logits_of(6, 5000, "fp32", 4)
+    k = [1 << 32, (1 << 32) + 3, (1 << 40) + 17, -(1 << 32) + 5, (1 << 62), 9]
+    top_k = torch.tensor(k, dtype=torch.int64, device="cuda")
+    same(z.cuda(), u.cuda(), [(0.9, n if 0 < n < 5000 else 0, 0.9, 0.0) for n in k], temperature=0.9, top_k=top_k, top_p=0.9)

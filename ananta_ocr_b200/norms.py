@@ -168,6 +168,8 @@ def _backward(dstream, dnormed, y, residual, weight, gate, post, eps, scale, nee
     key = (rows, hidden, values[13], values[15], post is None, gate is None)
     size = _SIZES.get(key)
     if size is None:
+        if len(_SIZES) >= 1024:                   # (a training loop with other numbers of rows in each step)
+            _SIZES.clear()
         size = _SIZES[key] = L.load().dash_add_norm_bwd_workspace_size(_BWD(*values, *(0,) * 13))
     ws = y.new_empty(size, dtype=torch.uint8)
     _call("dash_add_norm_bwd", _BWD(*values, at(ds), 0 if ds is None else ds.stride(0), dh.data_ptr(), dh.stride(0), at(dy),

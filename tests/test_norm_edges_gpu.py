@@ -45,3 +45,12 @@ def test_gradients_of_streams_of_any_size(power, eps, hidden, dt):
         if post:
             t["residual"].mul_(2.0 ** power)
             check_grads(t, None, dh, grads_of(t, None, dh, eps), eps, 1.0)
+
+
+def test_many_numbers_of_rows():
+    """What is kept for a number of rows is bounded, and so is a call's workspace."""
+    y = torch.randn(2100, 8, device="cuda")
+    w = torch.ones(8, device="cuda")
+    for rows in range(1, 2100):
+        norms.add_rms_norm_backward(None, y[:rows], y[:rows], None, w, 1e-6)
+    assert len(norms._SIZES) <= 1024

@@ -106,3 +106,13 @@ def test_small_inner_values(tokens):
     assert torch.equal(r.ids.cpu(), ids)
     off = (r.out.double().cpu() - out).abs()
     assert (off <= tol).all(), (off / tol).max()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", [(256, 64, 104, 64, 16, 0), (16, 64, 248, 64, 16, 72), (256, 64, 152, 64, 16, 72), (16, 64, 296, 64, 16, 72),
+                                  (256, 64, 176, 64, 16, 72), (16, 64, 344, 64, 16, 0)])
+def test_heights_of_tiles(case, dt):
+    """gate_up's tiles of 40, 48, 56, 56, 64 and 64 rows, none of which divides the width."""
+    tokens, hidden, ffn, experts, topk, shared = case
+    t, w = make(tokens, hidden, ffn, experts, shared, dt)
+    check(t, moe.moe_layer(t["x"], w, topk, residual=t["residual"]), topk)

@@ -21,3 +21,20 @@ def test_replaced_weights_are_the_ones_that_are_read():
         x, y = a.decode_step(), b.decode_step()
         assert torch.equal(x, y) and not torch.equal(x, before), name
         a.tok.copy_(b.tok)
+
+
+@pytest.mark.parametrize("batch", [1, 2, 5])
+def test_draft_steps_are_those_of_the_plain_forms(batch, monkeypatch):
+    """As the decode steps' test, with the same roots on both sides: always compared."""
+    a, b = start(make(batch)), start(make(batch))
+    extra = torch.randint(0, 1000, (batch, 4), generator=torch.Generator().manual_seed(5)).cuda()
+    a.decode_step()
+    root = a.tok.clone()
+    got = a.draft_step(extra)[1].float()
+    monkeypatch.setattr(norms, "rms_norm", plain_norm)
+    monkeypatch.setattr(norms, "add_rms_norm", plain_add)
+    monkeypatch.setattr(moe, "moe_layer", plain_moe)
+    b.decode_step()
+    b.tok.copy_(root)
+    want = b.draft_step(extra)[1].float()
+    assert torch.isfinite(got).all() and (got - want).abs().max() <= 0.02 * want.abs().max()

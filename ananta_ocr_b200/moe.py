@@ -28,11 +28,17 @@ class MoeWeights:
     [experts, hidden, ffn], bf16 or fp16, contiguous; optionally one shared expert of its
     own width, [2 * shared_ffn, hidden] and [hidden, shared_ffn].  hidden and the widths
     are multiples of 8.  The handle keeps the tensors alive; it holds no copies, so that
-    weights updated in place are the ones that are read."""
+    weights updated in place are the ones that are read, and so is other memory that a tensor
+    was given (``.data``, a module's ``to``), which is looked over as at first."""
 
     def __init__(self, gate: torch.Tensor, gate_up: torch.Tensor, down: torch.Tensor,
                  shared_gate_up: Optional[torch.Tensor] = None, shared_down: Optional[torch.Tensor] = None):
         self.tensors = [gate, gate_up, down, shared_gate_up, shared_down]
+        self._check()
+
+    def _check(self):
+        self.seen = None
+        gate, gate_up, down, shared_gate_up, shared_down = self.tensors
         _need_cuda(*self.tensors)
         if gate_up.dim() != 3 or down.dim() != 3 or gate.dim() != 2:
             raise ValueError("gate must be [experts, hidden], gate_up [experts, 2 * ffn, hidden], down [experts, hidden, ffn]")
@@ -55,6 +61,17 @@ class MoeWeights:
         self.experts, self.hidden, self.ffn, self.shared_ffn = E, H, F, S
         self.gate_f32 = 1 if gate.dtype is torch.float32 else 0
         self._sizes = {}
+        self.seen = self._now()
+
+    def _now(self):
+        return [None if t is None else (t.data_ptr(), t.dtype) for t in self.tensors]
+
+    def addresses(self):
+        """Of the tensors as they are now (0: none)."""
+        now = self._now()
+        if now != self.seen:
+            self._check()
+        return [0 if n is None else n[0] for n in now]
 
     def workspace_bytes(self, tokens: int, topk: int) -> int:
         n = self._sizes.get((tokens, topk))
@@ -85,7 +102,7 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     weights that ask for them, or carry tangents, are refused).  Scores are computed to 64 bits, everything
     else in fp32 (the FFN's inner values as the sum of two numbers of the weights' type), and
     rounded once."""
-    T = x.shape[0]
+    at = weights.addresses()
     if x.dim() != 2 or x.shape[1] != weights.hidden or x.dtype is not weights.dtype or x.get_device() != weights.index:
         _need_cuda(x)
         raise ValueError(f"x must be [tokens, {weights.hidden}] {weights.dtype} on {weights.device}")
@@ -97,6 +114,7 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
             if v is not None and v.requires_grad:
                 raise NotImplementedError("moe_layer has no gradients")
     _no_tangents("moe_layer", x, residual, *weights.tensors)
+    T = x.shape[0]
     x = _aligned(x)
     res = None if residual is None else _aligned(residual)
     out = x.new_empty(x.shape)
@@ -105,10 +123,8 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     if T:
         size = weights.workspace_bytes(T, topk)
         ws = x.new_empty(size, dtype=torch.uint8)
-        t = weights.tensors
         _call("dash_moe", _ARGS(
-            x.data_ptr(), x.stride(0), t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(),
-            0 if t[3] is None else t[3].data_ptr(), 0 if t[4] is None else t[4].data_ptr(),
+            x.data_ptr(), x.stride(0), *at,
             0 if res is None else res.data_ptr(), 0 if res is None else res.stride(0), out.data_ptr(), weights.hidden,
             ids.data_ptr(), w.data_ptr(), T, weights.hidden, weights.ffn, weights.experts, topk, weights.shared_ffn,
             _DT[x.dtype], weights.gate_f32, 1 if renormalize else 0, scale, ws.data_ptr(), size,

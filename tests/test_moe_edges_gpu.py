@@ -116,3 +116,32 @@ def test_heights_of_tiles(case, dt):
     tokens, hidden, ffn, experts, topk, shared = case
     t, w = make(tokens, hidden, ffn, experts, shared, dt)
     check(t, moe.moe_layer(t["x"], w, topk, residual=t["residual"]), topk)
+
+
+def test_weights_of_other_memory():
+    """A tensor's .data can be other memory (a module's `to`): it is read, or refused where it does not fit."""
+    t, w = make(4, 64, 32, 6, 8)
+    moe.moe_layer(t["x"], w, 2)
+    n, nw = make(4, 64, 32, 6, 8, seed=1)
+    want = moe.moe_layer(t["x"], nw, 2)
+    old = [v.data for v in w.tensors]
+    for a, b in zip(w.tensors, nw.tensors):
+        a.data = b.data.clone()
+    assert torch.equal(moe.moe_layer(t["x"], w, 2).out, want.out)
+    for a in w.tensors:
+        a.data = a.data.half()
+    with pytest.raises(ValueError):
+        moe.moe_layer(t["x"], w, 2)
+    half = dict(zip(("gate", "gu", "down", "sgu", "sd"), w.tensors), x=t["x"].half(), residual=None)
+    check(half, moe.moe_layer(half["x"], w, 2), 2, residual=False)
+    for a, b in zip(w.tensors, old):
+        a.data = b
+    w.tensors[2].data = old[2][:, :56].contiguous()
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            moe.moe_layer(t["x"], w, 2)
+    w.tensors[2].data = old[2].cpu()
+    with pytest.raises(RuntimeError):
+        moe.moe_layer(t["x"], w, 2)
+    w.tensors[2].data = old[2]
+    check(t, moe.moe_layer(t["x"], w, 2, residual=t["residual"]), 2)

@@ -12,13 +12,13 @@
 //   moe_combine_kernel  the weighted sum in the picks' order, and the residual
 //
 // Each kernel is launched while the one before it runs and waits for its results on the
-// GPU: gate_up's CTAs bring the shared expert's weights into L2 while the router
-// works, and down's CTAs take the places of gate_up's as they end.  Each waits for all of the kernel before it
-// before it reads anything: down takes the sorted picks from gate_up, which waited for the router.  (Reading
+// GPU: gate_up's CTAs bring a shared expert's weights into L2 while the router works, if
+// they are few, and down's CTAs take the places of gate_up's as they end.  Each waits for all of the kernel before
+// it before it reads what that one wrote: down takes the sorted picks from gate_up, which waited for the router.  (Reading
 // the router's picks while gate_up's last tiles were under way, and filling the rings with weights, took 1
 // to 2.5 us less, but nothing promises that what the kernel before last has written is visible then.)
 //
-// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 27.2 / 56.3 / 90.1 us
+// Measured (64 experts of 896, 6 picked, 2 shared, hidden 1,280, bf16; CUDA graph): 27.6 / 56.5 / 90.2 us
 // for 1 / 8 / 64 tokens, where the weights at the copy rate take 8.4 / 38.7 / 69.2.  While gate_up
 // and down stream, they read at 7.1 TB/s; the rest is the order of things.  One token, by the
 // global timer: scores 2.5 us, picks 3.8, sorted by expert in every CTA 6.4, the first
@@ -413,9 +413,12 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
     prefetch_tmap(&maps.sb);
     prefetch_tmap(&maps.sw);
   }
-  if (!DOWN && a.shared_ffn) {
-    // the shared expert's weights into L2, while the router works
-    const int64_t bytes = (int64_t)a.shared_ffn * a.hidden * 2, piece = 4096;
+  // The shared expert's weights into L2, while the router works.  14 MB of them (the layer above): 3 to 8 tokens 1 us
+  // less.  50 MB: 1 token 47 us, without 44; 402 MB, more than L2 holds: 1 token 126 and 118, 64 tokens 284 and 263.
+  constexpr int64_t kFetchMost = (int64_t)24 << 20;
+  const int64_t bytes = (int64_t)a.shared_ffn * a.hidden * 2;
+  if (!DOWN && 3 * bytes <= kFetchMost) {
+    const int64_t piece = 4096;
     for (int64_t at = ((int64_t)tid * gridDim.x + blockIdx.x) * piece; at < 3 * bytes; at += (int64_t)gridDim.x * kThreads * piece) {
       const bool up = at < 2 * bytes;
       const char* p = up ? static_cast<const char*>(a.shared_gate_up) + at : static_cast<const char*>(a.shared_down) + (at - 2 * bytes);
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(256, 3) moe_ffn_kernel(const __grid_constant__
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *holder;
-  // Each kernel waits here for the one before it: gate_up for the router's picks, down for
+  // Both wait here for the kernel before: gate_up for the router's picks, down for
   // the sorted picks and act.  (Nothing is read before this kernel's own wait: only what the kernel
   // directly before has written, or itself waited for and passed on, is sure to be there.)
   uint8_t* sorted = static_cast<uint8_t*>(a.workspace) + buf.sorted;

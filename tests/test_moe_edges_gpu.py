@@ -145,3 +145,10 @@ def test_weights_of_other_memory():
         moe.moe_layer(t["x"], w, 2)
     w.tensors[2].data = old[2]
     check(t, moe.moe_layer(t["x"], w, 2, residual=t["residual"]), 2)
+
+
+@pytest.mark.parametrize("tokens", [2, 20])
+def test_wide_shared_experts(tokens):
+    """More weights than are fetched ahead."""
+    t, w = make(tokens, 4096, 64, 3, 1032)
+    check(t, moe.moe_layer(t["x"], w, 2, residual=t["residual"]), 2)

@@ -50,7 +50,10 @@ constexpr int kTable = 256;                      // 2^(j / 256)
 // (the slice lies behind Shared, whose size is a multiple of its alignment)
 constexpr int kSliceMost = 128 * 1024;           // bytes of a slice kept in shared memory
 constexpr int kSliceTwo = 68 * 1024;             // the same with two CTAs on an SM
-constexpr int kSliceMany = 20 * 1024;            // with four
+// With four, which Shared leaves 12 KB each: at 15 KB only three ran at once, and rows cut for four in two waves
+// (70 rows of 60,000, bf16: greedy 18.8 us, top-p 0.9 74; left in global memory, 13.4 and 55; 72 of 32,000, fp32,
+// where clusters of 8 do not fill every SM: 17.5 and 51, 19.5 and 55).
+constexpr int kSliceMany = 12 * 1024;
 // Up to so many rows a CTA has 512 threads (two on an SM, slices in shared memory), above it 256
 // (four).  64 rows of 129,280 (fp32) with settings of their own 59 us, with 256 threads 78; with
 // top-k 20 alone 37 and 30.  Distributions of 128 rows (bf16), top-k 50: 88 and 52.
@@ -75,8 +78,9 @@ struct alignas(16) Shared {
   uint64_t found_before, found_here;             // of the digit that was looked for
   uint32_t found;
   int32_t last;                                  // cutoff index, exchanged
-  int32_t any[kMaxCluster];
 };
+static_assert(4 * (sizeof(Shared) + kSliceMany + 1024) <= 228 * 1024 && 2 * (sizeof(Shared) + kSliceTwo + 1024) <= 228 * 1024,
+              "as many CTAs on an SM as their names say");
 
 // -inf and NaN: 0 (out); otherwise in the order of the values, -0 as 0
 __device__ __forceinline__ uint32_t key_of(float z) {

@@ -61,17 +61,16 @@ class MoeWeights:
         self.experts, self.hidden, self.ffn, self.shared_ffn = E, H, F, S
         self.gate_f32 = 1 if gate.dtype is torch.float32 else 0
         self._sizes = {}
-        self.seen = self._now()
-
-    def _now(self):
-        return [None if t is None else (t.data_ptr(), t.dtype) for t in self.tensors]
+        self.given = [t for t in self.tensors if t is not None]
+        self.seen = [t.data_ptr() for t in self.given], [t.dtype for t in self.given]
 
     def addresses(self):
         """Of the tensors as they are now (0: none)."""
-        now = self._now()
-        if now != self.seen:
+        if self.seen is None or self.seen[0] != [t.data_ptr() for t in self.given] or \
+                self.seen[1] != [t.dtype for t in self.given]:
             self._check()
-        return [0 if n is None else n[0] for n in now]
+        at = self.seen[0]
+        return at if len(at) == 5 else [*at, 0, 0]
 
     def workspace_bytes(self, tokens: int, topk: int) -> int:
         n = self._sizes.get((tokens, topk))
@@ -110,8 +109,8 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
                                  residual.get_device() != weights.index):
         raise ValueError("residual must have x's shape, type and device")
     if torch.is_grad_enabled():
-        for v in (x, residual, *weights.tensors):
-            if v is not None and v.requires_grad:
+        for v in (x, *weights.given) if residual is None else (x, residual, *weights.given):
+            if v.requires_grad:
                 raise NotImplementedError("moe_layer has no gradients")
     _no_tangents("moe_layer", x, residual, *weights.tensors)
     T = x.shape[0]

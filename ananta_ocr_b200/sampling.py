@@ -51,8 +51,10 @@ def probs(logits: torch.Tensor, *, temperature: Setting = 1.0, top_k: Union[int,
     keeps nothing is all 0).  No gradients: logits and settings that ask for them, or
     carry tangents, are refused."""
     rows = _check(logits)
-    if torch.is_grad_enabled() and any(torch.is_tensor(t) and t.requires_grad for t in (logits, temperature, top_p, min_p)):
-        raise NotImplementedError("probs has no gradients")
+    if torch.is_grad_enabled():
+        for t in (logits, temperature, top_p, min_p):
+            if torch.is_tensor(t) and t.requires_grad:
+                raise NotImplementedError("probs has no gradients")
     _no_tangents("probs", logits, temperature, top_p, min_p)
     out = logits.new_empty(logits.shape, dtype=torch.float32)
     _run(logits, rows, None, temperature, top_k, top_p, min_p, None, out)

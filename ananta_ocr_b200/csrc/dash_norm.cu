@@ -12,8 +12,9 @@
 // Bound by memory: y and residual in, s and h out (forward); those two and the
 // gradients of s and h in, those of y and residual out (backward).  Rows of 1,280, bf16: forward
 // 36,992 of them 66 us (5.8 TB/s; 78 with post and gate), 8 of them 5.2 us from a graph;
-// gradients of 9,248 plain ones 27 us (22 at the copy rate), of 36,992 with post and gate 146 us
-// (87): there the issue of instructions is 60% busy with 15 warps on an SM, which is what the
+// gradients of 9,248 plain ones 27 us (22 at the copy rate), of 36,992 with post and gate 143 us
+// (87, the column sums' kernel among them).  With post or gate the forward's issue of instructions is 72% busy and memory 52%;
+// in the gradients the issue of instructions is 60% busy with 15 warps on an SM, which is what the
 // column sums and weights in registers leave room for.
 #include "dash_common.cuh"
 #include "dash_internal.h"
@@ -902,7 +903,7 @@ NormCut norm_cut(const DashNormArgs& a, int E) {
       c.nv *= 2, warps = (vecs + 32 * c.nv - 1) / (32 * c.nv);
   c.threads = warps * 32;
   const int most = 148 * max(1, min(8, kNormThreads / c.threads));
-  // chunks of at least 4 rows where there are enough rows for all CTAs
+  // rows dealt evenly, in chunks that lie within a group
   const int64_t groups = a.rows / a.group_rows;
   const int64_t want = (a.rows + most - 1) / most;
   c.chunk = min((int64_t)a.group_rows, max((int64_t)1, want));

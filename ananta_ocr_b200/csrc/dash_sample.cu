@@ -95,8 +95,10 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 
 // exp((z - top) / t) in units of 2^-43, relative error below 3e-12: with y = (z - top) / (t ln 2) * 256
 // = 256 k + j + r, |r| <= 1, it is 2^k * 2^(j/256) * exp(r ln2 / 256), the last factor by its series
-// (the term behind the cubic one is 2.2e-12).  Eight 64-bit operations per weight; the
-// largest logit has 1 exactly, an infinite one, too.
+// (the term behind the cubic one is 2.2e-12).  `add` is rounded, too: 1.1e-16 * |top| / t, which passes that where
+// |top| / t is above 3e4 (bf16 and fp16 logits are 7 t apart there or more, fp32 ones 0.0009 t, and above 1e9 nothing
+// but the largest has a weight).  Eight 64-bit operations per weight; the largest logit has 1 exactly, an
+// infinite one, too.
 struct Weight {
   float top;                                     // largest logit
   double mul, add;                               // y = z * mul + add
@@ -203,8 +205,8 @@ __device__ void total_of(Shared& S, cg::cluster_group& cl, int C, int rank, bool
 template <int kThreads>
 __device__ void digit_of(Shared& S, uint64_t want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // thread t: the four bins from 4 t down, counted from the top
   constexpr int PER = kBins / kThreads;
+  // thread t: PER bins from PER * t down, counted from the top
   uint64_t v[PER], own = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {

@@ -98,7 +98,7 @@ def moe_layer(x: torch.Tensor, weights: MoeWeights, topk: int, *, renormalize: b
     picked ones) times ``scale``.
 
     x, residual [tokens, hidden] of the weights' type, at most 256 tokens; no gradients (inputs and
-    weights that ask for them, or carry tangents, are refused).  Scores are computed to 64 bits, everything
+    weights that ask for them, or carry tangents, are refused).  Scores are 64-bit sums, everything
     else in fp32 (the FFN's inner values as the sum of two numbers of the weights' type), and
     rounded once."""
     at = weights.addresses()

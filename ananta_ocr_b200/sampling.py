@@ -47,8 +47,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: Setting = 1.0,
 
 def probs(logits: torch.Tensor, *, temperature: Setting = 1.0, top_k: Union[int, torch.Tensor] = 0, top_p: Setting = 1.0,
           min_p: Setting = 0.0) -> torch.Tensor:
-    """fp32 [rows, vocab]: the kept tokens' probabilities, 0 for the others (a row that
-    keeps nothing is all 0).  No gradients: logits and settings that ask for them, or
+    """fp32 [rows, vocab]: the kept tokens' probabilities, 0 for the others and for those below 2^-44
+    of the largest's (a row that keeps nothing is all 0).  No gradients: logits and settings that ask for them, or
     carry tangents, are refused."""
     rows = _check(logits)
     if torch.is_grad_enabled():

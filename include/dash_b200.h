@@ -1097,7 +1097,7 @@ int dash_add_norm_bwd(const DashNormBwdArgs* args, dash_stream_t stream);
  *   (k <= 0: all), of those the shortest head that holds the share p of their sum of e
  *   (p >= 1: all; always the first), of those the ones with e >= m
  *   tokens: the first kept i whose running sum of e, in the vocabulary's order, exceeds u
- *   times the kept sum; probs: e_i / kept sum for kept tokens, else 0
+ *   times the kept sum; probs: e_i / kept sum for kept tokens, else 0 (e below 2^-44 counts as 0)
  * t <= 0: the largest z alone.  A row that nothing is left of gives -1 and zeros.  Sums are
  * whole numbers of 2^-43 of the largest e, so that no order of adding changes them.  Either
  * of tokens and probs may be NULL.  vocab <= 2^20.  */
@@ -1124,9 +1124,9 @@ int dash_sample(const DashSampleArgs* args, dash_stream_t stream);
  *   smallest), in that order; w = softmax(score)[ids] (renorm: over their sum) * scale
  *   out = residual + sum_j w_j down[ids_j] act_j + shared_down act_s
  *   act = silu(g) * u of gate_up x, whose first half of rows is g, its second u
- * x, the experts and out are of one 16-bit type.  Scores are exact to 64 bits, act is kept
- * as the sum of two 16-bit numbers (with fp16, beyond its range it is infinite), everything else is
- * fp32, rounded once.  hidden, ffn and shared_ffn are multiples of 8; all rows and pointers
+ * x, the experts and out are of one 16-bit type.  Scores are 64-bit sums, act is kept
+ * as the sum of two 16-bit numbers (with fp16 the second one 2^11 times as large; beyond its range act is
+ * infinite), everything else is fp32, rounded once.  hidden, ffn and shared_ffn are multiples of 8; all rows and pointers
  * 16-byte aligned.  out may lie on residual.  workspace: dash_moe_workspace_size bytes.  */
 typedef struct {
   const void* x;          int64_t x_stride;         /* [tokens, hidden] */

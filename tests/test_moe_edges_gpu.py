@@ -152,3 +152,16 @@ def test_wide_shared_experts(tokens):
     """More weights than are fetched ahead."""
     t, w = make(tokens, 4096, 64, 3, 1032)
     check(t, moe.moe_layer(t["x"], w, 2, residual=t["residual"]), 2)
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 64])
+def test_calls_repeat_themselves(tokens):
+    """Whatever the workspace held before: bit for bit."""
+    t, w = make(tokens, 1280, 896, 64, 1792)
+    want = moe.moe_layer(t["x"], w, 6, residual=t["residual"])
+    size = w.workspace_bytes(tokens, 6)
+    for byte in (0xff, 0x7f, 0x00, 0x5a) * 3:
+        torch.full((size,), byte, dtype=torch.uint8, device="cuda")          # (freed at once, and the next to be handed out)
+        r = moe.moe_layer(t["x"], w, 6, residual=t["residual"])
+        for a, b in zip(r, want):
+            assert torch.equal(a, b)
